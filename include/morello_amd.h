@@ -630,6 +630,117 @@ int mrl_action_apply(const mrl_spec *spec, const mrl_action *action, mrl_rewrite
 int mrl_run_action_timed(const mrl_spec *spec, void *const *params, const mrl_action *action, uint32_t steps,
                          double *device_ms_total);
 
+/* ---- A cache of keys and values in pages ---------------------------------------------------
+ * No counterpart in the reference, whose Compose attends to dense tensors.  A serving program keeps the keys and
+ * values of its requests in pages of `page_size` slots; a request's pages are listed, in order, in its row of a page
+ * table, and its key j is in slot j % page_size of the page at column j / page_size.  Per step:
+ *   mrl_run_page_tables     the requests' lengths -> page tables, slots and positions, on the device
+ *   mrl_run_rotary          (in each layer) queries and keys turned by their tokens' positions, keys and values into their slots
+ *   mrl_run_paged_attention (in each layer) the new tokens' attention over their requests' pages
+ * The three only enqueue on `stream` (NULL = default stream), take no device memory of their own and make no call that a
+ * capture forbids: they may be recorded into a graph as they are.  What a call has to know of the requests it reads on the
+ * device; the descriptors hold what is fixed between steps, so that a recorded call stays good while lengths change.  `params`
+ * holds device pointers in the order given at each call, none NULL unless said so, aligned as their element type at least; In
+ * parameters must not alias written ones except where said so.  Buffers and stream belong to the device given to mrl_init,
+ * which is the calling thread's current one (MRL_ERR_NO_DEVICE otherwise).  Strides count elements; all strides of a tensor
+ * zero means dense in the order its indices are named; negative ones are refused (MRL_ERR_BAD_SPEC), and so are strides under which two elements
+ * of a written tensor could fall together.  Descriptors are zero-initialised before their fields are set. */
+
+/* Lengths of requests -> what a step of them needs.  Request r has max(cached[r], 0) tokens in the cache and
+ * max(added[r], 0) new ones, which are rows starts[r] .. starts[r + 1] - 1 of the step's tensors; new tokens past `tokens` rows are
+ * left out.  A request's pages for its new tokens come off the end of the free list, request after request, as many as
+ * its length wants beyond ceil(cached / page_size) and table_width allows.
+ * params:
+ *   0  cached      i32 [requests]
+ *   1  added       i32 [requests]
+ *   2  free list   i32 [free_pages]   page numbers, of which
+ *   3  free count  i32 [1]            the first so many are free (taken as 0 .. free_pages)
+ *   4  page table  i32 [requests][table_width]  (InOut) new pages' columns are written, -1 where the list has run out; others are left
+ *   5  starts      i32 [requests + 1] (Out)
+ *   6  lengths     i32 [requests]     (Out) keys of the request once the step's are written
+ *   7  slots       i32 [tokens]       (Out) page * page_size + place in it; -1 for a token without a page below `pages`, and behind the last token
+ *   8  positions   i32 [tokens]       (Out) places of the tokens in their requests, from 0; 0 behind the last token
+ *   9  free left   i32 [2]            (Out) pages left on the list; pages that were wanting
+ * The call reads nothing that it writes but columns of the page table that it leaves: run again on the same inputs it gives the
+ * same.  The next step's free count is free left's first entry (two buffers that take turns). */
+typedef struct {
+  uint32_t requests, table_width, page_size;
+  uint32_t pages;       /* of the cache: page numbers are below it; pages * page_size < 2^31 */
+  uint32_t tokens;      /* rows of the step's tensors */
+  uint32_t free_pages;  /* entries of the free list, 0 allowed (parameter 2 may then be NULL) */
+} mrl_page_tables;
+int mrl_page_tables_check(const mrl_page_tables *op);
+int mrl_run_page_tables(const mrl_page_tables *op, void *const *params, void *stream);
+int mrl_page_tables_plan(const mrl_page_tables *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
+/* Rotary positions with up to four axes (time, height and width, say).  Each head's first 2 * P dims are P pairs, P the sum of
+ * `sections`: dims i and P + i, or 2 i and 2 i + 1 with `adjacent`.  The first sections[0] pairs follow axis 0, the next sections[1]
+ * axis 1, and so on: pair i turns by the angle positions[axis][token] * frequencies[i],
+ *     (x, y) -> (x cos - y sin, y cos + x sin),
+ * or back by it with `inverse`: the gradient's way through the op.  The dims behind the pairs are copied.  Angles are formed
+ * in 64 bits, sums in 32, and each result is rounded once.
+ * page_size 0: keys go to a dense tensor [tokens][kv_heads][head_dim], values are not touched (parameters 2, 5 and 8 may be NULL).
+ * Otherwise keys and values go to their slots in the cache; a token whose slot is not one of pages * page_size is left out of
+ * it.  Slots of different tokens differ: of tokens that share one, any's elements are kept.  kv_heads 0: queries alone (1, 2, 5, 7, 8 may be NULL).
+ * params:
+ *   0  q            [tokens][q_heads][head_dim]
+ *   1  k            [tokens][kv_heads][head_dim]
+ *   2  v            [tokens][kv_heads][head_dim]
+ *   3  positions    i32 [axes][tokens]
+ *   4  frequencies  f32 [P]
+ *   5  slots        i32 [tokens]
+ *   6  q out        [tokens][q_heads][head_dim]          (Out; may be q itself with q's strides)
+ *   7  keys         [pages][page_size][kv_heads][head_dim] or dense (Out; dense may be k itself with k's strides)
+ *   8  values       [pages][page_size][kv_heads][head_dim]          (Out) */
+#define MRL_MAX_AXES 4
+typedef struct {
+  int32_t dtype;                   /* of q, k, v and where they go: MRL_BF16 or MRL_F32 */
+  uint32_t tokens, q_heads, kv_heads, head_dim;
+  uint32_t axes;                   /* 1 .. MRL_MAX_AXES */
+  uint32_t sections[MRL_MAX_AXES]; /* pairs of each axis; 2 * their sum is at most head_dim and at most 1024 */
+  int32_t adjacent, inverse;
+  uint32_t page_size, pages;       /* pages * page_size < 2^31 */
+  int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2]; /* of a token, of a head */
+  int64_t key_strides[3], value_strides[3];  /* of a page, of a slot, of a head (dense keys: the first is not used, the second a token's) */
+} mrl_rotary;
+int mrl_rotary_check(const mrl_rotary *op);
+int mrl_run_rotary(const mrl_rotary *op, void *const *params, void *stream);
+int mrl_rotary_plan(const mrl_rotary *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
+/* Attention of each request's new tokens over its pages, the new tokens' own keys among them.  With n = starts[r + 1] - starts[r]
+ * new tokens, the i-th of them stands at p = lengths[r] - n + i and sees the keys j of its request with j <= p, j > p - window
+ * (window 0: no such bound), j < lengths[r], whose page is one of the cache's (page numbers from 0 to pages - 1; a column past the
+ * table or a number outside hides its keys).  Query head h reads key/value head h / (q_heads / kv_heads).
+ *     out = sum_j softmax_j(scale * q . k_j) v_j over the keys seen, zeros where none is or all score -infinity
+ * What a hidden slot holds, NaN or infinity, does not matter.  Rows of q and out outside starts[0] .. starts[requests] are
+ * neither read nor written.  starts do not fall (whatever they are, no row outside 0 .. tokens is touched).
+ * Scores, statistics and sums are held in 32 bits; bf16: probabilities are rounded to bf16 for the product with the values.
+ * params:
+ *   0  q           [tokens][q_heads][head_dim]
+ *   1  keys        [pages][page_size][kv_heads][head_dim]
+ *   2  values      [pages][page_size][kv_heads][head_dim]
+ *   3  page table  i32 [requests][table_width]
+ *   4  starts      i32 [requests + 1]
+ *   5  lengths     i32 [requests]
+ *   6  out         [tokens][q_heads][head_dim]  (Out)
+ *   7  workspace   mrl_paged_attention_workspace_bytes() bytes, 16-byte aligned, what it holds does not matter; may be
+ *                  NULL where that is 0.  A call owns it from its first kernel to its last: calls that may overlap in
+ *                  time (other streams, graphs launched side by side) have one each. */
+typedef struct {
+  int32_t dtype;        /* of q, keys, values and out: MRL_BF16 or MRL_F32 */
+  uint32_t tokens, requests, q_heads, kv_heads, head_dim;  /* head_dim up to 1024; q_heads a multiple of kv_heads */
+  uint32_t page_size, pages, table_width;
+  uint32_t max_new;     /* new tokens of any one request, where the program knows a bound (it chooses kernels; results do not depend on it); 0: tokens */
+  uint32_t window;
+  float scale;          /* 0: 1 / sqrt(head_dim) */
+  int64_t q_strides[2], out_strides[2];      /* of a token, of a head */
+  int64_t key_strides[3], value_strides[3];  /* of a page, of a slot, of a head */
+} mrl_paged_attention;
+int mrl_paged_attention_check(const mrl_paged_attention *op);
+size_t mrl_paged_attention_workspace_bytes(const mrl_paged_attention *op);
+int mrl_run_paged_attention(const mrl_paged_attention *op, void *const *params, void *stream);
+int mrl_paged_attention_plan(const mrl_paged_attention *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,12 +19,16 @@ import numpy as np
 from . import _binding as B
 
 
+_PAGED_CALLS = ("mrl_run_page_tables", "mrl_run_rotary", "mrl_run_paged_attention", "mrl_page_tables_plan", "mrl_rotary_plan", "mrl_paged_attention_plan")
+
+
 class MorelloError(RuntimeError):
     def __init__(self, status: int, where: str):
         lib = B.load()
         msg = lib.mrl_status_string(status).decode()
         detail = lib.mrl_last_error().decode()
-        with_detail = status == 4 or where == "mrl_run_noalloc"   # the calls that set the detail they fail with
+        # the calls that set the detail they fail with
+        with_detail = status == 4 or where == "mrl_run_noalloc" or (status != 6 and where in _PAGED_CALLS)
         super().__init__(f"{where}: {msg}" + (f" ({detail})" if detail and with_detail else ""))
         self.status = status
 
@@ -574,6 +578,90 @@ class Compose:
         arr = _pointers[len(ptrs)](*ptrs)
         _check(B.load().mrl_run_compose(C.byref(self._c), arr, None), "mrl_run_compose")
         synchronize()
+
+
+class _PagedOp:
+    """An operator over a cache in pages: a descriptor that stays the same between steps, device pointers per call."""
+    _name, _params = "", 0
+
+    def check(self) -> int:
+        return int(getattr(B.load(), f"mrl_{self._name}_check")(C.byref(self._c)))
+
+    def plan(self) -> "Plan":
+        return _plan_of(getattr(B.load(), f"mrl_{self._name}_plan"), self._c, f"mrl_{self._name}_plan")
+
+    def run_async(self, ptrs: Sequence[Optional[int]], stream=None):
+        """Enqueues the call on `stream` (a Stream, or a HIP stream's handle as an integer; None = the default stream) and
+        returns.  `ptrs`: device pointers in the order include/morello_amd.h gives, None or 0 where one may be NULL."""
+        if len(ptrs) != self._params:
+            raise ValueError(f"{self._params} parameters")
+        handle = stream.handle if isinstance(stream, Stream) else C.c_void_p(stream or 0)
+        _check(self._run(C.byref(self._c), _pointers[self._params](*ptrs), handle), f"mrl_run_{self._name}")
+
+    def run_device(self, ptrs: Sequence[Optional[int]]):
+        self.run_async(ptrs)
+        synchronize()
+
+    def _finish(self):
+        self._run = getattr(B.load(), f"mrl_run_{self._name}")
+
+
+def _set_strides(c, **given):
+    for name, values in given.items():
+        field = getattr(c, name)
+        if values is None:
+            continue
+        if len(values) != len(field):
+            raise ValueError(f"{name}: {len(field)} strides")
+        for i, v in enumerate(values):
+            field[i] = v
+
+
+class PageTables(_PagedOp):
+    """Lengths of requests -> page tables, slots and positions of a step's new tokens (mrl_page_tables).
+    Parameters: cached, added, free list, free count, page table (InOut), starts, lengths, slots, positions, free left; all i32."""
+    _name, _params = "page_tables", 10
+
+    def __init__(self, requests, table_width, page_size, pages, tokens, free_pages):
+        self._c = B.PageTablesC(requests, table_width, page_size, pages, tokens, free_pages)
+        self._finish()
+
+
+class Rotary(_PagedOp):
+    """Queries and keys turned by their tokens' positions, keys and values into their slots of a cache in pages, or (page_size 0) keys to
+    a dense tensor (mrl_rotary).  `sections`: pairs of dims that follow each axis of the positions.
+    Parameters: q, k, v, positions, frequencies, slots, q out, keys, values."""
+    _name, _params = "rotary", 9
+
+    def __init__(self, dtype, tokens, q_heads, kv_heads, head_dim, sections, adjacent=False, inverse=False, page_size=0, pages=0,
+                 q_strides=None, k_strides=None, v_strides=None, q_out_strides=None, key_strides=None, value_strides=None):
+        self._c = B.RotaryC()
+        c = self._c
+        c.dtype, c.tokens, c.q_heads, c.kv_heads, c.head_dim = int(dtype), tokens, q_heads, kv_heads, head_dim
+        if not 1 <= len(sections) <= B.MAX_AXES:
+            raise ValueError(f"1 to {B.MAX_AXES} sections")
+        c.axes = len(sections)
+        for i, n in enumerate(sections):
+            c.sections[i] = n
+        c.adjacent, c.inverse, c.page_size, c.pages = int(adjacent), int(inverse), page_size, pages
+        _set_strides(c, q_strides=q_strides, k_strides=k_strides, v_strides=v_strides, q_out_strides=q_out_strides,
+                     key_strides=key_strides, value_strides=value_strides)
+        self._finish()
+
+
+class PagedAttention(_PagedOp):
+    """Attention of each request's new tokens over its pages of keys and values (mrl_paged_attention).
+    Parameters: q, keys, values, page table, starts, lengths, out, workspace (workspace_bytes() bytes)."""
+    _name, _params = "paged_attention", 8
+
+    def __init__(self, dtype, tokens, requests, q_heads, kv_heads, head_dim, page_size, pages, table_width, max_new=0, window=0, scale=0.0,
+                 q_strides=None, out_strides=None, key_strides=None, value_strides=None):
+        self._c = B.PagedAttentionC(int(dtype), tokens, requests, q_heads, kv_heads, head_dim, page_size, pages, table_width, max_new, window, scale)
+        _set_strides(self._c, q_strides=q_strides, out_strides=out_strides, key_strides=key_strides, value_strides=value_strides)
+        self._finish()
+
+    def workspace_bytes(self) -> int:
+        return int(B.load().mrl_paged_attention_workspace_bytes(C.byref(self._c)))
 
 
 class PlanStep:

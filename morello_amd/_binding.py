@@ -102,6 +102,27 @@ class PlanC(C.Structure):
     _fields_ = [("n_steps", C.c_uint32), ("scratch_bytes", C.c_uint64), ("cost_ns", C.c_double)]
 
 
+MAX_AXES = 4
+
+
+class PageTablesC(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("requests", "table_width", "page_size", "pages", "tokens", "free_pages")]
+
+
+class RotaryC(C.Structure):
+    _fields_ = [("dtype", C.c_int32)] + [(n, C.c_uint32) for n in ("tokens", "q_heads", "kv_heads", "head_dim", "axes")] + [
+        ("sections", C.c_uint32 * MAX_AXES), ("adjacent", C.c_int32), ("inverse", C.c_int32), ("page_size", C.c_uint32), ("pages", C.c_uint32)] + [
+        (n, C.c_int64 * 2) for n in ("q_strides", "k_strides", "v_strides", "q_out_strides")] + [
+        (n, C.c_int64 * 3) for n in ("key_strides", "value_strides")]
+
+
+class PagedAttentionC(C.Structure):
+    _fields_ = [("dtype", C.c_int32)] + [(n, C.c_uint32) for n in (
+        "tokens", "requests", "q_heads", "kv_heads", "head_dim", "page_size", "pages", "table_width", "max_new", "window")] + [
+        ("scale", C.c_float)] + [(n, C.c_int64 * 2) for n in ("q_strides", "out_strides")] + [
+        (n, C.c_int64 * 3) for n in ("key_strides", "value_strides")]
+
+
 # name -> (restype, argtypes); every symbol include/morello_amd.h declares.
 SIGNATURES = {
     "mrl_init": (C.c_int, [C.c_int]),
@@ -176,6 +197,16 @@ SIGNATURES = {
     "mrl_compose_plan": (C.c_int, [C.POINTER(ComposeC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
     "mrl_device_info": (C.c_int, [C.c_char_p, C.c_size_t, C.POINTER(C.c_int), C.POINTER(C.c_int),
                                   C.POINTER(C.c_size_t)]),
+    "mrl_page_tables_check": (C.c_int, [C.POINTER(PageTablesC)]),
+    "mrl_run_page_tables": (C.c_int, [C.POINTER(PageTablesC), _VPP, C.c_void_p]),
+    "mrl_page_tables_plan": (C.c_int, [C.POINTER(PageTablesC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_rotary_check": (C.c_int, [C.POINTER(RotaryC)]),
+    "mrl_run_rotary": (C.c_int, [C.POINTER(RotaryC), _VPP, C.c_void_p]),
+    "mrl_rotary_plan": (C.c_int, [C.POINTER(RotaryC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_paged_attention_check": (C.c_int, [C.POINTER(PagedAttentionC)]),
+    "mrl_run_paged_attention": (C.c_int, [C.POINTER(PagedAttentionC), _VPP, C.c_void_p]),
+    "mrl_paged_attention_plan": (C.c_int, [C.POINTER(PagedAttentionC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionC)]),
 }
 
 _lib = None

@@ -6,6 +6,7 @@
 
 #include <cstdio>
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <map>
 #include <memory>
@@ -16,6 +17,7 @@
 #include "host_stage.h"
 #include "kernels.h"
 #include "layout_factor.h"
+#include "paged.h"
 
 namespace {
 
@@ -1830,7 +1832,7 @@ uint32_t mrl_target_kernels(const char **names, uint32_t cap) {
       "k_softmax_cols",
       "k_softmax_generic", "k_softmax_cols_short", "k_parts", "k_parts_block", "k_parts_rows", "k_parts_cols", "k_broadcast", "k_broadcast_rows", "k_broadcast_fill_rows", "k_fill", "k_fill16", "k_fill_zero", "k_move_rows", "k_move_runs",
       "k_move_tiled", "k_move_tiled_as", "k_move_tiled8v", "k_move_tiled16", "k_move_tiled16v", "k_move_tiled32", "k_move_gather", "k_move_generic", "k_relayout", "k_convert4", "k_copy1",
-      "k_copy16", "k_pad_rows", "k_pad_rows_pair", "k_widen_bf16"};
+      "k_copy16", "k_pad_rows", "k_pad_rows_pair", "k_widen_bf16", "k_page_tables", "k_rotary", "k_paged_attn_generic"};
   const uint32_t n = sizeof families / sizeof families[0];
   for (uint32_t i = 0; i < n && i < cap && names; i++) names[i] = families[i];
   return n;
@@ -2731,6 +2733,252 @@ int mrl_device_info(char *name, size_t name_len, int *compute_units, int *clock_
   if (clock_khz) *clock_khz = prop.clockRate;
   if (total_mem_bytes) *total_mem_bytes = prop.totalGlobalMem;
   return MRL_OK;
+}
+
+}  // extern "C"
+
+// ---- The cache of keys and values in pages: checks of the descriptors, strides filled in, launches ----
+namespace {
+
+int bad(int status, const char *what) {
+  g_last_error = what;
+  return status;
+}
+
+constexpr uint32_t MOST_TOKENS = 1u << 23;          // a workgroup to each, of up to 256 threads, is still a launch
+constexpr int64_t MOST_STRIDE = int64_t(1) << 40;   // products of strides and indices stay far from 2^63
+
+// Strides of a tensor with dims `n`, slowest first, and `inner` contiguous elements behind them; all zero: dense.  `written`: no two
+// elements of it may fall together.
+int fill_strides(const int64_t *given, const uint32_t *n, int dims, uint32_t inner, bool written, const char *name, int64_t *out) {
+  bool dense = true;
+  for (int d = 0; d < dims; d++) {
+    if (given[d] < 0 || given[d] > MOST_STRIDE) return bad(MRL_ERR_BAD_SPEC, (std::string(name) + ": a stride is negative or past 2^40").c_str());
+    dense = dense && given[d] == 0;
+  }
+  if (dense) {
+    int64_t run = inner;
+    for (int d = dims - 1; d >= 0; d--) out[d] = run, run *= n[d];
+    return MRL_OK;
+  }
+  for (int d = 0; d < dims; d++) out[d] = given[d];
+  if (!written) return MRL_OK;
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + dims, [&](int x, int y) { return out[x] < out[y]; });
+  int64_t span = inner;   // elements that the dims so far reach over
+  for (int i = 0; i < dims; i++) {
+    const int d = order[i];
+    if (n[d] <= 1) continue;
+    if (out[d] < span) return bad(MRL_ERR_BAD_SPEC, (std::string(name) + ": elements of a written tensor overlap").c_str());
+    span += out[d] * (int64_t(n[d]) - 1);
+  }
+  return MRL_OK;
+}
+
+int check_cache(uint32_t page_size, uint32_t pages) {
+  if (page_size == 0 || pages == 0) return bad(MRL_ERR_BAD_SPEC, "page_size and pages are at least 1");
+  if (uint64_t(page_size) * pages > 0x7fffffffull) return bad(MRL_ERR_TOO_LARGE, "pages * page_size is past 2^31 - 1");
+  return MRL_OK;
+}
+
+int check_heads(int dtype, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
+  if (!valid_dtype(dtype)) return bad(MRL_ERR_BAD_SPEC, "unknown dtype");
+  if (dtype != MRL_BF16 && dtype != MRL_F32) return bad(MRL_ERR_UNSUPPORTED, "dtype is bf16 or f32");
+  if (tokens == 0 || head_dim == 0) return bad(MRL_ERR_BAD_SPEC, "tokens and head_dim are at least 1");
+  if (tokens > MOST_TOKENS) return bad(MRL_ERR_TOO_LARGE, "tokens is past 2^23");
+  if (q_heads > 65535 || kv_heads > 65535 || (uint64_t(q_heads) + 2ull * kv_heads) * head_dim > (1u << 24)) return bad(MRL_ERR_TOO_LARGE, "heads * head_dim is past 2^24");
+  return MRL_OK;
+}
+
+// The device the library was initialised for is the calling thread's current one.
+int on_the_device() {
+  int rc;
+  if (g_device < 0 && (rc = mrl_init(0)) != MRL_OK) return rc;
+  int current = -1;
+  HIP_TRY(hipGetDevice(&current));
+  if (current != g_device) return bad(MRL_ERR_NO_DEVICE, "the calling thread's current device is not the one the library was initialised for");
+  return MRL_OK;
+}
+
+int launched(hipError_t e, const char *what) { return e == hipSuccess ? MRL_OK : hip_fail(e, what); }
+
+int check_page_tables(const mrl_page_tables *op) {
+  if (!op) return MRL_ERR_NULL;
+  if (op->requests == 0 || op->table_width == 0 || op->tokens == 0) return bad(MRL_ERR_BAD_SPEC, "requests, table_width and tokens are at least 1");
+  const int rc = check_cache(op->page_size, op->pages);
+  if (rc != MRL_OK) return rc;
+  if (op->tokens > MOST_TOKENS || op->free_pages > 0x7fffffffu) return bad(MRL_ERR_TOO_LARGE, "tokens is past 2^23, or free_pages past 2^31 - 1");
+  if (uint64_t(op->requests) * op->table_width > 0x7fffffffull || uint64_t(op->table_width) * op->page_size > 0x7fffffffull)
+    return bad(MRL_ERR_TOO_LARGE, "the page table, or the tokens that a row of it holds, are past 2^31 - 1");
+  return MRL_OK;
+}
+
+int run_page_tables(const mrl_page_tables &op, void *const *params, hipStream_t stream) {
+  for (int i = 0; i < 10; i++)
+    if (!params[i] && !(i == 2 && op.free_pages == 0)) return MRL_ERR_NULL;
+  mrl::PageTablesArgs a;
+  a.cached = (const int32_t *)params[0], a.added = (const int32_t *)params[1], a.free_list = (const int32_t *)params[2], a.free_count = (const int32_t *)params[3];
+  a.table = (int32_t *)params[4], a.starts = (int32_t *)params[5], a.lengths = (int32_t *)params[6], a.slots = (int32_t *)params[7], a.positions = (int32_t *)params[8];
+  a.free_left = (int32_t *)params[9];
+  a.requests = op.requests, a.width = op.table_width, a.page_size = op.page_size, a.pages = op.pages, a.tokens = op.tokens, a.free_pages = op.free_pages;
+  return launched(mrl::launch_page_tables(a, stream), "page tables");
+}
+
+// Checks, and everything of the arguments but the pointers.
+int rotary_args(const mrl_rotary *op, mrl::RotaryArgs *a) {
+  if (!op) return MRL_ERR_NULL;
+  int rc = check_heads(op->dtype, op->tokens, op->q_heads, op->kv_heads, op->head_dim);
+  if (rc != MRL_OK) return rc;
+  if (op->q_heads == 0) return bad(MRL_ERR_BAD_SPEC, "q_heads is at least 1");
+  if (op->axes == 0 || op->axes > MRL_MAX_AXES) return bad(MRL_ERR_BAD_SPEC, "axes is 1 to 4");
+  uint64_t pairs = 0;
+  for (uint32_t i = 0; i < MRL_MAX_AXES; i++) {
+    if (i >= op->axes && op->sections[i]) return bad(MRL_ERR_BAD_SPEC, "a section without an axis");
+    pairs += op->sections[i];
+    a->section_end[i] = uint32_t(std::min<uint64_t>(pairs, 1024));
+  }
+  if (pairs == 0 || 2 * pairs > op->head_dim || pairs > 512) return bad(MRL_ERR_BAD_SPEC, "the sections' pairs are at least 1, their dims at most head_dim and 1024");
+  if (op->page_size == 0 && op->pages != 0) return bad(MRL_ERR_BAD_SPEC, "pages without a page_size");
+  const bool paged = op->page_size != 0;
+  if (paged && (rc = check_cache(op->page_size, op->pages)) != MRL_OK) return rc;
+  if (paged && op->kv_heads == 0) return bad(MRL_ERR_BAD_SPEC, "a cache without key and value heads");
+  a->tokens = op->tokens, a->q_heads = op->q_heads, a->kv_heads = op->kv_heads, a->head_dim = op->head_dim, a->pairs = uint32_t(pairs);
+  a->dtype = op->dtype, a->adjacent = op->adjacent != 0, a->inverse = op->inverse != 0, a->page_size = op->page_size, a->slot_count = op->page_size * op->pages;
+  const uint32_t q_dims[2] = {op->tokens, op->q_heads}, k_dims[2] = {op->tokens, op->kv_heads}, cache[3] = {op->pages, op->page_size, op->kv_heads};
+  int64_t s[3] = {0, 0, 0};
+  if ((rc = fill_strides(op->q_strides, q_dims, 2, op->head_dim, false, "q", s)) != MRL_OK) return rc;
+  a->q_t = s[0], a->q_h = s[1];
+  if ((rc = fill_strides(op->q_out_strides, q_dims, 2, op->head_dim, true, "q out", s)) != MRL_OK) return rc;
+  a->qo_t = s[0], a->qo_h = s[1];
+  a->k_t = a->k_h = a->v_t = a->v_h = a->key_p = a->key_s = a->key_h = a->val_p = a->val_s = a->val_h = 0;
+  if (op->kv_heads) {
+    if ((rc = fill_strides(op->k_strides, k_dims, 2, op->head_dim, false, "k", s)) != MRL_OK) return rc;
+    a->k_t = s[0], a->k_h = s[1];
+    if (paged) {
+      if ((rc = fill_strides(op->v_strides, k_dims, 2, op->head_dim, false, "v", s)) != MRL_OK) return rc;
+      a->v_t = s[0], a->v_h = s[1];
+      if ((rc = fill_strides(op->key_strides, cache, 3, op->head_dim, true, "keys", s)) != MRL_OK) return rc;
+      a->key_p = s[0], a->key_s = s[1], a->key_h = s[2];
+      if ((rc = fill_strides(op->value_strides, cache, 3, op->head_dim, true, "values", s)) != MRL_OK) return rc;
+      a->val_p = s[0], a->val_s = s[1], a->val_h = s[2];
+    } else {
+      if ((rc = fill_strides(op->key_strides + 1, k_dims, 2, op->head_dim, true, "keys", s)) != MRL_OK) return rc;
+      a->key_s = s[0], a->key_h = s[1];
+    }
+  }
+  return MRL_OK;
+}
+
+int run_rotary(mrl::RotaryArgs &a, void *const *params, hipStream_t stream) {
+  const bool keys = a.kv_heads != 0, paged = a.page_size != 0;
+  const bool wanted[9] = {true, keys, paged, true, true, paged, true, keys, paged};
+  for (int i = 0; i < 9; i++)
+    if (wanted[i] && !params[i]) return MRL_ERR_NULL;
+  if (params[6] == params[0] && (a.q_t != a.qo_t || a.q_h != a.qo_h)) return bad(MRL_ERR_BAD_SPEC, "q out is q, with other strides");
+  if (keys && !paged && params[7] == params[1] && (a.k_t != a.key_s || a.k_h != a.key_h)) return bad(MRL_ERR_BAD_SPEC, "keys is k, with other strides");
+  a.q = params[0], a.k = keys ? params[1] : nullptr, a.v = paged ? params[2] : nullptr, a.positions = (const int32_t *)params[3], a.frequencies = (const float *)params[4];
+  a.slots = paged ? (const int32_t *)params[5] : nullptr, a.q_out = params[6], a.keys = keys ? params[7] : nullptr, a.values = paged ? params[8] : nullptr;
+  return launched(mrl::launch_rotary(a, stream), "rotary");
+}
+
+int paged_attention_args(const mrl_paged_attention *op, mrl::PagedAttnArgs *a) {
+  if (!op) return MRL_ERR_NULL;
+  int rc = check_heads(op->dtype, op->tokens, op->q_heads, op->kv_heads, op->head_dim);
+  if (rc != MRL_OK) return rc;
+  if (op->requests == 0 || op->kv_heads == 0 || op->table_width == 0 || op->q_heads == 0 || op->q_heads % op->kv_heads)
+    return bad(MRL_ERR_BAD_SPEC, "requests, table_width and kv_heads are at least 1, q_heads a multiple of kv_heads");
+  if ((rc = check_cache(op->page_size, op->pages)) != MRL_OK) return rc;
+  if (op->head_dim > 1024) return bad(MRL_ERR_UNSUPPORTED, "head_dim is at most 1024");
+  if (!(std::fabs(op->scale) <= 3.0e38f)) return bad(MRL_ERR_BAD_SPEC, "scale is finite");
+  if (uint64_t(op->requests) * op->table_width > 0x7fffffffull || uint64_t(op->table_width) * op->page_size > 0x7fffffffull)
+    return bad(MRL_ERR_TOO_LARGE, "the page table, or the tokens that a row of it holds, are past 2^31 - 1");
+  a->tokens = op->tokens, a->requests = op->requests, a->q_heads = op->q_heads, a->kv_heads = op->kv_heads, a->group = op->q_heads / op->kv_heads, a->head_dim = op->head_dim;
+  a->page_size = op->page_size, a->pages = op->pages, a->width = op->table_width, a->window = op->window, a->dtype = op->dtype;
+  a->max_new = op->max_new ? std::min(op->max_new, op->tokens) : op->tokens;
+  a->scale = op->scale != 0.0f ? op->scale : 1.0f / std::sqrt(float(op->head_dim));
+  const uint32_t q_dims[2] = {op->tokens, op->q_heads}, cache[3] = {op->pages, op->page_size, op->kv_heads};
+  int64_t s[3] = {0, 0, 0};
+  if ((rc = fill_strides(op->q_strides, q_dims, 2, op->head_dim, false, "q", s)) != MRL_OK) return rc;
+  a->q_t = s[0], a->q_h = s[1];
+  if ((rc = fill_strides(op->out_strides, q_dims, 2, op->head_dim, true, "out", s)) != MRL_OK) return rc;
+  a->o_t = s[0], a->o_h = s[1];
+  if ((rc = fill_strides(op->key_strides, cache, 3, op->head_dim, false, "keys", s)) != MRL_OK) return rc;
+  a->key_p = s[0], a->key_s = s[1], a->key_h = s[2];
+  if ((rc = fill_strides(op->value_strides, cache, 3, op->head_dim, false, "values", s)) != MRL_OK) return rc;
+  a->val_p = s[0], a->val_s = s[1], a->val_h = s[2];
+  return MRL_OK;
+}
+
+int run_paged_attention(mrl::PagedAttnArgs &a, void *const *params, hipStream_t stream) {
+  for (int i = 0; i < 7; i++)
+    if (!params[i]) return MRL_ERR_NULL;
+  if (!params[7] && mrl::paged_attn_workspace_bytes(a)) return MRL_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(params[7]) & 15) return bad(MRL_ERR_UNSUPPORTED, "the workspace is not 16-byte aligned");
+  a.q = params[0], a.keys = params[1], a.values = params[2], a.table = (const int32_t *)params[3], a.starts = (const int32_t *)params[4], a.lengths = (const int32_t *)params[5];
+  a.out = params[6], a.workspace = (uint8_t *)params[7];
+  return launched(mrl::launch_paged_attn(a, stream), "attention over pages");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mrl_page_tables_check(const mrl_page_tables *op) { return check_page_tables(op); }
+int mrl_run_page_tables(const mrl_page_tables *op, void *const *params, void *stream) {
+  int rc = check_page_tables(op);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_page_tables(*op, params, (hipStream_t)stream);
+}
+int mrl_page_tables_plan(const mrl_page_tables *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  const int rc = check_page_tables(op);
+  if (rc != MRL_OK) return rc;
+  return plan_with(10, plan, steps, cap, [&](void *const *params, Workspace &) { return run_page_tables(*op, params, nullptr); });
+}
+
+int mrl_rotary_check(const mrl_rotary *op) {
+  mrl::RotaryArgs a;
+  return rotary_args(op, &a);
+}
+int mrl_run_rotary(const mrl_rotary *op, void *const *params, void *stream) {
+  mrl::RotaryArgs a;
+  int rc = rotary_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_rotary(a, params, (hipStream_t)stream);
+}
+int mrl_rotary_plan(const mrl_rotary *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  mrl::RotaryArgs a;
+  const int rc = rotary_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  return plan_with(9, plan, steps, cap, [&](void *const *params, Workspace &) { return run_rotary(a, params, nullptr); });
+}
+
+int mrl_paged_attention_check(const mrl_paged_attention *op) {
+  mrl::PagedAttnArgs a;
+  return paged_attention_args(op, &a);
+}
+size_t mrl_paged_attention_workspace_bytes(const mrl_paged_attention *op) {
+  mrl::PagedAttnArgs a;
+  return paged_attention_args(op, &a) == MRL_OK ? mrl::paged_attn_workspace_bytes(a) : 0;
+}
+int mrl_run_paged_attention(const mrl_paged_attention *op, void *const *params, void *stream) {
+  mrl::PagedAttnArgs a;
+  int rc = paged_attention_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_paged_attention(a, params, (hipStream_t)stream);
+}
+int mrl_paged_attention_plan(const mrl_paged_attention *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  mrl::PagedAttnArgs a;
+  int rc = paged_attention_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  rc = plan_with(8, plan, steps, cap, [&](void *const *params, Workspace &) { return run_paged_attention(a, params, nullptr); });
+  if (rc == MRL_OK) plan->scratch_bytes = mrl::paged_attn_workspace_bytes(a);
+  return rc;
 }
 
 }  // extern "C"
