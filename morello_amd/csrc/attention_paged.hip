@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.h"
+#include "attention_paged.h"
 
 namespace mrl {
 namespace {
@@ -103,12 +103,116 @@ hipError_t launch_generic(const PagedAttnArgs &a, hipStream_t stream) {
   return plan::last_error();
 }
 
+// Tiles that more than one workgroup has a piece of: out = sum_v O_v 2^(m_v - M) / sum_v l_v 2^(m_v - M), M the largest m_v, over the pieces in their order
+// (the parts formula of morello/src/spec.rs:107-132 in base 2).  blockIdx.x: the worker that begins the tile, blockIdx.y: a share of its rows.
+struct MergeArgs {
+  const float *partials;
+  const uint32_t *tiles;
+  uint32_t bq, row_floats, group;
+  FastDiv by_group, by_quads;
+};
+template <class T>
+__global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
+  const uint32_t worker = blockIdx.x;
+  const uint32_t *d = a.tiles + worker * 8;
+  const uint32_t more = d[0], row0 = d[2], rows = d[3], kv = d[4];
+  const int32_t start = int32_t(d[1]);
+  if (!more) return;
+  const uint32_t quads = (p.head_dim + 3) / 4, stat = a.row_floats - 4;
+  constexpr uint32_t U = 4;   // pieces asked for at a time
+  for (uint32_t x = blockIdx.y * THREADS + threadIdx.x; x < rows * quads; x += gridDim.y * THREADS) {
+    const uint32_t i = a.by_quads.div(x), dim = (x - i * quads) * 4;
+    // piece 0 lies in the first worker's place 1, the others in place 0 of the workers behind it
+    auto piece = [&](uint32_t v) { return a.partials + ((uint64_t(worker + v) * 2 + (v == 0)) * a.bq + i) * a.row_floats; };
+    float m = -3.0e38f, l = 0;
+    attn::v4f sum = {0, 0, 0, 0};
+    for (uint32_t v0 = 0; v0 <= more; v0 += U) {
+      float ms[U], ls[U];
+      attn::v4f os[U];
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) {
+        const float *from = piece(min(v0 + u, more));
+        ms[u] = from[stat], ls[u] = from[stat + 1], os[u] = *(const attn::v4f *)(from + dim);
+      }
+      float most = m;
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) most = fmaxf(most, ms[u]);
+      const float old = __builtin_amdgcn_exp2f(m - most);
+      sum *= old, l *= old, m = most;
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++)
+        if (v0 + u <= more) {
+          const float f = __builtin_amdgcn_exp2f(ms[u] - m);
+          sum += os[u] * f, l += ls[u] * f;
+        }
+    }
+    sum *= l == 0.0f ? 0.0f : 1.0f / l;
+    const uint32_t row = row0 + i, token = a.by_group.div(row), head = kv * p.group + (row - token * p.group);
+    T *out = (T *)p.out + int64_t(start + int32_t(token)) * p.o_t + int64_t(head) * p.o_h + dim;
+    if constexpr (sizeof(T) == 2) {
+      typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+      *(v4bf *)out = v4bf{(__bf16)sum[0], (__bf16)sum[1], (__bf16)sum[2], (__bf16)sum[3]};
+    } else {
+      *(attn::v4f *)out = sum;
+    }
+  }
+}
+
+// How a call runs, by sizes, types and strides.
+struct Choice {
+  bool tiled = false;          // else the generic kernel
+  int qb = 1;
+  paged::Work work = {};
+  size_t partial_bytes = 0, bytes = 0;
+};
+
+Choice choose(const PagedAttnArgs &a) {
+  Choice c;
+  const int size = a.dtype == MRL_BF16 ? 2 : 4;
+  auto chunks = [&](int64_t n) { return n * size % 16 == 0; };
+  const double scale = std::fabs(a.scale);
+  // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, 16 slots of a page within what an offset of 31 bits reaches.
+  c.tiled = a.page_size % 16 == 0 && a.head_dim <= 128 && chunks(a.head_dim) && chunks(a.q_t) && chunks(a.q_h) && chunks(a.o_t) && chunks(a.o_h) && chunks(a.key_p) &&
+            chunks(a.key_s) && chunks(a.key_h) && chunks(a.val_p) && chunks(a.val_s) && chunks(a.val_h) && a.key_s < (1 << 24) && a.val_s < (1 << 24) &&
+            uint64_t(a.tokens) * a.group < (1u << 31) && scale > 1e-30 && scale < 1e30;
+  if (!c.tiled) return c;
+  const uint64_t rows = uint64_t(a.max_new) * a.group;
+  c.qb = rows <= 16 ? 1 : 2;
+  paged::Work &w = c.work;
+  w.min_rows = 0, w.max_rows = 0xffffffffu;
+  // (max_new is the program's word: a request of more tokens would have more tiles than one)
+  w.single = uint64_t(a.tokens) * a.group <= 16u * c.qb;
+  w.workers = paged::keys_workers(a, c.qb);
+  w.direct = false;
+  c.partial_bytes = size_t(w.workers) * 2 * 16 * c.qb * paged::keys_row_floats(a) * sizeof(float);
+  c.bytes = c.partial_bytes + size_t(w.workers) * 32;
+  return c;
+}
+
+template <class T>
+hipError_t launch_merge(const PagedAttnArgs &a, const Choice &c, hipStream_t stream) {
+  MergeArgs m;
+  m.partials = c.work.partials, m.tiles = c.work.tiles, m.bq = 16 * c.qb, m.row_floats = paged::keys_row_floats(a), m.group = a.group;
+  m.by_group = FastDiv(a.group), m.by_quads = FastDiv((a.head_dim + 3) / 4);
+  plan::work(plan::UNIT_STREAM, 0, double(c.partial_bytes) / 2);
+  MRL_LAUNCH(k_paged_attn_merge<T>, dim3(c.work.workers, 1), dim3(THREADS), 0, stream, a, m);
+  return plan::last_error();
+}
+
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnArgs &) { return 0; }
+size_t paged_attn_workspace_bytes(const PagedAttnArgs &a) { return choose(a).bytes; }
 
 hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream) {
-  return a.dtype == MRL_BF16 ? launch_generic<u16>(a, stream) : launch_generic<float>(a, stream);
+  const bool bf16 = a.dtype == MRL_BF16;
+  auto aligned = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  Choice c = choose(a);
+  if (!c.tiled || !aligned(a.q) || !aligned(a.keys) || !aligned(a.values) || !aligned(a.out))
+    return bf16 ? launch_generic<u16>(a, stream) : launch_generic<float>(a, stream);
+  c.work.partials = reinterpret_cast<float *>(a.workspace), c.work.tiles = reinterpret_cast<uint32_t *>(a.workspace + c.partial_bytes);
+  const hipError_t e = paged::launch_keys(a, c.work, c.qb, stream);
+  if (e != hipSuccess || c.work.direct) return e;
+  return bf16 ? launch_merge<u16>(a, c, stream) : launch_merge<float>(a, c, stream);
 }
 
 }  // namespace mrl

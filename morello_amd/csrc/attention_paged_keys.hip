@@ -1,0 +1,482 @@
+// Attention over pages with the KEYS dealt to the waves of a workgroup: for few query rows per request (a decoding step, some tokens at once)
+// and for f32.
+//
+// A workgroup owns a piece of a tile (attention_paged.h) of 16 * QB rows; each of its W waves takes every W-th block of 32 keys, and the waves'
+// (O, m, l) meet at the end in LDS.  Both products are formed transposed, in blocks of 16 x 16: S^T = K.Q^T, O^T += V^T.P^T, so that
+// a lane owns a query row (l % 16 of the block's columns): running reference, denominator and rescaling are its scalars.  The index that
+// a product sums over may be dealt to lanes in any order that both operands share: lane group g = l / 16 holds keys 4 g .. 4 g + 3 of each 16
+// in its accumulators of the first product, and these are the operand of the second as they stand.
+//   bf16: v_mfma 16x16x32; V's operand through the transposing read; P rounded to bf16 (2^-8), the denominators from a row of ones, so that
+//         they are the sums of the very numbers that weigh the values.
+//   f32:  v_mfma 16x16x4; a 16-byte read of a K row is four steps of dims, a 16-byte read of a V row four blocks of output dims
+//         (dim 64 q + 4 (l % 16) + i is row l % 16 of block 4 q + i).
+// Keys and values go from their pages straight into LDS, 16 bytes a lane, through a buffer resource per 16 keys: a page's numbers are whole sixteens of
+// slots, so 16 keys lie behind each other.  The resource ends behind the last key that a row of the tile sees: what lies behind (or on no
+// page at all) arrives as zeros, whatever the slots hold.  The pages' numbers are fetched 32 blocks at a time, a lane each, and read from
+// the lanes.
+//
+// Exponentials are taken in base 2 of s * c - m, c = scale * log2 e; the reference m is the row's largest score so far in the first
+// blocks, and moves later only when a score has outgrown it by 2^40.
+#include <algorithm>
+
+#include "attention_paged.h"
+
+namespace mrl {
+namespace paged {
+namespace {
+
+using namespace attn;
+
+constexpr int KEYS = 32;      // keys per block
+constexpr int FOLLOWED = 4;   // blocks of a wave whose maxima the reference follows
+
+template <class T, int D, int QB, int W>
+struct Form {
+  static constexpr bool BF16 = sizeof(T) == 2;
+  static constexpr int TH = 64 * W, BQ = 16 * QB;
+  static constexpr int ROW = D * int(sizeof(T)), CHUNKS = ROW / 16, SLOTS = ROW / 32;
+  static constexpr int TILE = KEYS * ROW, LOADS = TILE / 1024, ROWS_PER_LOAD = 1024 / ROW, HALF = LOADS / 2;
+  static constexpr int ROWS_PER_LINE = ROW >= 256 ? 1 : 256 / ROW;   // rows per 256-byte line of banks
+  static constexpr int NDB = D / 16;                                  // 16-row blocks of O^T
+  static constexpr int ROW_FLOATS = D + 4;                            // of a partial result: O, reference, denominator
+  static_assert(ROWS_PER_LOAD <= 16 && LOADS < 32 && LOADS % 2 == 0, "a load stays within 16 keys");
+  // K rows are XOR-swizzled by 16-byte chunk, bf16's V rows by 32-byte slot (attention_keys.hip); an f32 V row is read whole.
+  __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1) & 15; }
+  __device__ static constexpr int v_swizzle(int row) { return BF16 ? (row / ROWS_PER_LINE) & (SLOTS - 1) & 15 : 0; }
+  // The waves' tiles, or after the loop their O, references and denominators; behind them, per wave, the weights of a block whose values are not
+  // all finite (KEYS rows of 16 floats), then what the dealing shares.
+  static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
+  static constexpr int AREA = TILES > TRIPLES ? TILES : TRIPLES;
+  static constexpr int WEIGHTS = W * KEYS * 16 * 4;
+  using Deal = Dealer<TH, BQ, KEYS>;
+  static constexpr int LDS = AREA + WEIGHTS + int(sizeof(typename Deal::Shared));
+};
+
+__device__ inline float over_lane_groups(float x) {   // the largest over the four lane groups, in all of them
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (two & 0x7f800000) == 0x7f800000; }   // NaN or infinity among them
+
+// p.head_dim may be below D, in whole 16-byte chunks: zeros behind it.
+template <class T, int D, int QB, int W>
+__global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work work, FastDiv by_group, FastDiv by_page16, float c) {
+  using F = Form<T, D, QB, W>;
+  constexpr bool BF16 = F::BF16;
+  constexpr int ROW = F::ROW, TILE = F::TILE, LOADS = F::LOADS, HALF = F::HALF, NDB = F::NDB;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lgp = lane >> 4;
+  typename F::Deal deal(p, work, by_group, reinterpret_cast<typename F::Deal::Shared *>(lds + F::AREA + F::WEIGHTS));
+  uint8_t *const k_tile = lds + wave * 2 * TILE, *const v_tile = k_tile + TILE;
+  float *const weights = reinterpret_cast<float *>(lds + F::AREA) + wave * (KEYS * 16);
+  const uint32_t row_bytes = p.head_dim * uint32_t(sizeof(T));
+  const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();   // a score that weighs nothing
+  const uint32_t groups_per_page = p.page_size / 16;
+
+  // One instruction fills 1 KiB of a tile, lane l its slot l: rows i * ROWS_PER_LOAD + l / CHUNKS, the chunk that belongs there.  The
+  // second 16 keys are as the first, from their own base.
+  uint32_t k_src[HALF], v_src[HALF];
+  {
+    const int ld_row = lane / F::CHUNKS, ld_pc = lane % F::CHUNKS;
+#pragma unroll
+    for (int i = 0; i < HALF; i++) {
+      const int row = i * F::ROWS_PER_LOAD + ld_row;
+      const uint32_t k_at = (ld_pc ^ F::k_swizzle(row)) << 4;
+      const uint32_t v_at = BF16 ? (((ld_pc >> 1) ^ F::v_swizzle(row)) << 5) | ((ld_pc & 1) << 4) : ld_pc << 4;
+      k_src[i] = k_at < row_bytes ? row * uint32_t(p.key_s * sizeof(T)) + k_at : OUTSIDE;
+      v_src[i] = v_at < row_bytes ? row * uint32_t(p.val_s * sizeof(T)) + v_at : OUTSIDE;
+    }
+  }
+  const uint32_t k_dst = lds_address(k_tile), v_dst = lds_address(v_tile);
+  // Lane-dependent parts of the operands' addresses.
+  constexpr int NC = ROW / 64;   // 64-byte pieces of a K row: bf16 a step of 32 dims, f32 four steps of 4
+  constexpr int NV = BF16 ? NDB : D / 64;
+  uint32_t k_lane[NC], v_lane[NV];
+#pragma unroll
+  for (int i = 0; i < NC; i++) k_lane[i] = lr * ROW + (((4 * i + lgp) ^ F::k_swizzle(lr)) << 4);
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int vrow = 4 * lgp + (lr >> 2);
+    v_lane[i] = BF16 ? vrow * ROW + ((i ^ F::v_swizzle(vrow)) << 5) + (lr & 3) * 8 : 4 * lgp * ROW + i * 256 + lr * 16;
+  }
+  constexpr int ALL_BUT_ONE_TILE = 0x0F70 | (LOADS & 15) | ((LOADS >> 4) << 14), ALL = 0x0F70, READS_DONE = 0xC07F;
+
+  bool described = false;
+  Piece t = {};
+  while (deal.next(t)) {
+    // (what the dealing shared has been read; the triples of the piece before too)
+    const uint8_t *const key_head = (const uint8_t *)p.keys + int64_t(t.head) * p.key_h * int64_t(sizeof(T));
+    const uint8_t *const val_head = (const uint8_t *)p.values + int64_t(t.head) * p.val_h * int64_t(sizeof(T));
+    const int32_t *const pages = p.table + uint64_t(t.request) * p.width;
+
+    // This lane's rows: queries, and the keys they see, [lo, hi].
+    v4i qf[QB][NC];
+    int32_t lo[QB], hi[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+      const uint32_t i = 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * p.group + (row - token * p.group);
+      const int32_t at = t.at + int32_t(token);
+      hi[qb] = i < t.rows ? min(at, int32_t(t.end) - 1) : -1;
+      lo[qb] = p.window ? int32_t(max(int64_t(at) - int64_t(p.window) + 1, int64_t(0))) : 0;
+      const uint8_t *q = (const uint8_t *)p.q + (int64_t(t.start + int32_t(token)) * p.q_t + int64_t(head) * p.q_h) * int64_t(sizeof(T));
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        const uint32_t from = j * 64 + lgp * 16;
+        qf[qb][j] = from < row_bytes ? *(const v4i *)(q + from) : v4i{0, 0, 0, 0};
+      }
+    }
+    // Blocks that every row sees whole lie in [all_from, all_to).
+    const int32_t first_at = t.at + int32_t(by_group.div(t.row0)), last_at = t.at + int32_t(by_group.div(t.row0 + t.rows - 1));
+    const int32_t all_to = min(first_at + 1, int32_t(t.end));
+    const int32_t all_from = p.window ? int32_t(min(max(int64_t(last_at) - int64_t(p.window) + 1, int64_t(0)), int64_t(0x7fffffff))) : 0;
+
+    // The pages' numbers of this wave's next 32 blocks, both sixteens of each, one a lane; places in the page.
+    int32_t page_here = -1, page_next = -1;
+    uint32_t place_here = 0, place_next = 0;
+    auto fetch_pages = [&](uint32_t n, int32_t &page, uint32_t &place) {   // of the wave's blocks n .. n + 31
+      const uint32_t group = (t.first_block + t.b0 + wave + (n + (lane >> 1)) * W) * 2 + (lane & 1);
+      page = -1;
+      const uint32_t column = by_page16.div(group);
+      place = (group - column * groups_per_page) * 16;
+      if (t.b0 + wave + (n + (lane >> 1)) * W < t.b1 && group * 16 < t.end) {
+        const int32_t number = pages[column];
+        if (number >= 0 && uint32_t(number) < p.pages) page = number;
+      }
+    };
+    // Of the wave's n-th block: 16 keys each.
+    auto page_of = [&](uint32_t n, int half) { return __builtin_amdgcn_readlane(page_here, (n & 31) * 2 + half); };
+    auto issue = [&](uint32_t n, const uint8_t *head, int64_t s_page, int64_t s_slot, const uint32_t *src, uint32_t dst) {
+      const uint32_t key0 = (t.first_block + t.b0 + wave + n * W) * KEYS;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const int32_t page = page_of(n, half);
+        const uint32_t place = __builtin_amdgcn_readlane(place_here, (n & 31) * 2 + half);
+        const uint32_t from = key0 + 16 * half;
+        const uint32_t rows = page < 0 || from >= t.end ? 0 : min(t.end - from, 16u);
+        const uint8_t *base = head + (int64_t(max(page, 0)) * s_page + int64_t(place) * s_slot) * int64_t(sizeof(T));
+        const int bytes = rows ? int((rows - 1) * uint32_t(s_slot * sizeof(T)) + row_bytes) : 0;
+        const uint64_t at = reinterpret_cast<uint64_t>(base), same = uint64_t(uniform(uint32_t(at >> 32))) << 32 | uniform(uint32_t(at));   // (in scalar registers)
+        const auto from_buf = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(same), 0, uniform(bytes), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < HALF; i++) dma16_ordered(from_buf, src[i], dst + (half * HALF + i) * 1024);
+      }
+    };
+    auto issue_k = [&](uint32_t n) { issue(n, key_head, p.key_p, p.key_s, k_src, k_dst); };
+    auto issue_v = [&](uint32_t n) { issue(n, val_head, p.val_p, p.val_s, v_src, v_dst); };
+
+    v4f o[NDB][QB], den[QB];
+    float m_run[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+      m_run[qb] = NO_REFERENCE;
+      den[qb] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int db = 0; db < NDB; db++) o[db][qb] = v4f{0, 0, 0, 0};
+    }
+    auto mfma16 = [](v4i a, auto b, v4f acc) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
+    };
+    auto mfma4 = [](float a, float b, v4f acc) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); };
+
+    // This wave's blocks: t.b0 + wave, + W, ..
+    const uint32_t mine = t.b1 - t.b0 > uint32_t(wave) ? (t.b1 - t.b0 - wave + W - 1) / W : 0;
+    __syncthreads();   // the tiles are free: everybody has read the piece before
+    if (mine) {
+      fetch_pages(0, page_here, place_here);
+      issue_k(0);
+      issue_v(0);
+      bool start = true;
+      __builtin_amdgcn_s_waitcnt(ALL);
+      for (uint32_t n = 0; n < mine; n++) {
+        const bool more = n + 1 < mine;
+        const uint32_t block = t.first_block + t.b0 + wave + n * W;
+        // In flight at this point, oldest first: K of this block, V of this block.
+        if (!start) __builtin_amdgcn_s_waitcnt(ALL_BUT_ONE_TILE);
+        asm volatile("" ::: "memory");
+        v4f s[2][QB];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++) s[kb][qb] = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < NC; j++) {
+            const v4i a = *(const v4i *)(k_tile + k_lane[j] + kb * 16 * ROW);
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) {
+              if constexpr (BF16) {
+                s[kb][qb] = mfma16(a, qf[qb][j], s[kb][qb]);
+              } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[kb][qb] = mfma4(__int_as_float(a[r]), __int_as_float(qf[qb][j][r]), s[kb][qb]);
+              }
+            }
+          }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(READS_DONE);   // K's operands are in registers: its tile may be filled again
+        const bool gone0 = page_of(n, 0) < 0, gone1 = page_of(n, 1) < 0;
+        // (V of the next block is asked for with the same numbers, so they move on behind this block's second product)
+        if (more && ((n + 1) & 31) == 0) fetch_pages(n + 1, page_next, place_next);
+        if (more) {
+          if (((n + 1) & 31) == 0) page_here = page_next, place_here = place_next;
+          issue_k(n + 1);
+        }
+        const int32_t key0 = int32_t(block * KEYS);
+        const bool masked = key0 < all_from || key0 + KEYS > all_to || gone0 || gone1;
+        if (masked) {
+#pragma unroll
+          for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const int32_t key = key0 + kb * 16 + 4 * lgp + r;
+                if (key < lo[qb] || key > hi[qb] || (kb ? gone1 : gone0)) s[kb][qb][r] = hidden;
+              }
+        }
+        auto move_reference = [&]() {
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++) {
+            float mx = s[0][qb][0] * c;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[kb][qb][r] * c);
+            mx = over_lane_groups(mx);
+            const float m_new = fmaxf(m_run[qb], mx);
+            const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+            m_run[qb] = m_new;
+            den[qb] *= alpha;
+#pragma unroll
+            for (int db = 0; db < NDB; db++) o[db][qb] *= alpha;
+          }
+        };
+        const bool fresh = n < FOLLOWED;
+        float e[2][QB][4];
+        float pmax = 0.0f;
+        auto exponentials = [&]() {
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                e[kb][qb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qb][r], c, -m_run[qb]));
+                pmax = fmaxf(pmax, e[kb][qb][r]);
+              }
+        };
+        if (fresh) move_reference();
+        exponentials();
+        if (!fresh && __any(!(pmax < STALE_REFERENCE))) {
+          move_reference();
+          exponentials();
+        }
+        start = false;
+        v8bf pb[QB];
+        if constexpr (BF16) {
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) pb[qb][kb * 4 + r] = (__bf16)e[kb][qb][r];
+        }
+        if (more) __builtin_amdgcn_s_waitcnt(ALL_BUT_ONE_TILE);   // V of this block is in; K of the next may still be under way
+        else __builtin_amdgcn_s_waitcnt(ALL);
+        asm volatile("" ::: "memory");
+        bool odd = false;   // a value that is not finite, in a block that not every row sees whole: a weight of zero would not hide it
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < TILE / 1024; i++) {
+            const v4i x = *(const v4i *)(v_tile + i * 1024 + lane * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) odd = odd || (BF16 ? odd_bf16(x[j]) : (x[j] & 0x7f800000) == 0x7f800000);
+          }
+        }
+        if (__any(odd)) {
+          // Key by key: a row takes what it sees.
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++) {
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const int32_t in_block = kb * 16 + 4 * lgp + r, key = key0 + in_block;
+                const bool seen = key >= lo[qb] && key <= hi[qb] && !(kb ? gone1 : gone0);
+                float x = e[kb][qb][r];
+                if constexpr (BF16) x = float(pb[qb][kb * 4 + r]);
+                weights[in_block * 16 + lr] = seen ? x : -1.0f;
+              }
+#pragma unroll 1
+            for (int key = 0; key < KEYS; key++) {
+              const float x = weights[key * 16 + lr];
+              const bool seen = !(x < 0.0f);
+#pragma unroll
+              for (int db = 0; db < NDB; db++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                  float v;
+                  if constexpr (BF16) {
+                    const uint32_t at = key * ROW + ((db ^ F::v_swizzle(key)) << 5) + (4 * lgp + r) * 2;
+                    v = __uint_as_float(uint32_t(*(const uint16_t *)(v_tile + at)) << 16);
+                  } else {
+                    const uint32_t dim = 64 * (db / 4) + 4 * (4 * lgp + r) + db % 4;
+                    v = *(const float *)(v_tile + key * ROW + dim * 4);
+                  }
+                  if (seen) o[db][qb][r] = __builtin_fmaf(x, v, o[db][qb][r]);
+                }
+            }
+          }
+        } else if constexpr (BF16) {
+#pragma unroll
+          for (int db = 0; db < NDB; db++) {
+            const v2i lo2 = read_tr16(v_tile + v_lane[db]), hi2 = read_tr16(v_tile + v_lane[db] + 16 * ROW);
+            const v4i a = {lo2[0], lo2[1], hi2[0], hi2[1]};
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) o[db][qb] = mfma16(a, pb[qb], o[db][qb]);
+          }
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+              for (int i = 0; i < NV; i++) {
+                const v4i a = *(const v4i *)(v_tile + v_lane[i] + (kb * 16 + r) * ROW);
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                  for (int j = 0; j < 4; j++) o[4 * i + j][qb] = mfma4(__int_as_float(a[j]), e[kb][qb][r], o[4 * i + j][qb]);
+              }
+        }
+        if constexpr (BF16) {
+          const v4i ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++) den[qb] = mfma16(ones, pb[qb], den[qb]);
+        } else {
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) den[qb][r] += e[kb][qb][r];
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(READS_DONE);
+        if (more) issue_v(n + 1);
+      }
+    }
+
+    // The waves' triples meet: quads of O in LDS as [wave][block column][quad][lane], then [wave][block column][reference, denominator][row].
+    // Quad x of a lane holds dims quad_dim(x) .. + 3.
+    auto quad_dim = [&](int x) { return BF16 ? 16 * x + 4 * lgp : 64 * (x / 4) + 16 * lgp + 4 * (x % 4); };
+    __syncthreads();   // all tiles have been read
+    v4f *const quads = (v4f *)lds;
+    float *const stats = (float *)(lds + W * QB * D * 64);
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+#pragma unroll
+      for (int x = 0; x < NDB; x++) {
+        v4f quad;
+        if constexpr (BF16) quad = o[x][qb];
+        else quad = v4f{o[x / 4 * 4][qb][x % 4], o[x / 4 * 4 + 1][qb][x % 4], o[x / 4 * 4 + 2][qb][x % 4], o[x / 4 * 4 + 3][qb][x % 4]};
+        quads[((wave * QB + qb) * NDB + x) * 64 + lane] = quad;
+      }
+      float l = den[qb][0];
+      if constexpr (!BF16) {
+        l = (den[qb][0] + den[qb][1]) + (den[qb][2] + den[qb][3]);
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+      }
+      if (lgp == 0) stats[(wave * QB + qb) * 32 + lr] = m_run[qb], stats[(wave * QB + qb) * 32 + 16 + lr] = l;
+    }
+    __syncthreads();
+    const bool whole = F::Deal::whole(t);
+    float *const part = whole ? nullptr : deal.place(t, F::ROW_FLOATS);
+    if (!whole && t.b0 == 0) {
+      described = true;
+      if (tid == 0) deal.describe(t);
+    }
+#pragma unroll
+    for (int x = wave; x < QB * NDB; x += W) {
+      const int qb = x / NDB;
+      const uint32_t i = 16 * qb + lr;
+      if (i >= t.rows) continue;
+      float mm = -3.0e38f, l = 0.0f;
+      float f[W];
+#pragma unroll
+      for (int j = 0; j < W; j++) f[j] = stats[(j * QB + qb) * 32 + lr], mm = fmaxf(mm, f[j]);
+      v4f sum = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < W; j++) {
+        f[j] = __builtin_amdgcn_exp2f(f[j] - mm);
+        l += stats[(j * QB + qb) * 32 + 16 + lr] * f[j];
+        sum += quads[((j * QB + qb) * NDB + x % NDB) * 64 + lane] * f[j];
+      }
+      const uint32_t dim = quad_dim(x % NDB);
+      if (!whole) {
+        float *to = part + i * F::ROW_FLOATS;
+        *(v4f *)(to + dim) = sum;
+        if (dim == 0) to[D] = mm, to[D + 1] = l;
+        continue;
+      }
+      if (dim >= p.head_dim) continue;
+      sum *= l == 0.0f ? 0.0f : 1.0f / l;
+      const uint32_t row = t.row0 + i, token = by_group.div(row), head = t.head * p.group + (row - token * p.group);
+      T *out = (T *)p.out + int64_t(t.start + int32_t(token)) * p.o_t + int64_t(head) * p.o_h + dim;
+      if constexpr (BF16) {
+        typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+        *(v4bf *)out = v4bf{(__bf16)sum[0], (__bf16)sum[1], (__bf16)sum[2], (__bf16)sum[3]};
+      } else {
+        *(v4f *)out = sum;
+      }
+    }
+  }
+  if (tid == 0) deal.finish(described);
+}
+
+template <class T, int D, int QB, int W>
+hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
+  using F = Form<T, D, QB, W>;
+  static std::atomic<uint64_t> lds_limit_set{0};
+  if (!plan::recording()) {
+    const hipError_t e = raise_lds_limit(lds_limit_set, (const void *)k_paged_attn<T, D, QB, W>, F::LDS);
+    if (e != hipSuccess) return e;
+  }
+  work.round_blocks = W;
+  const uint32_t grid = work.direct ? a.requests * a.kv_heads : work.workers;
+  const double keys = double(a.width) * a.page_size * a.requests;   // (all that the table holds: the lengths are on the device)
+  plan::work(F::BF16 ? plan::UNIT_MFMA_BF16 : plan::UNIT_MFMA_F32, 4.0 * a.tokens * a.q_heads * D * double(a.width) * a.page_size,
+             2.0 * sizeof(T) * a.kv_heads * a.head_dim * keys + 2.0 * sizeof(T) * a.tokens * double(a.q_heads) * a.head_dim);
+  MRL_LAUNCH((k_paged_attn<T, D, QB, W>), dim3(grid), dim3(F::TH), F::LDS, stream, a, work, FastDiv(a.group), FastDiv(a.page_size / 16), a.scale * LOG2E);
+  return plan::last_error();
+}
+
+template <class T, int D>
+uint32_t per_unit(int qb) {   // workgroups that a compute unit's LDS holds
+  constexpr int W = sizeof(T) == 4 && D == 128 ? 4 : 8;
+  return std::max(1, std::min(2, 160 * 1024 / (qb == 1 ? Form<T, D, 1, W>::LDS : Form<T, D, 2, W>::LDS)));
+}
+}  // namespace
+
+uint32_t keys_row_floats(const PagedAttnArgs &a) { return (a.head_dim <= 64 ? 64 : 128) + 4; }
+
+uint32_t keys_workers(const PagedAttnArgs &a, int qb) {
+  const bool narrow = a.head_dim <= 64;
+  return g_compute_units * (a.dtype == MRL_BF16 ? (narrow ? per_unit<__bf16, 64>(qb) : per_unit<__bf16, 128>(qb)) : (narrow ? per_unit<float, 64>(qb) : per_unit<float, 128>(qb)));
+}
+
+hipError_t launch_keys(const PagedAttnArgs &a, const Work &work, int qb, hipStream_t stream) {
+  const bool narrow = a.head_dim <= 64;
+  if (a.dtype == MRL_BF16) {
+    if (narrow) return qb == 1 ? launch_one<__bf16, 64, 1, 8>(a, work, stream) : launch_one<__bf16, 64, 2, 8>(a, work, stream);
+    return qb == 1 ? launch_one<__bf16, 128, 1, 8>(a, work, stream) : launch_one<__bf16, 128, 2, 8>(a, work, stream);
+  }
+  if (narrow) return qb == 1 ? launch_one<float, 64, 1, 8>(a, work, stream) : launch_one<float, 64, 2, 8>(a, work, stream);
+  return qb == 1 ? launch_one<float, 128, 1, 4>(a, work, stream) : launch_one<float, 128, 2, 4>(a, work, stream);
+}
+
+}  // namespace paged
+}  // namespace mrl
