@@ -104,26 +104,31 @@ hipError_t launch_generic(const PagedAttnArgs &a, hipStream_t stream) {
 }
 
 // Tiles that more than one workgroup has a piece of: out = sum_v O_v 2^(m_v - M) / sum_v l_v 2^(m_v - M), M the largest m_v, over the pieces in their order
-// (the parts formula of morello/src/spec.rs:107-132 in base 2).  blockIdx.x: the worker that begins the tile, blockIdx.y: a share of its rows.
+// (the parts formula of morello/src/spec.rs:107-132 in base 2).  blockIdx.x: the worker that begins the tile, those of the first kernel before those of
+// the second; blockIdx.y: a share of the tile's rows.
 struct MergeArgs {
-  const float *partials;
-  const uint32_t *tiles;
-  uint32_t bq, row_floats, group;
+  struct {
+    const float *partials;
+    const uint32_t *tiles;
+    uint32_t workers, bq;
+  } of[2];
+  uint32_t row_floats;
   FastDiv by_group, by_quads;
 };
 template <class T>
 __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
-  const uint32_t worker = blockIdx.x;
-  const uint32_t *d = a.tiles + worker * 8;
+  const uint32_t second = blockIdx.x >= a.of[0].workers, worker = blockIdx.x - (second ? a.of[0].workers : 0), bq = a.of[second].bq;
+  const float *const partials = a.of[second].partials;
+  const uint32_t *d = a.of[second].tiles + worker * 8;
   const uint32_t more = d[0], row0 = d[2], rows = d[3], kv = d[4];
   const int32_t start = int32_t(d[1]);
   if (!more) return;
   const uint32_t quads = (p.head_dim + 3) / 4, stat = a.row_floats - 4;
-  constexpr uint32_t U = 4;   // pieces asked for at a time
+  constexpr uint32_t U = 16;   // pieces asked for at a time
   for (uint32_t x = blockIdx.y * THREADS + threadIdx.x; x < rows * quads; x += gridDim.y * THREADS) {
     const uint32_t i = a.by_quads.div(x), dim = (x - i * quads) * 4;
     // piece 0 lies in the first worker's place 1, the others in place 0 of the workers behind it
-    auto piece = [&](uint32_t v) { return a.partials + ((uint64_t(worker + v) * 2 + (v == 0)) * a.bq + i) * a.row_floats; };
+    auto piece = [&](uint32_t v) { return partials + ((uint64_t(worker + v) * 2 + (v == 0)) * bq + i) * a.row_floats; };
     float m = -3.0e38f, l = 0;
     attn::v4f sum = {0, 0, 0, 0};
     for (uint32_t v0 = 0; v0 <= more; v0 += U) {
@@ -158,12 +163,12 @@ __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, M
   }
 }
 
-// How a call runs, by sizes, types and strides.
+// How a call runs, by sizes, types and strides: on tiles of 16 * qb rows, of 128, or small requests on the former and the others on the latter.
 struct Choice {
   bool tiled = false;          // else the generic kernel
-  int qb = 1;
-  paged::Work work = {};
-  size_t partial_bytes = 0, bytes = 0;
+  int qb = 0;                  // 0: no tiles of 16 or 32 rows
+  paged::Work keys = {}, chunk = {};
+  size_t keys_bytes = 0, chunk_bytes = 0, bytes = 0;   // of partial results, of the workspace
 };
 
 Choice choose(const PagedAttnArgs &a) {
@@ -177,25 +182,36 @@ Choice choose(const PagedAttnArgs &a) {
             uint64_t(a.tokens) * a.group < (1u << 31) && scale > 1e-30 && scale < 1e30;
   if (!c.tiled) return c;
   const uint64_t rows = uint64_t(a.max_new) * a.group;
-  c.qb = rows <= 16 ? 1 : 2;
-  paged::Work &w = c.work;
-  w.min_rows = 0, w.max_rows = 0xffffffffu;
-  // (max_new is the program's word: a request of more tokens would have more tiles than one)
-  w.single = uint64_t(a.tokens) * a.group <= 16u * c.qb;
-  w.workers = paged::keys_workers(a, c.qb);
-  w.direct = false;
-  c.partial_bytes = size_t(w.workers) * 2 * 16 * c.qb * paged::keys_row_floats(a) * sizeof(float);
-  c.bytes = c.partial_bytes + size_t(w.workers) * 32;
+  const bool chunk = a.dtype == MRL_BF16 && rows > 32;
+  if (!chunk) c.qb = rows <= 16 ? 1 : 2;
+  else if (a.requests > 1) c.qb = 1;
+  const size_t row_bytes = paged::row_floats(a) * sizeof(float);
+  if (c.qb) {
+    paged::Work &w = c.keys;
+    w.min_rows = 1, w.max_rows = chunk ? 16 : 0x7fffffff;
+    // (max_new is the program's word: a request of more tokens would have more tiles than one)
+    w.single = chunk || uint64_t(a.tokens) * a.group <= 16u * c.qb;
+    w.workers = paged::keys_workers(a, c.qb);
+    c.keys_bytes = size_t(w.workers) * 2 * 16 * c.qb * row_bytes;
+  }
+  if (chunk) {
+    paged::Work &w = c.chunk;
+    w.min_rows = c.qb ? 17 : 1, w.max_rows = 0x7fffffff;
+    w.workers = paged::chunk_workers(a);
+    c.chunk_bytes = size_t(w.workers) * 2 * paged::CHUNK_ROWS * row_bytes;
+  }
+  c.bytes = c.keys_bytes + c.chunk_bytes + size_t(c.keys.workers + c.chunk.workers) * 32 + size_t(c.chunk.workers) * paged::LIST * 64;
   return c;
 }
 
 template <class T>
 hipError_t launch_merge(const PagedAttnArgs &a, const Choice &c, hipStream_t stream) {
   MergeArgs m;
-  m.partials = c.work.partials, m.tiles = c.work.tiles, m.bq = 16 * c.qb, m.row_floats = paged::keys_row_floats(a), m.group = a.group;
-  m.by_group = FastDiv(a.group), m.by_quads = FastDiv((a.head_dim + 3) / 4);
-  plan::work(plan::UNIT_STREAM, 0, double(c.partial_bytes) / 2);
-  MRL_LAUNCH(k_paged_attn_merge<T>, dim3(c.work.workers, 1), dim3(THREADS), 0, stream, a, m);
+  m.of[0] = {c.keys.partials, c.keys.tiles, c.keys.workers, 16u * c.qb};
+  m.of[1] = {c.chunk.partials, c.chunk.tiles, c.chunk.workers, paged::CHUNK_ROWS};
+  m.row_floats = paged::row_floats(a), m.by_group = FastDiv(a.group), m.by_quads = FastDiv((a.head_dim + 3) / 4);
+  plan::work(plan::UNIT_STREAM, 0, double(c.keys_bytes + c.chunk_bytes) / 2);
+  MRL_LAUNCH(k_paged_attn_merge<T>, dim3(c.keys.workers + c.chunk.workers, c.chunk.workers ? 8 : 1), dim3(THREADS), 0, stream, a, m);
   return plan::last_error();
 }
 
@@ -209,9 +225,12 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream) {
   Choice c = choose(a);
   if (!c.tiled || !aligned(a.q) || !aligned(a.keys) || !aligned(a.values) || !aligned(a.out))
     return bf16 ? launch_generic<u16>(a, stream) : launch_generic<float>(a, stream);
-  c.work.partials = reinterpret_cast<float *>(a.workspace), c.work.tiles = reinterpret_cast<uint32_t *>(a.workspace + c.partial_bytes);
-  const hipError_t e = paged::launch_keys(a, c.work, c.qb, stream);
-  if (e != hipSuccess || c.work.direct) return e;
+  c.keys.partials = reinterpret_cast<float *>(a.workspace), c.chunk.partials = reinterpret_cast<float *>(a.workspace + c.keys_bytes);
+  c.keys.tiles = reinterpret_cast<uint32_t *>(a.workspace + c.keys_bytes + c.chunk_bytes), c.chunk.tiles = c.keys.tiles + c.keys.workers * 8, c.chunk.lists = c.chunk.tiles + c.chunk.workers * 8;
+  hipError_t e = hipSuccess;
+  if (c.chunk.workers) e = paged::launch_chunk(a, c.chunk, stream);
+  if (e == hipSuccess && c.qb) e = paged::launch_keys(a, c.keys, c.qb, stream);
+  if (e != hipSuccess || c.keys.direct) return e;
   return bf16 ? launch_merge<u16>(a, c, stream) : launch_merge<float>(a, c, stream);
 }
 

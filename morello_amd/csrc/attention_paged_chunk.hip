@@ -1,0 +1,509 @@
+// Attention over pages for chunks of new tokens in bf16: tiles of 128 query rows (tokens times the query heads of a key/value head).
+//
+// Eight waves: four take 32 rows each over the first half of a piece's keys, four the same rows over the second half; the halves' (O, m, l) meet at
+// the end.  The loop is that of the fused kernel over dense tensors (attention.hip): S^T = K.Q^T and O^T += V^T.P^T in 16 x 16 blocks of the
+// bf16 MFMA, keys and values straight from memory into LDS (two K tiles and three V tiles of 64 keys per half), and the two halves one slot apart,
+// so that one's products run beside the other's exponentials.  What differs:
+//   - a wave fetches 16 of a block's 64 keys, which lie behind each other in a page: one page number per block and wave, out of a register that holds 64
+//     blocks' numbers, a lane each; the buffer resource over them ends behind the last key that a row of the tile sees (zeros come from there);
+//   - rows see keys up to their own place (and, with a window, not those too far before): blocks that some row of the wave does not see whole have their
+//     scores masked;  there, where values are not all finite, the second product goes key by key, for a weight of zero would not hide them;
+//   - exponentials in base 2 of s * c - m with c = scale * log2 e;
+//   - work comes in pieces (attention_paged.h).
+// What bounds it: the issue of MFMA and vector instructions, as there.
+#include <algorithm>
+
+#include "attention_paged.h"
+
+namespace mrl {
+namespace paged {
+namespace {
+
+using namespace attn;
+
+constexpr int BKV = 64, QG = 4, BQ = CHUNK_ROWS, TH = 512;
+constexpr int PRIO_A = 2, PRIO_B = 0;   // of a wave in its slot of products, of exponentials
+using Deal = Dealer<TH, BQ, BKV, 4>;
+
+template <int D>
+struct Dims {
+  static constexpr int ROW = D * 2, TILE = BKV * ROW, HALF = 5 * TILE;   // bytes of a row, of a block, of a half's tiles
+  static constexpr int CHUNKS = ROW / 16, SLOTS = ROW / 32, ROWS_PER_LINE = ROW >= 256 ? 1 : 256 / ROW, ROWS_PER_LOAD = 1024 / ROW;
+  static constexpr int PER_WAVE = 16 / ROWS_PER_LOAD;                    // loads of a wave's 16 keys
+  static constexpr int MERGE_ROWS = D / 2 + 4;                           // a lane's O, two references and two denominators
+  static constexpr int MERGE = QG * MERGE_ROWS * 64 * 4;
+  static constexpr int LDS = 2 * HALF > MERGE ? 2 * HALF : MERGE;
+  static_assert(int(sizeof(Deal::Shared)) <= LDS, "what the dealing shares lies where the tiles do");
+  __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1); }
+  __device__ static constexpr int v_swizzle(int row) { return (row / ROWS_PER_LINE) & (SLOTS - 1); }
+};
+
+__device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (two & 0x7f800000) == 0x7f800000; }   // NaN or infinity among them
+
+template <int D>
+__global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
+  typedef Dims<D> DD;
+  constexpr int ROW = DD::ROW, TILE = DD::TILE, HALF = DD::HALF, PER_WAVE = DD::PER_WAVE;
+  constexpr int NC = D / 32, NDB = D / 16, NKB = BKV / 16, NKC = BKV / 32;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qg = wave % QG, half = wave / QG;   // rows 32 qg .. of the tile; half of the keys
+  const int lr = lane & 15, lgp = lane >> 4;
+  const uint32_t worker = xcd_run(blockIdx.x, gridDim.x);
+  uint8_t *const my_lds = lds + half * HALF;
+  const uint32_t row_bytes = kernargs().p.head_dim * 2, k_slot = uint32_t(kernargs().p.key_s * 2), v_slot = uint32_t(kernargs().p.val_s * 2);
+
+  // A load fills 1 KiB, lane l its slot l; the swizzles are applied where a lane fetches from.
+  uint32_t k_src[PER_WAVE], v_src[PER_WAVE];
+#pragma unroll
+  for (int i = 0; i < PER_WAVE; i++) {
+    const int row = i * DD::ROWS_PER_LOAD + lane / DD::CHUNKS, pc = lane % DD::CHUNKS;
+    const uint32_t k_at = (pc ^ DD::k_swizzle(row)) << 4, v_at = (((pc >> 1) ^ DD::v_swizzle(row)) << 5) | ((pc & 1) << 4);
+    k_src[i] = k_at < row_bytes ? row * k_slot + k_at : OUTSIDE;
+    v_src[i] = v_at < row_bytes ? row * v_slot + v_at : OUTSIDE;
+  }
+  // Operands' addresses in a tile: of output block db and of step j these with 32 db and 64 j exclusive-ored in (rows are whole multiples of both, and tiles of 1 KiB).
+  const uint32_t v_lane = (4 * lgp + (lr >> 2)) * ROW + (DD::v_swizzle(4 * lgp + (lr >> 2)) << 5) + (lr & 3) * 8;
+  const uint32_t k_lane = lr * ROW + ((lgp ^ DD::k_swizzle(lr)) << 4);
+  constexpr int WAIT_BUT_TWO = 0x0F70 | ((2 * PER_WAVE) & 15) | (((2 * PER_WAVE) >> 4) << 14);
+  const v4i ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
+  auto mfma = [](v4i a, auto b, v4f acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
+  };
+
+  bool described = false;
+  uint64_t cur = 0;
+  do {
+    uint32_t *const notes = kernargs().w.lists + uint64_t(worker) * (LIST * 16);
+    const uint32_t count = Deal(kernargs(), reinterpret_cast<Deal::Shared *>(lds)).deal(worker, notes, cur);
+    __syncthreads();
+    for (uint32_t number = 0; number < count; number++) {
+    const Kernargs &k = kernargs();
+    const Piece t = Deal::read(k.w.lists + uint64_t(worker) * (LIST * 16), number);
+    const float c = k.c;
+    const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
+    const uint32_t group = k.p.group, window = k.p.window;
+    const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();
+    const int my_blocks = int(t.b1 - t.b0), steps = (my_blocks + 1) / 2;
+    const int nblocks = half ? my_blocks - steps : steps;
+    const uint32_t first_block = t.begin / BKV + t.b0 + (half ? steps : 0);
+    const uint8_t *const key_head = (const uint8_t *)k.p.keys + int64_t(t.head) * k.p.key_h * 2;
+    const uint8_t *const val_head = (const uint8_t *)k.p.values + int64_t(t.head) * k.p.val_h * 2;
+    const int64_t key_page = k.p.key_p * 2, val_page = k.p.val_p * 2;
+    const int32_t *const pages = k.p.table + uint64_t(t.request) * k.p.width;
+    const uint32_t page_count = k.p.pages, groups_per_page = k.p.page_size / 16;
+
+    // The places of this lane's two rows (a row sees the keys up to it, below t.end and, with a window, behind it less the window; -1 where the tile
+    // has no such row), and the keys that all of the wave's rows see, [all_from, all_to).
+    int32_t row_at[2];
+    v4i qf[2][NC];
+#pragma unroll
+    for (int qb = 0; qb < 2; qb++) {
+      const uint32_t i = 32 * qg + 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * group + (row - token * group);
+      row_at[qb] = i < t.rows ? t.at + int32_t(token) : -1;
+      if (!half) {
+        const uint8_t *q = (const uint8_t *)k.p.q + (int64_t(t.start + int32_t(token)) * k.p.q_t + int64_t(head) * k.p.q_h) * 2;
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+          const uint32_t from = j * 64 + lgp * 16;
+          qf[qb][j] = from < row_bytes ? *(const v4i *)(q + from) : v4i{0, 0, 0, 0};
+        }
+      }
+    }
+    const uint32_t wave_first = t.row0 + min(32u * qg, t.rows - 1), wave_last = t.row0 + min(32u * qg + 31, t.rows - 1);
+    const int32_t all_to = min(t.at + int32_t(by_group.div(wave_first)) + 1, int32_t(t.end));
+    const int32_t all_from = window ? int32_t(max(int64_t(t.at) + by_group.div(wave_last) - int64_t(window) + 1, int64_t(0))) : 0;
+
+    // Of 64 of this half's blocks, a lane each: the page of this wave's sixteen keys and the place in it, and which blocks have sixteens on no page.
+    // (K runs two blocks ahead: its numbers move on before the bits of the block whose scores are masked do.)
+    int32_t page_here = -1;
+    uint64_t gone_here[NKB] = {}, gone_next[NKB] = {};
+    auto fetch_pages = [&](uint32_t kb, uint64_t *gone) {   // blocks kb .. kb + 63
+#pragma unroll
+      for (int g = 0; g < NKB; g++) {
+        const uint32_t group = (first_block + kb + lane) * 4 + g, column = by_page16.div(group);
+        int32_t number = -1;
+        if (int(kb) + lane < nblocks && group * 16 < t.end) {
+          number = pages[column];
+          if (uint32_t(number) >= page_count) number = -1;
+        }
+        gone[g] = __ballot(number < 0);
+        if (g == qg) page_here = number;
+      }
+    };
+    // The wave's 16 keys of block kb in their page.
+    auto resource = [&](const uint8_t *head, int64_t page_bytes, uint32_t slot_bytes, int32_t page, int kb) {
+      const uint32_t group16 = (first_block + kb) * 4 + qg, from = group16 * 16, place = (group16 - by_page16.div(group16) * groups_per_page) * 16;
+      const uint32_t rows = page < 0 || kb >= nblocks || from >= t.end ? 0 : min(t.end - from, 16u);
+      const uint64_t base = reinterpret_cast<uint64_t>(head) + uint64_t(max(page, 0)) * page_bytes + uint64_t(place) * slot_bytes;
+      return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(base)), 0, uniform(int(rows ? (rows - 1) * slot_bytes + row_bytes : 0)), 0x00020000);
+    };
+    auto page_of = [&](int kb) { return __builtin_amdgcn_readlane(page_here, kb & 63); };
+    const uint32_t k_dst0 = lds_address(my_lds) + qg * PER_WAVE * 1024, v_dst0 = k_dst0 + 2 * TILE;
+
+    v4f o[NDB][2], den[2];
+    float m_run[2] = {NO_REFERENCE, NO_REFERENCE};
+#pragma unroll
+    for (int qb = 0; qb < 2; qb++) {
+      den[qb] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int db = 0; db < NDB; db++) o[db][qb] = v4f{0, 0, 0, 0};
+    }
+    // K block kb goes to K tile kb & 1, V block kb to V tile kb % 3; blocks past the half's last bring zeros to tiles that nobody reads, so that
+    // every slot issues the same number of loads.  V of a block is asked for a slot after K of it, with the page that was looked up then.
+    int32_t page_v = -1;
+
+    v4f s[NKB][2];
+    v8bf pb[NKC][2];
+    // Before the first slot: Q and half 0's K(0); behind the barrier V(0), K(1) and all of half 1's, which have half 0's first slot to land in.
+    if (nblocks > 0) fetch_pages(0, gone_here);
+    auto issue_k = [&](int kb) {
+      page_v = page_of(kb);
+      const auto from = resource(key_head, key_page, k_slot, page_v, kb);
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; i++) dma16(from, k_src[i], k_dst0 + (kb & 1) * TILE + i * 1024);
+    };
+    auto issue_v = [&](int kb) {
+      const auto from = resource(val_head, val_page, v_slot, page_v, kb);
+#pragma unroll
+      for (int i = 0; i < PER_WAVE; i++) dma16(from, v_src[i], v_dst0 + (kb % 3) * TILE + i * 1024);
+    };
+    if (nblocks > 0 && !half) issue_k(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    {
+      // Q's operands from half 0 to half 1 through V tiles 1 and 2 of half 1, which no fetch touches before that half's first slot of exponentials.
+      static_assert(QG * D * 64 <= 2 * TILE, "the exchange fits the two tiles");
+      v4i *qx = (v4i *)(lds + HALF + 3 * TILE) + qg * (2 * NC * 64) + lane;
+      if (!half) {
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+          for (int j = 0; j < NC; j++) qx[(qb * NC + j) * 64] = qf[qb][j];
+      }
+      __syncthreads();
+      if (half) {
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+          for (int j = 0; j < NC; j++) qf[qb][j] = qx[(qb * NC + j) * 64];
+      }
+    }
+    if (nblocks > 0) {
+      if (half) issue_k(0);
+      issue_v(0);
+      issue_k(1);
+    }
+    if (half) {
+      __builtin_amdgcn_s_waitcnt(WAIT_BUT_TWO);   // K(0)
+      __syncthreads();
+    }
+    // Where a slot's operands are: formed in the slot and not kept (the compiler would hold all of them in registers over the loop, which has none to spare).
+    auto here = [&](const uint8_t *tile, uint32_t at) {
+      uint32_t x = uint32_t(tile - lds) + at;
+      asm volatile("" : "+v"(x));
+      return x;
+    };
+    auto read_v = [&](uint32_t v_here, int db, int kc) {
+      const uint8_t *a = lds + (v_here ^ (db << 5)) + kc * 32 * ROW;
+      const v2i lo2 = read_tr16(a), hi2 = read_tr16(a + 16 * ROW);
+      return v4i{lo2[0], lo2[1], hi2[0], hi2[1]};
+    };
+    // A slot of products: steps of two MFMAs on one operand out of LDS, which is read AHEAD steps before.
+    constexpr int PV_ROWS = NDB + 1, PV_STEPS = NKC * PV_ROWS, QK_STEPS = NC * NKB, AHEAD = 2, RING = AHEAD + 1;
+    v4i ring[RING];
+    auto run_steps = [&](auto first_c, auto last_c, const uint8_t *lv, const uint8_t *lk) {
+      constexpr int FIRST = decltype(first_c)::value, LAST = decltype(last_c)::value;
+      const uint32_t v_here = here(lv, v_lane), k_here = here(lk, k_lane);
+      auto fetch = [&](int x) {
+        if (x < PV_STEPS) {
+          if (x % PV_ROWS < NDB) ring[x % RING] = read_v(v_here, x % PV_ROWS, x / PV_ROWS);
+        } else {
+          ring[x % RING] = *(const v4i *)(lds + (k_here ^ ((x - PV_STEPS) / NKB << 6)) + (x - PV_STEPS) % NKB * 16 * ROW);
+        }
+      };
+#pragma unroll
+      for (int x = FIRST; x < LAST && x < FIRST + AHEAD; x++) fetch(x);
+#pragma unroll
+      for (int x = FIRST; x < LAST; x++) {
+        if (x + AHEAD < LAST) fetch(x + AHEAD);
+        const v4i a = ring[x % RING];
+        if (x < PV_STEPS) {
+          const int db = x % PV_ROWS, kc = x / PV_ROWS;
+          if (db < NDB) {
+            o[db][0] = mfma(a, pb[kc][0], o[db][0]);
+            o[db][1] = mfma(a, pb[kc][1], o[db][1]);
+          } else {
+            den[0] = mfma(ones, pb[kc][0], den[0]);
+            den[1] = mfma(ones, pb[kc][1], den[1]);
+          }
+        } else {
+          const int kb = (x - PV_STEPS) % NKB, j = (x - PV_STEPS) / NKB;
+          s[kb][0] = mfma(a, qf[0][j], s[kb][0]);
+          s[kb][1] = mfma(a, qf[1][j], s[kb][1]);
+        }
+      }
+      auto reads_group = [&](int x) {   // the builtin wants literal sizes
+        if (x >= PV_STEPS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        else if (x % PV_ROWS < NDB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      };
+#pragma unroll
+      for (int x = FIRST; x < LAST && x < FIRST + AHEAD; x++) reads_group(x);
+#pragma unroll
+      for (int x = FIRST; x < LAST; x++) {
+        if (x + AHEAD < LAST) reads_group(x + AHEAD);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      }
+    };
+    auto zero_s = [&]() {
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++) s[kb][0] = s[kb][1] = v4f{0, 0, 0, 0};
+    };
+    using std::integral_constant;
+    // Of the block whose weights pb holds: which of its sixteens are on no page, and whether some row does not see it whole.
+    uint32_t gone_bits = 0;
+    bool masked = false;
+    // The second product of a masked block whose values are not all finite: a key at a time, its values against its weights alone, and of the product only the
+    // columns (rows of queries) that see it.
+    auto slow_product = [&](int kb, const uint8_t *lv) {
+      const int32_t key0 = int32_t((first_block + kb) * BKV);
+#pragma unroll
+      for (int kc = 0; kc < NKC; kc++) {
+#pragma unroll 1
+        for (int x = 0; x < 32; x++) {   // key 32 kc + x: element 4 (x / 16) + x % 4 of lane group (x % 16) / 4
+          const int32_t key = key0 + 32 * kc + x;
+          const bool on = key < int32_t(t.end) && !((gone_bits >> (2 * kc + x / 16)) & 1);
+          const bool seen0 = on && key <= row_at[0] && (!window || key > int64_t(row_at[0]) - window), seen1 = on && key <= row_at[1] && (!window || key > int64_t(row_at[1]) - window);
+          const int element = 4 * (x / 16) + x % 4, bits = lgp == x % 16 / 4 ? element % 2 ? int(0xffff0000) : 0xffff : 0;
+          const v4i only = {element / 2 == 0 ? bits : 0, element / 2 == 1 ? bits : 0, element / 2 == 2 ? bits : 0, element / 2 == 3 ? bits : 0};
+          const uint32_t v_here = here(lv, v_lane);
+          const v4i p0 = __builtin_bit_cast(v4i, pb[kc][0]) & only, p1 = __builtin_bit_cast(v4i, pb[kc][1]) & only;
+#pragma unroll
+          for (int db = 0; db < NDB; db++) {
+            const v4i a = read_v(v_here, db, kc) & only;
+            const v4f y0 = mfma(a, p0, v4f{0, 0, 0, 0}), y1 = mfma(a, p1, v4f{0, 0, 0, 0});
+            o[db][0] += seen0 ? y0 : v4f{0, 0, 0, 0};
+            o[db][1] += seen1 ? y1 : v4f{0, 0, 0, 0};
+            asm volatile("" ::: "memory");   // (one at a time: it need not be fast, and has few registers)
+          }
+        }
+      }
+    };
+    auto odd_values = [&](const uint8_t *lv) {
+      bool odd = false;
+#pragma unroll 4
+      for (int i = 0; i < TILE / 1024; i++) {
+        const v4i x = *(const v4i *)(lv + i * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) odd = odd || odd_bf16(x[j]);
+      }
+      return __any(odd);
+    };
+    // V of the block before slot j, in V tile `vstage`, for the second product.  Where the slow one has been done, zeros, in the V tile that is free in this slot:
+    // the fast one then adds nothing but the denominators.  (Were it left out there, its sums would be in other registers after either branch.)
+    auto values_of = [&](int j, int vstage) {
+      const uint8_t *const lv = my_lds + (2 + vstage) * TILE;
+      if (!masked || !odd_values(lv)) return lv;
+      slow_product(j - 1, lv);
+      uint8_t *const zeros = my_lds + (2 + (vstage + 2) % 3) * TILE;
+#pragma unroll 1
+      for (int i = 0; i < TILE / 1024; i++) *(v4i *)(zeros + i * 1024 + lane * 16) = v4i{0, 0, 0, 0};
+      return (const uint8_t *)zeros;
+    };
+    // Products of slot j: O += V.P of block j - 1, S = K.Q of block j; the first and the last slot have one of the two.
+    auto slot_a = [&](int j, int vstage) {
+      __builtin_amdgcn_s_setprio(PRIO_A);
+      zero_s();
+      const uint8_t *const lv = values_of(j, vstage);
+      run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, lv, my_lds + (j & 1) * TILE);
+    };
+    auto slot_b = [&](int j) {
+      __builtin_amdgcn_s_setprio(PRIO_B);
+      if (((j + 2) & 63) == 0) fetch_pages(j + 2, gone_next);
+      if ((j & 63) == 0 && j) {
+#pragma unroll
+        for (int g = 0; g < NKB; g++) gone_here[g] = gone_next[g];
+      }
+      gone_bits = 0;
+#pragma unroll
+      for (int g = 0; g < NKB; g++) gone_bits |= uint32_t((gone_here[g] >> (j & 63)) & 1) << g;
+      const int32_t key0 = int32_t((first_block + j) * BKV);
+      masked = key0 < all_from || key0 + BKV > all_to || gone_bits;
+      if (masked) {
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) {
+          const int32_t last = min(row_at[qb], int32_t(t.end) - 1) - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
+#pragma unroll
+          for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r > last ? hidden : s[kb][qb][r];
+        }
+        if (window) {
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++) {
+            const int32_t first = int32_t(max(int64_t(row_at[qb]) - window + 1, int64_t(0))) - key0 - 4 * lgp;
+#pragma unroll
+            for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r < first ? hidden : s[kb][qb][r];
+          }
+        }
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+          if ((gone_bits >> kb) & 1) s[kb][0] = s[kb][1] = v4f{hidden, hidden, hidden, hidden};
+      }
+      auto move_reference = [&]() {
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) {
+          float mx = s[0][qb][0] * c;
+#pragma unroll
+          for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[kb][qb][r] * c);
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float m_new = fmaxf(m_run[qb], mx), alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+          m_run[qb] = m_new;
+          den[qb] *= alpha;
+#pragma unroll
+          for (int db = 0; db < NDB; db++) o[db][qb] *= alpha;
+        }
+      };
+      if (j == 0) move_reference();
+      float pmax[2] = {0.0f, 0.0f};   // the block's largest exponential per row: what tells a stale reference
+      // The fetches of V(j + 1) and K(j + 2) go out one at a time between the exponentials.
+      const int32_t page_k = page_of(j + 2);
+      const auto v_from = resource(val_head, val_page, v_slot, page_v, j + 1), k_from = resource(key_head, key_page, k_slot, page_k, j + 2);
+      page_v = page_k;
+      const uint32_t kdst = k_dst0 + (j & 1) * TILE, vdst = v_dst0 + ((j + 1) % 3) * TILE;
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qb][r], c, -m_run[qb]));
+            pmax[qb] = fmaxf(pmax[qb], e);
+            pb[kb / 2][qb][(kb % 2) * 4 + r] = (__bf16)e;
+            constexpr int EVERY = 16 / PER_WAVE;
+            const int n = (kb * 2 + qb) * 4 + r;   // 0 .. 31
+            if (n % EVERY == EVERY - 1) {
+              const int i = n / EVERY;
+              if (i < PER_WAVE) dma16(v_from, v_src[i], vdst + i * 1024);
+              else dma16(k_from, k_src[i - PER_WAVE], kdst + (i - PER_WAVE) * 1024);
+            }
+          }
+      if (j > 0 && __any(!(pmax[0] < STALE_REFERENCE) || !(pmax[1] < STALE_REFERENCE))) {
+        move_reference();
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+          for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              pb[kb / 2][qb][(kb % 2) * 4 + r] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qb][r], c, -m_run[qb]));
+      }
+      __builtin_amdgcn_s_waitcnt(WAIT_BUT_TWO);
+    };
+    // Every wave passes steps + 1 pairs of barriers; a half with fewer blocks idles through the rest.
+    if (nblocks > 0) {
+      zero_s();
+      run_steps(integral_constant<int, PV_STEPS>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, my_lds, my_lds);
+    }
+    __syncthreads();
+    if (nblocks > 0) slot_b(0);
+    __syncthreads();
+    int vstage = 0;   // V tile of block j - 1
+    for (int j = 1; j < nblocks; j++) {
+      slot_a(j, vstage);
+      vstage = vstage == 2 ? 0 : vstage + 1;
+      __syncthreads();
+      slot_b(j);
+      __syncthreads();
+    }
+    if (nblocks > 0) run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS>{}, values_of(nblocks, vstage), my_lds);
+    for (int j = max(nblocks, 1); j <= steps; j++) {
+      __syncthreads();
+      __syncthreads();
+    }
+    if (!half) __syncthreads();
+
+    // The halves meet: (O, m, l) of half 1 through LDS to the wave of half 0 that has the same rows.  The fetches past the last block must not land on it.
+    const float l_own[2] = {den[0][0], den[1][0]};
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    constexpr int MQ = DD::MERGE_ROWS / 4;   // a lane's quads: O^T's blocks, then (m, m, l, l)
+    v4f *mbuf = (v4f *)lds + qg * (MQ * 64) + lane;
+    if (half) {
+#pragma unroll
+      for (int db = 0; db < NDB; db++)
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) mbuf[(db * 2 + qb) * 64] = o[db][qb];
+      mbuf[(NDB * 2) * 64] = v4f{m_run[0], m_run[1], l_own[0], l_own[1]};
+    }
+    __syncthreads();
+    const Kernargs &e = kernargs();
+    const bool whole = t.whole();
+    if (!whole && t.b0 == 0) {
+      described = true;
+      if (tid == 0) describe(e.w, worker, t);
+    }
+    if (!half) {
+      float *const part = whole ? nullptr : partial_place(e.w, worker, t, BQ, D + 4);
+      const v4f ml = mbuf[(NDB * 2) * 64];
+#pragma unroll
+      for (int qb = 0; qb < 2; qb++) {
+        const uint32_t i = 32 * qg + 16 * qb + lr;
+        const float m1 = ml[qb], l1 = ml[2 + qb], mm = fmaxf(m_run[qb], m1);
+        const float a0 = __builtin_amdgcn_exp2f(m_run[qb] - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm), l = l_own[qb] * a0 + l1 * a1;
+        if (i >= t.rows) continue;
+        if (!whole) {
+          float *to = part + i * (D + 4);
+#pragma unroll
+          for (int db = 0; db < NDB; db++) *(v4f *)(to + db * 16 + 4 * lgp) = o[db][qb] * a0 + mbuf[(db * 2 + qb) * 64] * a1;
+          if (lgp == 0) to[D] = mm, to[D + 1] = l;
+          continue;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l, w0 = a0 * inv, w1 = a1 * inv;
+        const uint32_t row = t.row0 + i, token = e.by_group.div(row), head = t.head * e.p.group + (row - token * e.p.group);
+        __bf16 *out = (__bf16 *)e.p.out + int64_t(t.start + int32_t(token)) * e.p.o_t + int64_t(head) * e.p.o_h;
+        typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int db = 0; db < NDB; db++) {
+          const v4f v = o[db][qb] * w0 + mbuf[(db * 2 + qb) * 64] * w1;
+          const uint32_t dim = db * 16 + 4 * lgp;
+          if (dim < e.p.head_dim) *(v4bf *)(out + dim) = v4bf{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        }
+      }
+    }
+    __syncthreads();   // (the next piece's tiles, or the dealing, come where the halves met)
+    }
+  } while (cur != ~uint64_t(0));
+  if (tid == 0 && !described) kernargs().w.tiles[worker * 8] = 0;
+}
+
+template <int D>
+hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
+  constexpr int LDS = Dims<D>::LDS;
+  static std::atomic<uint64_t> lds_limit_set{0};
+  if (!plan::recording()) {
+    const hipError_t e = raise_lds_limit(lds_limit_set, (const void *)k_paged_attn<D>, LDS);
+    if (e != hipSuccess) return e;
+  }
+  work.round_blocks = 8;
+  plan::work(plan::UNIT_MFMA_BF16, 4.0 * a.tokens * a.q_heads * D * double(a.width) * a.page_size,
+             4.0 * a.kv_heads * a.head_dim * double(a.width) * a.page_size * a.requests + 4.0 * a.tokens * double(a.q_heads) * a.head_dim);
+  MRL_LAUNCH(k_paged_attn<D>, dim3(work.workers), dim3(TH), LDS, stream, Kernargs{a, work, FastDiv(a.group), FastDiv(a.page_size / 16), a.scale * LOG2E});
+  return plan::last_error();
+}
+
+}  // namespace
+
+uint32_t chunk_workers(const PagedAttnArgs &) { return g_compute_units; }
+
+hipError_t launch_chunk(const PagedAttnArgs &a, const Work &work, hipStream_t stream) {
+  return a.head_dim <= 64 ? launch_one<64>(a, work, stream) : launch_one<128>(a, work, stream);
+}
+
+}  // namespace paged
+}  // namespace mrl

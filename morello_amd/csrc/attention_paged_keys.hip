@@ -43,13 +43,11 @@ struct Form {
   // K rows are XOR-swizzled by 16-byte chunk, bf16's V rows by 32-byte slot (attention_keys.hip); an f32 V row is read whole.
   __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1) & 15; }
   __device__ static constexpr int v_swizzle(int row) { return BF16 ? (row / ROWS_PER_LINE) & (SLOTS - 1) & 15 : 0; }
-  // The waves' tiles, or after the loop their O, references and denominators; behind them, per wave, the weights of a block whose values are not
-  // all finite (KEYS rows of 16 floats), then what the dealing shares.
+  // The waves' tiles, or after the loop their O, references and denominators; behind them what the dealing shares, and the pieces that it has noted.
   static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
   static constexpr int AREA = TILES > TRIPLES ? TILES : TRIPLES;
-  static constexpr int WEIGHTS = W * KEYS * 16 * 4;
-  using Deal = Dealer<TH, BQ, KEYS>;
-  static constexpr int LDS = AREA + WEIGHTS + int(sizeof(typename Deal::Shared));
+  using Deal = Dealer<TH, BQ, KEYS, 3>;
+  static constexpr int NOTES = AREA + int(sizeof(typename Deal::Shared)), LDS = NOTES + LIST * 64;
 };
 
 __device__ inline float over_lane_groups(float x) {   // the largest over the four lane groups, in all of them
@@ -58,9 +56,9 @@ __device__ inline float over_lane_groups(float x) {   // the largest over the fo
 }
 __device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (two & 0x7f800000) == 0x7f800000; }   // NaN or infinity among them
 
-// p.head_dim may be below D, in whole 16-byte chunks: zeros behind it.
+// The head dim may be below D, in whole 16-byte chunks: zeros behind it.
 template <class T, int D, int QB, int W>
-__global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work work, FastDiv by_group, FastDiv by_page16, float c) {
+__global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
   using F = Form<T, D, QB, W>;
   constexpr bool BF16 = F::BF16;
   constexpr int ROW = F::ROW, TILE = F::TILE, LOADS = F::LOADS, HALF = F::HALF, NDB = F::NDB;
@@ -68,12 +66,10 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lgp = lane >> 4;
-  typename F::Deal deal(p, work, by_group, reinterpret_cast<typename F::Deal::Shared *>(lds + F::AREA + F::WEIGHTS));
+  const uint32_t worker = xcd_run(blockIdx.x, gridDim.x);
+  uint32_t *const notes = reinterpret_cast<uint32_t *>(lds + F::NOTES);
   uint8_t *const k_tile = lds + wave * 2 * TILE, *const v_tile = k_tile + TILE;
-  float *const weights = reinterpret_cast<float *>(lds + F::AREA) + wave * (KEYS * 16);
-  const uint32_t row_bytes = p.head_dim * uint32_t(sizeof(T));
-  const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();   // a score that weighs nothing
-  const uint32_t groups_per_page = p.page_size / 16;
+  const uint32_t row_bytes = kernargs().p.head_dim * uint32_t(sizeof(T)), k_slot = uint32_t(kernargs().p.key_s * sizeof(T)), v_slot = uint32_t(kernargs().p.val_s * sizeof(T));
 
   // One instruction fills 1 KiB of a tile, lane l its slot l: rows i * ROWS_PER_LOAD + l / CHUNKS, the chunk that belongs there.  The
   // second 16 keys are as the first, from their own base.
@@ -85,8 +81,8 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
       const int row = i * F::ROWS_PER_LOAD + ld_row;
       const uint32_t k_at = (ld_pc ^ F::k_swizzle(row)) << 4;
       const uint32_t v_at = BF16 ? (((ld_pc >> 1) ^ F::v_swizzle(row)) << 5) | ((ld_pc & 1) << 4) : ld_pc << 4;
-      k_src[i] = k_at < row_bytes ? row * uint32_t(p.key_s * sizeof(T)) + k_at : OUTSIDE;
-      v_src[i] = v_at < row_bytes ? row * uint32_t(p.val_s * sizeof(T)) + v_at : OUTSIDE;
+      k_src[i] = k_at < row_bytes ? row * k_slot + k_at : OUTSIDE;
+      v_src[i] = v_at < row_bytes ? row * v_slot + v_at : OUTSIDE;
     }
   }
   const uint32_t k_dst = lds_address(k_tile), v_dst = lds_address(v_tile);
@@ -104,23 +100,28 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
   constexpr int ALL_BUT_ONE_TILE = 0x0F70 | (LOADS & 15) | ((LOADS >> 4) << 14), ALL = 0x0F70, READS_DONE = 0xC07F;
 
   bool described = false;
-  Piece t = {};
-  while (deal.next(t)) {
-    // (what the dealing shared has been read; the triples of the piece before too)
-    const uint8_t *const key_head = (const uint8_t *)p.keys + int64_t(t.head) * p.key_h * int64_t(sizeof(T));
-    const uint8_t *const val_head = (const uint8_t *)p.values + int64_t(t.head) * p.val_h * int64_t(sizeof(T));
-    const int32_t *const pages = p.table + uint64_t(t.request) * p.width;
+  uint64_t cur = 0;
+  do {
+    const uint32_t count = typename F::Deal(kernargs(), reinterpret_cast<typename F::Deal::Shared *>(lds + F::AREA)).deal(worker, notes, cur);
+    __syncthreads();
+    for (uint32_t number = 0; number < count; number++) {
+    const Kernargs &k = kernargs();
+    const Piece t = F::Deal::read(notes, number);
+    const float c = k.c;
+    const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
+    const uint32_t group = k.p.group, window = k.p.window, first_block = t.begin / KEYS + t.b0 + wave;
+    const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();   // a score that weighs nothing
 
     // This lane's rows: queries, and the keys they see, [lo, hi].
     v4i qf[QB][NC];
     int32_t lo[QB], hi[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
-      const uint32_t i = 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * p.group + (row - token * p.group);
+      const uint32_t i = 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * group + (row - token * group);
       const int32_t at = t.at + int32_t(token);
       hi[qb] = i < t.rows ? min(at, int32_t(t.end) - 1) : -1;
-      lo[qb] = p.window ? int32_t(max(int64_t(at) - int64_t(p.window) + 1, int64_t(0))) : 0;
-      const uint8_t *q = (const uint8_t *)p.q + (int64_t(t.start + int32_t(token)) * p.q_t + int64_t(head) * p.q_h) * int64_t(sizeof(T));
+      lo[qb] = window ? int32_t(max(int64_t(at) - int64_t(window) + 1, int64_t(0))) : 0;
+      const uint8_t *q = (const uint8_t *)k.p.q + (int64_t(t.start + int32_t(token)) * k.p.q_t + int64_t(head) * k.p.q_h) * int64_t(sizeof(T));
 #pragma unroll
       for (int j = 0; j < NC; j++) {
         const uint32_t from = j * 64 + lgp * 16;
@@ -130,41 +131,41 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
     // Blocks that every row sees whole lie in [all_from, all_to).
     const int32_t first_at = t.at + int32_t(by_group.div(t.row0)), last_at = t.at + int32_t(by_group.div(t.row0 + t.rows - 1));
     const int32_t all_to = min(first_at + 1, int32_t(t.end));
-    const int32_t all_from = p.window ? int32_t(min(max(int64_t(last_at) - int64_t(p.window) + 1, int64_t(0)), int64_t(0x7fffffff))) : 0;
+    const int32_t all_from = window ? int32_t(max(int64_t(last_at) - int64_t(window) + 1, int64_t(0))) : 0;
 
-    // The pages' numbers of this wave's next 32 blocks, both sixteens of each, one a lane; places in the page.
-    int32_t page_here = -1, page_next = -1;
-    uint32_t place_here = 0, place_next = 0;
-    auto fetch_pages = [&](uint32_t n, int32_t &page, uint32_t &place) {   // of the wave's blocks n .. n + 31
-      const uint32_t group = (t.first_block + t.b0 + wave + (n + (lane >> 1)) * W) * 2 + (lane & 1);
-      page = -1;
-      const uint32_t column = by_page16.div(group);
-      place = (group - column * groups_per_page) * 16;
-      if (t.b0 + wave + (n + (lane >> 1)) * W < t.b1 && group * 16 < t.end) {
+    // The pages' numbers of 32 of this wave's blocks, both sixteens of each, one a lane, and the places in the page.
+    int32_t page_here = -1;
+    uint32_t place_here = 0;
+    const int32_t *const pages = k.p.table + uint64_t(t.request) * k.p.width;
+    const uint32_t page_count = k.p.pages, groups_per_page = k.p.page_size / 16;
+    auto fetch_pages = [&](uint32_t n) {   // of the wave's blocks n .. n + 31
+      const uint32_t mine = n + (lane >> 1), group16 = (first_block + mine * W) * 2 + (lane & 1), column = by_page16.div(group16);
+      page_here = -1, place_here = (group16 - column * groups_per_page) * 16;
+      if (t.b0 + wave + mine * W < t.b1 && group16 * 16 < t.end) {
         const int32_t number = pages[column];
-        if (number >= 0 && uint32_t(number) < p.pages) page = number;
+        if (uint32_t(number) < page_count) page_here = number;
       }
     };
-    // Of the wave's n-th block: 16 keys each.
+    // Of the wave's n-th block, 16 keys each: through a resource that ends behind the last one that a row sees.
     auto page_of = [&](uint32_t n, int half) { return __builtin_amdgcn_readlane(page_here, (n & 31) * 2 + half); };
-    auto issue = [&](uint32_t n, const uint8_t *head, int64_t s_page, int64_t s_slot, const uint32_t *src, uint32_t dst) {
-      const uint32_t key0 = (t.first_block + t.b0 + wave + n * W) * KEYS;
+    auto issue = [&](uint32_t n, const uint8_t *head, int64_t page_bytes, uint32_t slot_bytes, const uint32_t *src, uint32_t dst) {
+      const uint32_t key0 = (first_block + n * W) * KEYS;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int32_t page = page_of(n, half);
-        const uint32_t place = __builtin_amdgcn_readlane(place_here, (n & 31) * 2 + half);
-        const uint32_t from = key0 + 16 * half;
+        const uint32_t place = __builtin_amdgcn_readlane(place_here, (n & 31) * 2 + half), from = key0 + 16 * half;
         const uint32_t rows = page < 0 || from >= t.end ? 0 : min(t.end - from, 16u);
-        const uint8_t *base = head + (int64_t(max(page, 0)) * s_page + int64_t(place) * s_slot) * int64_t(sizeof(T));
-        const int bytes = rows ? int((rows - 1) * uint32_t(s_slot * sizeof(T)) + row_bytes) : 0;
-        const uint64_t at = reinterpret_cast<uint64_t>(base), same = uint64_t(uniform(uint32_t(at >> 32))) << 32 | uniform(uint32_t(at));   // (in scalar registers)
-        const auto from_buf = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(same), 0, uniform(bytes), 0x00020000);
+        const uint64_t base = reinterpret_cast<uint64_t>(head) + uint64_t(max(page, 0)) * page_bytes + uint64_t(place) * slot_bytes;
+        const auto from_buf = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(base)), 0, uniform(int(rows ? (rows - 1) * slot_bytes + row_bytes : 0)), 0x00020000);
 #pragma unroll
         for (int i = 0; i < HALF; i++) dma16_ordered(from_buf, src[i], dst + (half * HALF + i) * 1024);
       }
     };
-    auto issue_k = [&](uint32_t n) { issue(n, key_head, p.key_p, p.key_s, k_src, k_dst); };
-    auto issue_v = [&](uint32_t n) { issue(n, val_head, p.val_p, p.val_s, v_src, v_dst); };
+    const uint8_t *const key_head = (const uint8_t *)k.p.keys + int64_t(t.head) * k.p.key_h * int64_t(sizeof(T));
+    const uint8_t *const val_head = (const uint8_t *)k.p.values + int64_t(t.head) * k.p.val_h * int64_t(sizeof(T));
+    const int64_t key_page = k.p.key_p * int64_t(sizeof(T)), val_page = k.p.val_p * int64_t(sizeof(T));
+    auto issue_k = [&](uint32_t n) { issue(n, key_head, key_page, k_slot, k_src, k_dst); };
+    auto issue_v = [&](uint32_t n) { issue(n, val_head, val_page, v_slot, v_src, v_dst); };
 
     v4f o[NDB][QB], den[QB];
     float m_run[QB];
@@ -182,16 +183,14 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
 
     // This wave's blocks: t.b0 + wave, + W, ..
     const uint32_t mine = t.b1 - t.b0 > uint32_t(wave) ? (t.b1 - t.b0 - wave + W - 1) / W : 0;
-    __syncthreads();   // the tiles are free: everybody has read the piece before
     if (mine) {
-      fetch_pages(0, page_here, place_here);
+      fetch_pages(0);
       issue_k(0);
       issue_v(0);
       bool start = true;
       __builtin_amdgcn_s_waitcnt(ALL);
       for (uint32_t n = 0; n < mine; n++) {
         const bool more = n + 1 < mine;
-        const uint32_t block = t.first_block + t.b0 + wave + n * W;
         // In flight at this point, oldest first: K of this block, V of this block.
         if (!start) __builtin_amdgcn_s_waitcnt(ALL_BUT_ONE_TILE);
         asm volatile("" ::: "memory");
@@ -217,24 +216,21 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(READS_DONE);   // K's operands are in registers: its tile may be filled again
         const bool gone0 = page_of(n, 0) < 0, gone1 = page_of(n, 1) < 0;
-        // (V of the next block is asked for with the same numbers, so they move on behind this block's second product)
-        if (more && ((n + 1) & 31) == 0) fetch_pages(n + 1, page_next, place_next);
         if (more) {
-          if (((n + 1) & 31) == 0) page_here = page_next, place_here = place_next;
+          if (((n + 1) & 31) == 0) fetch_pages(n + 1);
           issue_k(n + 1);
         }
-        const int32_t key0 = int32_t(block * KEYS);
+        const int32_t key0 = int32_t((first_block + n * W) * KEYS);
         const bool masked = key0 < all_from || key0 + KEYS > all_to || gone0 || gone1;
         if (masked) {
 #pragma unroll
-          for (int kb = 0; kb < 2; kb++)
+          for (int qb = 0; qb < QB; qb++) {
+            const int32_t last = hi[qb] - key0 - 4 * lgp, first = lo[qb] - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++)
+            for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const int32_t key = key0 + kb * 16 + 4 * lgp + r;
-                if (key < lo[qb] || key > hi[qb] || (kb ? gone1 : gone0)) s[kb][qb][r] = hidden;
-              }
+              for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r > last || kb * 16 + r < first || (kb ? gone1 : gone0) ? hidden : s[kb][qb][r];
+          }
         }
         auto move_reference = [&]() {
 #pragma unroll
@@ -296,40 +292,51 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
           }
         }
         if (__any(odd)) {
-          // Key by key: a row takes what it sees.
+          // A key at a time, its values against its weights alone, and of the product only the columns (query rows) that see it.
+          if constexpr (BF16) {
+#pragma unroll 1
+            for (int x = 0; x < KEYS; x++) {   // element 4 (x / 16) + x % 4 of lane group (x % 16) / 4
+              const int element = 4 * (x / 16) + x % 4, bits = lgp == x % 16 / 4 ? element % 2 ? int(0xffff0000) : 0xffff : 0;
+              const v4i only = {element / 2 == 0 ? bits : 0, element / 2 == 1 ? bits : 0, element / 2 == 2 ? bits : 0, element / 2 == 3 ? bits : 0};
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++) {
+              for (int db = 0; db < NDB; db++) {
+                const v2i lo2 = read_tr16(v_tile + v_lane[db]), hi2 = read_tr16(v_tile + v_lane[db] + 16 * ROW);
+                const v4i a = v4i{lo2[0], lo2[1], hi2[0], hi2[1]} & only;
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) {
+                  const v4f y = mfma16(a, __builtin_bit_cast(v4i, pb[qb]) & only, v4f{0, 0, 0, 0});
+                  o[db][qb] += key0 + x >= lo[qb] && key0 + x <= hi[qb] && !(x < 16 ? gone0 : gone1) ? y : v4f{0, 0, 0, 0};
+                }
+                asm volatile("" ::: "memory");   // (one at a time: it need not be fast, and has few registers)
+              }
+            }
+          } else {
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const int32_t in_block = kb * 16 + 4 * lgp + r, key = key0 + in_block;
-                const bool seen = key >= lo[qb] && key <= hi[qb] && !(kb ? gone1 : gone0);
-                float x = e[kb][qb][r];
-                if constexpr (BF16) x = float(pb[qb][kb * 4 + r]);
-                weights[in_block * 16 + lr] = seen ? x : -1.0f;
-              }
+              for (int r = 0; r < 4; r++)
 #pragma unroll 1
-            for (int key = 0; key < KEYS; key++) {
-              const float x = weights[key * 16 + lr];
-              const bool seen = !(x < 0.0f);
+                for (int g = 0; g < 4; g++) {
+                  const int32_t key = key0 + kb * 16 + 4 * g + r;
 #pragma unroll
-              for (int db = 0; db < NDB; db++)
+                  for (int i = 0; i < NV; i++) {
+                    const v4i a = *(const v4i *)(v_tile + v_lane[i] + (kb * 16 + r) * ROW);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                  float v;
-                  if constexpr (BF16) {
-                    const uint32_t at = key * ROW + ((db ^ F::v_swizzle(key)) << 5) + (4 * lgp + r) * 2;
-                    v = __uint_as_float(uint32_t(*(const uint16_t *)(v_tile + at)) << 16);
-                  } else {
-                    const uint32_t dim = 64 * (db / 4) + 4 * (4 * lgp + r) + db % 4;
-                    v = *(const float *)(v_tile + key * ROW + dim * 4);
+                    for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                      for (int j = 0; j < 4; j++) {
+                        const v4f y = mfma4(lgp == g ? __int_as_float(a[j]) : 0.0f, lgp == g ? e[kb][qb][r] : 0.0f, v4f{0, 0, 0, 0});
+                        o[4 * i + j][qb] += key >= lo[qb] && key <= hi[qb] && !(kb ? gone1 : gone0) ? y : v4f{0, 0, 0, 0};
+                      }
+                    asm volatile("" ::: "memory");
                   }
-                  if (seen) o[db][qb][r] = __builtin_fmaf(x, v, o[db][qb][r]);
                 }
-            }
           }
-        } else if constexpr (BF16) {
+          // What is left of the block are its denominators: the product below adds zeros.
+#pragma unroll 1
+          for (int i = 0; i < TILE / 1024; i++) *(v4i *)(v_tile + i * 1024 + lane * 16) = v4i{0, 0, 0, 0};
+        }
+        if constexpr (BF16) {
 #pragma unroll
           for (int db = 0; db < NDB; db++) {
             const v2i lo2 = read_tr16(v_tile + v_lane[db]), hi2 = read_tr16(v_tile + v_lane[db] + 16 * ROW);
@@ -393,11 +400,12 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
       if (lgp == 0) stats[(wave * QB + qb) * 32 + lr] = m_run[qb], stats[(wave * QB + qb) * 32 + 16 + lr] = l;
     }
     __syncthreads();
-    const bool whole = F::Deal::whole(t);
-    float *const part = whole ? nullptr : deal.place(t, F::ROW_FLOATS);
+    const Kernargs &e = kernargs();
+    const bool whole = t.whole();
+    float *const part = whole ? nullptr : partial_place(e.w, worker, t, F::BQ, F::ROW_FLOATS);
     if (!whole && t.b0 == 0) {
       described = true;
-      if (tid == 0) deal.describe(t);
+      if (tid == 0) describe(e.w, worker, t);
     }
 #pragma unroll
     for (int x = wave; x < QB * NDB; x += W) {
@@ -422,10 +430,10 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
         if (dim == 0) to[D] = mm, to[D + 1] = l;
         continue;
       }
-      if (dim >= p.head_dim) continue;
+      if (dim >= e.p.head_dim) continue;
       sum *= l == 0.0f ? 0.0f : 1.0f / l;
-      const uint32_t row = t.row0 + i, token = by_group.div(row), head = t.head * p.group + (row - token * p.group);
-      T *out = (T *)p.out + int64_t(t.start + int32_t(token)) * p.o_t + int64_t(head) * p.o_h + dim;
+      const uint32_t row = t.row0 + i, token = e.by_group.div(row), head = t.head * e.p.group + (row - token * e.p.group);
+      T *out = (T *)e.p.out + int64_t(t.start + int32_t(token)) * e.p.o_t + int64_t(head) * e.p.o_h + dim;
       if constexpr (BF16) {
         typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
         *(v4bf *)out = v4bf{(__bf16)sum[0], (__bf16)sum[1], (__bf16)sum[2], (__bf16)sum[3]};
@@ -433,8 +441,10 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(PagedAttnArgs p, Work wor
         *(v4f *)out = sum;
       }
     }
-  }
-  if (tid == 0) deal.finish(described);
+    __syncthreads();   // (the next piece's tiles, or the dealing, come where the triples met)
+    }
+  } while (cur != ~uint64_t(0));
+  if (tid == 0 && !described && !kernargs().w.direct) kernargs().w.tiles[worker * 8] = 0;
 }
 
 template <class T, int D, int QB, int W>
@@ -450,7 +460,7 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
   const double keys = double(a.width) * a.page_size * a.requests;   // (all that the table holds: the lengths are on the device)
   plan::work(F::BF16 ? plan::UNIT_MFMA_BF16 : plan::UNIT_MFMA_F32, 4.0 * a.tokens * a.q_heads * D * double(a.width) * a.page_size,
              2.0 * sizeof(T) * a.kv_heads * a.head_dim * keys + 2.0 * sizeof(T) * a.tokens * double(a.q_heads) * a.head_dim);
-  MRL_LAUNCH((k_paged_attn<T, D, QB, W>), dim3(grid), dim3(F::TH), F::LDS, stream, a, work, FastDiv(a.group), FastDiv(a.page_size / 16), a.scale * LOG2E);
+  MRL_LAUNCH((k_paged_attn<T, D, QB, W>), dim3(grid), dim3(F::TH), F::LDS, stream, Kernargs{a, work, FastDiv(a.group), FastDiv(a.page_size / 16), a.scale * LOG2E});
   return plan::last_error();
 }
 
@@ -460,8 +470,6 @@ uint32_t per_unit(int qb) {   // workgroups that a compute unit's LDS holds
   return std::max(1, std::min(2, 160 * 1024 / (qb == 1 ? Form<T, D, 1, W>::LDS : Form<T, D, 2, W>::LDS)));
 }
 }  // namespace
-
-uint32_t keys_row_floats(const PagedAttnArgs &a) { return (a.head_dim <= 64 ? 64 : 128) + 4; }
 
 uint32_t keys_workers(const PagedAttnArgs &a, int qb) {
   const bool narrow = a.head_dim <= 64;
