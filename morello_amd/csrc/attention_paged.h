@@ -8,7 +8,7 @@
 // The host chooses a number of workgroups; each finds its own share by itself, from the same lengths (some thousand bytes out of a cache,
 // no launch before the kernel).  Shares are equal runs of one line on which the tiles lie, request by request, tile by tile, head by head:
 //   few tiles for the workgroups: a tile's length on the line is its blocks rounded up to the share, and the share so small that
-//     the pieces are just as many as workgroups: each has one piece, a tile's pieces meet in the merging launch;
+//     the pieces are at most as many as workgroups: each has one piece, a tile's pieces meet in the merging launch;
 //   else: a tile's length is its blocks and some for what a tile costs besides, the share what all come to over the workgroups.
 // A workgroup's run may begin and end inside a tile: there it leaves a partial result (O, m, l: the sum of the values, the reference in the
 // exponent's base of two, the denominator) instead of the tile's rows, one for the tile it does not begin (place 0) and one for the tile it
@@ -67,8 +67,9 @@ __device__ inline uint32_t quotient(uint64_t x, uint64_t y) { return uint32_t(do
 
 constexpr int LIST = 16;   // pieces that a workgroup notes at a time
 
-// OVERHEAD: what a tile costs besides its blocks, in blocks: the trips to memory before its first one, and its results.
-template <int TH, int BQ, int BK, int OVERHEAD>
+// What a tile costs besides its blocks (the trips to memory before its first one, its results), in blocks: OVERHEAD where the chip has all it can do, START
+// where a workgroup waits for nothing but its own loads.
+template <int TH, int BQ, int BK, int OVERHEAD, int START>
 struct Dealer {
   // Shared memory of the dealing: nothing in it is kept over a piece.
   struct Shared {
@@ -198,14 +199,13 @@ struct Dealer {
       if (one) break;
     }
     const uint64_t heads = k.p.kv_heads, workers = k.w.workers, all_tiles = scan(tiles) * heads, all_blocks = scan(sum) * heads;
-    const bool few = all_tiles * 4 < workers * 3;
-    uint64_t share;
-    if (few) {
+    uint64_t share = max(uint64_t(quotient(all_blocks + all_tiles * (1 + OVERHEAD) + workers - 1, workers)), uint64_t(1));
+    bool few = false;
+    if (all_tiles < workers) {   // a piece to each, where that is no longer than equal shares and the second start that they cost
       const uint64_t spare = workers - all_tiles, round = k.w.round_blocks;
-      share = (uint64_t(quotient(all_blocks + spare - 1, spare)) + round - 1) / round * round;
-      share = max(share, round);
-    } else {
-      share = max(uint64_t(quotient(all_blocks + all_tiles * (1 + OVERHEAD) + workers - 1, workers)), uint64_t(1));
+      const uint64_t single = max((uint64_t(quotient(all_blocks + spare - 1, spare)) + round - 1) / round * round, round);
+      few = single <= share + START;
+      if (few) share = single;
     }
     const uint64_t stop = share * (worker + 1);
     cur = max(cur, share * worker);

@@ -115,16 +115,11 @@ struct MergeArgs {
   uint32_t row_floats;
   FastDiv by_group, by_quads;
 };
-template <class T>
-__global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
-  const uint32_t second = blockIdx.x >= a.of[0].workers, worker = blockIdx.x - (second ? a.of[0].workers : 0), bq = a.of[second].bq;
-  const float *const partials = a.of[second].partials;
-  const uint32_t *d = a.of[second].tiles + worker * 8;
-  const uint32_t more = d[0], row0 = d[2], rows = d[3], kv = d[4];
-  const int32_t start = int32_t(d[1]);
-  if (!more) return;
+// U: pieces asked for at a time.
+template <class T, uint32_t U>
+__device__ inline void merge_rows(const PagedAttnArgs &p, const MergeArgs &a, const float *partials, uint32_t worker, uint32_t more, uint32_t bq, int32_t start, uint32_t row0,
+                                  uint32_t rows, uint32_t kv) {
   const uint32_t quads = (p.head_dim + 3) / 4, stat = a.row_floats - 4;
-  constexpr uint32_t U = 16;   // pieces asked for at a time
   for (uint32_t x = blockIdx.y * THREADS + threadIdx.x; x < rows * quads; x += gridDim.y * THREADS) {
     const uint32_t i = a.by_quads.div(x), dim = (x - i * quads) * 4;
     // piece 0 lies in the first worker's place 1, the others in place 0 of the workers behind it
@@ -162,6 +157,20 @@ __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, M
     }
   }
 }
+template <class T>
+__global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
+  const uint32_t second = blockIdx.x >= a.of[0].workers, worker = blockIdx.x - (second ? a.of[0].workers : 0), bq = a.of[second].bq;
+  const float *const partials = a.of[second].partials;
+  const uint32_t *d = a.of[second].tiles + worker * 8;
+  const uint32_t more = d[0], row0 = d[2], rows = d[3], kv = d[4];
+  const int32_t start = int32_t(d[1]);
+  if (!more) return;
+  if (more < 2) merge_rows<T, 2>(p, a, partials, worker, more, bq, start, row0, rows, kv);
+  else if (more < 4) merge_rows<T, 4>(p, a, partials, worker, more, bq, start, row0, rows, kv);
+  else merge_rows<T, 16>(p, a, partials, worker, more, bq, start, row0, rows, kv);
+}
+
+constexpr uint32_t DIRECT_KEYS = 1024;
 
 // How a call runs, by sizes, types and strides: on tiles of 16 * qb rows, of 128, or small requests on the former and the others on the latter.
 struct Choice {
@@ -191,7 +200,9 @@ Choice choose(const PagedAttnArgs &a) {
     w.min_rows = 1, w.max_rows = chunk ? 16 : 0x7fffffff;
     // (max_new is the program's word: a request of more tokens would have more tiles than one)
     w.single = chunk || uint64_t(a.tokens) * a.group <= 16u * c.qb;
-    w.workers = paged::keys_workers(a, c.qb);
+    // Tables of some hundred keys at most: a workgroup to each request and head does them in some rounds, with nothing to find out before and no second launch.
+    w.direct = w.single && !chunk && uint64_t(a.width) * a.page_size <= DIRECT_KEYS;
+    w.workers = w.direct ? 0 : paged::keys_workers(a, c.qb);
     c.keys_bytes = size_t(w.workers) * 2 * 16 * c.qb * row_bytes;
   }
   if (chunk) {

@@ -23,7 +23,7 @@ using namespace attn;
 
 constexpr int BKV = 64, QG = 4, BQ = CHUNK_ROWS, TH = 512;
 constexpr int PRIO_A = 2, PRIO_B = 0;   // of a wave in its slot of products, of exponentials
-using Deal = Dealer<TH, BQ, BKV, 4>;
+using Deal = Dealer<TH, BQ, BKV, 4, 5>;
 
 template <int D>
 struct Dims {

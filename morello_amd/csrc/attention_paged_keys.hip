@@ -46,7 +46,7 @@ struct Form {
   // The waves' tiles, or after the loop their O, references and denominators; behind them what the dealing shares, and the pieces that it has noted.
   static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
   static constexpr int AREA = TILES > TRIPLES ? TILES : TRIPLES;
-  using Deal = Dealer<TH, BQ, KEYS, 3>;
+  using Deal = Dealer<TH, BQ, KEYS, 3, BF16 ? 3 * W : W>;
   static constexpr int NOTES = AREA + int(sizeof(typename Deal::Shared)), LDS = NOTES + LIST * 64;
 };
 
