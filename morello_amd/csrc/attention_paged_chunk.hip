@@ -21,9 +21,8 @@ namespace {
 
 using namespace attn;
 
-constexpr int BKV = 64, QG = 4, BQ = CHUNK_ROWS, TH = 512;
+constexpr int BKV = 64, QG = 4, BQ = 32 * QG, TH = 512;
 constexpr int PRIO_A = 2, PRIO_B = 0;   // of a wave in its slot of products, of exponentials
-using Deal = Dealer<TH, BQ, BKV, 4, 5>;
 
 template <int D>
 struct Dims {
@@ -32,8 +31,8 @@ struct Dims {
   static constexpr int PER_WAVE = 16 / ROWS_PER_LOAD;                    // loads of a wave's 16 keys
   static constexpr int MERGE_ROWS = D / 2 + 4;                           // a lane's O, two references and two denominators
   static constexpr int MERGE = QG * MERGE_ROWS * 64 * 4;
-  static constexpr int LDS = 2 * HALF > MERGE ? 2 * HALF : MERGE;
-  static_assert(int(sizeof(Deal::Shared)) <= LDS, "what the dealing shares lies where the tiles do");
+  static constexpr int LDS = 2 * HALF;
+  static_assert(MERGE <= LDS, "what meets at the end lies where the tiles did");
   __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1); }
   __device__ static constexpr int v_swizzle(int row) { return (row / ROWS_PER_LINE) & (SLOTS - 1); }
 };
@@ -50,7 +49,6 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qg = wave % QG, half = wave / QG;   // rows 32 qg .. of the tile; half of the keys
   const int lr = lane & 15, lgp = lane >> 4;
-  const uint32_t worker = xcd_run(blockIdx.x, gridDim.x);
   uint8_t *const my_lds = lds + half * HALF;
   const uint32_t row_bytes = kernargs().p.head_dim * 2, k_slot = uint32_t(kernargs().p.key_s * 2), v_slot = uint32_t(kernargs().p.val_s * 2);
 
@@ -72,15 +70,10 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
   };
 
-  bool described = false;
-  uint64_t cur = 0;
-  do {
-    uint32_t *const notes = kernargs().w.lists + uint64_t(worker) * (LIST * 16);
-    const uint32_t count = Deal(kernargs(), reinterpret_cast<Deal::Shared *>(lds)).deal(worker, notes, cur);
-    __syncthreads();
-    for (uint32_t number = 0; number < count; number++) {
+  Worker worker(kernargs().w);
+  Piece t;
+  while (worker.next(kernargs(), &t)) {
     const Kernargs &k = kernargs();
-    const Piece t = Deal::read(k.w.lists + uint64_t(worker) * (LIST * 16), number);
     const float c = k.c;
     const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
     const uint32_t group = k.p.group, window = k.p.window;
@@ -445,11 +438,11 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     const Kernargs &e = kernargs();
     const bool whole = t.whole();
     if (!whole && t.b0 == 0) {
-      described = true;
-      if (tid == 0) describe(e.w, worker, t);
+      worker.described = true;
+      if (tid == 0) worker.describe(e.w, t);
     }
     if (!half) {
-      float *const part = whole ? nullptr : partial_place(e.w, worker, t, BQ, D + 4);
+      float *const part = whole ? nullptr : worker.place(e.w, t, BQ * (D + 4));
       const v4f ml = mbuf[(NDB * 2) * 64];
 #pragma unroll
       for (int qb = 0; qb < 2; qb++) {
@@ -476,10 +469,9 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
         }
       }
     }
-    __syncthreads();   // (the next piece's tiles, or the dealing, come where the halves met)
-    }
-  } while (cur != ~uint64_t(0));
-  if (tid == 0 && !described) kernargs().w.tiles[worker * 8] = 0;
+    __syncthreads();   // (the next piece's tiles come where the halves met)
+  }
+  if (tid == 0 && !worker.described) kernargs().w.merges[worker.number * 8] = 0;
 }
 
 template <int D>
@@ -490,7 +482,6 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
     const hipError_t e = raise_lds_limit(lds_limit_set, (const void *)k_paged_attn<D>, LDS);
     if (e != hipSuccess) return e;
   }
-  work.round_blocks = 8;
   plan::work(plan::UNIT_MFMA_BF16, 4.0 * a.tokens * a.q_heads * D * double(a.width) * a.page_size,
              4.0 * a.kv_heads * a.head_dim * double(a.width) * a.page_size * a.requests + 4.0 * a.tokens * double(a.q_heads) * a.head_dim);
   MRL_LAUNCH(k_paged_attn<D>, dim3(work.workers), dim3(TH), LDS, stream, Kernargs{a, work, FastDiv(a.group), FastDiv(a.page_size / 16), a.scale * LOG2E});
@@ -499,7 +490,10 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
 
 }  // namespace
 
-uint32_t chunk_workers(const PagedAttnArgs &) { return g_compute_units; }
+void chunk_work(const PagedAttnArgs &, Work *w) {
+  w->workers = std::min(MOST_WORKERS, g_compute_units);   // (one of D = 128 to a compute unit's LDS)
+  w->bq_log2 = 7, w->block_log2 = 6, w->least = 8, w->overhead = 7, w->second = 7;
+}
 
 hipError_t launch_chunk(const PagedAttnArgs &a, const Work &work, hipStream_t stream) {
   return a.head_dim <= 64 ? launch_one<64>(a, work, stream) : launch_one<128>(a, work, stream);

@@ -28,6 +28,7 @@ namespace {
 using namespace attn;
 
 constexpr int KEYS = 32;      // keys per block
+constexpr int WAVES = 4;
 constexpr int FOLLOWED = 4;   // blocks of a wave whose maxima the reference follows
 
 template <class T, int D, int QB, int W>
@@ -43,11 +44,11 @@ struct Form {
   // K rows are XOR-swizzled by 16-byte chunk, bf16's V rows by 32-byte slot (attention_keys.hip); an f32 V row is read whole.
   __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1) & 15; }
   __device__ static constexpr int v_swizzle(int row) { return BF16 ? (row / ROWS_PER_LINE) & (SLOTS - 1) & 15 : 0; }
-  // The waves' tiles, or after the loop their O, references and denominators; behind them what the dealing shares, and the pieces that it has noted.
+  // The waves' tiles, or after the loop their O, references and denominators.
   static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
-  static constexpr int AREA = TILES > TRIPLES ? TILES : TRIPLES;
-  using Deal = Dealer<TH, BQ, KEYS, 3, BF16 ? 3 * W : W>;
-  static constexpr int NOTES = AREA + int(sizeof(typename Deal::Shared)), LDS = NOTES + LIST * 64;
+  static constexpr int LDS = TILES > TRIPLES ? TILES : TRIPLES;
+  // Workgroups of a compute unit: by LDS, and by registers (a wave per SIMD each).
+  static constexpr int BY_LDS = 160 * 1024 / LDS, RESIDENT = BY_LDS >= 4 && QB == 1 ? 4 : BY_LDS >= 2 ? 2 : 1;
 };
 
 __device__ inline float over_lane_groups(float x) {   // the largest over the four lane groups, in all of them
@@ -58,7 +59,7 @@ __device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (t
 
 // The head dim may be below D, in whole 16-byte chunks: zeros behind it.
 template <class T, int D, int QB, int W>
-__global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, D, QB, W>::RESIDENT))) void k_paged_attn(Kernargs) {
   using F = Form<T, D, QB, W>;
   constexpr bool BF16 = F::BF16;
   constexpr int ROW = F::ROW, TILE = F::TILE, LOADS = F::LOADS, HALF = F::HALF, NDB = F::NDB;
@@ -66,8 +67,6 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lgp = lane >> 4;
-  const uint32_t worker = xcd_run(blockIdx.x, gridDim.x);
-  uint32_t *const notes = reinterpret_cast<uint32_t *>(lds + F::NOTES);
   uint8_t *const k_tile = lds + wave * 2 * TILE, *const v_tile = k_tile + TILE;
   const uint32_t row_bytes = kernargs().p.head_dim * uint32_t(sizeof(T)), k_slot = uint32_t(kernargs().p.key_s * sizeof(T)), v_slot = uint32_t(kernargs().p.val_s * sizeof(T));
 
@@ -99,14 +98,8 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
   }
   constexpr int ALL_BUT_ONE_TILE = 0x0F70 | (LOADS & 15) | ((LOADS >> 4) << 14), ALL = 0x0F70, READS_DONE = 0xC07F;
 
-  bool described = false;
-  uint64_t cur = 0;
-  do {
-    const uint32_t count = typename F::Deal(kernargs(), reinterpret_cast<typename F::Deal::Shared *>(lds + F::AREA)).deal(worker, notes, cur);
-    __syncthreads();
-    for (uint32_t number = 0; number < count; number++) {
-    const Kernargs &k = kernargs();
-    const Piece t = F::Deal::read(notes, number);
+  const bool direct = kernargs().w.direct;
+  auto run = [&](const Kernargs &k, const Piece &t, Worker *worker) {
     const float c = k.c;
     const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
     const uint32_t group = k.p.group, window = k.p.window, first_block = t.begin / KEYS + t.b0 + wave;
@@ -402,10 +395,10 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
     __syncthreads();
     const Kernargs &e = kernargs();
     const bool whole = t.whole();
-    float *const part = whole ? nullptr : partial_place(e.w, worker, t, F::BQ, F::ROW_FLOATS);
+    float *const part = whole ? nullptr : worker->place(e.w, t, F::BQ * F::ROW_FLOATS);
     if (!whole && t.b0 == 0) {
-      described = true;
-      if (tid == 0) describe(e.w, worker, t);
+      worker->described = true;
+      if (tid == 0) worker->describe(e.w, t);
     }
 #pragma unroll
     for (int x = wave; x < QB * NDB; x += W) {
@@ -441,10 +434,18 @@ __global__ __launch_bounds__(64 * W) void k_paged_attn(Kernargs) {
         *(v4f *)out = sum;
       }
     }
-    __syncthreads();   // (the next piece's tiles, or the dealing, come where the triples met)
-    }
-  } while (cur != ~uint64_t(0));
-  if (tid == 0 && !described && !kernargs().w.direct) kernargs().w.tiles[worker * 8] = 0;
+  };
+  Piece t;
+  if (direct) {
+    if (direct_piece(kernargs(), &t)) run(kernargs(), t, nullptr);
+    return;
+  }
+  Worker worker(kernargs().w);
+  while (worker.next(kernargs(), &t)) {
+    run(kernargs(), t, &worker);
+    __syncthreads();   // (the triples have been read)
+  }
+  if (tid == 0 && !worker.described) kernargs().w.merges[worker.number * 8] = 0;
 }
 
 template <class T, int D, int QB, int W>
@@ -455,7 +456,6 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
     const hipError_t e = raise_lds_limit(lds_limit_set, (const void *)k_paged_attn<T, D, QB, W>, F::LDS);
     if (e != hipSuccess) return e;
   }
-  work.round_blocks = W;
   const uint32_t grid = work.direct ? a.requests * a.kv_heads : work.workers;
   const double keys = double(a.width) * a.page_size * a.requests;   // (all that the table holds: the lengths are on the device)
   plan::work(F::BF16 ? plan::UNIT_MFMA_BF16 : plan::UNIT_MFMA_F32, 4.0 * a.tokens * a.q_heads * D * double(a.width) * a.page_size,
@@ -464,26 +464,31 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
   return plan::last_error();
 }
 
-template <class T, int D>
-uint32_t per_unit(int qb) {   // workgroups that a compute unit's LDS holds
-  constexpr int W = sizeof(T) == 4 && D == 128 ? 4 : 8;
-  return std::max(1, std::min(2, 160 * 1024 / (qb == 1 ? Form<T, D, 1, W>::LDS : Form<T, D, 2, W>::LDS)));
+// Calls f with the form's types and sizes.
+template <class F>
+auto with_form(const PagedAttnArgs &a, int qb, F f) {
+  constexpr int W = WAVES;
+  const bool narrow = a.head_dim <= 64;
+  if (a.dtype == MRL_BF16) {
+    if (narrow) return qb == 1 ? f(Form<__bf16, 64, 1, W>()) : f(Form<__bf16, 64, 2, W>());
+    return qb == 1 ? f(Form<__bf16, 128, 1, W>()) : f(Form<__bf16, 128, 2, W>());
+  }
+  if (narrow) return qb == 1 ? f(Form<float, 64, 1, W>()) : f(Form<float, 64, 2, W>());
+  return qb == 1 ? f(Form<float, 128, 1, W>()) : f(Form<float, 128, 2, W>());
+}
+template <class T, int D, int QB, int W>
+hipError_t launch_form(Form<T, D, QB, W>, const PagedAttnArgs &a, const Work &work, hipStream_t stream) {
+  return launch_one<T, D, QB, W>(a, work, stream);
 }
 }  // namespace
 
-uint32_t keys_workers(const PagedAttnArgs &a, int qb) {
-  const bool narrow = a.head_dim <= 64;
-  return g_compute_units * (a.dtype == MRL_BF16 ? (narrow ? per_unit<__bf16, 64>(qb) : per_unit<__bf16, 128>(qb)) : (narrow ? per_unit<float, 64>(qb) : per_unit<float, 128>(qb)));
+void keys_work(const PagedAttnArgs &a, int qb, Work *w) {
+  w->workers = std::min(MOST_WORKERS, g_compute_units * with_form(a, qb, [](auto f) { return uint32_t(decltype(f)::RESIDENT); }));
+  w->bq_log2 = qb == 1 ? 4 : 5, w->block_log2 = 5, w->least = WAVES, w->overhead = 3, w->second = 3 * WAVES;
 }
 
 hipError_t launch_keys(const PagedAttnArgs &a, const Work &work, int qb, hipStream_t stream) {
-  const bool narrow = a.head_dim <= 64;
-  if (a.dtype == MRL_BF16) {
-    if (narrow) return qb == 1 ? launch_one<__bf16, 64, 1, 8>(a, work, stream) : launch_one<__bf16, 64, 2, 8>(a, work, stream);
-    return qb == 1 ? launch_one<__bf16, 128, 1, 8>(a, work, stream) : launch_one<__bf16, 128, 2, 8>(a, work, stream);
-  }
-  if (narrow) return qb == 1 ? launch_one<float, 64, 1, 8>(a, work, stream) : launch_one<float, 64, 2, 8>(a, work, stream);
-  return qb == 1 ? launch_one<float, 128, 1, 4>(a, work, stream) : launch_one<float, 128, 2, 4>(a, work, stream);
+  return with_form(a, qb, [&](auto f) { return launch_form(f, a, work, stream); });
 }
 
 }  // namespace paged
