@@ -3,18 +3,23 @@
 //
 // A TILE is up to 16, 32 or 128 query rows of one request that read the same key/value head: row i of a request is its token i / G at query head i % G of the
 // G = q_heads / kv_heads that share it, so that keys and values are fetched once for all of them.  A tile's keys come in BLOCKS; how many it has
-// follows from the lengths, which are on the device.  So a launch of one workgroup (k_paged_attn_deal) lays the tiles on a line, request by request, head by
-// head (what shares a head's keys and values runs beside each other, on one XCD, and finds them in its L2), and cuts the line in equal shares:
-//   few tiles for the workgroups: a tile's length on the line is its blocks rounded up to the share, and the share so small that
-//     the pieces are at most as many as workgroups: each has one piece;
-//   else: a tile's length is its blocks and some for what a tile costs besides, the share what all come to over the workgroups.
+// follows from the lengths, which are on the device.  The host chooses a number of workgroups, and each finds its own share from the lengths before it begins.
+//
+// All tiles lie on a line, request by request, head by head (what shares a head's keys and values runs beside each other, on one XCD, and finds them in its
+// L2), and the line is cut in equal shares:
+//   few tiles for the workgroups: a tile's length on the line is its request's most blocks rounded up to the share, and the share so small that the
+//     pieces are at most as many as workgroups: each has one piece;
+//   else: a tile's length is its blocks and some for what a tile costs besides.  Tile t's keys end bq / G tokens behind tile t - 1's, so lengths grow evenly up to what
+//     a window allows; taken as that (at least the tile's blocks), the place of any tile is a formula, and no list of tiles is needed.
 // A workgroup's share may begin and end inside a tile: there it leaves a partial result (O, m, l: the sum of the values, the reference in the
 // exponent's base of two, the denominator) instead of the tile's rows, one for the tile it does not begin (place 0) and one for the tile it
 // begins and does not end (place 1).  Who begins a tile and does not end it describes it for a last launch, which puts the pieces together in their order.  No
 // atomics: results do not depend on who is first.  Where a table holds so few keys that a workgroup does a request's head in some rounds, there is
-// one to each and nothing is dealt (`direct`).
-// (Pieces off a queue, whoever is free: no faster where memory bounds them -- of equal shares of a decoding step's keys the first was done after 115 us, the last
-// after 157, but whoever is done leaves its bandwidth to the others -- and slower where pieces are short.)
+// one to each and nothing is shared out (`direct`).
+//
+// Tried and left: the dealing in a launch of its own that notes every tile's place (9 us and a gap in front of a decoding step; here 3 us of the kernel); pieces off a
+// queue, whoever is free (no faster where memory bounds them: of equal shares of a decoding step's keys the first was done after 115 us, the last after
+// 157, but whoever is done leaves its bandwidth to the others; slower where pieces are short).
 #pragma once
 #include "attention.h"
 #include "paged.h"
@@ -22,37 +27,14 @@
 namespace mrl {
 namespace paged {
 
-constexpr uint32_t MOST_WORKERS = 1024;   // threads of the dealing's workgroup
-
-// What the dealing leaves in the workspace.
-struct Line {
-  uint64_t share;      // of each workgroup
-  uint32_t tiles;      // that are noted (of all heads together one)
-  uint32_t unused[5];
-};
-struct Start {         // of a workgroup's share: tile, head, place in the tile
-  uint32_t tile, head, at, unused;
-};
-struct Tile {
-  uint32_t request, row0, rows;      // rows row0 .. row0 + rows - 1 of the request
-  int32_t start, at;                 // the tensors' row of the request's token 0, and its place among the keys (may be below zero)
-  uint32_t begin, end;               // keys that some row sees lie in [begin, end)
-  uint32_t blocks, length;           // their blocks, and the tile's length on the line
-  uint32_t first, behind;            // tiles of its request (of those noted together): these follow each other once for every head
-  uint32_t unused[5];
-};
-
 struct Work {
   uint32_t min_rows, max_rows;   // requests of so many query rows; others' are left to another kernel
+  bool once;                     // no request is expected to have more than a tile: its keys and values are read once
   bool direct;                   // a workgroup to each (request, head): nothing is dealt
   uint32_t workers;
   uint32_t bq_log2, block_log2;  // of a tile's rows, of a block's keys
   uint32_t least;                // the least blocks that a tile is cut to where workgroups are to spare
   uint32_t overhead, second;     // what a tile costs besides its blocks, in blocks, where the chip has all it can do; what a second piece costs a workgroup that has no other
-  uint32_t most_tiles;           // that there is room to note
-  Line *line;
-  Start *starts;                 // [workers]
-  Tile *tiles;                   // [most_tiles]
   uint32_t *merges;              // [workers][8]: see describe()
   float *partials;               // [workers][2][rows of a tile][row_floats]
 };
@@ -72,6 +54,11 @@ __device__ inline const Kernargs &kernargs() {
   return *(const Kernargs *)s;
 }
 
+// attn::dma16_ordered for what is read once: it leaves the caches to others.
+__device__ inline void dma16_once(__amdgpu_buffer_rsrc_t from, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" : : "s"(lds_addr), "v"(voff), "s"(from) : "memory");
+}
+
 __device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline uint64_t uniform(uint64_t x) { return uint64_t(uniform(uint32_t(x >> 32))) << 32 | uniform(uint32_t(x)); }
@@ -89,65 +76,205 @@ __device__ inline Request read_request(const PagedAttnArgs &p, const Work &w, ui
   return q;
 }
 
-// The keys that a tile sees, and their blocks.
-__device__ inline Tile measure(const PagedAttnArgs &p, FastDiv by_group, const Request &q, uint32_t row0, uint32_t rows, uint32_t block_log2) {
-  Tile t = {};
-  const int32_t known = min(max(q.length, 0), int32_t(p.width * p.page_size));
+// One tile's piece, in scalar registers.
+struct Piece {
+  uint32_t request, head, row0, rows;   // rows row0 .. row0 + rows - 1 of the request, at key/value head `head`
+  int32_t start, at;                    // the tensors' row of the request's token 0, and its place among the keys (may be below zero)
+  uint32_t begin, end, blocks;          // keys that some row of the tile sees lie in [begin, end), in so many blocks
+  uint32_t b0, b1;                      // the piece's, counted from the one that holds `begin`
+  __device__ bool whole() const { return b0 == 0 && b1 == blocks; }
+};
+// Tile `tile` of a request, as a whole.
+__device__ inline Piece tile_of(const Kernargs &k, const Request &q, uint32_t tile) {
+  Piece t = {};
+  const uint32_t row0 = tile << k.w.bq_log2, rows = min(uint32_t(q.n) * k.p.group - row0, 1u << k.w.bq_log2);
+  const int32_t known = min(max(q.length, 0), int32_t(k.p.width * k.p.page_size));
   t.row0 = row0, t.rows = rows, t.start = q.start, t.at = int32_t(max(int64_t(q.length) - q.n, -(int64_t(1) << 30)));
-  const int64_t last = int64_t(t.at) + by_group.div(row0 + rows - 1), first = int64_t(t.at) + by_group.div(row0);
+  const int64_t last = int64_t(t.at) + k.by_group.div(row0 + rows - 1), first = int64_t(t.at) + k.by_group.div(row0);
   t.end = uint32_t(min(max(last + 1, int64_t(0)), int64_t(known)));
-  t.begin = p.window ? uint32_t(min(max(first - int64_t(p.window) + 1, int64_t(0)), int64_t(t.end))) : 0;
-  t.blocks = t.end > t.begin ? ((t.end - 1) >> block_log2) - (t.begin >> block_log2) + 1 : 0;
+  t.begin = k.p.window ? uint32_t(min(max(first - int64_t(k.p.window) + 1, int64_t(0)), int64_t(t.end))) : 0;
+  t.blocks = t.b1 = t.end > t.begin ? ((t.end - 1) >> k.w.block_log2) - (t.begin >> k.w.block_log2) + 1 : 0;
   return t;
 }
 
 // floor(x / y) for x < 2^52 and a quotient below 2^32 (a quotient that is no whole number is at least 1 / y off one: more than a rounding in 64 bits).
 __device__ inline uint32_t quotient(uint64_t x, uint64_t y) { return uint32_t(double(x) / double(y)); }
 
-// One tile's piece, in scalar registers.
-struct Piece {
-  uint32_t request, head, row0, rows;
-  int32_t start, at;
-  uint32_t begin, end, blocks;
-  uint32_t b0, b1;   // its blocks, counted from the one that holds `begin`
-  __device__ bool whole() const { return b0 == 0 && b1 == blocks; }
-};
+// A request's tiles on the line, of one head.
+struct Lengths {
+  uint32_t tiles;
+  uint32_t first, slope, most, grown;   // tile t: first + t * slope / 256 for t below `grown`, then `most`; in the few tiles' way `most` for all
 
-// A workgroup's way along its share of the line; everybody calls it.
-struct Worker {
-  uint32_t number = xcd_run(blockIdx.x, gridDim.x);
-  uint32_t tile, head, at;   // where it stands
-  uint32_t left;             // of its share
-  bool described = false;
-
-  __device__ Worker(const Work &w) {
-    const volatile Start *s = w.starts + number;
-    tile = uniform(s->tile), head = uniform(s->head), at = uniform(s->at), left = uniform(uint32_t(w.line->share));
+  __device__ uint64_t before(uint32_t t) const {   // of the tiles before tile t
+    const uint64_t x = min(t, grown);
+    return x * first + ((x * (x - (x != 0)) / 2 * slope) >> 8) + uint64_t(t - uint32_t(x)) * most;
   }
+  __device__ uint32_t of(uint32_t t) const { return uint32_t(before(t + 1) - before(t)); }
+  __device__ uint64_t all() const { return before(tiles); }
+  // The tile that holds place x.
+  __device__ uint32_t tile_at(uint64_t x) const {
+    uint32_t lo = 0, hi = tiles;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (before(mid) <= x) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  }
+};
+// A tile has at most (keys it sees) / 2^block_log2 + 2 blocks, and tile t sees at most at + (t + 1) * bq / G + 1 keys, or window + bq / G + 1.
+// (Two more, as the eighths of `slope` are rounded where they are summed.)
+__device__ inline Lengths lengths_of(const Kernargs &k, const Request &q) {
+  Lengths l;
+  const uint32_t bq = 1u << k.w.bq_log2, step = bq / k.p.group + 1, more = 4 + k.w.overhead;
+  const uint32_t at = uint32_t(min(max(int64_t(q.length) - q.n, int64_t(0)), int64_t(k.p.width * k.p.page_size)));
+  l.tiles = (uint32_t(q.n) * k.p.group + bq - 1) >> k.w.bq_log2;
+  l.slope = ((bq * 256 / k.p.group) >> k.w.block_log2) + 1;
+  l.first = (uint32_t((uint64_t(at) + step) >> k.w.block_log2)) + more;
+  l.grown = 0xffffffffu, l.most = 0;
+  if (k.p.window) {
+    l.most = uint32_t((uint64_t(k.p.window) + step) >> k.w.block_log2) + more;
+    l.grown = l.first >= l.most ? 0 : quotient(uint64_t(l.most - l.first) * 256, l.slope) + 1;
+  }
+  return l;
+}
+// In the few tiles' way, each as long as the longest can be.
+__device__ inline uint32_t most_blocks(const Kernargs &k, const Request &q, uint32_t tiles) {
+  const Piece last = tile_of(k, q, tiles - 1);
+  if (tiles == 1) return max(last.blocks, 1u);
+  return k.p.window ? min(((last.end + 1) >> k.w.block_log2) + 2, uint32_t((uint64_t(k.p.window) + (1u << k.w.bq_log2) / k.p.group + 1) >> k.w.block_log2) + 2)
+                    : max(last.blocks, 1u);
+}
+
+// A workgroup's way along its share of the line; everybody calls it.  TH: threads of the workgroup.
+template <int TH>
+struct Worker {
+  struct Shared {
+    uint64_t sums[3][TH / 64];
+    uint32_t found[4];
+  };
+  uint32_t number = xcd_run(blockIdx.x, gridDim.x);
+  uint32_t request = 0xffffffffu, head = 0, tile = 0, at = 0;   // where it stands
+  uint32_t share = 1, left = 0;
+  bool few = false, described = false;
+
+  __device__ Lengths lengths(const Kernargs &k, const Request &q) const {
+    Lengths l = lengths_of(k, q);
+    if (few) l.grown = 0, l.most = quotient(uint64_t(most_blocks(k, q, l.tiles)) + share - 1, share) * share;
+    return l;
+  }
+
+  // Finds its start; `sh` is free again behind the caller's next barrier.
+  __device__ Worker(const Kernargs &k, Shared *sh) {
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const uint64_t heads = k.p.kv_heads, workers = k.w.workers;
+    // How many tiles, how long the line, how many blocks in the few tiles' way.
+    uint64_t tiles = 0, line = 0, blocks = 0;
+    Request q = {0, 0, 0};
+    for (uint32_t r = tid; r < k.p.requests; r += TH) {
+      q = read_request(k.p, k.w, r);
+      if (!q.n) continue;
+      const Lengths l = lengths_of(k, q);
+      tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(k, q, l.tiles);
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) tiles += __shfl_xor(tiles, d), line += __shfl_xor(line, d), blocks += __shfl_xor(blocks, d);
+    if (lane == 0) sh->sums[0][wave] = tiles, sh->sums[1][wave] = line, sh->sums[2][wave] = blocks;
+    if (tid == 0) sh->found[0] = 0xffffffffu;
+    __syncthreads();
+    tiles = line = blocks = 0;
+#pragma unroll
+    for (int i = 0; i < TH / 64; i++) tiles += sh->sums[0][i], line += sh->sums[1][i], blocks += sh->sums[2][i];
+    tiles = uniform(tiles) * heads, line = uniform(line) * heads, blocks = uniform(blocks) * heads;
+    share = max(quotient(line + workers - 1, workers), 1u);
+    if (tiles < workers) {   // a piece to each, where that is no longer than equal shares and the second piece that they may come to
+      const uint32_t spare = uint32_t(workers - tiles), single = max((quotient(blocks + spare - 1, spare) + k.w.least - 1) / k.w.least, 1u) * k.w.least;
+      few = single <= share + k.w.second;
+      if (few) share = single;
+    }
+    // The request that holds its start.
+    const uint64_t from = uint64_t(share) * number;
+    uint64_t base = 0;
+    for (uint32_t r0 = 0; r0 < k.p.requests; r0 += TH) {
+      if (k.p.requests > TH) {
+        q = {0, 0, 0};
+        if (r0 + tid < k.p.requests) q = read_request(k.p, k.w, r0 + tid);
+      }
+      Lengths l = {};
+      uint64_t mine = 0;
+      if (q.n) l = lengths(k, q), mine = l.all();
+      uint64_t sum = mine * heads;
+      const uint64_t all_mine = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint64_t below = __shfl_up(sum, d);
+        if (lane >= d) sum += below;
+      }
+      __syncthreads();   // (the sums before have been read)
+      if (lane == 63) sh->sums[0][wave] = sum;
+      __syncthreads();
+      uint64_t off = base, all = 0;
+#pragma unroll
+      for (int i = 0; i < TH / 64; i++) {
+        const uint64_t x = sh->sums[0][i];
+        if (i < int(wave)) off += x;
+        all += x;
+      }
+      off += sum - all_mine;
+      if (q.n && from >= off && from < off + all_mine) {
+        const uint32_t h = quotient(from - off, mine);
+        const uint64_t in_head = from - off - h * mine;
+        const uint32_t t = l.tile_at(in_head);
+        sh->found[0] = r0 + tid, sh->found[1] = h, sh->found[2] = t, sh->found[3] = uint32_t(in_head - l.before(t));
+      }
+      base += uniform(all);
+      if (from < base) break;
+    }
+    __syncthreads();
+    request = uniform(sh->found[0]), head = uniform(sh->found[1]), tile = uniform(sh->found[2]), at = uniform(sh->found[3]);
+    left = request < k.p.requests ? share : 0;
+  }
+
   // The next piece that has something to do; false: there is none.
   __device__ bool next(const Kernargs &k, Piece *out) {
-    const uint32_t tiles = uniform(k.w.line->tiles);
-    while (left && tile < tiles) {
-      const volatile Tile *t = k.w.tiles + tile;
-      const uint32_t blocks = uniform(t->blocks), length = uniform(t->length), first = uniform(t->first), behind = uniform(t->behind);
-      out->request = uniform(t->request), out->head = head, out->row0 = uniform(t->row0), out->rows = uniform(t->rows), out->start = uniform(int32_t(t->start));
-      out->at = uniform(int32_t(t->at)), out->begin = uniform(t->begin), out->end = uniform(t->end), out->blocks = blocks;
-      out->b0 = min(at, blocks), out->b1 = min(at + min(left, length - at), blocks);
-      const bool any = out->b0 < out->b1 || (blocks == 0 && at == 0);
+    while (left) {
+      Request q = read_request(k.p, k.w, request);
+      q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
+      const Lengths l = lengths(k, q);
+      const uint32_t length = uniform(l.of(tile));
+      Piece t = tile_of(k, q, tile);
+      t.request = request, t.head = head, t.b0 = min(at, t.blocks), t.b1 = min(at + min(left, length - at), t.blocks);
+      const bool any = t.b0 < t.b1 || (t.blocks == 0 && at == 0);
       left -= min(left, length - at), at = 0, tile++;
-      if (tile == behind && head + 1 < k.p.kv_heads) tile = first, head++;
-      else if (tile == behind) head = 0;
-      if (any) return true;
+      if (tile == l.tiles) {
+        tile = 0, head++;
+        if (head == k.p.kv_heads && left) {   // the next request of this kernel's
+          head = 0;
+          const uint32_t lane = threadIdx.x & 63;
+          uint64_t some = 0;
+          for (request++; request < k.p.requests; request += 64) {
+            some = __ballot(request + lane < k.p.requests && read_request(k.p, k.w, min(request + lane, k.p.requests - 1)).n != 0);
+            if (some) break;
+          }
+          if (some) request += __builtin_ctzll(some);
+          else left = 0;
+        }
+      }
+      if (any) {
+        *out = t;
+        out->start = uniform(t.start), out->at = uniform(t.at), out->begin = uniform(t.begin), out->end = uniform(t.end), out->blocks = uniform(t.blocks);
+        out->b0 = uniform(t.b0), out->b1 = uniform(t.b1), out->row0 = uniform(t.row0), out->rows = uniform(t.rows);
+        return true;
+      }
     }
     return false;
   }
   // Where a piece that is not its tile leaves its partial result.
   __device__ float *place(const Work &w, const Piece &t, uint32_t piece_floats) const { return w.partials + (uint64_t(number) * 2 + (t.b0 == 0)) * piece_floats; }
-  // By one thread, of a tile that this workgroup begins and others end: how many of them, and which rows.  Its last block lies `b1 .. blocks` behind this share's end, but
-  // for the last share's.
+  // By one thread, of a tile that this workgroup begins and others end: how many of them, and which rows.  (Its share ends behind block b1 - 1.)
   __device__ void describe(const Work &w, const Piece &t) const {
     uint32_t *d = w.merges + number * 8;
-    d[0] = 1 + quotient(t.blocks - 1 - t.b1, w.line->share), d[1] = uint32_t(t.start), d[2] = t.row0, d[3] = t.rows, d[4] = t.head;
+    d[0] = 1 + (t.blocks - 1 - t.b1) / share, d[1] = uint32_t(t.start), d[2] = t.row0, d[3] = t.rows, d[4] = t.head;
   }
 };
 
@@ -157,8 +284,8 @@ __device__ inline bool direct_piece(const Kernargs &k, Piece *out) {
   Request q = read_request(k.p, k.w, request);
   q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
   if (!q.n) return false;
-  const Tile t = measure(k.p, k.by_group, q, 0, uint32_t(q.n) * k.p.group, k.w.block_log2);
-  *out = {request, worker - request * k.p.kv_heads, t.row0, t.rows, t.start, t.at, t.begin, t.end, t.blocks, 0, t.blocks};
+  *out = tile_of(k, q, 0);
+  out->request = request, out->head = worker - request * k.p.kv_heads;
   return true;
 }
 

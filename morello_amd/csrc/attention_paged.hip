@@ -103,132 +103,6 @@ hipError_t launch_generic(const PagedAttnArgs &a, hipStream_t stream) {
   return plan::last_error();
 }
 
-// ---- Dealing: the tiles on a line, its shares (attention_paged.h). ----
-struct DealArgs {
-  PagedAttnArgs p;
-  FastDiv by_group;
-  paged::Work work[2];   // a workgroup to each
-};
-constexpr int DEAL = int(paged::MOST_WORKERS), DEAL_WAVES = DEAL / 64;
-
-// x: the sum over the threads before this one; returns the sum over all.
-__device__ inline uint64_t scan(uint64_t &x, uint64_t *wave_sums) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t sum = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t below = __shfl_up(sum, d);
-    if (lane >= d) sum += below;
-  }
-  __syncthreads();   // (the sums of the scan before have been read)
-  if (lane == 63) wave_sums[wave] = sum;
-  __syncthreads();
-  uint64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < DEAL_WAVES; w++) {
-    if (w < wave) before += wave_sums[w];
-    all += wave_sums[w];
-  }
-  x = before + sum - x;
-  return all;
-}
-// The last of 1024 ascending numbers that is at most x (the first one is).
-template <class N>
-__device__ inline uint32_t last_up_to(const N *numbers, N x) {
-  uint32_t lo = 0;
-#pragma unroll
-  for (uint32_t step = DEAL / 2; step; step /= 2)
-    if (numbers[lo + step] <= x) lo += step;
-  return lo;
-}
-
-// Requests 1024 at a time, their tiles 1024 at a time, a thread each; once for how much there is (and once more where that was more than one such chunk), then to note them.
-// Of a chunk, request r's tiles lie at heads * (lengths of the tiles before r's) + head * (lengths of r's) + (lengths of r's before it).
-__global__ __launch_bounds__(DEAL) void k_paged_attn_deal(DealArgs a) {
-  using namespace paged;
-  __shared__ uint64_t wave_sums[DEAL_WAVES];
-  __shared__ uint32_t first[DEAL], tiles_of[DEAL];          // of a request: its first tile in the chunk of requests, how many
-  __shared__ int32_t n_of[DEAL], start_of[DEAL], length_of[DEAL];
-  __shared__ uint64_t line[DEAL + 1];                       // lengths of the chunk's tiles before a tile
-  __shared__ uint32_t request_of[DEAL];
-  const Work &w = a.work[blockIdx.x];
-  const uint32_t tid = threadIdx.x, heads = a.p.kv_heads;
-  uint32_t r0 = 0, t0 = 0, tiles = 0, left = 0, request = 0, noted = 0;
-  Tile t = {};
-  // The next chunk: a tile to a thread (t.rows = 0: none).
-  auto next_chunk = [&](bool start) {
-    if (start) r0 = t0 = tiles = 0, left = w.most_tiles;   // (starts that do not fall never come to more; others are cut off here)
-    else t0 += DEAL;
-    while (t0 >= tiles) {
-      if (!start) r0 += DEAL;
-      start = false;
-      if (r0 >= a.p.requests || !left) return false;
-      Request q = {0, 0, 0};
-      if (r0 + tid < a.p.requests) q = read_request(a.p, w, r0 + tid);
-      const uint32_t mine = (uint32_t(q.n) * a.p.group + (1u << w.bq_log2) - 1) >> w.bq_log2;
-      uint64_t at = mine;
-      tiles = uint32_t(min(scan(at, wave_sums), uint64_t(left))), t0 = 0, left -= tiles;
-      first[tid] = uint32_t(at), tiles_of[tid] = mine, n_of[tid] = q.n, start_of[tid] = q.start, length_of[tid] = q.length;
-      __syncthreads();
-    }
-    t.rows = 0, t.blocks = 0;
-    if (t0 + tid < tiles) {
-      request = last_up_to(first, t0 + tid);
-      const Request q = {n_of[request], start_of[request], length_of[request]};
-      const uint32_t row0 = (t0 + tid - first[request]) << w.bq_log2;
-      t = measure(a.p, a.by_group, q, row0, min(uint32_t(q.n) * a.p.group - row0, 1u << w.bq_log2), w.block_log2);
-    }
-    return true;
-  };
-  uint64_t sum_tiles = 0, sum_blocks = 0;
-  uint32_t chunks = 0;
-  for (bool more = next_chunk(true); more; more = next_chunk(false)) {
-    sum_tiles += t.rows != 0, sum_blocks += t.blocks, chunks++;
-    if (tiles <= DEAL && a.p.requests <= DEAL) break;
-  }
-  const uint64_t all_tiles = scan(sum_tiles, wave_sums) * heads, all_blocks = scan(sum_blocks, wave_sums) * heads, workers = w.workers;
-  uint64_t share = quotient(all_blocks + all_tiles * (1 + w.overhead) + workers - 1, workers);
-  bool few = false;
-  if (all_tiles < workers) {   // a piece to each, where that is no longer than equal shares and the second piece that they may come to
-    const uint32_t spare = uint32_t(workers - all_tiles), single = max((quotient(all_blocks + spare - 1, spare) + w.least - 1) / w.least, 1u) * w.least;
-    few = single <= share + w.second;
-    if (few) share = single;
-  }
-  share = max(share, uint64_t(1));
-  uint64_t base = 0;   // of the chunk, on the line
-  const uint64_t my_start = share * tid;
-  bool open = tid < w.workers;   // this workgroup's start is not found yet
-  const bool again = !(chunks == 1 && tiles <= DEAL && a.p.requests <= DEAL);
-  for (bool more = again ? next_chunk(true) : chunks == 1; more; more = again && next_chunk(false)) {
-    if (t.rows) t.length = few ? (quotient(max(t.blocks, 1u) + share - 1, share)) * uint32_t(share) : t.blocks + 1 + w.overhead;
-    uint64_t at = t.rows ? t.length : 0;
-    const uint64_t all = scan(at, wave_sums);   // (its barriers: what the chunk before noted has been read)
-    line[tid] = at, request_of[tid] = request;
-    if (tid == 0) line[DEAL] = all;
-    __syncthreads();
-    const uint32_t count = min(tiles - t0, uint32_t(DEAL));
-    if (t.rows) {
-      t.request = r0 + request;
-      t.first = noted + max(first[request], t0) - t0, t.behind = noted + min(first[request] + tiles_of[request] - t0, count);
-      w.tiles[noted + tid] = t;
-    }
-    if (open && my_start < base + all * heads) {
-      const uint64_t here = my_start - base;
-      const uint32_t of = request_of[last_up_to(line, uint64_t(quotient(here, heads)))];
-      const uint32_t lo = max(first[of], t0) - t0, hi = min(first[of] + tiles_of[of] - t0, count);
-      const uint64_t rest = here - line[lo] * heads, each = line[hi] - line[lo];
-      const uint32_t head = quotient(rest, each);
-      const uint64_t in_head = line[lo] + (rest - head * each);
-      const uint32_t x = last_up_to(line, in_head);
-      w.starts[tid] = {noted + x, head, uint32_t(in_head - line[x]), 0};
-      open = false;
-    }
-    base += all * heads, noted += count;
-  }
-  if (open) w.starts[tid] = {0xffffffffu, 0, 0, 0};
-  if (tid == 0) w.line->share = share, w.line->tiles = noted;
-}
-
 // ---- Tiles in pieces: out = sum_v O_v 2^(m_v - M) / sum_v l_v 2^(m_v - M), M the largest m_v, over the pieces in their order (the parts formula of
 // morello/src/spec.rs:107-132 in base 2). ----
 struct MergeArgs {
@@ -303,24 +177,17 @@ struct Choice {
   bool tiled = false;                 // else the generic kernel
   int qb = 0;                         // 0: no tiles of 16 or 32 rows
   paged::Work keys = {}, chunk = {};  // workers = 0: none of them
-  size_t keys_at[5] = {}, chunk_at[5] = {}, bytes = 0;   // what the Work points at, in the workspace; all of it
+  size_t keys_at = 0, chunk_at = 0, bytes = 0;   // partial results in the workspace, descriptions behind them; all of it
 };
 
-void lay_out(const PagedAttnArgs &a, paged::Work &w, size_t *at, size_t *bytes) {
-  const uint64_t bq = uint64_t(1) << w.bq_log2;
-  w.most_tiles = uint32_t(((uint64_t(a.tokens) * a.group + bq - 1) >> w.bq_log2) + a.requests);
-  auto take = [&](size_t n) {
-    const size_t from = *bytes;
-    *bytes += (n + 255) & ~size_t(255);
-    return from;
-  };
-  at[0] = take(sizeof(paged::Line)), at[1] = take(w.workers * sizeof(paged::Start)), at[2] = take(w.most_tiles * sizeof(paged::Tile)), at[3] = take(w.workers * 32);
-  at[4] = take(2 * w.workers * bq * paged::row_floats(a) * sizeof(float));
+size_t partial_bytes(const PagedAttnArgs &a, const paged::Work &w) { return (size_t(2 * w.workers) << w.bq_log2) * paged::row_floats(a) * sizeof(float); }
+size_t take(const PagedAttnArgs &a, const paged::Work &w, size_t *bytes) {
+  const size_t at = *bytes;
+  *bytes += partial_bytes(a, w) + w.workers * 32;
+  return at;
 }
-void place(paged::Work &w, const size_t *at, uint8_t *workspace) {
-  w.line = reinterpret_cast<paged::Line *>(workspace + at[0]), w.starts = reinterpret_cast<paged::Start *>(workspace + at[1]);
-  w.tiles = reinterpret_cast<paged::Tile *>(workspace + at[2]), w.merges = reinterpret_cast<uint32_t *>(workspace + at[3]);
-  w.partials = reinterpret_cast<float *>(workspace + at[4]);
+void place(const PagedAttnArgs &a, paged::Work &w, size_t at) {
+  w.partials = reinterpret_cast<float *>(a.workspace + at), w.merges = reinterpret_cast<uint32_t *>(a.workspace + at + partial_bytes(a, w));
 }
 
 Choice choose(const PagedAttnArgs &a) {
@@ -342,29 +209,18 @@ Choice choose(const PagedAttnArgs &a) {
   if (c.qb) {
     paged::Work &w = c.keys;
     paged::keys_work(a, c.qb, &w);
-    w.min_rows = 1, w.max_rows = chunk ? 16 : 0x7fffffff;
+    w.min_rows = 1, w.max_rows = chunk ? 16 : 0x7fffffff, w.once = chunk || rows <= 16u * c.qb;
     // Tables of some hundred keys at most: a workgroup to each request and head does them in some rounds, with nothing to find out before and no launch behind.
-    // (max_new is the program's word: a request of more tokens would have more tiles than one)
+    // (max_new is the program's word: a request of more tokens would have more tiles than one, unless all rows there are make no second one)
     w.direct = !chunk && uint64_t(a.tokens) * a.group <= 16u * c.qb && uint64_t(a.width) * a.page_size <= DIRECT_KEYS;
-    if (!w.direct) lay_out(a, w, c.keys_at, &c.bytes);
+    if (!w.direct) c.keys_at = take(a, w, &c.bytes);
   }
   if (chunk) {
     paged::chunk_work(a, &c.chunk);
     c.chunk.min_rows = c.qb ? 17 : 1, c.chunk.max_rows = 0x7fffffff;
-    lay_out(a, c.chunk, c.chunk_at, &c.bytes);
+    c.chunk_at = take(a, c.chunk, &c.bytes);
   }
   return c;
-}
-
-hipError_t launch_deal(const PagedAttnArgs &a, const Choice &c, hipStream_t stream) {
-  DealArgs d;
-  d.p = a, d.by_group = FastDiv(a.group);
-  int n = 0;
-  if (c.chunk.workers) d.work[n++] = c.chunk;
-  if (c.keys.workers) d.work[n++] = c.keys;
-  plan::work(plan::UNIT_STREAM, 0, 12.0 * a.requests + 64.0 * (c.chunk.most_tiles + c.keys.most_tiles));
-  MRL_LAUNCH(k_paged_attn_deal, dim3(n), dim3(DEAL), 0, stream, d);
-  return plan::last_error();
 }
 
 template <class T>
@@ -389,9 +245,9 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream) {
   if (!c.tiled || !aligned(a.q) || !aligned(a.keys) || !aligned(a.values) || !aligned(a.out))
     return bf16 ? launch_generic<u16>(a, stream) : launch_generic<float>(a, stream);
   if (c.keys.direct) return paged::launch_keys(a, c.keys, c.qb, stream);
-  place(c.keys, c.keys_at, a.workspace), place(c.chunk, c.chunk_at, a.workspace);
-  hipError_t e = launch_deal(a, c, stream);
-  if (e == hipSuccess && c.chunk.workers) e = paged::launch_chunk(a, c.chunk, stream);
+  place(a, c.keys, c.keys_at), place(a, c.chunk, c.chunk_at);
+  hipError_t e = hipSuccess;
+  if (c.chunk.workers) e = paged::launch_chunk(a, c.chunk, stream);
   if (e == hipSuccess && c.keys.workers) e = paged::launch_keys(a, c.keys, c.qb, stream);
   if (e != hipSuccess) return e;
   return bf16 ? launch_merge<u16>(a, c, stream) : launch_merge<float>(a, c, stream);

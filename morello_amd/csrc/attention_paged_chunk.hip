@@ -70,7 +70,8 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
   };
 
-  Worker worker(kernargs().w);
+  Worker<TH> worker(kernargs(), reinterpret_cast<Worker<TH>::Shared *>(lds));
+  __syncthreads();
   Piece t;
   while (worker.next(kernargs(), &t)) {
     const Kernargs &k = kernargs();
@@ -491,7 +492,7 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
 }  // namespace
 
 void chunk_work(const PagedAttnArgs &, Work *w) {
-  w->workers = std::min(MOST_WORKERS, g_compute_units);   // (one of D = 128 to a compute unit's LDS)
+  w->workers = g_compute_units;   // (one of D = 128 to a compute unit's LDS)
   w->bq_log2 = 7, w->block_log2 = 6, w->least = 8, w->overhead = 7, w->second = 7;
 }
 

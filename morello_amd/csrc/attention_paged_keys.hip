@@ -99,10 +99,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
   constexpr int ALL_BUT_ONE_TILE = 0x0F70 | (LOADS & 15) | ((LOADS >> 4) << 14), ALL = 0x0F70, READS_DONE = 0xC07F;
 
   const bool direct = kernargs().w.direct;
-  auto run = [&](const Kernargs &k, const Piece &t, Worker *worker) {
+  auto run = [&](const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
     const float c = k.c;
     const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
     const uint32_t group = k.p.group, window = k.p.window, first_block = t.begin / KEYS + t.b0 + wave;
+    const bool once = k.w.once;
     const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();   // a score that weighs nothing
 
     // This lane's rows: queries, and the keys they see, [lo, hi].
@@ -150,8 +151,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
         const uint32_t rows = page < 0 || from >= t.end ? 0 : min(t.end - from, 16u);
         const uint64_t base = reinterpret_cast<uint64_t>(head) + uint64_t(max(page, 0)) * page_bytes + uint64_t(place) * slot_bytes;
         const auto from_buf = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(base)), 0, uniform(int(rows ? (rows - 1) * slot_bytes + row_bytes : 0)), 0x00020000);
+        if (once) {
 #pragma unroll
-        for (int i = 0; i < HALF; i++) dma16_ordered(from_buf, src[i], dst + (half * HALF + i) * 1024);
+          for (int i = 0; i < HALF; i++) dma16_once(from_buf, src[i], dst + (half * HALF + i) * 1024);
+        } else {
+#pragma unroll
+          for (int i = 0; i < HALF; i++) dma16_ordered(from_buf, src[i], dst + (half * HALF + i) * 1024);
+        }
       }
     };
     const uint8_t *const key_head = (const uint8_t *)k.p.keys + int64_t(t.head) * k.p.key_h * int64_t(sizeof(T));
@@ -440,7 +446,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
     if (direct_piece(kernargs(), &t)) run(kernargs(), t, nullptr);
     return;
   }
-  Worker worker(kernargs().w);
+  Worker<64 * W> worker(kernargs(), reinterpret_cast<typename Worker<64 * W>::Shared *>(lds));
+  __syncthreads();
   while (worker.next(kernargs(), &t)) {
     run(kernargs(), t, &worker);
     __syncthreads();   // (the triples have been read)
@@ -483,7 +490,7 @@ hipError_t launch_form(Form<T, D, QB, W>, const PagedAttnArgs &a, const Work &wo
 }  // namespace
 
 void keys_work(const PagedAttnArgs &a, int qb, Work *w) {
-  w->workers = std::min(MOST_WORKERS, g_compute_units * with_form(a, qb, [](auto f) { return uint32_t(decltype(f)::RESIDENT); }));
+  w->workers = g_compute_units * with_form(a, qb, [](auto f) { return uint32_t(decltype(f)::RESIDENT); });
   w->bq_log2 = qb == 1 ? 4 : 5, w->block_log2 = 5, w->least = WAVES, w->overhead = 3, w->second = 3 * WAVES;
 }
 
