@@ -28,7 +28,6 @@ namespace mrl {
 namespace paged {
 
 struct Work {
-  uint32_t min_rows, max_rows;   // requests of so many query rows; others' are left to another kernel
   bool once;                     // no request is expected to have more than a tile: its keys and values are read once
   bool direct;                   // a workgroup to each (request, head): nothing is dealt
   uint32_t workers;
@@ -63,17 +62,14 @@ __device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfir
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline uint64_t uniform(uint64_t x) { return uint64_t(uniform(uint32_t(x >> 32))) << 32 | uniform(uint32_t(x)); }
 
-// A request: its new tokens (0: none of this kernel's), their first row, and its length.
+// A request: its new tokens, their first row, and its length.
 struct Request {
   int32_t n, start, length;
 };
-__device__ inline Request read_request(const PagedAttnArgs &p, const Work &w, uint32_t r) {
+__device__ inline Request read_request(const PagedAttnArgs &p, uint32_t r) {
   const int32_t most = int32_t(p.tokens);
   const int32_t s0 = min(max(p.starts[r], 0), most), s1 = min(max(p.starts[r + 1], 0), most);
-  Request q = {max(s1 - s0, 0), s0, p.lengths[r]};
-  const uint32_t rows = uint32_t(q.n) * p.group;
-  if (rows < w.min_rows || rows > w.max_rows) q.n = 0;
-  return q;
+  return {max(s1 - s0, 0), s0, p.lengths[r]};
 }
 
 // One tile's piece, in scalar registers.
@@ -172,7 +168,7 @@ struct Worker {
     uint64_t tiles = 0, line = 0, blocks = 0;
     Request q = {0, 0, 0};
     for (uint32_t r = tid; r < k.p.requests; r += TH) {
-      q = read_request(k.p, k.w, r);
+      q = read_request(k.p, r);
       if (!q.n) continue;
       const Lengths l = lengths_of(k, q);
       tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(k, q, l.tiles);
@@ -198,7 +194,7 @@ struct Worker {
     for (uint32_t r0 = 0; r0 < k.p.requests; r0 += TH) {
       if (k.p.requests > TH) {
         q = {0, 0, 0};
-        if (r0 + tid < k.p.requests) q = read_request(k.p, k.w, r0 + tid);
+        if (r0 + tid < k.p.requests) q = read_request(k.p, r0 + tid);
       }
       Lengths l = {};
       uint64_t mine = 0;
@@ -238,7 +234,7 @@ struct Worker {
   // The next piece that has something to do; false: there is none.
   __device__ bool next(const Kernargs &k, Piece *out) {
     while (left) {
-      Request q = read_request(k.p, k.w, request);
+      Request q = read_request(k.p, request);
       q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
       const Lengths l = lengths(k, q);
       const uint32_t length = uniform(l.of(tile));
@@ -248,12 +244,12 @@ struct Worker {
       left -= min(left, length - at), at = 0, tile++;
       if (tile == l.tiles) {
         tile = 0, head++;
-        if (head == k.p.kv_heads && left) {   // the next request of this kernel's
+        if (head == k.p.kv_heads && left) {   // the next request with new tokens
           head = 0;
           const uint32_t lane = threadIdx.x & 63;
           uint64_t some = 0;
           for (request++; request < k.p.requests; request += 64) {
-            some = __ballot(request + lane < k.p.requests && read_request(k.p, k.w, min(request + lane, k.p.requests - 1)).n != 0);
+            some = __ballot(request + lane < k.p.requests && read_request(k.p, min(request + lane, k.p.requests - 1)).n != 0);
             if (some) break;
           }
           if (some) request += __builtin_ctzll(some);
@@ -281,7 +277,7 @@ struct Worker {
 // In a `direct` launch: the workgroup's one tile, as a whole; false: it has none.
 __device__ inline bool direct_piece(const Kernargs &k, Piece *out) {
   const uint32_t worker = xcd_run(blockIdx.x, gridDim.x), request = worker / k.p.kv_heads;
-  Request q = read_request(k.p, k.w, request);
+  Request q = read_request(k.p, request);
   q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
   if (!q.n) return false;
   *out = tile_of(k, q, 0);

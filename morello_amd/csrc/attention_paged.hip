@@ -106,12 +106,9 @@ hipError_t launch_generic(const PagedAttnArgs &a, hipStream_t stream) {
 // ---- Tiles in pieces: out = sum_v O_v 2^(m_v - M) / sum_v l_v 2^(m_v - M), M the largest m_v, over the pieces in their order (the parts formula of
 // morello/src/spec.rs:107-132 in base 2). ----
 struct MergeArgs {
-  struct {
-    const uint32_t *merges;
-    const float *partials;
-    uint32_t workers, bq;
-  } of[2];
-  uint32_t row_floats;
+  const uint32_t *merges;
+  const float *partials;
+  uint32_t bq, row_floats;   // rows of a tile
   FastDiv by_group, by_quads;
 };
 // U: pieces asked for at a time.
@@ -156,15 +153,14 @@ __device__ inline void merge_rows(const PagedAttnArgs &p, const MergeArgs &a, co
     }
   }
 }
-// blockIdx.x: the workgroup that begins the tile, those of the first kernel before those of the second; blockIdx.y: a share of its rows.
+// blockIdx.x: the workgroup that begins the tile; blockIdx.y: a share of its rows.
 template <class T>
 __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
-  const uint32_t second = blockIdx.x >= a.of[0].workers, worker = blockIdx.x - (second ? a.of[0].workers : 0);
-  const uint32_t *d = a.of[second].merges + worker * 8;
-  const uint32_t piece_floats = a.of[second].bq * a.row_floats, more = d[0], row0 = d[2], rows = d[3], kv = d[4];
+  const uint32_t *d = a.merges + blockIdx.x * 8;
+  const uint32_t piece_floats = a.bq * a.row_floats, more = d[0], row0 = d[2], rows = d[3], kv = d[4];
   const int32_t start = int32_t(d[1]);
   if (!more) return;
-  const float *const partials = a.of[second].partials + 2 * uint64_t(worker) * piece_floats;
+  const float *const partials = a.partials + 2 * uint64_t(blockIdx.x) * piece_floats;
   if (more < 2) merge_rows<T, 2>(p, a, partials, more, piece_floats, start, row0, rows, kv);
   else if (more < 4) merge_rows<T, 4>(p, a, partials, more, piece_floats, start, row0, rows, kv);
   else merge_rows<T, 16>(p, a, partials, more, piece_floats, start, row0, rows, kv);
@@ -172,65 +168,53 @@ __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, M
 
 constexpr uint32_t DIRECT_KEYS = 1024;
 
-// How a call runs, by sizes, types and strides: on tiles of 16 * qb rows, of 128, or small requests on the former and the others on the latter.
+// How a call runs, by sizes, types and strides.
 struct Choice {
-  bool tiled = false;                 // else the generic kernel
-  int qb = 0;                         // 0: no tiles of 16 or 32 rows
-  paged::Work keys = {}, chunk = {};  // workers = 0: none of them
-  size_t keys_at = 0, chunk_at = 0, bytes = 0;   // partial results in the workspace, descriptions behind them; all of it
+  bool tiled = false;        // else the generic kernel
+  int qb = 0;                // on tiles of 16 * qb rows; 0: of 128
+  paged::Work work = {};
+  size_t partial_bytes = 0, bytes = 0;   // of partial results in the workspace, of all of it (the descriptions lie behind)
 };
-
-size_t partial_bytes(const PagedAttnArgs &a, const paged::Work &w) { return (size_t(2 * w.workers) << w.bq_log2) * paged::row_floats(a) * sizeof(float); }
-size_t take(const PagedAttnArgs &a, const paged::Work &w, size_t *bytes) {
-  const size_t at = *bytes;
-  *bytes += partial_bytes(a, w) + w.workers * 32;
-  return at;
-}
-void place(const PagedAttnArgs &a, paged::Work &w, size_t at) {
-  w.partials = reinterpret_cast<float *>(a.workspace + at), w.merges = reinterpret_cast<uint32_t *>(a.workspace + at + partial_bytes(a, w));
-}
 
 Choice choose(const PagedAttnArgs &a) {
   Choice c;
   const int size = a.dtype == MRL_BF16 ? 2 : 4;
   auto chunks = [&](int64_t n) { return n * size % 16 == 0; };
   const double scale = std::fabs(a.scale);
-  // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, 16 slots of a page within what an offset of 31 bits reaches; a line of blocks that
+  // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, the slots of a page, and neighbouring pages, within 2 GB; a line of blocks that
   // 256 shares of 32 bits cover.
   c.tiled = a.page_size % 16 == 0 && a.head_dim <= 128 && chunks(a.head_dim) && chunks(a.q_t) && chunks(a.q_h) && chunks(a.o_t) && chunks(a.o_h) && chunks(a.key_p) &&
             chunks(a.key_s) && chunks(a.key_h) && chunks(a.val_p) && chunks(a.val_s) && chunks(a.val_h) && a.key_s < (1 << 24) && a.val_s < (1 << 24) &&
+            a.key_p < (1 << 29) && a.val_p < (1 << 29) && a.key_s * a.page_size < (1 << 29) && a.val_s * a.page_size < (1 << 29) &&
             uint64_t(a.tokens) * a.group < (1u << 31) &&
             (double(a.tokens) * a.group / 16 + a.requests) * a.kv_heads * (double(a.width) * a.page_size / 32 + 16) < double(1ull << 39) && scale > 1e-30 && scale < 1e30;
   if (!c.tiled) return c;
   const uint64_t rows = uint64_t(a.max_new) * a.group;
-  const bool chunk = a.dtype == MRL_BF16 && rows > 32;
-  if (!chunk) c.qb = rows <= 16 ? 1 : 2;
-  else if (a.requests > 1) c.qb = 1;
-  if (c.qb) {
-    paged::Work &w = c.keys;
+  paged::Work &w = c.work;
+  if (a.dtype == MRL_BF16 && rows > 32) {
+    // Requests of few rows among others go the same way: a tile of 128 rows streams its keys at what memory delivers, too (a decoding step of 48 requests up to 16384
+    // keys that way 167 us, on tiles of 16 rows 143; 18 such requests beside 6 chunks in a launch of their own on those: 53 us, 39 together).
+    paged::chunk_work(a, &w);
+  } else {
+    c.qb = rows <= 16 ? 1 : 2;
     paged::keys_work(a, c.qb, &w);
-    w.min_rows = 1, w.max_rows = chunk ? 16 : 0x7fffffff, w.once = chunk || rows <= 16u * c.qb;
+    w.once = rows <= 16u * c.qb;
     // Tables of some hundred keys at most: a workgroup to each request and head does them in some rounds, with nothing to find out before and no launch behind.
     // (max_new is the program's word: a request of more tokens would have more tiles than one, unless all rows there are make no second one)
-    w.direct = !chunk && uint64_t(a.tokens) * a.group <= 16u * c.qb && uint64_t(a.width) * a.page_size <= DIRECT_KEYS;
-    if (!w.direct) c.keys_at = take(a, w, &c.bytes);
+    w.direct = uint64_t(a.tokens) * a.group <= 16u * c.qb && uint64_t(a.width) * a.page_size <= DIRECT_KEYS;
   }
-  if (chunk) {
-    paged::chunk_work(a, &c.chunk);
-    c.chunk.min_rows = c.qb ? 17 : 1, c.chunk.max_rows = 0x7fffffff;
-    c.chunk_at = take(a, c.chunk, &c.bytes);
+  if (!w.direct) {
+    c.partial_bytes = (size_t(2 * w.workers) << w.bq_log2) * paged::row_floats(a) * sizeof(float);
+    c.bytes = c.partial_bytes + w.workers * 32;
   }
   return c;
 }
 
 template <class T>
 hipError_t launch_merge(const PagedAttnArgs &a, const Choice &c, hipStream_t stream) {
-  MergeArgs m;
-  m.of[0] = {c.chunk.merges, c.chunk.partials, c.chunk.workers, 1u << c.chunk.bq_log2};
-  m.of[1] = {c.keys.merges, c.keys.partials, c.keys.workers, 1u << c.keys.bq_log2};
-  m.row_floats = paged::row_floats(a), m.by_group = FastDiv(a.group), m.by_quads = FastDiv((a.head_dim + 3) / 4);
+  const MergeArgs m = {c.work.merges, c.work.partials, 1u << c.work.bq_log2, paged::row_floats(a), FastDiv(a.group), FastDiv((a.head_dim + 3) / 4)};
   plan::work(plan::UNIT_STREAM, 0, double(c.bytes) / 2);
-  MRL_LAUNCH(k_paged_attn_merge<T>, dim3(c.chunk.workers + c.keys.workers, c.chunk.workers ? 8 : 2), dim3(THREADS), 0, stream, a, m);
+  MRL_LAUNCH(k_paged_attn_merge<T>, dim3(c.work.workers, c.qb ? 2 : 8), dim3(THREADS), 0, stream, a, m);
   return plan::last_error();
 }
 
@@ -244,12 +228,9 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream) {
   Choice c = choose(a);
   if (!c.tiled || !aligned(a.q) || !aligned(a.keys) || !aligned(a.values) || !aligned(a.out))
     return bf16 ? launch_generic<u16>(a, stream) : launch_generic<float>(a, stream);
-  if (c.keys.direct) return paged::launch_keys(a, c.keys, c.qb, stream);
-  place(a, c.keys, c.keys_at), place(a, c.chunk, c.chunk_at);
-  hipError_t e = hipSuccess;
-  if (c.chunk.workers) e = paged::launch_chunk(a, c.chunk, stream);
-  if (e == hipSuccess && c.keys.workers) e = paged::launch_keys(a, c.keys, c.qb, stream);
-  if (e != hipSuccess) return e;
+  c.work.partials = reinterpret_cast<float *>(a.workspace), c.work.merges = reinterpret_cast<uint32_t *>(a.workspace + c.partial_bytes);
+  const hipError_t e = c.qb ? paged::launch_keys(a, c.work, c.qb, stream) : paged::launch_chunk(a, c.work, stream);
+  if (e != hipSuccess || c.work.direct) return e;
   return bf16 ? launch_merge<u16>(a, c, stream) : launch_merge<float>(a, c, stream);
 }
 

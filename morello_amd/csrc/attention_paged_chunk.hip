@@ -86,7 +86,7 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     const uint8_t *const val_head = (const uint8_t *)k.p.values + int64_t(t.head) * k.p.val_h * 2;
     const int64_t key_page = k.p.key_p * 2, val_page = k.p.val_p * 2;
     const int32_t *const pages = k.p.table + uint64_t(t.request) * k.p.width;
-    const uint32_t page_count = k.p.pages, groups_per_page = k.p.page_size / 16;
+    const uint32_t page_count = k.p.pages;
 
     // The places of this lane's two rows (a row sees the keys up to it, below t.end and, with a window, behind it less the window; -1 where the tile
     // has no such row), and the keys that all of the wave's rows see, [all_from, all_to).
@@ -112,8 +112,9 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     // Of 64 of this half's blocks, a lane each: the page of this wave's sixteen keys and the place in it, and which blocks have sixteens on no page.
     // (K runs two blocks ahead: its numbers move on before the bits of the block whose scores are masked do.)
     int32_t page_here = -1;
-    uint64_t gone_here[NKB] = {}, gone_next[NKB] = {};
-    auto fetch_pages = [&](uint32_t kb, uint64_t *gone) {   // blocks kb .. kb + 63
+    uint64_t gone_here[NKB] = {}, gone_next[NKB] = {}, any_here = 0, any_next = 0;
+    auto fetch_pages = [&](uint32_t kb, uint64_t *gone, uint64_t &any) {   // blocks kb .. kb + 63
+      any = 0;
 #pragma unroll
       for (int g = 0; g < NKB; g++) {
         const uint32_t group = (first_block + kb + lane) * 4 + g, column = by_page16.div(group);
@@ -122,18 +123,40 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
           number = pages[column];
           if (uint32_t(number) >= page_count) number = -1;
         }
-        gone[g] = __ballot(number < 0);
+        gone[g] = __ballot(number < 0), any |= gone[g];
         if (g == qg) page_here = number;
       }
     };
-    // The wave's 16 keys of block kb in their page.
-    auto resource = [&](const uint8_t *head, int64_t page_bytes, uint32_t slot_bytes, int32_t page, int kb) {
-      const uint32_t group16 = (first_block + kb) * 4 + qg, from = group16 * 16, place = (group16 - by_page16.div(group16) * groups_per_page) * 16;
-      const uint32_t rows = page < 0 || kb >= nblocks || from >= t.end ? 0 : min(t.end - from, 16u);
-      const uint64_t base = reinterpret_cast<uint64_t>(head) + uint64_t(max(page, 0)) * page_bytes + uint64_t(place) * slot_bytes;
-      return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(base)), 0, uniform(int(rows ? (rows - 1) * slot_bytes + row_bytes : 0)), 0x00020000);
+    // The wave's 16 keys of a block in their page: how far behind the head's first page they begin, and the bytes from there to the end of the last one
+    // that a row sees (none on no page).  Found block after block.
+    struct Span {
+      uint64_t keys, values;
+      uint32_t key_bytes, value_bytes;
     };
-    auto page_of = [&](int kb) { return __builtin_amdgcn_readlane(page_here, kb & 63); };
+    const uint32_t page_slots = k.p.page_size, place_step = uniform(BKV % page_slots);
+    const bool alike = k_slot == v_slot && key_page == val_page;   // (what keys and values have in common need not be found twice)
+    uint32_t place = uniform((first_block * BKV + 16 * qg) % page_slots);
+    // Blocks whose sixteen are seen whole.
+    const int whole_blocks = t.end < uint32_t(16 * qg + 16) ? 0 : min(nblocks, int((t.end - 16 * qg - 16) / BKV + 1) - int(first_block));
+    auto next_span = [&](int kb) {
+      const int32_t page = __builtin_amdgcn_readlane(page_here, kb & 63);
+      uint32_t rows = 16;
+      if (kb >= whole_blocks) {
+        const uint32_t from = (first_block + kb) * BKV + 16 * qg;
+        rows = kb >= nblocks || from >= t.end ? 0 : min(t.end - from, 16u);
+      }
+      if (page < 0) rows = 0;
+      Span s;
+      s.keys = uint64_t(uint32_t(page)) * uint32_t(key_page) + uint64_t(place * k_slot), s.key_bytes = rows ? (rows - 1) * k_slot + row_bytes : 0;
+      s.values = s.keys, s.value_bytes = s.key_bytes;
+      if (!alike) s.values = uint64_t(uint32_t(page)) * uint32_t(val_page) + uint64_t(place * v_slot), s.value_bytes = rows ? (rows - 1) * v_slot + row_bytes : 0;
+      place += place_step;
+      if (place >= page_slots) place -= page_slots;
+      return s;
+    };
+    auto resource = [](const uint8_t *head, uint64_t at, uint32_t bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(reinterpret_cast<uint64_t>(head) + at)), 0, int(uniform(bytes)), 0x00020000);
+    };
     const uint32_t k_dst0 = lds_address(my_lds) + qg * PER_WAVE * 1024, v_dst0 = k_dst0 + 2 * TILE;
 
     v4f o[NDB][2], den[2];
@@ -146,20 +169,20 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     }
     // K block kb goes to K tile kb & 1, V block kb to V tile kb % 3; blocks past the half's last bring zeros to tiles that nobody reads, so that
     // every slot issues the same number of loads.  V of a block is asked for a slot after K of it, with the page that was looked up then.
-    int32_t page_v = -1;
+    Span span = {}, span_of_v = {};   // of the block whose K is asked for last, and of the one before
 
     v4f s[NKB][2];
     v8bf pb[NKC][2];
     // Before the first slot: Q and half 0's K(0); behind the barrier V(0), K(1) and all of half 1's, which have half 0's first slot to land in.
-    if (nblocks > 0) fetch_pages(0, gone_here);
+    if (nblocks > 0) fetch_pages(0, gone_here, any_here);
     auto issue_k = [&](int kb) {
-      page_v = page_of(kb);
-      const auto from = resource(key_head, key_page, k_slot, page_v, kb);
+      span_of_v = span, span = next_span(kb);
+      const auto from = resource(key_head, span.keys, span.key_bytes);
 #pragma unroll
       for (int i = 0; i < PER_WAVE; i++) dma16(from, k_src[i], k_dst0 + (kb & 1) * TILE + i * 1024);
     };
-    auto issue_v = [&](int kb) {
-      const auto from = resource(val_head, val_page, v_slot, page_v, kb);
+    auto issue_v = [&](int kb) {   // (of the block whose K was asked for last)
+      const auto from = resource(val_head, span.values, span.value_bytes);
 #pragma unroll
       for (int i = 0; i < PER_WAVE; i++) dma16(from, v_src[i], v_dst0 + (kb % 3) * TILE + i * 1024);
     };
@@ -257,6 +280,22 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     // Of the block whose weights pb holds: which of its sixteens are on no page, and whether some row does not see it whole.
     uint32_t gone_bits = 0;
     bool masked = false;
+    // What slot B of block j wants to know is found in slot A: slot B is the longer of the two with it (2040 cycles against 1400, of 2.4 us a step; a wave issues an
+    // instruction every 6 or 7 cycles there, scalar ones too).
+    uint32_t masked_next = 0;
+    auto prepare = [&](int j) {
+      if (((j + 2) & 63) == 0) fetch_pages(j + 2, gone_next, any_next);
+      if ((j & 63) == 0 && j) {
+        any_here = any_next;
+#pragma unroll
+        for (int g = 0; g < NKB; g++) gone_here[g] = gone_next[g];
+      }
+      const int32_t key0 = int32_t((first_block + j) * BKV);
+      masked_next = uniform(uint32_t(key0 < all_from || key0 + BKV > all_to || ((any_here >> (j & 63)) & 1)));
+      span_of_v = span, span = next_span(j + 2);
+      span.keys = uniform(span.keys), span.key_bytes = uniform(span.key_bytes);
+      asm volatile("" : "+s"(span.keys), "+s"(span.key_bytes), "+s"(masked_next));   // (here, and not where it is used)
+    };
     // The second product of a masked block whose values are not all finite: a key at a time, its values against its weights alone, and of the product only the
     // columns (rows of queries) that see it.
     auto slow_product = [&](int kb, const uint8_t *lv) {
@@ -309,21 +348,17 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       __builtin_amdgcn_s_setprio(PRIO_A);
       zero_s();
       const uint8_t *const lv = values_of(j, vstage);
+      prepare(j);
       run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, lv, my_lds + (j & 1) * TILE);
     };
     auto slot_b = [&](int j) {
       __builtin_amdgcn_s_setprio(PRIO_B);
-      if (((j + 2) & 63) == 0) fetch_pages(j + 2, gone_next);
-      if ((j & 63) == 0 && j) {
-#pragma unroll
-        for (int g = 0; g < NKB; g++) gone_here[g] = gone_next[g];
-      }
-      gone_bits = 0;
-#pragma unroll
-      for (int g = 0; g < NKB; g++) gone_bits |= uint32_t((gone_here[g] >> (j & 63)) & 1) << g;
+      masked = masked_next;
       const int32_t key0 = int32_t((first_block + j) * BKV);
-      masked = key0 < all_from || key0 + BKV > all_to || gone_bits;
       if (masked) {
+        gone_bits = 0;
+#pragma unroll
+        for (int g = 0; g < NKB; g++) gone_bits |= uint32_t((gone_here[g] >> (j & 63)) & 1) << g;
 #pragma unroll
         for (int qb = 0; qb < 2; qb++) {
           const int32_t last = min(row_at[qb], int32_t(t.end) - 1) - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
@@ -366,9 +401,7 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       if (j == 0) move_reference();
       float pmax[2] = {0.0f, 0.0f};   // the block's largest exponential per row: what tells a stale reference
       // The fetches of V(j + 1) and K(j + 2) go out one at a time between the exponentials.
-      const int32_t page_k = page_of(j + 2);
-      const auto v_from = resource(val_head, val_page, v_slot, page_v, j + 1), k_from = resource(key_head, key_page, k_slot, page_k, j + 2);
-      page_v = page_k;
+      const auto v_from = resource(val_head, span_of_v.values, span_of_v.value_bytes), k_from = resource(key_head, span.keys, span.key_bytes);
       const uint32_t kdst = k_dst0 + (j & 1) * TILE, vdst = v_dst0 + ((j + 1) % 3) * TILE;
 #pragma unroll
       for (int kb = 0; kb < NKB; kb++)
@@ -402,6 +435,7 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     // Every wave passes steps + 1 pairs of barriers; a half with fewer blocks idles through the rest.
     if (nblocks > 0) {
       zero_s();
+      prepare(0);
       run_steps(integral_constant<int, PV_STEPS>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, my_lds, my_lds);
     }
     __syncthreads();
