@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -595,15 +596,20 @@ class _PagedOp:
         returns.  `ptrs`: device pointers in the order include/morello_amd.h gives, None or 0 where one may be NULL."""
         if len(ptrs) != self._params:
             raise ValueError(f"{self._params} parameters")
-        handle = stream.handle if isinstance(stream, Stream) else C.c_void_p(stream or 0)
-        _check(self._run(C.byref(self._c), _pointers[self._params](*ptrs), handle), f"mrl_run_{self._name}")
+        try:
+            packed = self._pack(*ptrs)   # (0.13 us; an array of c_void_p takes 0.68)
+        except struct.error:
+            packed = self._pack(*[p or 0 for p in ptrs])
+        status = self._run(self._ref, packed, stream.handle if isinstance(stream, Stream) else stream)
+        if status:
+            _check(status, f"mrl_run_{self._name}")
 
     def run_device(self, ptrs: Sequence[Optional[int]]):
         self.run_async(ptrs)
         synchronize()
 
     def _finish(self):
-        self._run = getattr(B.load(), f"mrl_run_{self._name}")
+        self._run, self._ref, self._pack = getattr(B.load(), f"mrl_run_{self._name}"), C.byref(self._c), struct.Struct(f"{self._params}P").pack
 
 
 def _set_strides(c, **given):

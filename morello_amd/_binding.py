@@ -198,13 +198,13 @@ SIGNATURES = {
     "mrl_device_info": (C.c_int, [C.c_char_p, C.c_size_t, C.POINTER(C.c_int), C.POINTER(C.c_int),
                                   C.POINTER(C.c_size_t)]),
     "mrl_page_tables_check": (C.c_int, [C.POINTER(PageTablesC)]),
-    "mrl_run_page_tables": (C.c_int, [C.POINTER(PageTablesC), _VPP, C.c_void_p]),
+    "mrl_run_page_tables": (C.c_int, [C.POINTER(PageTablesC), C.c_void_p, C.c_void_p]),
     "mrl_page_tables_plan": (C.c_int, [C.POINTER(PageTablesC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
     "mrl_rotary_check": (C.c_int, [C.POINTER(RotaryC)]),
-    "mrl_run_rotary": (C.c_int, [C.POINTER(RotaryC), _VPP, C.c_void_p]),
+    "mrl_run_rotary": (C.c_int, [C.POINTER(RotaryC), C.c_void_p, C.c_void_p]),
     "mrl_rotary_plan": (C.c_int, [C.POINTER(RotaryC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
     "mrl_paged_attention_check": (C.c_int, [C.POINTER(PagedAttentionC)]),
-    "mrl_run_paged_attention": (C.c_int, [C.POINTER(PagedAttentionC), _VPP, C.c_void_p]),
+    "mrl_run_paged_attention": (C.c_int, [C.POINTER(PagedAttentionC), C.c_void_p, C.c_void_p]),
     "mrl_paged_attention_plan": (C.c_int, [C.POINTER(PagedAttentionC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
     "mrl_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionC)]),
 }

@@ -286,7 +286,8 @@ __device__ inline bool direct_piece(const Kernargs &k, Piece *out) {
 }
 
 // Floats of a row of a partial result: O of the head dim the kernels are built for, reference, denominator, and two that are not used.
-inline uint32_t row_floats(const PagedAttnArgs &a) { return (a.head_dim <= 64 ? 64 : 128) + 4; }
+inline uint32_t kernel_dims(const PagedAttnArgs &a) { return a.head_dim <= 64 ? 64 : a.dtype == MRL_F32 && a.head_dim <= 96 ? (a.head_dim <= 80 ? 80 : 96) : 128; }
+inline uint32_t row_floats(const PagedAttnArgs &a) { return kernel_dims(a) + 4; }
 // attention_paged_chunk.hip: tiles of 128 rows, bf16.  The Work's fixed numbers, and the launch.
 void chunk_work(const PagedAttnArgs &a, Work *w);
 hipError_t launch_chunk(const PagedAttnArgs &a, const Work &work, hipStream_t stream);

@@ -8,8 +8,8 @@
 // in its accumulators of the first product, and these are the operand of the second as they stand.
 //   bf16: v_mfma 16x16x32; V's operand through the transposing read; P rounded to bf16 (2^-8), the denominators from a row of ones, so that
 //         they are the sums of the very numbers that weigh the values.
-//   f32:  v_mfma 16x16x4; a 16-byte read of a K row is four steps of dims, a 16-byte read of a V row four blocks of output dims
-//         (dim 64 q + 4 (l % 16) + i is row l % 16 of block 4 q + i).
+//   f32:  v_mfma 16x16x4; a 16-byte read of a K row is four steps of dims, a V row is read in words.  The matrix cores bound it (1/16 of bf16's rate), so
+//         there are forms for 80 and 96 dims, too, and a tile of up to 16 rows does half of a form of 32.
 // Keys and values go from their pages straight into LDS, 16 bytes a lane, through a buffer resource per 16 keys: a page's numbers are whole sixteens of
 // slots, so 16 keys lie behind each other.  The resource ends behind the last key that a row of the tile sees: what lies behind (or on no
 // page at all) arrives as zeros, whatever the slots hold.  The pages' numbers are fetched 32 blocks at a time, a lane each, and read from
@@ -36,13 +36,14 @@ struct Form {
   static constexpr bool BF16 = sizeof(T) == 2;
   static constexpr int TH = 64 * W, BQ = 16 * QB;
   static constexpr int ROW = D * int(sizeof(T)), CHUNKS = ROW / 16, SLOTS = ROW / 32;
-  static constexpr int TILE = KEYS * ROW, LOADS = TILE / 1024, ROWS_PER_LOAD = 1024 / ROW, HALF = LOADS / 2;
+  static constexpr int TILE = KEYS * ROW, LOADS = TILE / 1024, HALF = LOADS / 2;
   static constexpr int ROWS_PER_LINE = ROW >= 256 ? 1 : 256 / ROW;   // rows per 256-byte line of banks
   static constexpr int NDB = D / 16;                                  // 16-row blocks of O^T
   static constexpr int ROW_FLOATS = D + 4;                            // of a partial result: O, reference, denominator
-  static_assert(ROWS_PER_LOAD <= 16 && LOADS < 32 && LOADS % 2 == 0, "a load stays within 16 keys");
-  // K rows are XOR-swizzled by 16-byte chunk, bf16's V rows by 32-byte slot (attention_keys.hip); an f32 V row is read whole.
-  __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1) & 15; }
+  static_assert(16 * ROW % 1024 == 0 && LOADS < 64, "16 keys are whole loads");
+  // K rows of 2^n bytes are XOR-swizzled by 16-byte chunk, bf16's V rows by 32-byte slot (attention_keys.hip); the others lie as they are: 16 lanes read 16 words of
+  // an f32 row of V, and what meets in the banks by that is read while the products are busy.
+  __device__ static constexpr int k_swizzle(int row) { return CHUNKS & (CHUNKS - 1) ? 0 : (row / ROWS_PER_LINE) & (CHUNKS - 1) & 15; }
   __device__ static constexpr int v_swizzle(int row) { return BF16 ? (row / ROWS_PER_LINE) & (SLOTS - 1) & 15 : 0; }
   // The waves' tiles, or after the loop their O, references and denominators.
   static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
@@ -70,14 +71,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
   uint8_t *const k_tile = lds + wave * 2 * TILE, *const v_tile = k_tile + TILE;
   const uint32_t row_bytes = kernargs().p.head_dim * uint32_t(sizeof(T)), k_slot = uint32_t(kernargs().p.key_s * sizeof(T)), v_slot = uint32_t(kernargs().p.val_s * sizeof(T));
 
-  // One instruction fills 1 KiB of a tile, lane l its slot l: rows i * ROWS_PER_LOAD + l / CHUNKS, the chunk that belongs there.  The
-  // second 16 keys are as the first, from their own base.
+  // One instruction fills 1 KiB of a tile, lane l its slot l: row and chunk that belong there.  The second 16 keys are as the first, from their
+  // own base.
   uint32_t k_src[HALF], v_src[HALF];
   {
-    const int ld_row = lane / F::CHUNKS, ld_pc = lane % F::CHUNKS;
 #pragma unroll
     for (int i = 0; i < HALF; i++) {
-      const int row = i * F::ROWS_PER_LOAD + ld_row;
+      const int row = (i * 64 + lane) / F::CHUNKS, ld_pc = (i * 64 + lane) % F::CHUNKS;
       const uint32_t k_at = (ld_pc ^ F::k_swizzle(row)) << 4;
       const uint32_t v_at = BF16 ? (((ld_pc >> 1) ^ F::v_swizzle(row)) << 5) | ((ld_pc & 1) << 4) : ld_pc << 4;
       k_src[i] = k_at < row_bytes ? row * k_slot + k_at : OUTSIDE;
@@ -86,20 +86,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
   }
   const uint32_t k_dst = lds_address(k_tile), v_dst = lds_address(v_tile);
   // Lane-dependent parts of the operands' addresses.
-  constexpr int NC = ROW / 64;   // 64-byte pieces of a K row: bf16 a step of 32 dims, f32 four steps of 4
-  constexpr int NV = BF16 ? NDB : D / 64;
-  uint32_t k_lane[NC], v_lane[NV];
+  constexpr int NC = D * int(sizeof(T)) / 64;   // 64-byte pieces of a K row: bf16 a step of 32 dims, f32 four steps of 4
+  uint32_t k_lane[NC], v_lane[NDB];
 #pragma unroll
   for (int i = 0; i < NC; i++) k_lane[i] = lr * ROW + (((4 * i + lgp) ^ F::k_swizzle(lr)) << 4);
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
+  for (int i = 0; i < NDB; i++) {
     const int vrow = 4 * lgp + (lr >> 2);
-    v_lane[i] = BF16 ? vrow * ROW + ((i ^ F::v_swizzle(vrow)) << 5) + (lr & 3) * 8 : 4 * lgp * ROW + i * 256 + lr * 16;
+    v_lane[i] = BF16 ? vrow * ROW + ((i ^ F::v_swizzle(vrow)) << 5) + (lr & 3) * 8 : 4 * lgp * ROW + i * 64 + lr * 4;
   }
   constexpr int ALL_BUT_ONE_TILE = 0x0F70 | (LOADS & 15) | ((LOADS >> 4) << 14), ALL = 0x0F70, READS_DONE = 0xC07F;
 
   const bool direct = kernargs().w.direct;
-  auto run = [&](const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
+  // NQ: of the QB columns of 16 rows, those that the tile has rows in.
+  auto run = [&](auto columns, const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
+    constexpr int NQ = decltype(columns)::value;
     const float c = k.c;
     const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
     const uint32_t group = k.p.group, window = k.p.window, first_block = t.begin / KEYS + t.b0 + wave;
@@ -107,10 +108,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
     const float hidden = c > 0 ? -__builtin_inff() : __builtin_inff();   // a score that weighs nothing
 
     // This lane's rows: queries, and the keys they see, [lo, hi].
-    v4i qf[QB][NC];
-    int32_t lo[QB], hi[QB];
+    v4i qf[NQ][NC];
+    int32_t lo[NQ], hi[NQ];
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
+    for (int qb = 0; qb < NQ; qb++) {
       const uint32_t i = 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * group + (row - token * group);
       const int32_t at = t.at + int32_t(token);
       hi[qb] = i < t.rows ? min(at, int32_t(t.end) - 1) : -1;
@@ -166,10 +167,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
     auto issue_k = [&](uint32_t n) { issue(n, key_head, key_page, k_slot, k_src, k_dst); };
     auto issue_v = [&](uint32_t n) { issue(n, val_head, val_page, v_slot, v_src, v_dst); };
 
-    v4f o[NDB][QB], den[QB];
-    float m_run[QB];
+    v4f o[NDB][NQ], den[NQ];
+    float m_run[NQ];
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
+    for (int qb = 0; qb < NQ; qb++) {
       m_run[qb] = NO_REFERENCE;
       den[qb] = v4f{0, 0, 0, 0};
 #pragma unroll
@@ -193,16 +194,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
         // In flight at this point, oldest first: K of this block, V of this block.
         if (!start) __builtin_amdgcn_s_waitcnt(ALL_BUT_ONE_TILE);
         asm volatile("" ::: "memory");
-        v4f s[2][QB];
+        v4f s[2][NQ];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++) s[kb][qb] = v4f{0, 0, 0, 0};
+          for (int qb = 0; qb < NQ; qb++) s[kb][qb] = v4f{0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < NC; j++) {
             const v4i a = *(const v4i *)(k_tile + k_lane[j] + kb * 16 * ROW);
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) {
+            for (int qb = 0; qb < NQ; qb++) {
               if constexpr (BF16) {
                 s[kb][qb] = mfma16(a, qf[qb][j], s[kb][qb]);
               } else {
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
         const bool masked = key0 < all_from || key0 + KEYS > all_to || gone0 || gone1;
         if (masked) {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++) {
+          for (int qb = 0; qb < NQ; qb++) {
             const int32_t last = hi[qb] - key0 - 4 * lgp, first = lo[qb] - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
         }
         auto move_reference = [&]() {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++) {
+          for (int qb = 0; qb < NQ; qb++) {
             float mx = s[0][qb][0] * c;
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
@@ -249,11 +250,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
           }
         };
         const bool fresh = n < FOLLOWED;
-        float e[2][QB][4];
+        float e[2][NQ][4];
         float pmax = 0.0f;
         auto exponentials = [&]() {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++)
+          for (int qb = 0; qb < NQ; qb++)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -269,10 +270,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
           exponentials();
         }
         start = false;
-        v8bf pb[QB];
+        v8bf pb[NQ];
         if constexpr (BF16) {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++)
+          for (int qb = 0; qb < NQ; qb++)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
                 const v2i lo2 = read_tr16(v_tile + v_lane[db]), hi2 = read_tr16(v_tile + v_lane[db] + 16 * ROW);
                 const v4i a = v4i{lo2[0], lo2[1], hi2[0], hi2[1]} & only;
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++) {
+                for (int qb = 0; qb < NQ; qb++) {
                   const v4f y = mfma16(a, __builtin_bit_cast(v4i, pb[qb]) & only, v4f{0, 0, 0, 0});
                   o[db][qb] += key0 + x >= lo[qb] && key0 + x <= hi[qb] && !(x < 16 ? gone0 : gone1) ? y : v4f{0, 0, 0, 0};
                 }
@@ -318,15 +319,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
                 for (int g = 0; g < 4; g++) {
                   const int32_t key = key0 + kb * 16 + 4 * g + r;
 #pragma unroll
-                  for (int i = 0; i < NV; i++) {
-                    const v4i a = *(const v4i *)(v_tile + v_lane[i] + (kb * 16 + r) * ROW);
+                  for (int db = 0; db < NDB; db++) {
+                    const float a = *(const float *)(v_tile + v_lane[db] + (kb * 16 + r) * ROW);
 #pragma unroll
-                    for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-                      for (int j = 0; j < 4; j++) {
-                        const v4f y = mfma4(lgp == g ? __int_as_float(a[j]) : 0.0f, lgp == g ? e[kb][qb][r] : 0.0f, v4f{0, 0, 0, 0});
-                        o[4 * i + j][qb] += key >= lo[qb] && key <= hi[qb] && !(kb ? gone1 : gone0) ? y : v4f{0, 0, 0, 0};
-                      }
+                    for (int qb = 0; qb < NQ; qb++) {
+                      const v4f y = mfma4(lgp == g ? a : 0.0f, lgp == g ? e[kb][qb][r] : 0.0f, v4f{0, 0, 0, 0});
+                      o[db][qb] += key >= lo[qb] && key <= hi[qb] && !(kb ? gone1 : gone0) ? y : v4f{0, 0, 0, 0};
+                    }
                     asm volatile("" ::: "memory");
                   }
                 }
@@ -341,7 +340,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
             const v2i lo2 = read_tr16(v_tile + v_lane[db]), hi2 = read_tr16(v_tile + v_lane[db] + 16 * ROW);
             const v4i a = {lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) o[db][qb] = mfma16(a, pb[qb], o[db][qb]);
+            for (int qb = 0; qb < NQ; qb++) o[db][qb] = mfma16(a, pb[qb], o[db][qb]);
           }
         } else {
 #pragma unroll
@@ -349,21 +348,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-              for (int i = 0; i < NV; i++) {
-                const v4i a = *(const v4i *)(v_tile + v_lane[i] + (kb * 16 + r) * ROW);
+              for (int db = 0; db < NDB; db++) {
+                const float a = *(const float *)(v_tile + v_lane[db] + (kb * 16 + r) * ROW);
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-                  for (int j = 0; j < 4; j++) o[4 * i + j][qb] = mfma4(__int_as_float(a[j]), e[kb][qb][r], o[4 * i + j][qb]);
+                for (int qb = 0; qb < NQ; qb++) o[db][qb] = mfma4(a, e[kb][qb][r], o[db][qb]);
               }
         }
         if constexpr (BF16) {
           const v4i ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++) den[qb] = mfma16(ones, pb[qb], den[qb]);
+          for (int qb = 0; qb < NQ; qb++) den[qb] = mfma16(ones, pb[qb], den[qb]);
         } else {
 #pragma unroll
-          for (int qb = 0; qb < QB; qb++)
+          for (int qb = 0; qb < NQ; qb++)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -376,27 +373,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
     }
 
     // The waves' triples meet: quads of O in LDS as [wave][block column][quad][lane], then [wave][block column][reference, denominator][row].
-    // Quad x of a lane holds dims quad_dim(x) .. + 3.
-    auto quad_dim = [&](int x) { return BF16 ? 16 * x + 4 * lgp : 64 * (x / 4) + 16 * lgp + 4 * (x % 4); };
+    // Quad x of a lane holds dims 16 x + 4 lgp .. + 3.
     __syncthreads();   // all tiles have been read
     v4f *const quads = (v4f *)lds;
-    float *const stats = (float *)(lds + W * QB * D * 64);
+    float *const stats = (float *)(lds + W * NQ * D * 64);
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
+    for (int qb = 0; qb < NQ; qb++) {
 #pragma unroll
-      for (int x = 0; x < NDB; x++) {
-        v4f quad;
-        if constexpr (BF16) quad = o[x][qb];
-        else quad = v4f{o[x / 4 * 4][qb][x % 4], o[x / 4 * 4 + 1][qb][x % 4], o[x / 4 * 4 + 2][qb][x % 4], o[x / 4 * 4 + 3][qb][x % 4]};
-        quads[((wave * QB + qb) * NDB + x) * 64 + lane] = quad;
-      }
+      for (int x = 0; x < NDB; x++) quads[((wave * NQ + qb) * NDB + x) * 64 + lane] = o[x][qb];
       float l = den[qb][0];
       if constexpr (!BF16) {
         l = (den[qb][0] + den[qb][1]) + (den[qb][2] + den[qb][3]);
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
       }
-      if (lgp == 0) stats[(wave * QB + qb) * 32 + lr] = m_run[qb], stats[(wave * QB + qb) * 32 + 16 + lr] = l;
+      if (lgp == 0) stats[(wave * NQ + qb) * 32 + lr] = m_run[qb], stats[(wave * NQ + qb) * 32 + 16 + lr] = l;
     }
     __syncthreads();
     const Kernargs &e = kernargs();
@@ -407,22 +398,23 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
       if (tid == 0) worker->describe(e.w, t);
     }
 #pragma unroll
-    for (int x = wave; x < QB * NDB; x += W) {
-      const int qb = x / NDB;
+    for (int x0 = 0; x0 < NQ * NDB; x0 += W) {
+      const int x = x0 + wave, qb = x / NDB;
+      if (NQ * NDB % W && x >= NQ * NDB) break;
       const uint32_t i = 16 * qb + lr;
       if (i >= t.rows) continue;
       float mm = -3.0e38f, l = 0.0f;
       float f[W];
 #pragma unroll
-      for (int j = 0; j < W; j++) f[j] = stats[(j * QB + qb) * 32 + lr], mm = fmaxf(mm, f[j]);
+      for (int j = 0; j < W; j++) f[j] = stats[(j * NQ + qb) * 32 + lr], mm = fmaxf(mm, f[j]);
       v4f sum = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < W; j++) {
         f[j] = __builtin_amdgcn_exp2f(f[j] - mm);
-        l += stats[(j * QB + qb) * 32 + 16 + lr] * f[j];
-        sum += quads[((j * QB + qb) * NDB + x % NDB) * 64 + lane] * f[j];
+        l += stats[(j * NQ + qb) * 32 + 16 + lr] * f[j];
+        sum += quads[((j * NQ + qb) * NDB + x % NDB) * 64 + lane] * f[j];
       }
-      const uint32_t dim = quad_dim(x % NDB);
+      const uint32_t dim = x % NDB * 16 + 4 * lgp;
       if (!whole) {
         float *to = part + i * F::ROW_FLOATS;
         *(v4f *)(to + dim) = sum;
@@ -441,15 +433,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
       }
     }
   };
+  auto run_piece = [&](const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
+    if constexpr (!BF16 && QB > 1) {
+      if (t.rows <= 16) return run(std::integral_constant<int, 1>{}, k, t, worker);
+    }
+    run(std::integral_constant<int, QB>{}, k, t, worker);
+  };
   Piece t;
   if (direct) {
-    if (direct_piece(kernargs(), &t)) run(kernargs(), t, nullptr);
+    if (direct_piece(kernargs(), &t)) run_piece(kernargs(), t, nullptr);
     return;
   }
   Worker<64 * W> worker(kernargs(), reinterpret_cast<typename Worker<64 * W>::Shared *>(lds));
   __syncthreads();
   while (worker.next(kernargs(), &t)) {
-    run(kernargs(), t, &worker);
+    run_piece(kernargs(), t, &worker);
     __syncthreads();   // (the triples have been read)
   }
   if (tid == 0 && !worker.described) kernargs().w.merges[worker.number * 8] = 0;
@@ -481,6 +479,8 @@ auto with_form(const PagedAttnArgs &a, int qb, F f) {
     return qb == 1 ? f(Form<__bf16, 128, 1, W>()) : f(Form<__bf16, 128, 2, W>());
   }
   if (narrow) return qb == 1 ? f(Form<float, 64, 1, W>()) : f(Form<float, 64, 2, W>());
+  if (a.head_dim <= 80) return qb == 1 ? f(Form<float, 80, 1, W>()) : f(Form<float, 80, 2, W>());
+  if (a.head_dim <= 96) return qb == 1 ? f(Form<float, 96, 1, W>()) : f(Form<float, 96, 2, W>());
   return qb == 1 ? f(Form<float, 128, 1, W>()) : f(Form<float, 128, 2, W>());
 }
 template <class T, int D, int QB, int W>
