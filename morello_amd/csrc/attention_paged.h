@@ -142,15 +142,28 @@ __device__ inline uint32_t most_blocks(const Kernargs &k, const Request &q, uint
                     : max(last.blocks, 1u);
 }
 
-// A workgroup's way along its share of the line; everybody calls it.  TH: threads of the workgroup.
-template <int TH>
+// Sums over the lanes up to each.
+template <int CTRL, int ROWS>
+__device__ inline uint64_t moved(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(x)), CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(x >> 32)), CTRL, ROWS, 0xf, false);
+  return uint64_t(hi) << 32 | lo;
+}
+__device__ inline uint64_t sums_up_to(uint64_t x) {
+  x += moved<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8: within sixteens
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);   // row_bcast 15, 31: the last of a sixteen, of a half, to those behind
+  return x + moved<0x143, 0xc>(x);
+}
+__device__ inline uint32_t of_lane(uint32_t x, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(x), lane)); }
+__device__ inline uint64_t of_lane(uint64_t x, int lane) { return uint64_t(of_lane(uint32_t(x >> 32), lane)) << 32 | of_lane(uint32_t(x), lane); }
+
+// A workgroup's way along its share of the line; every wave goes it for itself, so that no wave waits for another.
 struct Worker {
-  struct Shared {
-    uint64_t sums[3][TH / 64];
-    uint32_t found[4];
-  };
   uint32_t number = xcd_run(blockIdx.x, gridDim.x);
   uint32_t request = 0xffffffffu, head = 0, tile = 0, at = 0;   // where it stands
+  Request q = {0, 0, 0};                                        // the request there
   uint32_t share = 1, left = 0;
   bool few = false, described = false;
 
@@ -160,82 +173,59 @@ struct Worker {
     return l;
   }
 
-  // Finds its start; `sh` is free again behind the caller's next barrier.
-  __device__ Worker(const Kernargs &k, Shared *sh) {
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  // Finds its start, a lane to a request.
+  __device__ Worker(const Kernargs &k) {
+    const uint32_t lane = threadIdx.x & 63, requests = k.p.requests;
     const uint64_t heads = k.p.kv_heads, workers = k.w.workers;
     // How many tiles, how long the line, how many blocks in the few tiles' way.
     uint64_t tiles = 0, line = 0, blocks = 0;
-    Request q = {0, 0, 0};
-    for (uint32_t r = tid; r < k.p.requests; r += TH) {
-      q = read_request(k.p, r);
-      if (!q.n) continue;
-      const Lengths l = lengths_of(k, q);
-      tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(k, q, l.tiles);
+    Request mine = {0, 0, 0};
+    for (uint32_t r = lane; r < requests; r += 64) {
+      mine = read_request(k.p, r);
+      if (!mine.n) continue;
+      const Lengths l = lengths_of(k, mine);
+      tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(k, mine, l.tiles);
     }
-#pragma unroll
-    for (int d = 32; d; d /= 2) tiles += __shfl_xor(tiles, d), line += __shfl_xor(line, d), blocks += __shfl_xor(blocks, d);
-    if (lane == 0) sh->sums[0][wave] = tiles, sh->sums[1][wave] = line, sh->sums[2][wave] = blocks;
-    if (tid == 0) sh->found[0] = 0xffffffffu;
-    __syncthreads();
-    tiles = line = blocks = 0;
-#pragma unroll
-    for (int i = 0; i < TH / 64; i++) tiles += sh->sums[0][i], line += sh->sums[1][i], blocks += sh->sums[2][i];
-    tiles = uniform(tiles) * heads, line = uniform(line) * heads, blocks = uniform(blocks) * heads;
-    share = max(quotient(line + workers - 1, workers), 1u);
+    tiles = of_lane(sums_up_to(tiles), 63) * heads, line = of_lane(sums_up_to(line), 63) * heads, blocks = of_lane(sums_up_to(blocks), 63) * heads;
+    share = uniform(max(quotient(line + workers - 1, workers), 1u));
     if (tiles < workers) {   // a piece to each, where that is no longer than equal shares and the second piece that they may come to
-      const uint32_t spare = uint32_t(workers - tiles), single = max((quotient(blocks + spare - 1, spare) + k.w.least - 1) / k.w.least, 1u) * k.w.least;
+      const uint32_t spare = uint32_t(workers - tiles), single = max((uniform(quotient(blocks + spare - 1, spare)) + k.w.least - 1) / k.w.least, 1u) * k.w.least;
       few = single <= share + k.w.second;
       if (few) share = single;
     }
     // The request that holds its start.
     const uint64_t from = uint64_t(share) * number;
     uint64_t base = 0;
-    for (uint32_t r0 = 0; r0 < k.p.requests; r0 += TH) {
-      if (k.p.requests > TH) {
-        q = {0, 0, 0};
-        if (r0 + tid < k.p.requests) q = read_request(k.p, r0 + tid);
+    for (uint32_t r0 = 0; r0 < requests; r0 += 64) {
+      if (requests > 64) {
+        mine = {0, 0, 0};
+        if (r0 + lane < requests) mine = read_request(k.p, r0 + lane);
       }
       Lengths l = {};
-      uint64_t mine = 0;
-      if (q.n) l = lengths(k, q), mine = l.all();
-      uint64_t sum = mine * heads;
-      const uint64_t all_mine = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const uint64_t below = __shfl_up(sum, d);
-        if (lane >= d) sum += below;
+      uint64_t length = 0;
+      if (mine.n) l = lengths(k, mine), length = l.all();
+      const uint64_t sum = sums_up_to(length * heads), off = base + sum - length * heads;
+      const bool here = mine.n && from >= off && from < base + sum;
+      const uint64_t where = __ballot(here);
+      if (where) {
+        uint32_t h = 0, t = 0, in_tile = 0;
+        if (here) {
+          h = quotient(from - off, length);
+          const uint64_t in_head = from - off - h * length;
+          t = l.tile_at(in_head), in_tile = uint32_t(in_head - l.before(t));
+        }
+        const int it = __builtin_ctzll(where);
+        request = r0 + it, head = of_lane(h, it), tile = of_lane(t, it), at = of_lane(in_tile, it), left = share;
+        q = {int32_t(of_lane(uint32_t(mine.n), it)), int32_t(of_lane(uint32_t(mine.start), it)), int32_t(of_lane(uint32_t(mine.length), it))};
+        break;
       }
-      __syncthreads();   // (the sums before have been read)
-      if (lane == 63) sh->sums[0][wave] = sum;
-      __syncthreads();
-      uint64_t off = base, all = 0;
-#pragma unroll
-      for (int i = 0; i < TH / 64; i++) {
-        const uint64_t x = sh->sums[0][i];
-        if (i < int(wave)) off += x;
-        all += x;
-      }
-      off += sum - all_mine;
-      if (q.n && from >= off && from < off + all_mine) {
-        const uint32_t h = quotient(from - off, mine);
-        const uint64_t in_head = from - off - h * mine;
-        const uint32_t t = l.tile_at(in_head);
-        sh->found[0] = r0 + tid, sh->found[1] = h, sh->found[2] = t, sh->found[3] = uint32_t(in_head - l.before(t));
-      }
-      base += uniform(all);
-      if (from < base) break;
+      base += of_lane(sum, 63);
     }
-    __syncthreads();
-    request = uniform(sh->found[0]), head = uniform(sh->found[1]), tile = uniform(sh->found[2]), at = uniform(sh->found[3]);
-    left = request < k.p.requests ? share : 0;
   }
 
   // The next piece that has something to do; false: there is none.
   __device__ bool next(const Kernargs &k, Piece *out) {
     while (left) {
-      Request q = read_request(k.p, request);
-      q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
       const Lengths l = lengths(k, q);
       const uint32_t length = uniform(l.of(tile));
       Piece t = tile_of(k, q, tile);
@@ -248,12 +238,19 @@ struct Worker {
           head = 0;
           const uint32_t lane = threadIdx.x & 63;
           uint64_t some = 0;
+          Request mine = {0, 0, 0};
           for (request++; request < k.p.requests; request += 64) {
-            some = __ballot(request + lane < k.p.requests && read_request(k.p, min(request + lane, k.p.requests - 1)).n != 0);
+            mine = {0, 0, 0};
+            if (request + lane < k.p.requests) mine = read_request(k.p, request + lane);
+            some = __ballot(mine.n != 0);
             if (some) break;
           }
-          if (some) request += __builtin_ctzll(some);
-          else left = 0;
+          left = some ? left : 0;
+          if (some) {
+            const int it = __builtin_ctzll(some);
+            request += it;
+            q = {int32_t(of_lane(uint32_t(mine.n), it)), int32_t(of_lane(uint32_t(mine.start), it)), int32_t(of_lane(uint32_t(mine.length), it))};
+          }
         }
       }
       if (any) {

@@ -70,8 +70,7 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
   };
 
-  Worker<TH> worker(kernargs(), reinterpret_cast<Worker<TH>::Shared *>(lds));
-  __syncthreads();
+  Worker worker(kernargs());
   Piece t;
   while (worker.next(kernargs(), &t)) {
     const Kernargs &k = kernargs();

@@ -28,7 +28,7 @@ namespace {
 using namespace attn;
 
 constexpr int KEYS = 32;      // keys per block
-constexpr int WAVES = 4;
+constexpr int WAVES = 4;      // of a workgroup; where it has a head of a request to itself and LDS allows, twice as many
 constexpr int FOLLOWED = 4;   // blocks of a wave whose maxima the reference follows
 
 template <class T, int D, int QB, int W>
@@ -48,8 +48,8 @@ struct Form {
   // The waves' tiles, or after the loop their O, references and denominators.
   static constexpr int TILES = W * 2 * TILE, TRIPLES = W * (QB * D * 64 + QB * 128);
   static constexpr int LDS = TILES > TRIPLES ? TILES : TRIPLES;
-  // Workgroups of a compute unit: by LDS, and by registers (a wave per SIMD each).
-  static constexpr int BY_LDS = 160 * 1024 / LDS, RESIDENT = BY_LDS >= 4 && QB == 1 ? 4 : BY_LDS >= 2 ? 2 : 1;
+  // Waves of a SIMD, and workgroups of a compute unit, by LDS and by registers.
+  static constexpr int BY_LDS = 160 * 1024 / LDS * W / 4, ON_SIMD = BY_LDS >= 4 && QB == 1 ? 4 : BY_LDS >= 2 ? 2 : 1, RESIDENT = ON_SIMD * 4 / W;
 };
 
 __device__ inline float over_lane_groups(float x) {   // the largest over the four lane groups, in all of them
@@ -60,7 +60,7 @@ __device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (t
 
 // The head dim may be below D, in whole 16-byte chunks: zeros behind it.
 template <class T, int D, int QB, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, D, QB, W>::RESIDENT))) void k_paged_attn(Kernargs) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, D, QB, W>::ON_SIMD))) void k_paged_attn(Kernargs) {
   using F = Form<T, D, QB, W>;
   constexpr bool BF16 = F::BF16;
   constexpr int ROW = F::ROW, TILE = F::TILE, LOADS = F::LOADS, HALF = F::HALF, NDB = F::NDB;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
 
   const bool direct = kernargs().w.direct;
   // NQ: of the QB columns of 16 rows, those that the tile has rows in.
-  auto run = [&](auto columns, const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
+  auto run = [&](auto columns, const Kernargs &k, const Piece &t, Worker *worker) {
     constexpr int NQ = decltype(columns)::value;
     const float c = k.c;
     const FastDiv by_group = k.by_group, by_page16 = k.by_page16;
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
       }
     }
   };
-  auto run_piece = [&](const Kernargs &k, const Piece &t, Worker<64 * W> *worker) {
+  auto run_piece = [&](const Kernargs &k, const Piece &t, Worker *worker) {
     if constexpr (!BF16 && QB > 1) {
       if (t.rows <= 16) return run(std::integral_constant<int, 1>{}, k, t, worker);
     }
@@ -444,8 +444,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
     if (direct_piece(kernargs(), &t)) run_piece(kernargs(), t, nullptr);
     return;
   }
-  Worker<64 * W> worker(kernargs(), reinterpret_cast<typename Worker<64 * W>::Shared *>(lds));
-  __syncthreads();
+  Worker worker(kernargs());
   while (worker.next(kernargs(), &t)) {
     run_piece(kernargs(), t, &worker);
     __syncthreads();   // (the triples have been read)
@@ -470,18 +469,18 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
 }
 
 // Calls f with the form's types and sizes.
+template <class T, int D, class F>
+auto with_rows(int qb, bool direct, F f) {
+  constexpr int MORE = Form<T, D, 1, 2 * WAVES>::LDS <= 160 * 1024 ? 2 * WAVES : WAVES;
+  if (direct) return qb == 1 ? f(Form<T, D, 1, MORE>()) : f(Form<T, D, 2, MORE>());
+  return qb == 1 ? f(Form<T, D, 1, WAVES>()) : f(Form<T, D, 2, WAVES>());
+}
 template <class F>
-auto with_form(const PagedAttnArgs &a, int qb, F f) {
-  constexpr int W = WAVES;
-  const bool narrow = a.head_dim <= 64;
-  if (a.dtype == MRL_BF16) {
-    if (narrow) return qb == 1 ? f(Form<__bf16, 64, 1, W>()) : f(Form<__bf16, 64, 2, W>());
-    return qb == 1 ? f(Form<__bf16, 128, 1, W>()) : f(Form<__bf16, 128, 2, W>());
-  }
-  if (narrow) return qb == 1 ? f(Form<float, 64, 1, W>()) : f(Form<float, 64, 2, W>());
-  if (a.head_dim <= 80) return qb == 1 ? f(Form<float, 80, 1, W>()) : f(Form<float, 80, 2, W>());
-  if (a.head_dim <= 96) return qb == 1 ? f(Form<float, 96, 1, W>()) : f(Form<float, 96, 2, W>());
-  return qb == 1 ? f(Form<float, 128, 1, W>()) : f(Form<float, 128, 2, W>());
+auto with_form(const PagedAttnArgs &a, int qb, bool direct, F f) {
+  if (a.dtype == MRL_BF16) return a.head_dim <= 64 ? with_rows<__bf16, 64>(qb, direct, f) : with_rows<__bf16, 128>(qb, direct, f);
+  if (a.head_dim <= 64) return with_rows<float, 64>(qb, direct, f);
+  if (a.head_dim <= 80) return with_rows<float, 80>(qb, direct, f);
+  return a.head_dim <= 96 ? with_rows<float, 96>(qb, direct, f) : with_rows<float, 128>(qb, direct, f);
 }
 template <class T, int D, int QB, int W>
 hipError_t launch_form(Form<T, D, QB, W>, const PagedAttnArgs &a, const Work &work, hipStream_t stream) {
@@ -490,12 +489,12 @@ hipError_t launch_form(Form<T, D, QB, W>, const PagedAttnArgs &a, const Work &wo
 }  // namespace
 
 void keys_work(const PagedAttnArgs &a, int qb, Work *w) {
-  w->workers = g_compute_units * with_form(a, qb, [](auto f) { return uint32_t(decltype(f)::RESIDENT); });
+  w->workers = g_compute_units * with_form(a, qb, false, [](auto f) { return uint32_t(decltype(f)::RESIDENT); });
   w->bq_log2 = qb == 1 ? 4 : 5, w->block_log2 = 5, w->least = WAVES, w->overhead = 3, w->second = 3 * WAVES;
 }
 
 hipError_t launch_keys(const PagedAttnArgs &a, const Work &work, int qb, hipStream_t stream) {
-  return with_form(a, qb, [&](auto f) { return launch_form(f, a, work, stream); });
+  return with_form(a, qb, work.direct, [&](auto f) { return launch_form(f, a, work, stream); });
 }
 
 }  // namespace paged
