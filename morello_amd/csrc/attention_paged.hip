@@ -111,59 +111,89 @@ struct MergeArgs {
   uint32_t bq, row_floats;   // rows of a tile
   FastDiv by_group, by_quads;
 };
-// U: pieces asked for at a time.
-template <class T, uint32_t U>
-__device__ inline void merge_rows(const PagedAttnArgs &p, const MergeArgs &a, const float *partials, uint32_t more, uint32_t piece_floats, int32_t start, uint32_t row0, uint32_t rows,
-                                  uint32_t kv) {
-  const uint32_t quads = (p.head_dim + 3) / 4, stat = a.row_floats - 4;
-  for (uint32_t x = blockIdx.y * THREADS + threadIdx.x; x < rows * quads; x += gridDim.y * THREADS) {
-    const uint32_t i = a.by_quads.div(x), dim = (x - i * quads) * 4;
-    // piece 0 lies in the first workgroup's place 1, the others in place 0 of those behind it
-    auto piece = [&](uint32_t v) { return partials + (2 * uint64_t(v) + (v == 0)) * piece_floats + i * a.row_floats; };
-    float m = -3.0e38f, l = 0;
-    attn::v4f sum = {0, 0, 0, 0};
-    for (uint32_t v0 = 0; v0 <= more; v0 += U) {
-      float ms[U], ls[U];
-      attn::v4f os[U];
+// Pieces put together so far.
+struct Sum {
+  float m, l;
+  attn::v4f o;
+};
+constexpr Sum NOTHING = {-3.0e38f, 0, {0, 0, 0, 0}};
+// Pieces first .. last of four dims of a row, U asked for at a time; from(v): the row's of piece v.
+template <uint32_t U, class F>
+__device__ inline Sum sum_of(uint32_t first, uint32_t last, uint32_t stat, uint32_t dim, F from) {
+  Sum s = NOTHING;
+  for (uint32_t v0 = first; v0 <= last; v0 += U) {
+    float ms[U], ls[U];
+    attn::v4f os[U];
 #pragma unroll
-      for (uint32_t u = 0; u < U; u++) {
-        const float *from = piece(min(v0 + u, more));
-        ms[u] = from[stat], ls[u] = from[stat + 1], os[u] = *(const attn::v4f *)(from + dim);
+    for (uint32_t u = 0; u < U; u++) {
+      const float *x = from(min(v0 + u, last));
+      ms[u] = x[stat], ls[u] = x[stat + 1], os[u] = *(const attn::v4f *)(x + dim);
+    }
+    float most = s.m;
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) most = fmaxf(most, ms[u]);
+    const float old = __builtin_amdgcn_exp2f(s.m - most);
+    s.o *= old, s.l *= old, s.m = most;
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+      if (v0 + u <= last) {
+        const float f = __builtin_amdgcn_exp2f(ms[u] - s.m);
+        s.o += os[u] * f, s.l += ls[u] * f;
       }
-      float most = m;
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) most = fmaxf(most, ms[u]);
-      const float old = __builtin_amdgcn_exp2f(m - most);
-      sum *= old, l *= old, m = most;
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++)
-        if (v0 + u <= more) {
-          const float f = __builtin_amdgcn_exp2f(ms[u] - m);
-          sum += os[u] * f, l += ls[u] * f;
-        }
-    }
-    sum *= l == 0.0f ? 0.0f : 1.0f / l;
-    const uint32_t row = row0 + i, token = a.by_group.div(row), head = kv * p.group + (row - token * p.group);
-    T *out = (T *)p.out + int64_t(start + int32_t(token)) * p.o_t + int64_t(head) * p.o_h + dim;
-    if constexpr (sizeof(T) == 2) {
-      typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
-      *(v4bf *)out = v4bf{(__bf16)sum[0], (__bf16)sum[1], (__bf16)sum[2], (__bf16)sum[3]};
-    } else {
-      *(attn::v4f *)out = sum;
-    }
   }
+  return s;
 }
-// blockIdx.x: the workgroup that begins the tile; blockIdx.y: a share of its rows.
+constexpr uint32_t MANY = 4;   // pieces from which on the waves of a workgroup share them
+// blockIdx.x: the workgroup that begins the tile; blockIdx.y: a share of its rows' dims, four to a thread.  What it takes is latency: a descriptor, then all pieces of a
+// thread at once.
 template <class T>
 __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, MergeArgs a) {
+  constexpr uint32_t WAVES = THREADS / 64;
+  __shared__ Sum met[WAVES][64];
   const uint32_t *d = a.merges + blockIdx.x * 8;
   const uint32_t piece_floats = a.bq * a.row_floats, more = d[0], row0 = d[2], rows = d[3], kv = d[4];
   const int32_t start = int32_t(d[1]);
   if (!more) return;
   const float *const partials = a.partials + 2 * uint64_t(blockIdx.x) * piece_floats;
-  if (more < 2) merge_rows<T, 2>(p, a, partials, more, piece_floats, start, row0, rows, kv);
-  else if (more < 4) merge_rows<T, 4>(p, a, partials, more, piece_floats, start, row0, rows, kv);
-  else merge_rows<T, 16>(p, a, partials, more, piece_floats, start, row0, rows, kv);
+  const uint32_t quads = (p.head_dim + 3) / 4, stat = a.row_floats - 4, all = rows * quads;
+  auto store = [&](const Sum &s, uint32_t i, uint32_t dim) {
+    const attn::v4f y = s.o * (s.l == 0.0f ? 0.0f : 1.0f / s.l);
+    const uint32_t row = row0 + i, token = a.by_group.div(row), head = kv * p.group + (row - token * p.group);
+    T *out = (T *)p.out + int64_t(start + int32_t(token)) * p.o_t + int64_t(head) * p.o_h + dim;
+    if constexpr (sizeof(T) == 2) {
+      typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+      *(v4bf *)out = v4bf{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]};
+    } else {
+      *(attn::v4f *)out = y;
+    }
+  };
+  // (piece 0 lies in the first workgroup's place 1, the others in place 0 of those behind it)
+  if (more < MANY) {
+    for (uint32_t x = blockIdx.y * THREADS + threadIdx.x; x < all; x += gridDim.y * THREADS) {
+      const uint32_t i = a.by_quads.div(x), dim = (x - i * quads) * 4;
+      auto from = [&](uint32_t v) { return partials + (2 * uint64_t(v) + (v == 0)) * piece_floats + i * a.row_floats; };
+      store(more < 2 ? sum_of<2>(0, more, stat, dim, from) : sum_of<MANY>(0, more, stat, dim, from), i, dim);
+    }
+    return;
+  }
+  const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64, each = more / WAVES + 1, first = wave * each, last = min(first + each - 1, more);
+  for (uint32_t x0 = blockIdx.y * 64; x0 < all; x0 += gridDim.y * 64) {
+    const uint32_t x = min(x0 + lane, all - 1), i = a.by_quads.div(x), dim = (x - i * quads) * 4;
+    auto from = [&](uint32_t v) { return partials + (2 * uint64_t(v) + (v == 0)) * piece_floats + i * a.row_floats; };
+    met[wave][lane] = first <= more ? sum_of<8>(first, last, stat, dim, from) : NOTHING;
+    __syncthreads();
+    if (wave == 0 && x0 + lane < all) {
+      Sum s = met[0][lane];
+#pragma unroll
+      for (uint32_t w = 1; w < WAVES; w++) {
+        const Sum &y = met[w][lane];
+        const float most = fmaxf(s.m, y.m), old = __builtin_amdgcn_exp2f(s.m - most), f = __builtin_amdgcn_exp2f(y.m - most);
+        s.o = s.o * old + y.o * f, s.l = s.l * old + y.l * f, s.m = most;
+      }
+      store(s, i, dim);
+    }
+    __syncthreads();
+  }
 }
 
 constexpr uint32_t DIRECT_KEYS = 1024;
