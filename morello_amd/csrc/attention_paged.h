@@ -107,16 +107,6 @@ struct Lengths {
   }
   __device__ uint32_t of(uint32_t t) const { return uint32_t(before(t + 1) - before(t)); }
   __device__ uint64_t all() const { return before(tiles); }
-  // The tile that holds place x.
-  __device__ uint32_t tile_at(uint64_t x) const {
-    uint32_t lo = 0, hi = tiles;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (before(mid) <= x) lo = mid;
-      else hi = mid;
-    }
-    return lo;
-  }
 };
 // A tile has at most (keys it sees) / 2^block_log2 + 2 blocks, and tile t sees at most at + (t + 1) * bq / G + 1 keys, or window + bq / G + 1.
 // (Two more, as the eighths of `slope` are rounded where they are summed.)
@@ -163,7 +153,8 @@ __device__ inline uint64_t of_lane(uint64_t x, int lane) { return uint64_t(of_la
 struct Worker {
   uint32_t number = xcd_run(blockIdx.x, gridDim.x);
   uint32_t request = 0xffffffffu, head = 0, tile = 0, at = 0;   // where it stands
-  Request q = {0, 0, 0};                                        // the request there
+  Request q = {0, 0, 0};                                        // the request there, and its tiles
+  Lengths l = {};
   uint32_t share = 1, left = 0;
   bool few = false, described = false;
 
@@ -171,6 +162,13 @@ struct Worker {
     Lengths l = lengths_of(k, q);
     if (few) l.grown = 0, l.most = quotient(uint64_t(most_blocks(k, q, l.tiles)) + share - 1, share) * share;
     return l;
+  }
+
+  // Takes the request that lane `it` has, of those from `first` on.
+  __device__ void stand(const Request &mine, const Lengths &of_mine, uint32_t first, int it) {
+    request = first + it;
+    q = {int32_t(of_lane(uint32_t(mine.n), it)), int32_t(of_lane(uint32_t(mine.start), it)), int32_t(of_lane(uint32_t(mine.length), it))};
+    l = {of_lane(of_mine.tiles, it), of_lane(of_mine.first, it), of_lane(of_mine.slope, it), of_lane(of_mine.most, it), of_lane(of_mine.grown, it)};
   }
 
   // Finds its start, a lane to a request.
@@ -201,22 +199,27 @@ struct Worker {
         mine = {0, 0, 0};
         if (r0 + lane < requests) mine = read_request(k.p, r0 + lane);
       }
-      Lengths l = {};
+      Lengths of_mine = {};
       uint64_t length = 0;
-      if (mine.n) l = lengths(k, mine), length = l.all();
+      if (mine.n) of_mine = lengths(k, mine), length = of_mine.all();
       const uint64_t sum = sums_up_to(length * heads), off = base + sum - length * heads;
       const bool here = mine.n && from >= off && from < base + sum;
       const uint64_t where = __ballot(here);
       if (where) {
-        uint32_t h = 0, t = 0, in_tile = 0;
-        if (here) {
-          h = quotient(from - off, length);
-          const uint64_t in_head = from - off - h * length;
-          t = l.tile_at(in_head), in_tile = uint32_t(in_head - l.before(t));
-        }
         const int it = __builtin_ctzll(where);
-        request = r0 + it, head = of_lane(h, it), tile = of_lane(t, it), at = of_lane(in_tile, it), left = share;
-        q = {int32_t(of_lane(uint32_t(mine.n), it)), int32_t(of_lane(uint32_t(mine.start), it)), int32_t(of_lane(uint32_t(mine.length), it))};
+        stand(mine, of_mine, r0, it);
+        const uint64_t all = of_lane(length, it), in_request = from - of_lane(off, it);
+        head = uniform(quotient(in_request, all)), left = share;
+        // The tile that holds the place in the head: the last that begins at or before it, found among 64 at a time.
+        const uint64_t in_head = in_request - head * all;
+        uint32_t step = 1;
+        while (step * 64 < l.tiles) step *= 64;
+        for (;; step /= 64) {
+          const uint32_t t = tile + lane * step;
+          tile += (__builtin_popcountll(__ballot(t < l.tiles && l.before(t) <= in_head)) - 1) * step;   // (of tiles that rise: the first lanes)
+          if (step == 1) break;
+        }
+        at = uniform(uint32_t(in_head - l.before(tile)));
         break;
       }
       base += of_lane(sum, 63);
@@ -226,7 +229,6 @@ struct Worker {
   // The next piece that has something to do; false: there is none.
   __device__ bool next(const Kernargs &k, Piece *out) {
     while (left) {
-      const Lengths l = lengths(k, q);
       const uint32_t length = uniform(l.of(tile));
       Piece t = tile_of(k, q, tile);
       t.request = request, t.head = head, t.b0 = min(at, t.blocks), t.b1 = min(at + min(left, length - at), t.blocks);
@@ -246,11 +248,7 @@ struct Worker {
             if (some) break;
           }
           left = some ? left : 0;
-          if (some) {
-            const int it = __builtin_ctzll(some);
-            request += it;
-            q = {int32_t(of_lane(uint32_t(mine.n), it)), int32_t(of_lane(uint32_t(mine.start), it)), int32_t(of_lane(uint32_t(mine.length), it))};
-          }
+          if (some) stand(mine, mine.n ? lengths(k, mine) : Lengths{}, request, __builtin_ctzll(some));
         }
       }
       if (any) {

@@ -221,7 +221,8 @@ Choice choose(const PagedAttnArgs &a) {
   if (!c.tiled) return c;
   const uint64_t rows = uint64_t(a.max_new) * a.group;
   paged::Work &w = c.work;
-  if (a.dtype == MRL_BF16 && rows > 32) {
+  const bool near = a.q_t < (1 << 22) && a.q_h < (1 << 28) / int64_t(a.group);   // (a tile's queries within 2 GB of its first)
+  if (a.dtype == MRL_BF16 && rows > 32 && near) {
     // Requests of few rows among others go the same way: a tile of 128 rows streams its keys at what memory delivers, too (a decoding step of 48 requests up to 16384
     // keys that way 167 us, on tiles of 16 rows 143; 18 such requests beside 6 chunks in a launch of their own on those: 53 us, 39 together).
     paged::chunk_work(a, &w);

@@ -29,8 +29,7 @@ struct Dims {
   static constexpr int ROW = D * 2, TILE = BKV * ROW, HALF = 5 * TILE;   // bytes of a row, of a block, of a half's tiles
   static constexpr int CHUNKS = ROW / 16, SLOTS = ROW / 32, ROWS_PER_LINE = ROW >= 256 ? 1 : 256 / ROW, ROWS_PER_LOAD = 1024 / ROW;
   static constexpr int PER_WAVE = 16 / ROWS_PER_LOAD;                    // loads of a wave's 16 keys
-  static constexpr int MERGE_ROWS = D / 2 + 4;                           // a lane's O, two references and two denominators
-  static constexpr int MERGE = QG * MERGE_ROWS * 64 * 4;
+  static constexpr int MEET = D / 16 + 1, MERGE = 2 * QG * MEET * 1024;   // quads of a lane where the halves meet: a sixteen of rows' O, reference and denominator
   static constexpr int LDS = 2 * HALF;
   static_assert(MERGE <= LDS, "what meets at the end lies where the tiles did");
   __device__ static constexpr int k_swizzle(int row) { return (row / ROWS_PER_LINE) & (CHUNKS - 1); }
@@ -89,19 +88,22 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
 
     // The places of this lane's two rows (a row sees the keys up to it, below t.end and, with a window, behind it less the window; -1 where the tile
     // has no such row), and the keys that all of the wave's rows see, [all_from, all_to).
+    // Q's operands go through V tiles 1 and 2 of half 1, which no fetch touches before that half's first slot of exponentials, as the lanes read them: each of the two waves that
+    // have the same rows asks for a sixteen of them.
     int32_t row_at[2];
-    v4i qf[2][NC];
+    static_assert(QG * D * 64 <= 2 * TILE, "the operands fit the two tiles");
+    const uint32_t first_token = uniform(by_group.div(t.row0));
+    const uint8_t *const q_first = (const uint8_t *)k.p.q + (int64_t(t.start + int32_t(first_token)) * k.p.q_t + int64_t(t.head * group) * k.p.q_h) * 2;
+    const uint32_t q_lds = lds_address(lds + HALF + 3 * TILE) + qg * (2 * NC * 1024);
 #pragma unroll
     for (int qb = 0; qb < 2; qb++) {
-      const uint32_t i = 32 * qg + 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = t.head * group + (row - token * group);
+      const uint32_t i = 32 * qg + 16 * qb + lr, row = t.row0 + min(i, t.rows - 1), token = by_group.div(row), head = row - token * group;
       row_at[qb] = i < t.rows ? t.at + int32_t(token) : -1;
-      if (!half) {
-        const uint8_t *q = (const uint8_t *)k.p.q + (int64_t(t.start + int32_t(token)) * k.p.q_t + int64_t(head) * k.p.q_h) * 2;
+      if (qb == half) {
+        const auto from = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uniform(reinterpret_cast<uint64_t>(q_first))), 0, int(OUTSIDE), 0x00020000);
+        const uint32_t at = ((token - first_token) * uint32_t(k.p.q_t) + head * uint32_t(k.p.q_h)) * 2;
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-          const uint32_t from = j * 64 + lgp * 16;
-          qf[qb][j] = from < row_bytes ? *(const v4i *)(q + from) : v4i{0, 0, 0, 0};
-        }
+        for (int j = 0; j < NC; j++) dma16(from, j * 64 + lgp * 16 < int(row_bytes) ? at + j * 64 + lgp * 16 : OUTSIDE, q_lds + (qb * NC + j) * 1024);
       }
     }
     const uint32_t wave_first = t.row0 + min(32u * qg, t.rows - 1), wave_last = t.row0 + min(32u * qg + 31, t.rows - 1);
@@ -172,7 +174,6 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
 
     v4f s[NKB][2];
     v8bf pb[NKC][2];
-    // Before the first slot: Q and half 0's K(0); behind the barrier V(0), K(1) and all of half 1's, which have half 0's first slot to land in.
     if (nblocks > 0) fetch_pages(0, gone_here, any_here);
     auto issue_k = [&](int kb) {
       span_of_v = span, span = next_span(kb);
@@ -185,35 +186,22 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
 #pragma unroll
       for (int i = 0; i < PER_WAVE; i++) dma16(from, v_src[i], v_dst0 + (kb % 3) * TILE + i * 1024);
     };
-    if (nblocks > 0 && !half) issue_k(0);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    {
-      // Q's operands from half 0 to half 1 through V tiles 1 and 2 of half 1, which no fetch touches before that half's first slot of exponentials.
-      static_assert(QG * D * 64 <= 2 * TILE, "the exchange fits the two tiles");
-      v4i *qx = (v4i *)(lds + HALF + 3 * TILE) + qg * (2 * NC * 64) + lane;
-      if (!half) {
-#pragma unroll
-        for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-          for (int j = 0; j < NC; j++) qx[(qb * NC + j) * 64] = qf[qb][j];
-      }
-      __syncthreads();
-      if (half) {
-#pragma unroll
-        for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-          for (int j = 0; j < NC; j++) qf[qb][j] = qx[(qb * NC + j) * 64];
-      }
-    }
+    // Before the first slot: Q and K(0), with V(0) and K(1) on their way.  Half 1 is a slot behind.
     if (nblocks > 0) {
-      if (half) issue_k(0);
+      issue_k(0);
       issue_v(0);
       issue_k(1);
+      __builtin_amdgcn_s_waitcnt(WAIT_BUT_TWO);
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
     }
-    if (half) {
-      __builtin_amdgcn_s_waitcnt(WAIT_BUT_TWO);   // K(0)
-      __syncthreads();
-    }
+    __syncthreads();
+    v4i qf[2][NC];
+#pragma unroll
+    for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+      for (int j = 0; j < NC; j++) qf[qb][j] = *(const v4i *)(lds + HALF + 3 * TILE + qg * (2 * NC * 1024) + (qb * NC + j) * 1024 + lane * 16);
+    if (half) __syncthreads();
     // Where a slot's operands are: formed in the slot and not kept (the compiler would hold all of them in registers over the loop, which has none to spare).
     auto here = [&](const uint8_t *tile, uint32_t at) {
       uint32_t x = uint32_t(tile - lds) + at;
@@ -455,19 +443,14 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     }
     if (!half) __syncthreads();
 
-    // The halves meet: (O, m, l) of half 1 through LDS to the wave of half 0 that has the same rows.  The fetches past the last block must not land on it.
-    const float l_own[2] = {den[0][0], den[1][0]};
+    // The halves meet in LDS: of the two waves that have the same rows, each puts a sixteen of them together.  The fetches past the last block must not land there.
     __builtin_amdgcn_s_waitcnt(0x0F70);
     __syncthreads();
-    constexpr int MQ = DD::MERGE_ROWS / 4;   // a lane's quads: O^T's blocks, then (m, m, l, l)
-    v4f *mbuf = (v4f *)lds + qg * (MQ * 64) + lane;
-    if (half) {
+    v4f *const given = (v4f *)lds + wave * (DD::MEET * 64) + lane;
+    const v4f *const taken = (const v4f *)lds + (wave ^ QG) * (DD::MEET * 64) + lane;
 #pragma unroll
-      for (int db = 0; db < NDB; db++)
-#pragma unroll
-        for (int qb = 0; qb < 2; qb++) mbuf[(db * 2 + qb) * 64] = o[db][qb];
-      mbuf[(NDB * 2) * 64] = v4f{m_run[0], m_run[1], l_own[0], l_own[1]};
-    }
+    for (int db = 0; db < NDB; db++) given[db * 64] = half ? o[db][0] : o[db][1];
+    given[NDB * 64] = half ? v4f{m_run[0], den[0][0], 0, 0} : v4f{m_run[1], den[1][0], 0, 0};
     __syncthreads();
     const Kernargs &e = kernargs();
     const bool whole = t.whole();
@@ -475,29 +458,26 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       worker.described = true;
       if (tid == 0) worker.describe(e.w, t);
     }
-    if (!half) {
-      float *const part = whole ? nullptr : worker.place(e.w, t, BQ * (D + 4));
-      const v4f ml = mbuf[(NDB * 2) * 64];
+    const uint32_t i = 32 * qg + 16 * half + lr;
+    if (i < t.rows) {
+      const v4f ml = taken[NDB * 64];
+      const float m_own = half ? m_run[1] : m_run[0], mm = fmaxf(m_own, ml[0]);
+      float own = __builtin_amdgcn_exp2f(m_own - mm), other = __builtin_amdgcn_exp2f(ml[0] - mm);
+      const float l = (half ? den[1][0] : den[0][0]) * own + ml[1] * other;
+      if (!whole) {
+        float *const to = worker.place(e.w, t, BQ * (D + 4)) + i * (D + 4);
 #pragma unroll
-      for (int qb = 0; qb < 2; qb++) {
-        const uint32_t i = 32 * qg + 16 * qb + lr;
-        const float m1 = ml[qb], l1 = ml[2 + qb], mm = fmaxf(m_run[qb], m1);
-        const float a0 = __builtin_amdgcn_exp2f(m_run[qb] - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm), l = l_own[qb] * a0 + l1 * a1;
-        if (i >= t.rows) continue;
-        if (!whole) {
-          float *to = part + i * (D + 4);
-#pragma unroll
-          for (int db = 0; db < NDB; db++) *(v4f *)(to + db * 16 + 4 * lgp) = o[db][qb] * a0 + mbuf[(db * 2 + qb) * 64] * a1;
-          if (lgp == 0) to[D] = mm, to[D + 1] = l;
-          continue;
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l, w0 = a0 * inv, w1 = a1 * inv;
+        for (int db = 0; db < NDB; db++) *(v4f *)(to + db * 16 + 4 * lgp) = (half ? o[db][1] : o[db][0]) * own + taken[db * 64] * other;
+        if (lgp == 0) to[D] = mm, to[D + 1] = l;
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        own *= inv, other *= inv;
         const uint32_t row = t.row0 + i, token = e.by_group.div(row), head = t.head * e.p.group + (row - token * e.p.group);
         __bf16 *out = (__bf16 *)e.p.out + int64_t(t.start + int32_t(token)) * e.p.o_t + int64_t(head) * e.p.o_h;
         typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int db = 0; db < NDB; db++) {
-          const v4f v = o[db][qb] * w0 + mbuf[(db * 2 + qb) * 64] * w1;
+          const v4f v = (half ? o[db][1] : o[db][0]) * own + taken[db * 64] * other;
           const uint32_t dim = db * 16 + 4 * lgp;
           if (dim < e.p.head_dim) *(v4bf *)(out + dim) = v4bf{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
         }
