@@ -62,6 +62,16 @@ __device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfir
 __device__ inline int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline uint64_t uniform(uint64_t x) { return uint64_t(uniform(uint32_t(x >> 32))) << 32 | uniform(uint32_t(x)); }
 
+// Of values' bits (two of bf16, one of f32): something but zero where one is infinite or no number: an exponent of ones runs over into the sign's bit.
+template <bool BF16>
+__device__ inline uint32_t not_finite(attn::v4i x) {
+  constexpr uint32_t EXPONENT = BF16 ? 0x7f807f80 : 0x7f800000, ONE = BF16 ? 0x00800080 : 0x00800000;
+  uint32_t over = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) over |= (uint32_t(x[j]) & EXPONENT) + ONE;
+  return over & (BF16 ? 0x80008000u : 0x80000000u);
+}
+
 // A request: its new tokens, their first row, and its length.
 struct Request {
   int32_t n, start, length;

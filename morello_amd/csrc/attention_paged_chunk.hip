@@ -36,8 +36,6 @@ struct Dims {
   __device__ static constexpr int v_swizzle(int row) { return (row / ROWS_PER_LINE) & (SLOTS - 1); }
 };
 
-__device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (two & 0x7f800000) == 0x7f800000; }   // NaN or infinity among them
-
 template <int D>
 __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
   typedef Dims<D> DD;
@@ -109,6 +107,9 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     const uint32_t wave_first = t.row0 + min(32u * qg, t.rows - 1), wave_last = t.row0 + min(32u * qg + 31, t.rows - 1);
     const int32_t all_to = min(t.at + int32_t(by_group.div(wave_first)) + 1, int32_t(t.end));
     const int32_t all_from = window ? int32_t(max(int64_t(t.at) + by_group.div(wave_last) - int64_t(window) + 1, int64_t(0))) : 0;
+    // (that all of the tile's see)
+    const int32_t tile_to = min(t.at + int32_t(first_token) + 1, int32_t(t.end));
+    const int32_t tile_from = window ? int32_t(max(int64_t(t.at) + by_group.div(t.row0 + t.rows - 1) - int64_t(window) + 1, int64_t(0))) : 0;
 
     // Of 64 of this half's blocks, a lane each: the page of this wave's sixteen keys and the place in it, and which blocks have sixteens on no page.
     // (K runs two blocks ahead: its numbers move on before the bits of the block whose scores are masked do.)
@@ -264,9 +265,10 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       for (int kb = 0; kb < NKB; kb++) s[kb][0] = s[kb][1] = v4f{0, 0, 0, 0};
     };
     using std::integral_constant;
-    // Of the block whose weights pb holds: which of its sixteens are on no page, and whether some row does not see it whole.
-    uint32_t gone_bits = 0;
-    bool masked = false;
+    // Of the block whose weights pb holds: which of its sixteens are on no page, and why some row does not see it whole: it does not see so far, or not so far back (with a window),
+    // or there is a sixteen on no page; `SOME`: one of these is true for a wave of this half.
+    constexpr uint32_t HIGH = 1, LOW = 2, GONE = 4, SOME = 8;
+    uint32_t gone_bits = 0, masked = 0;
     // What slot B of block j wants to know is found in slot A: slot B is the longer of the two with it (2040 cycles against 1400, of 2.4 us a step; a wave issues an
     // instruction every 6 or 7 cycles there, scalar ones too).
     uint32_t masked_next = 0;
@@ -278,7 +280,8 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
         for (int g = 0; g < NKB; g++) gone_here[g] = gone_next[g];
       }
       const int32_t key0 = int32_t((first_block + j) * BKV);
-      masked_next = uniform(uint32_t(key0 < all_from || key0 + BKV > all_to || ((any_here >> (j & 63)) & 1)));
+      const bool gone = (any_here >> (j & 63)) & 1;
+      masked_next = uniform((key0 + BKV > all_to ? HIGH : 0) | (key0 < all_from ? LOW : 0) | (gone ? GONE : 0) | (key0 + BKV > tile_to || key0 < tile_from || gone ? SOME : 0));
       span_of_v = span, span = next_span(j + 2);
       span.keys = uniform(span.keys), span.key_bytes = uniform(span.key_bytes);
       asm volatile("" : "+s"(span.keys), "+s"(span.key_bytes), "+s"(masked_next));   // (here, and not where it is used)
@@ -309,23 +312,27 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
         }
       }
     };
-    auto odd_values = [&](const uint8_t *lv) {
-      bool odd = false;
-#pragma unroll 4
-      for (int i = 0; i < TILE / 1024; i++) {
-        const v4i x = *(const v4i *)(lv + i * 1024 + lane * 16);
+    // Whether the values of a block that is masked for some wave are all finite is found in slot B, by each wave of the sixteen keys that it has fetched, and noted in the V tile that is free
+    // until the next slot B: zero where they are not.
+    auto note_values = [&](int vstage) {
+      asm volatile("" ::: "memory");
+      const uint8_t *const mine = my_lds + (2 + vstage) * TILE + qg * PER_WAVE * 1024 + lane * 16;
+      uint32_t odd = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) odd = odd || odd_bf16(x[j]);
-      }
-      return __any(odd);
+      for (int i = 0; i < PER_WAVE; i++) odd |= not_finite<true>(*(const v4i *)(mine + i * 1024));
+      const bool any = __any(odd != 0);
+      if (lane == 0) *(int *)(my_lds + (2 + (vstage + 2) % 3) * TILE + qg * 4) = any ? 0 : 1;
     };
-    // V of the block before slot j, in V tile `vstage`, for the second product.  Where the slow one has been done, zeros, in the V tile that is free in this slot:
+    // V of the block before slot j, in V tile `vstage`, for the second product.  Where the slow one has been done, zeros, in the tile with the notes (a note that another wave has
+    // overwritten was one of zero, or stood beside one):
     // the fast one then adds nothing but the denominators.  (Were it left out there, its sums would be in other registers after either branch.)
     auto values_of = [&](int j, int vstage) {
       const uint8_t *const lv = my_lds + (2 + vstage) * TILE;
-      if (!masked || !odd_values(lv)) return lv;
-      slow_product(j - 1, lv);
+      if (!(masked & (HIGH | LOW | GONE))) return lv;
       uint8_t *const zeros = my_lds + (2 + (vstage + 2) % 3) * TILE;
+      const v4i notes = *(const v4i *)zeros;
+      if (uniform(notes[0]) && uniform(notes[1]) && uniform(notes[2]) && uniform(notes[3])) return lv;
+      slow_product(j - 1, lv);
 #pragma unroll 1
       for (int i = 0; i < TILE / 1024; i++) *(v4i *)(zeros + i * 1024 + lane * 16) = v4i{0, 0, 0, 0};
       return (const uint8_t *)zeros;
@@ -338,23 +345,22 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       prepare(j);
       run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, lv, my_lds + (j & 1) * TILE);
     };
-    auto slot_b = [&](int j) {
+    auto slot_b = [&](int j, int vstage) {   // vstage: V tile of block j
       __builtin_amdgcn_s_setprio(PRIO_B);
       masked = masked_next;
-      const int32_t key0 = int32_t((first_block + j) * BKV);
       if (masked) {
-        gone_bits = 0;
+        const int32_t key0 = int32_t((first_block + j) * BKV);
+        if (masked & HIGH) {
 #pragma unroll
-        for (int g = 0; g < NKB; g++) gone_bits |= uint32_t((gone_here[g] >> (j & 63)) & 1) << g;
+          for (int qb = 0; qb < 2; qb++) {
+            const int32_t last = min(row_at[qb], int32_t(t.end) - 1) - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
 #pragma unroll
-        for (int qb = 0; qb < 2; qb++) {
-          const int32_t last = min(row_at[qb], int32_t(t.end) - 1) - key0 - 4 * lgp;   // (of this lane's four of each sixteen)
+            for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-          for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r > last ? hidden : s[kb][qb][r];
+              for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r > last ? hidden : s[kb][qb][r];
+          }
         }
-        if (window) {
+        if (masked & LOW) {
 #pragma unroll
           for (int qb = 0; qb < 2; qb++) {
             const int32_t first = int32_t(max(int64_t(row_at[qb]) - window + 1, int64_t(0))) - key0 - 4 * lgp;
@@ -364,9 +370,14 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
               for (int r = 0; r < 4; r++) s[kb][qb][r] = kb * 16 + r < first ? hidden : s[kb][qb][r];
           }
         }
+        gone_bits = 0;
+        if (masked & GONE) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
-          if ((gone_bits >> kb) & 1) s[kb][0] = s[kb][1] = v4f{hidden, hidden, hidden, hidden};
+          for (int g = 0; g < NKB; g++) gone_bits |= uint32_t((gone_here[g] >> (j & 63)) & 1) << g;
+#pragma unroll
+          for (int kb = 0; kb < NKB; kb++)
+            if ((gone_bits >> kb) & 1) s[kb][0] = s[kb][1] = v4f{hidden, hidden, hidden, hidden};
+        }
       }
       auto move_reference = [&]() {
 #pragma unroll
@@ -418,6 +429,7 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
               pb[kb / 2][qb][(kb % 2) * 4 + r] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qb][r], c, -m_run[qb]));
       }
       __builtin_amdgcn_s_waitcnt(WAIT_BUT_TWO);
+      if (masked) note_values(vstage);
     };
     // Every wave passes steps + 1 pairs of barriers; a half with fewer blocks idles through the rest.
     if (nblocks > 0) {
@@ -426,14 +438,14 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       run_steps(integral_constant<int, PV_STEPS>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, my_lds, my_lds);
     }
     __syncthreads();
-    if (nblocks > 0) slot_b(0);
+    if (nblocks > 0) slot_b(0, 0);
     __syncthreads();
     int vstage = 0;   // V tile of block j - 1
     for (int j = 1; j < nblocks; j++) {
       slot_a(j, vstage);
       vstage = vstage == 2 ? 0 : vstage + 1;
       __syncthreads();
-      slot_b(j);
+      slot_b(j, vstage);
       __syncthreads();
     }
     if (nblocks > 0) run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS>{}, values_of(nblocks, vstage), my_lds);

@@ -56,7 +56,6 @@ __device__ inline float over_lane_groups(float x) {   // the largest over the fo
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
 }
-__device__ inline bool odd_bf16(int two) { return (two & 0x7f80) == 0x7f80 || (two & 0x7f800000) == 0x7f800000; }   // NaN or infinity among them
 
 // The head dim may be below D, in whole 16-byte chunks: zeros behind it.
 template <class T, int D, int QB, int W>
@@ -282,16 +281,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
         if (more) __builtin_amdgcn_s_waitcnt(ALL_BUT_ONE_TILE);   // V of this block is in; K of the next may still be under way
         else __builtin_amdgcn_s_waitcnt(ALL);
         asm volatile("" ::: "memory");
-        bool odd = false;   // a value that is not finite, in a block that not every row sees whole: a weight of zero would not hide it
+        uint32_t odd = 0;   // a value that is not finite, in a block that not every row sees whole: a weight of zero would not hide it
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < TILE / 1024; i++) {
-            const v4i x = *(const v4i *)(v_tile + i * 1024 + lane * 16);
-#pragma unroll
-            for (int j = 0; j < 4; j++) odd = odd || (BF16 ? odd_bf16(x[j]) : (x[j] & 0x7f800000) == 0x7f800000);
-          }
+          for (int i = 0; i < TILE / 1024; i++) odd |= not_finite<BF16>(*(const v4i *)(v_tile + i * 1024 + lane * 16));
         }
-        if (__any(odd)) {
+        if (__any(odd != 0)) {
           // A key at a time, its values against its weights alone, and of the product only the columns (query rows) that see it.
           if constexpr (BF16) {
 #pragma unroll 1
