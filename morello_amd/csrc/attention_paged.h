@@ -279,16 +279,23 @@ struct Worker {
   }
 };
 
-// In a `direct` launch: the workgroup's one tile, as a whole; false: it has none.
-__device__ inline bool direct_piece(const Kernargs &k, Piece *out) {
-  const uint32_t worker = xcd_run(blockIdx.x, gridDim.x), request = worker / k.p.kv_heads;
-  Request q = read_request(k.p, request);
-  q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
-  if (!q.n) return false;
-  *out = tile_of(k, q, 0);
-  out->request = request, out->head = worker - request * k.p.kv_heads;
-  return true;
-}
+// In a `direct` launch: a request's head to a workgroup, tile after tile (one, where max_new says what is so).
+struct DirectWorker {
+  uint32_t request, head, tile = 0;
+  Request q;
+  __device__ DirectWorker(const Kernargs &k) {
+    const uint32_t worker = xcd_run(blockIdx.x, gridDim.x);
+    request = worker / k.p.kv_heads, head = worker - request * k.p.kv_heads;
+    q = read_request(k.p, request);
+    q.n = uniform(q.n), q.start = uniform(q.start), q.length = uniform(q.length);
+  }
+  __device__ bool next(const Kernargs &k, Piece *out) {
+    if (uint64_t(tile) << k.w.bq_log2 >= uint64_t(q.n) * k.p.group) return false;
+    *out = tile_of(k, q, tile++);
+    out->request = request, out->head = head;
+    return true;
+  }
+};
 
 // Floats of a row of a partial result: O of the head dim the kernels are built for, reference, denominator, and two that are not used.
 inline uint32_t kernel_dims(const PagedAttnArgs &a) { return a.head_dim <= 64 ? 64 : a.dtype == MRL_F32 && a.head_dim <= 96 ? (a.head_dim <= 80 ? 80 : 96) : 128; }

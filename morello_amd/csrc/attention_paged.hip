@@ -196,8 +196,6 @@ __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, M
   }
 }
 
-constexpr uint32_t DIRECT_KEYS = 1024;
-
 // How a call runs, by sizes, types and strides.
 struct Choice {
   bool tiled = false;        // else the generic kernel
@@ -230,9 +228,10 @@ Choice choose(const PagedAttnArgs &a) {
     c.qb = rows <= 16 ? 1 : 2;
     paged::keys_work(a, c.qb, &w);
     w.once = rows <= 16u * c.qb;
-    // Tables of some hundred keys at most: a workgroup to each request and head does them in some rounds, with nothing to find out before and no launch behind.
-    // (max_new is the program's word: a request of more tokens would have more tiles than one, unless all rows there are make no second one)
-    w.direct = uint64_t(a.tokens) * a.group <= 16u * c.qb && uint64_t(a.width) * a.page_size <= DIRECT_KEYS;
+    // Tables of some hundred keys: a request's head to a workgroup, with nothing to find out before and no launch behind.  us, so and shared out: bf16, 4 requests and 16 heads of
+    // 128 dims 9.1 and 14.0 at 512 keys, 15.3 and 18.2 at 1024, 27.5 and 22.3 at 2048; 16 requests and 8 such heads 10.2 and 17.6, 17.0 and 21.3, 30.0 and 33.9; 2 requests and a
+    // head of 64 dims 5.8 and 9.7, 8.7 and 10.0, 12.9 and 10.3; f32, the first 20.2 and 19.8 at 512, 33.9 and 24.4 at 1024.
+    w.direct = w.once && uint64_t(a.width) * a.page_size <= (a.dtype == MRL_BF16 ? 1024u : 512u);
   }
   if (!w.direct) {
     c.partial_bytes = (size_t(2 * w.workers) << w.bq_log2) * paged::row_floats(a) * sizeof(float);

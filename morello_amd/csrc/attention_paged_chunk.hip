@@ -516,9 +516,9 @@ hipError_t launch_one(const PagedAttnArgs &a, Work work, hipStream_t stream) {
 
 }  // namespace
 
-void chunk_work(const PagedAttnArgs &, Work *w) {
+void chunk_work(const PagedAttnArgs &a, Work *w) {
   w->workers = g_compute_units;   // (one of D = 128 to a compute unit's LDS)
-  w->bq_log2 = 7, w->block_log2 = 6, w->least = 8, w->overhead = 7, w->second = 7;
+  w->bq_log2 = 7, w->block_log2 = 6, w->least = 8, w->overhead = a.head_dim <= 64 ? 7 : 4, w->second = 7;
 }
 
 hipError_t launch_chunk(const PagedAttnArgs &a, const Work &work, hipStream_t stream) {

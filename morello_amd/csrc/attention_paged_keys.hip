@@ -436,7 +436,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(Form<T, 
   };
   Piece t;
   if (direct) {
-    if (direct_piece(kernargs(), &t)) run_piece(kernargs(), t, nullptr);
+    DirectWorker worker(kernargs());
+    while (worker.next(kernargs(), &t)) {
+      run_piece(kernargs(), t, nullptr);
+      __syncthreads();   // (the triples have been read)
+    }
     return;
   }
   Worker worker(kernargs());

@@ -62,6 +62,56 @@ def test_many_requests(gpu, dtype):
     run_and_check(Batch(dtype, [(c, min(n, 1)) for c, n in lengths], 2, 2, 64, 16, seed=19))
 
 
+def widened(batch, keys):
+    """With a table that has room for so many keys of a request: small tables and large ones are dealt to workgroups in ways of their own."""
+    width = -(-keys // batch.page)
+    batch.table = np.pad(batch.table, ((0, 0), (0, width - batch.width)), constant_values=-1)
+    batch.width = width
+    return batch
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,dim", [((4, 1), 64), ((6, 2), 128), ((3, 3), 80), ((16, 1), 96)])
+@pytest.mark.parametrize("lengths", [DECODE, CHUNKS], ids=["decode", "chunks"])
+def test_wide_tables(gpu, dtype, heads, dim, lengths):
+    run_and_check(widened(Batch(dtype, lengths, *heads, dim, 16, seed=51), 5000))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_requests_in_wide_tables(gpu, dtype):
+    rng = np.random.default_rng(2)
+    lengths = [(int(c), int(n)) for c, n in zip(rng.integers(0, 30, 700), rng.choice([0, 1, 1, 1, 2], 700))]
+    run_and_check(widened(Batch(dtype, lengths, 2, 1, 32, 16, seed=52), 2000))
+    run_and_check(widened(Batch(dtype, [(c, min(n, 1)) for c, n in lengths], 2, 2, 64, 16, seed=53), 2000))
+    lengths = [(int(c), int(n)) for c, n in zip(rng.integers(0, 300, 130), rng.choice([0, 0, 0, 1, 40], 130))]
+    run_and_check(widened(Batch(dtype, lengths, 4, 2, 64, 16, seed=54), 2000), window=100)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("keys", [400, 3000])
+def test_more_new_tokens_than_the_bound_says(gpu, dtype, keys):
+    """max_new is taken at its word for choosing kernels only: requests of more tokens have more tiles than one."""
+    run_and_check(widened(Batch(dtype, [(0, 1), (100, 70), (17, 33), (0, 0), (250, 2)], 4, 2, 64, 16, seed=55), keys), max_new=1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_queries_far_apart(gpu, dtype):
+    """Tokens whose queries lie 8 MB and more apart: past what one resource over a tile's queries would hold."""
+    b = widened(Batch(dtype, [(0, 20), (90, 3)], 2, 1, 64, 16, seed=56, spare_rows=0), 2000)
+    stride, size = 1 << 22, b.q.itemsize
+    q = M.DeviceBuffer(((b.tokens - 1) * stride + b.q_heads * b.dim) * size)
+    for t in range(b.tokens):
+        row = np.ascontiguousarray(b.q[t])
+        M._check(M.B.load().mrl_memcpy_h2d(q.ptr + t * stride * size, row.ctypes.data, row.nbytes), "mrl_memcpy_h2d")
+    op = b.op(max_new=20, q_strides=(stride, b.dim))
+    out = np.full((b.tokens, b.q_heads, b.dim), 5, np.float32).astype(b.q.dtype) if dtype == "f32" else np.full((b.tokens, b.q_heads, b.dim), 0x40a0, np.uint16)
+    bufs = [M.DeviceBuffer.from_numpy(a) for a in (b.keys, b.values, b.table, b.starts, b.totals, out, np.full(max(16, op.workspace_bytes()), 0xff, np.uint8))]
+    op.run_device([q.ptr] + [x.ptr for x in bufs])
+    b.check(bufs[5].to_numpy(out.dtype, out.shape))
+    for x in bufs + [q]:
+        x.free()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_rows_that_see_nothing(gpu, dtype):
     """Lengths below the new tokens, of zero and below; tables whose numbers lie outside the cache, or which end before the length: zeros where
