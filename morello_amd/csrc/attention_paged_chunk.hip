@@ -10,7 +10,13 @@
 //     scores masked;  there, where values are not all finite, the second product goes key by key, for a weight of zero would not hide them;
 //   - exponentials in base 2 of s * c - m with c = scale * log2 e;
 //   - work comes in pieces (attention_paged.h).
-// What bounds it: the issue of MFMA and vector instructions, as there.
+// What bounds it: the issue of MFMA and vector instructions, as there.  2048 new tokens behind 6001, 32 heads on 8 of 128 dims: 236 GFLOP in 225 to 258 us (the clock falls to 1.7 to 1.9 GHz under it),
+// 0.9 to 1.05 PFLOP/s, the matrix cores busy for 48 % of the cycles: per two blocks of keys a slot of products of 1400 cycles and one of exponentials of 2040, beside the other half's.
+// Short pieces cost more: finding the share 2.5 us, then per piece 1.5 (the tile's numbers), 2.2 (queries and pages, then keys), two slots more than blocks, and 1.3 for the meeting.  18 requests'
+// single tokens and 6 chunks of 100 to 777, heads of 64 dims: 4228 blocks, 17 to a workgroup in two or three pieces, 31 us, 15 % busy; 9 requests with a window of 1024, 5 chunks, 96 dims:
+// 52 us, 25 % busy.
+// Tried and left: waves without a row leaving out their products (286 us for 275: the branch costs the others more); for 64 dims tiles of 64 rows, two workgroups of four waves to a compute unit
+// (33.9 us for 31.4).
 #include <algorithm>
 
 #include "attention_paged.h"

@@ -8,7 +8,8 @@
 // have some among them leave a mark at their first, and the largest mark up to a token names its request.  Every page that is
 // drawn begins with a new token (the cached ones end in a page before), so the token that opens a page writes its column
 // of the table; slots on a page of an earlier step come from the table, whose columns below ceil(c / P) nobody writes.
-// What bounds it: the launch, and the trips to memory behind each other (lengths, then pages).
+// What bounds it: the launch, and the trips to memory behind each other (lengths, then pages): 16 requests' single tokens 5.4 us, 67 requests' 11 027 tokens and 171 new pages 6.4 us,
+// of which an empty launch takes 2 to 3.
 #include "paged.h"
 
 namespace mrl {
