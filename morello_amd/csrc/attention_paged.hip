@@ -209,12 +209,12 @@ Choice choose(const PagedAttnArgs &a) {
   const int size = a.dtype == MRL_BF16 ? 2 : 4;
   auto chunks = [&](int64_t n) { return n * size % 16 == 0; };
   const double scale = std::fabs(a.scale);
-  // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, the slots of a page, and neighbouring pages, within 2 GB; a line of blocks that
-  // 256 shares of 32 bits cover.
+  // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, the slots of a page, and neighbouring pages, within 2 GB; places of
+  // keys that some blocks more do not take past 31 bits; a line of blocks that 256 shares of 32 bits cover.
   c.tiled = a.page_size % 16 == 0 && a.head_dim <= 128 && chunks(a.head_dim) && chunks(a.q_t) && chunks(a.q_h) && chunks(a.o_t) && chunks(a.o_h) && chunks(a.key_p) &&
             chunks(a.key_s) && chunks(a.key_h) && chunks(a.val_p) && chunks(a.val_s) && chunks(a.val_h) && a.key_s < (1 << 24) && a.val_s < (1 << 24) &&
             a.key_p < (1 << 29) && a.val_p < (1 << 29) && a.key_s * a.page_size < (1 << 29) && a.val_s * a.page_size < (1 << 29) &&
-            uint64_t(a.tokens) * a.group < (1u << 31) &&
+            uint64_t(a.tokens) * a.group < (1u << 31) && uint64_t(a.width) * a.page_size <= 0x7fff0000u &&
             (double(a.tokens) * a.group / 16 + a.requests) * a.kv_heads * (double(a.width) * a.page_size / 32 + 16) < double(1ull << 39) && scale > 1e-30 && scale < 1e30;
   if (!c.tiled) return c;
   const uint64_t rows = uint64_t(a.max_new) * a.group;
@@ -231,7 +231,8 @@ Choice choose(const PagedAttnArgs &a) {
     // Tables of some hundred keys: a request's head to a workgroup, with nothing to find out before and no launch behind.  us, so and shared out: bf16, 4 requests and 16 heads of
     // 128 dims 9.1 and 14.0 at 512 keys, 15.3 and 18.2 at 1024, 27.5 and 22.3 at 2048; 16 requests and 8 such heads 10.2 and 17.6, 17.0 and 21.3, 30.0 and 33.9; 2 requests and a
     // head of 64 dims 5.8 and 9.7, 8.7 and 10.0, 12.9 and 10.3; f32, the first 20.2 and 19.8 at 512, 33.9 and 24.4 at 1024.
-    w.direct = w.once && uint64_t(a.width) * a.page_size <= (a.dtype == MRL_BF16 ? 1024u : 512u);
+    // (A million workgroups are still a launch.)
+    w.direct = w.once && uint64_t(a.width) * a.page_size <= (a.dtype == MRL_BF16 ? 1024u : 512u) && uint64_t(a.requests) * a.kv_heads <= 1u << 20;
   }
   if (!w.direct) {
     c.partial_bytes = (size_t(2 * w.workers) << w.bq_log2) * paged::row_floats(a) * sizeof(float);

@@ -95,3 +95,17 @@ def test_plans():
     # 16 bytes at a time, or an element where a stride or a section does not allow that
     assert "V = 8" in rotary(sections=[16, 8, 8]).plan().steps[0].kernel and "V = 1" in rotary(q_strides=(513, 64)).plan().steps[0].kernel
     assert "V = 4" in rotary(M.f32).plan().steps[0].kernel and "V = 1" in rotary(sections=[3]).plan().steps[0].kernel
+
+
+def test_which_kernels_attention_takes():
+    """By the rows that a request may have, the type and what a table holds; strides and sizes that the tiles cannot take go to the generic kernel."""
+    steps = lambda **given: [s.kernel.split(" ")[0] for s in attention(**given).plan().steps]
+    shared, direct, generic = ["k_paged_attn", "k_paged_attn_merge"], ["k_paged_attn"], ["k_paged_attn_generic"]
+    assert steps(max_new=1) == steps(max_new=1, table_width=64) == steps(max_new=1, table_width=32, dtype=M.f32) == direct
+    assert steps(max_new=1, table_width=65) == steps(max_new=1, table_width=33, dtype=M.f32) == steps() == steps(dtype=M.f32) == shared
+    assert steps(head_dim=136) == steps(head_dim=12) == steps(page_size=24) == steps(q_strides=(516, 64)) == steps(key_strides=(1 << 24, 1 << 24, 64)) == generic
+    # a workgroup to a request's head only where that is a launch
+    assert steps(max_new=1, requests=1 << 19, q_heads=2) == direct and steps(max_new=1, requests=1 << 20, q_heads=2) == shared
+    # places of keys near 2^31
+    assert steps(requests=1, table_width=(0x7fff0000 >> 4), pages=64) == shared and steps(requests=1, table_width=(0x7fff0000 >> 4) + 1, pages=64) == generic
+    assert attention(max_new=1).workspace_bytes() == 0 and attention(head_dim=136).workspace_bytes() == 0 and attention().workspace_bytes() > 0
