@@ -11,7 +11,8 @@
 //   - exponentials in base 2 of s * c - m with c = scale * log2 e;
 //   - work comes in pieces (attention_paged.h).
 // What bounds it: the issue of MFMA and vector instructions, as there.  2048 new tokens behind 6001, 32 heads on 8 of 128 dims: 236 GFLOP in 225 to 258 us (the clock falls to 1.7 to 1.9 GHz under it),
-// 0.9 to 1.05 PFLOP/s, the matrix cores busy for 48 % of the cycles: per two blocks of keys a slot of products of 1400 cycles and one of exponentials of 2040, beside the other half's.
+// 0.9 to 1.05 PFLOP/s, the matrix cores busy for 48 % of the cycles: per two blocks of keys a slot of products of 1880 cycles (its 68 MFMAs take 1088) and one of exponentials of 1680, beside the other half's;
+// no wave waits for memory.
 // Short pieces cost more: finding the share 2.5 us, then per piece 1.5 (the tile's numbers), 2.2 (queries and pages, then keys), two slots more than blocks, and 1.3 for the meeting.  18 requests'
 // single tokens and 6 chunks of 100 to 777, heads of 64 dims: 4228 blocks, 17 to a workgroup in two or three pieces, 31 us, 15 % busy; 9 requests with a window of 1024, 5 chunks, 96 dims:
 // 52 us, 25 % busy.
@@ -142,24 +143,15 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       uint32_t key_bytes, value_bytes;
     };
     const uint32_t page_slots = k.p.page_size, place_step = uniform(BKV % page_slots);
-    const bool alike = k_slot == v_slot && key_page == val_page;   // (what keys and values have in common need not be found twice)
     uint32_t place = uniform((first_block * BKV + 16 * qg) % page_slots);
-    // Blocks whose sixteen are seen whole.
-    const int whole_blocks = t.end < uint32_t(16 * qg + 16) ? 0 : min(nblocks, int((t.end - 16 * qg - 16) / BKV + 1) - int(first_block));
-    auto next_span = [&](int kb) {
-      const int32_t page = __builtin_amdgcn_readlane(page_here, kb & 63);
-      uint32_t rows = 16;
-      if (kb >= whole_blocks) {
-        const uint32_t from = (first_block + kb) * BKV + 16 * qg;
-        rows = kb >= nblocks || from >= t.end ? 0 : min(t.end - from, 16u);
-      }
-      if (page < 0) rows = 0;
+    auto next_span = [&](int kb) {   // (without branches: the slot goes on beside it)
+      const int32_t page = __builtin_amdgcn_readlane(page_here, kb & 63), seen = int32_t(t.end) - int32_t((first_block + kb) * BKV + 16 * qg);
+      const uint32_t rows = page < 0 || kb >= nblocks ? 0 : uint32_t(min(max(seen, 0), 16));
       Span s;
       s.keys = uint64_t(uint32_t(page)) * uint32_t(key_page) + uint64_t(place * k_slot), s.key_bytes = rows ? (rows - 1) * k_slot + row_bytes : 0;
-      s.values = s.keys, s.value_bytes = s.key_bytes;
-      if (!alike) s.values = uint64_t(uint32_t(page)) * uint32_t(val_page) + uint64_t(place * v_slot), s.value_bytes = rows ? (rows - 1) * v_slot + row_bytes : 0;
+      s.values = uint64_t(uint32_t(page)) * uint32_t(val_page) + uint64_t(place * v_slot), s.value_bytes = rows ? (rows - 1) * v_slot + row_bytes : 0;
       place += place_step;
-      if (place >= page_slots) place -= page_slots;
+      place -= place >= page_slots ? page_slots : 0;
       return s;
     };
     auto resource = [](const uint8_t *head, uint64_t at, uint32_t bytes) {
@@ -278,19 +270,23 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     // What slot B of block j wants to know is found in slot A: slot B is the longer of the two with it (2040 cycles against 1400, of 2.4 us a step; a wave issues an
     // instruction every 6 or 7 cycles there, scalar ones too).
     uint32_t masked_next = 0;
-    auto prepare = [&](int j) {
+    auto prepare_pages = [&](int j) {
       if (((j + 2) & 63) == 0) fetch_pages(j + 2, gone_next, any_next);
       if ((j & 63) == 0 && j) {
         any_here = any_next;
 #pragma unroll
         for (int g = 0; g < NKB; g++) gone_here[g] = gone_next[g];
       }
+    };
+    auto prepare = [&](int j) {
       const int32_t key0 = int32_t((first_block + j) * BKV);
       const bool gone = (any_here >> (j & 63)) & 1;
-      masked_next = uniform((key0 + BKV > all_to ? HIGH : 0) | (key0 < all_from ? LOW : 0) | (gone ? GONE : 0) | (key0 + BKV > tile_to || key0 < tile_from || gone ? SOME : 0));
+      masked_next = (key0 + BKV > all_to ? HIGH : 0) | (key0 < all_from ? LOW : 0) | (gone ? GONE : 0) | (key0 + BKV > tile_to || key0 < tile_from || gone ? SOME : 0);
       span_of_v = span, span = next_span(j + 2);
-      span.keys = uniform(span.keys), span.key_bytes = uniform(span.key_bytes);
-      asm volatile("" : "+s"(span.keys), "+s"(span.key_bytes), "+s"(masked_next));   // (here, and not where it is used)
+    };
+    auto prepared = [&]() {   // (here, and not where it is used)
+      masked_next = uniform(masked_next), span.keys = uniform(span.keys), span.key_bytes = uniform(span.key_bytes), span.values = uniform(span.values), span.value_bytes = uniform(span.value_bytes);
+      asm volatile("" : "+s"(span.keys), "+s"(span.key_bytes), "+s"(masked_next), "+s"(span.values), "+s"(span.value_bytes));
     };
     // The second product of a masked block whose values are not all finite: a key at a time, its values against its weights alone, and of the product only the
     // columns (rows of queries) that see it.
@@ -348,8 +344,10 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
       __builtin_amdgcn_s_setprio(PRIO_A);
       zero_s();
       const uint8_t *const lv = values_of(j, vstage);
+      prepare_pages(j);
       prepare(j);
       run_steps(integral_constant<int, 0>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, lv, my_lds + (j & 1) * TILE);
+      prepared();
     };
     auto slot_b = [&](int j, int vstage) {   // vstage: V tile of block j
       __builtin_amdgcn_s_setprio(PRIO_B);
@@ -440,7 +438,9 @@ __global__ __launch_bounds__(TH) void k_paged_attn(Kernargs) {
     // Every wave passes steps + 1 pairs of barriers; a half with fewer blocks idles through the rest.
     if (nblocks > 0) {
       zero_s();
+      prepare_pages(0);
       prepare(0);
+      prepared();
       run_steps(integral_constant<int, PV_STEPS>{}, integral_constant<int, PV_STEPS + QK_STEPS>{}, my_lds, my_lds);
     }
     __syncthreads();
