@@ -142,20 +142,6 @@ __device__ inline uint32_t most_blocks(const Kernargs &k, const Request &q, uint
                     : max(last.blocks, 1u);
 }
 
-// Sums over the lanes up to each.
-template <int CTRL, int ROWS>
-__device__ inline uint64_t moved(uint64_t x) {
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(x)), CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(x >> 32)), CTRL, ROWS, 0xf, false);
-  return uint64_t(hi) << 32 | lo;
-}
-__device__ inline uint64_t sums_up_to(uint64_t x) {
-  x += moved<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8: within sixteens
-  x += moved<0x112, 0xf>(x);
-  x += moved<0x114, 0xf>(x);
-  x += moved<0x118, 0xf>(x);
-  x += moved<0x142, 0xa>(x);   // row_bcast 15, 31: the last of a sixteen, of a half, to those behind
-  return x + moved<0x143, 0xc>(x);
-}
 __device__ inline uint32_t of_lane(uint32_t x, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(x), lane)); }
 __device__ inline uint64_t of_lane(uint64_t x, int lane) { return uint64_t(of_lane(uint32_t(x >> 32), lane)) << 32 | of_lane(uint32_t(x), lane); }
 

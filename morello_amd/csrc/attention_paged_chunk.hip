@@ -14,10 +14,10 @@
 // 0.9 to 1.05 PFLOP/s, the matrix cores busy for 48 % of the cycles: per two blocks of keys a slot of products of 1880 cycles (its 68 MFMAs take 1088) and one of exponentials of 1680, beside the other half's;
 // no wave waits for memory.
 // Short pieces cost more: finding the share 2.5 us, then per piece 1.5 (the tile's numbers), 2.2 (queries and pages, then keys), two slots more than blocks, and 1.3 for the meeting.  18 requests'
-// single tokens and 6 chunks of 100 to 777, heads of 64 dims: 4228 blocks, 17 to a workgroup in two or three pieces, 31 us, 15 % busy; 9 requests with a window of 1024, 5 chunks, 96 dims:
+// single tokens and 6 chunks of 100 to 777, heads of 64 dims: 4228 blocks, 17 to a workgroup in two or three pieces, 30 us, 15 % busy; 9 requests with a window of 1024, 5 chunks, 96 dims:
 // 52 us, 25 % busy.
 // Tried and left: waves without a row leaving out their products (286 us for 275: the branch costs the others more); for 64 dims tiles of 64 rows, two workgroups of four waves to a compute unit
-// (33.9 us for 31.4).
+// (33.9 us where these took 31.4).
 #include <algorithm>
 
 #include "attention_paged.h"

@@ -8,7 +8,7 @@
 // have some among them leave a mark at their first, and the largest mark up to a token names its request.  Every page that is
 // drawn begins with a new token (the cached ones end in a page before), so the token that opens a page writes its column
 // of the table; slots on a page of an earlier step come from the table, whose columns below ceil(c / P) nobody writes.
-// What bounds it: the launch, and the trips to memory behind each other (lengths, then pages): 16 requests' single tokens 5.4 us, 67 requests' 11 027 tokens and 171 new pages 6.4 us,
+// What bounds it: the launch, and the trips to memory behind each other (lengths, then pages): 16 requests' single tokens 4.8 us, 67 requests' 11 027 tokens and 171 new pages 6.0 us (with shuffles for the scans 5.3 and 6.4),
 // of which an empty launch takes 2 to 3.
 #include "paged.h"
 
@@ -21,12 +21,7 @@ constexpr int PASS = THREADS * EACH, WAVES = THREADS / 64;
 // x: the sum over the threads before this one; returns the sum over all.
 __device__ inline uint64_t scan(uint64_t &x, uint64_t *wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t sum = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t below = __shfl_up(sum, d);
-    if (lane >= d) sum += below;
-  }
+  const uint64_t sum = paged::sums_up_to(x);
   __syncthreads();   // (the sums of the scan before have been read)
   if (lane == 63) wave_sums[wave] = sum;
   __syncthreads();
@@ -109,11 +104,7 @@ __global__ __launch_bounds__(THREADS) void k_page_tables(PageTablesArgs p, FastD
 #pragma unroll
   for (int i = 0; i < EACH; i++) last = max(last, mark[tid * EACH + i]), own[i] = last;
   const int lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int32_t below = __shfl_up(last, d);
-    if (lane >= d) last = max(last, below);
-  }
+  last = paged::largest_up_to(last, -1);
   if (lane == 63) wave_marks[wave] = last;
   int32_t before = __shfl_up(last, 1);
   if (lane == 0) before = -1;

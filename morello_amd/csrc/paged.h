@@ -5,6 +5,31 @@
 
 namespace mrl {
 
+namespace paged {
+// Another lane's x, by DPP control CTRL and for the sixteens of lanes in ROWS; `none` where there is no such lane.
+template <int CTRL, int ROWS>
+__device__ inline int32_t moved(int32_t x, int32_t none) { return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false); }
+// x over the lanes up to each, f(x, control, rows) being x with what is moved to it; all lanes take part.  (No trips through LDS, as shuffles make.)
+template <class T, class F>
+__device__ inline T over_lanes_up_to(T x, F f) {
+  x = f(x, std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());   // row_shr 1, 2, 4, 8: within sixteens
+  x = f(x, std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  x = f(x, std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  x = f(x, std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  x = f(x, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());   // row_bcast 15, 31: the last of a sixteen, of a half, to those behind
+  return f(x, std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+}
+__device__ inline uint64_t sums_up_to(uint64_t x) {
+  return over_lanes_up_to(x, [](uint64_t y, auto ctrl, auto rows) {
+    const uint32_t lo = moved<ctrl(), rows()>(int32_t(uint32_t(y)), 0), hi = moved<ctrl(), rows()>(int32_t(uint32_t(y >> 32)), 0);
+    return y + (uint64_t(hi) << 32 | lo);
+  });
+}
+__device__ inline int32_t largest_up_to(int32_t x, int32_t least) {
+  return over_lanes_up_to(x, [=](int32_t y, auto ctrl, auto rows) { return max(y, moved<ctrl(), rows()>(y, least)); });
+}
+}  // namespace paged
+
 struct PageTablesArgs {
   const int32_t *cached, *added, *free_list, *free_count;
   int32_t *table, *starts, *lengths, *slots, *positions, *free_left;
