@@ -662,7 +662,8 @@ int mrl_run_action_timed(const mrl_spec *spec, void *const *params, const mrl_ac
  *   8  positions   i32 [tokens]       (Out) places of the tokens in their requests, from 0; 0 behind the last token
  *   9  free left   i32 [2]            (Out) pages left on the list; pages that were wanting
  * The call reads nothing that it writes but columns of the page table that it leaves: run again on the same inputs it gives the
- * same.  The next step's free count is free left's first entry (two buffers that take turns). */
+ * same.  The next step's cached are lengths, its free count free left's first entry, in buffers that take turns: a written parameter that
+ * overlaps another is refused (MRL_ERR_BAD_SPEC). */
 typedef struct {
   uint32_t requests, table_width, page_size;
   uint32_t pages;       /* of the cache: page numbers are below it; pages * page_size < 2^31 */

@@ -2816,6 +2816,13 @@ int check_page_tables(const mrl_page_tables *op) {
 int run_page_tables(const mrl_page_tables &op, void *const *params, hipStream_t stream) {
   for (int i = 0; i < 10; i++)
     if (!params[i] && !(i == 2 && op.free_pages == 0)) return MRL_ERR_NULL;
+  // Workgroups read lengths while others write: the next step's, say, over this one's would be read by some.
+  const uint64_t entries[10] = {op.requests, op.requests, op.free_pages, 1, uint64_t(op.requests) * op.table_width, op.requests + 1ull, op.requests, op.tokens, op.tokens, 2};
+  for (int i = 0; i < 10; i++)
+    for (int j = std::max(4, i + 1); j < 10; j++) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(params[i]), y = reinterpret_cast<uintptr_t>(params[j]);
+      if (x < y + 4 * entries[j] && y < x + 4 * entries[i]) return bad(MRL_ERR_BAD_SPEC, "a written parameter overlaps another");
+    }
   mrl::PageTablesArgs a;
   a.cached = (const int32_t *)params[0], a.added = (const int32_t *)params[1], a.free_list = (const int32_t *)params[2], a.free_count = (const int32_t *)params[3];
   a.table = (int32_t *)params[4], a.starts = (int32_t *)params[5], a.lengths = (int32_t *)params[6], a.slots = (int32_t *)params[7], a.positions = (int32_t *)params[8];

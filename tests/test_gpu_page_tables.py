@@ -119,3 +119,22 @@ def test_lengths_whose_sum_passes_32_bits(gpu):
     added = [2 ** 31 - 1] * 3
     for g, w in zip(run(op, [0, 0, 0], added, free, 4, table), by_hand(op, [0, 0, 0], added, free, 4, table)):
         assert np.array_equal(g, w)
+
+
+def test_refused_pointers(gpu):
+    """A written parameter over another: workgroups would read what others have written."""
+    op = M.PageTables(3, 4, 16, 32, 100, 5)
+    sizes = [3, 3, 5, 1, 12, 4, 3, 100, 100, 2]
+    buf = M.DeviceBuffer(4 * 4096)
+    at = [buf.ptr + 1024 * i for i in range(10)]
+    for i in range(10):
+        with pytest.raises(M.MorelloError) as err:
+            op.run_device([None if j == i else p for j, p in enumerate(at)])
+        assert err.value.status == 6
+        for j in range(max(4, i + 1), 10):
+            for over in (at[j], at[j] + 4 * (sizes[j] - 1), at[j] - 4 * (sizes[i] - 1)):   # on it, its last entry, its first
+                with pytest.raises(M.MorelloError) as err:
+                    op.run_device([over if k == i else p for k, p in enumerate(at)])
+                assert err.value.status == 3 and "overlaps" in str(err.value)
+    buf.free()
+    check(16, [(3, 2), (0, 1)])   # (buffers side by side are fine)
