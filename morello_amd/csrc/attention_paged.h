@@ -10,7 +10,7 @@
 //   few tiles for the workgroups: a tile's length on the line is its request's most blocks rounded up to the share, and the share so small that the
 //     pieces are at most as many as workgroups: each has one piece;
 //   else: a tile's length is its blocks and some for what a tile costs besides.  Tile t's keys end bq / G tokens behind tile t - 1's, so lengths grow evenly up to what
-//     a window allows; taken as that (at least the tile's blocks), the place of any tile is a formula, and no list of tiles is needed.
+//     a window or the table allows; taken as that (at least the tile's blocks), the place of any tile is a formula, and no list of tiles is needed.
 // A workgroup's share may begin and end inside a tile: there it leaves a partial result (O, m, l: the sum of the values, the reference in the
 // exponent's base of two, the denominator) instead of the tile's rows, one for the tile it does not begin (place 0) and one for the tile it
 // begins and does not end (place 1).  Who begins a tile and does not end it describes it for a last launch, which puts the pieces together in their order.  No
@@ -23,6 +23,7 @@
 #pragma once
 #include "attention.h"
 #include "paged.h"
+#include "paged_line.h"
 
 namespace mrl {
 namespace paged {
@@ -72,10 +73,8 @@ __device__ inline uint32_t not_finite(attn::v4i x) {
   return over & (BF16 ? 0x80008000u : 0x80000000u);
 }
 
-// A request: its new tokens, their first row, and its length.
-struct Request {
-  int32_t n, start, length;
-};
+__device__ inline Rules<FastDiv> rules(const Kernargs &k) { return {k.by_group, k.p.group, k.w.bq_log2, k.w.block_log2, k.p.width * k.p.page_size, k.p.window, k.w.overhead}; }
+
 __device__ inline Request read_request(const PagedAttnArgs &p, uint32_t r) {
   const int32_t most = int32_t(p.tokens);
   const int32_t s0 = min(max(p.starts[r], 0), most), s1 = min(max(p.starts[r + 1], 0), most);
@@ -93,53 +92,11 @@ struct Piece {
 // Tile `tile` of a request, as a whole.
 __device__ inline Piece tile_of(const Kernargs &k, const Request &q, uint32_t tile) {
   Piece t = {};
-  const uint32_t row0 = tile << k.w.bq_log2, rows = min(uint32_t(q.n) * k.p.group - row0, 1u << k.w.bq_log2);
-  const int32_t known = min(max(q.length, 0), int32_t(k.p.width * k.p.page_size));
-  t.row0 = row0, t.rows = rows, t.start = q.start, t.at = int32_t(max(int64_t(q.length) - q.n, -(int64_t(1) << 30)));
-  const int64_t last = int64_t(t.at) + k.by_group.div(row0 + rows - 1), first = int64_t(t.at) + k.by_group.div(row0);
-  t.end = uint32_t(min(max(last + 1, int64_t(0)), int64_t(known)));
-  t.begin = k.p.window ? uint32_t(min(max(first - int64_t(k.p.window) + 1, int64_t(0)), int64_t(t.end))) : 0;
-  t.blocks = t.b1 = t.end > t.begin ? ((t.end - 1) >> k.w.block_log2) - (t.begin >> k.w.block_log2) + 1 : 0;
+  const auto r = rules(k);
+  t.row0 = tile << r.bq_log2, t.rows = rows_of(r, q, tile), t.start = q.start;
+  const Seen s = seen_of(r, q, t.row0, t.rows);
+  t.at = s.at, t.begin = s.begin, t.end = s.end, t.blocks = t.b1 = s.blocks;
   return t;
-}
-
-// floor(x / y) for x < 2^52 and a quotient below 2^32 (a quotient that is no whole number is at least 1 / y off one: more than a rounding in 64 bits).
-__device__ inline uint32_t quotient(uint64_t x, uint64_t y) { return uint32_t(double(x) / double(y)); }
-
-// A request's tiles on the line, of one head.
-struct Lengths {
-  uint32_t tiles;
-  uint32_t first, slope, most, grown;   // tile t: first + t * slope / 256 for t below `grown`, then `most`; in the few tiles' way `most` for all
-
-  __device__ uint64_t before(uint32_t t) const {   // of the tiles before tile t
-    const uint64_t x = min(t, grown);
-    return x * first + ((x * (x - (x != 0)) / 2 * slope) >> 8) + uint64_t(t - uint32_t(x)) * most;
-  }
-  __device__ uint32_t of(uint32_t t) const { return uint32_t(before(t + 1) - before(t)); }
-  __device__ uint64_t all() const { return before(tiles); }
-};
-// A tile has at most (keys it sees) / 2^block_log2 + 2 blocks, and tile t sees at most at + (t + 1) * bq / G + 1 keys, or window + bq / G + 1.
-// (Two more, as the eighths of `slope` are rounded where they are summed.)
-__device__ inline Lengths lengths_of(const Kernargs &k, const Request &q) {
-  Lengths l;
-  const uint32_t bq = 1u << k.w.bq_log2, step = bq / k.p.group + 1, more = 4 + k.w.overhead;
-  const uint32_t at = uint32_t(min(max(int64_t(q.length) - q.n, int64_t(0)), int64_t(k.p.width * k.p.page_size)));
-  l.tiles = (uint32_t(q.n) * k.p.group + bq - 1) >> k.w.bq_log2;
-  l.slope = ((bq * 256 / k.p.group) >> k.w.block_log2) + 1;
-  l.first = (uint32_t((uint64_t(at) + step) >> k.w.block_log2)) + more;
-  l.grown = 0xffffffffu, l.most = 0;
-  if (k.p.window) {
-    l.most = uint32_t((uint64_t(k.p.window) + step) >> k.w.block_log2) + more;
-    l.grown = l.first >= l.most ? 0 : quotient(uint64_t(l.most - l.first) * 256, l.slope) + 1;
-  }
-  return l;
-}
-// In the few tiles' way, each as long as the longest can be.
-__device__ inline uint32_t most_blocks(const Kernargs &k, const Request &q, uint32_t tiles) {
-  const Piece last = tile_of(k, q, tiles - 1);
-  if (tiles == 1) return max(last.blocks, 1u);
-  return k.p.window ? min(((last.end + 1) >> k.w.block_log2) + 2, uint32_t((uint64_t(k.p.window) + (1u << k.w.bq_log2) / k.p.group + 1) >> k.w.block_log2) + 2)
-                    : max(last.blocks, 1u);
 }
 
 __device__ inline uint32_t of_lane(uint32_t x, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(x), lane)); }
@@ -155,8 +112,9 @@ struct Worker {
   bool few = false, described = false;
 
   __device__ Lengths lengths(const Kernargs &k, const Request &q) const {
-    Lengths l = lengths_of(k, q);
-    if (few) l.grown = 0, l.most = quotient(uint64_t(most_blocks(k, q, l.tiles)) + share - 1, share) * share;
+    const auto r = rules(k);
+    Lengths l = lengths_of(r, q);
+    if (few) make_few(&l, most_blocks(r, q, l.tiles), share);
     return l;
   }
 
@@ -177,16 +135,13 @@ struct Worker {
     for (uint32_t r = lane; r < requests; r += 64) {
       mine = read_request(k.p, r);
       if (!mine.n) continue;
-      const Lengths l = lengths_of(k, mine);
-      tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(k, mine, l.tiles);
+      const auto rule = rules(k);
+      const Lengths l = lengths_of(rule, mine);
+      tiles += l.tiles, line += l.all(), blocks += uint64_t(l.tiles) * most_blocks(rule, mine, l.tiles);
     }
     tiles = of_lane(sums_up_to(tiles), 63) * heads, line = of_lane(sums_up_to(line), 63) * heads, blocks = of_lane(sums_up_to(blocks), 63) * heads;
-    share = uniform(max(quotient(line + workers - 1, workers), 1u));
-    if (tiles < workers) {   // a piece to each, where that is no longer than equal shares and the second piece that they may come to
-      const uint32_t spare = uint32_t(workers - tiles), single = max((uniform(quotient(blocks + spare - 1, spare)) + k.w.least - 1) / k.w.least, 1u) * k.w.least;
-      few = single <= share + k.w.second;
-      if (few) share = single;
-    }
+    const Cut cut = cut_of(tiles, line, blocks, workers, k.w.least, k.w.second);
+    share = uniform(cut.share), few = uniform(uint32_t(cut.few));
     // The request that holds its start.
     const uint64_t from = uint64_t(share) * number;
     uint64_t base = 0;
@@ -205,7 +160,7 @@ struct Worker {
         const int it = __builtin_ctzll(where);
         stand(mine, of_mine, r0, it);
         const uint64_t all = of_lane(length, it), in_request = from - of_lane(off, it);
-        head = uniform(quotient(in_request, all)), left = share;
+        head = min(uniform(quotient(in_request, all)), k.p.kv_heads - 1), left = share;   // (past it only where starts that fall make a line that 64 bits do not hold)
         // The tile that holds the place in the head: the last that begins at or before it, found among 64 at a time.
         const uint64_t in_head = in_request - head * all;
         uint32_t step = 1;
@@ -261,7 +216,7 @@ struct Worker {
   // By one thread, of a tile that this workgroup begins and others end: how many of them, and which rows.  (Its share ends behind block b1 - 1.)
   __device__ void describe(const Work &w, const Piece &t) const {
     uint32_t *d = w.merges + number * 8;
-    d[0] = 1 + (t.blocks - 1 - t.b1) / share, d[1] = uint32_t(t.start), d[2] = t.row0, d[3] = t.rows, d[4] = t.head;
+    d[0] = pieces_behind(t.blocks, t.b1, share), d[1] = uint32_t(t.start), d[2] = t.row0, d[3] = t.rows, d[4] = t.head;
   }
 };
 

@@ -151,7 +151,8 @@ __global__ __launch_bounds__(THREADS) void k_paged_attn_merge(PagedAttnArgs p, M
   constexpr uint32_t WAVES = THREADS / 64;
   __shared__ Sum met[WAVES][64];
   const uint32_t *d = a.merges + blockIdx.x * 8;
-  const uint32_t piece_floats = a.bq * a.row_floats, more = d[0], row0 = d[2], rows = d[3], kv = d[4];
+  // (as many as there are workgroups behind: starts that fall could make a line that its shares do not cover)
+  const uint32_t piece_floats = a.bq * a.row_floats, more = min(d[0], gridDim.x - 1 - blockIdx.x), row0 = d[2], rows = d[3], kv = d[4];
   const int32_t start = int32_t(d[1]);
   if (!more) return;
   const float *const partials = a.partials + 2 * uint64_t(blockIdx.x) * piece_floats;
@@ -210,12 +211,12 @@ Choice choose(const PagedAttnArgs &a) {
   auto chunks = [&](int64_t n) { return n * size % 16 == 0; };
   const double scale = std::fabs(a.scale);
   // Pages of whole sixteens of slots, heads and strides of whole 16-byte chunks, the slots of a page, and neighbouring pages, within 2 GB; places of
-  // keys that some blocks more do not take past 31 bits; a line of blocks that 256 shares of 32 bits cover.
+  // keys that some blocks more do not take past 31 bits; a line of blocks that its shares cover.
   c.tiled = a.page_size % 16 == 0 && a.head_dim <= 128 && chunks(a.head_dim) && chunks(a.q_t) && chunks(a.q_h) && chunks(a.o_t) && chunks(a.o_h) && chunks(a.key_p) &&
             chunks(a.key_s) && chunks(a.key_h) && chunks(a.val_p) && chunks(a.val_s) && chunks(a.val_h) && a.key_s < (1 << 24) && a.val_s < (1 << 24) &&
             a.key_p < (1 << 29) && a.val_p < (1 << 29) && a.key_s * a.page_size < (1 << 29) && a.val_s * a.page_size < (1 << 29) &&
             uint64_t(a.tokens) * a.group < (1u << 31) && uint64_t(a.width) * a.page_size <= 0x7fff0000u &&
-            (double(a.tokens) * a.group / 16 + a.requests) * a.kv_heads * (double(a.width) * a.page_size / 32 + 16) < double(1ull << 39) && scale > 1e-30 && scale < 1e30;
+            paged::line_fits(a.tokens, a.requests, a.group, a.kv_heads, uint64_t(a.width) * a.page_size, g_compute_units) && scale > 1e-30 && scale < 1e30;
   if (!c.tiled) return c;
   const uint64_t rows = uint64_t(a.max_new) * a.group;
   paged::Work &w = c.work;
