@@ -643,8 +643,8 @@ int mrl_run_action_timed(const mrl_spec *spec, void *const *params, const mrl_ac
  * holds device pointers in the order given at each call, none NULL unless said so, aligned as their element type at least; In
  * parameters must not alias written ones except where said so.  Buffers and stream belong to the device given to mrl_init,
  * which is the calling thread's current one (MRL_ERR_NO_DEVICE otherwise).  Strides count elements; all strides of a tensor
- * zero means dense in the order its indices are named; negative ones are refused (MRL_ERR_BAD_SPEC), and so are strides under which two elements
- * of a written tensor could fall together.  Descriptors are zero-initialised before their fields are set. */
+ * zero means dense in the order its indices are named; negative ones and ones past 2^40 are refused (MRL_ERR_BAD_SPEC), and so are strides under which two elements
+ * of a written tensor could fall together, and those that take a tensor's last element past 2^60 (MRL_ERR_TOO_LARGE).  Descriptors are zero-initialised before their fields are set. */
 
 /* Lengths of requests -> what a step of them needs.  Request r has max(cached[r], 0) tokens in the cache and
  * max(added[r], 0) new ones, which are rows starts[r] .. starts[r + 1] - 1 of the step's tensors; new tokens past `tokens` rows are

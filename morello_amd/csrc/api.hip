@@ -2746,7 +2746,8 @@ int bad(int status, const char *what) {
 }
 
 constexpr uint32_t MOST_TOKENS = 1u << 23;          // a workgroup to each, of up to 256 threads, is still a launch
-constexpr int64_t MOST_STRIDE = int64_t(1) << 40;   // products of strides and indices stay far from 2^63
+constexpr int64_t MOST_STRIDE = int64_t(1) << 40;
+constexpr int64_t MOST_REACH = int64_t(1) << 60;    // elements from a tensor's first to behind its last: offsets in bytes stay within 63 bits
 
 // Strides of a tensor with dims `n`, slowest first, and `inner` contiguous elements behind them; all zero: dense.  `written`: no two
 // elements of it may fall together.
@@ -2761,7 +2762,13 @@ int fill_strides(const int64_t *given, const uint32_t *n, int dims, uint32_t inn
     for (int d = dims - 1; d >= 0; d--) out[d] = run, run *= n[d];
     return MRL_OK;
   }
-  for (int d = 0; d < dims; d++) out[d] = given[d];
+  int64_t reach = inner;
+  for (int d = 0; d < dims; d++) {
+    out[d] = given[d];
+    // (a product of the two alone may pass 63 bits)
+    if (n[d] > 1 && given[d] > (MOST_REACH - reach) / (int64_t(n[d]) - 1)) return bad(MRL_ERR_TOO_LARGE, (std::string(name) + ": the last element lies past 2^60").c_str());
+    reach += given[d] * (int64_t(n[d]) - 1);
+  }
   if (!written) return MRL_OK;
   int order[3] = {0, 1, 2};
   std::sort(order, order + dims, [&](int x, int y) { return out[x] < out[y]; });

@@ -109,3 +109,18 @@ def test_which_kernels_attention_takes():
     # places of keys near 2^31
     assert steps(requests=1, table_width=(0x7fff0000 >> 4), pages=64) == shared and steps(requests=1, table_width=(0x7fff0000 >> 4) + 1, pages=64) == generic
     assert attention(max_new=1).workspace_bytes() == 0 and attention(head_dim=136).workspace_bytes() == 0 and attention().workspace_bytes() > 0
+
+
+@pytest.mark.parametrize("op,given,status", [
+    (attention, dict(pages=1 << 23, key_strides=(1 << 40, 128, 64)), TOO_LARGE), (attention, dict(pages=(1 << 27) - 1, value_strides=(1 << 38, 128, 64)), TOO_LARGE),
+    (attention, dict(tokens=1 << 23, q_strides=(1 << 40, 64)), TOO_LARGE), (attention, dict(tokens=1 << 23, out_strides=(1 << 40, 64)), TOO_LARGE),
+    (attention, dict(pages=1 << 20, key_strides=(1 << 40, 128, 64)), OK), (attention, dict(pages=(1 << 20) + 1, key_strides=(1 << 40, 128, 64)), TOO_LARGE),
+    (attention, dict(pages=1 << 26, page_size=2, table_width=64, key_strides=(1 << 33, 1 << 39, 64)), OK), (attention, dict(pages=(1 << 27) - 1, key_strides=(0, 1 << 40, 1 << 40)), OK),
+    (rotary, dict(pages=1 << 23, key_strides=(1 << 40, 128, 64)), TOO_LARGE), (rotary, dict(pages=1 << 23, value_strides=(1 << 40, 128, 64)), TOO_LARGE),
+    (rotary, dict(pages=1 << 24, page_size=16, key_strides=(1 << 40, 1 << 40, 64)), TOO_LARGE), (rotary, dict(pages=64, page_size=16, key_strides=(1 << 40, 1 << 40, 64)), BAD_SPEC),
+    (rotary, dict(tokens=1 << 23, k_strides=(1 << 40, 64)), TOO_LARGE), (rotary, dict(tokens=1 << 23, q_out_strides=(1 << 40, 64)), TOO_LARGE),
+    (rotary, dict(tokens=1 << 23, page_size=0, pages=0, key_strides=(0, 1 << 40, 64)), TOO_LARGE), (rotary, dict(pages=1 << 20, key_strides=(1 << 39, 128, 64)), OK),
+])
+def test_strides_whose_products_pass_63_bits(op, given, status):
+    """A stride of 2^40 is legal, and so are 2^27 pages: together their last element has no 64-bit place."""
+    assert op(**given).check() == status
