@@ -625,7 +625,8 @@ def _set_strides(c, **given):
 
 class PageTables(_PagedOp):
     """Lengths of requests -> page tables, slots and positions of a step's new tokens (mrl_page_tables).
-    Parameters: cached, added, free list, free count, page table (InOut), starts, lengths, slots, positions, free left; all i32."""
+    Parameters: cached, added, free list, free count, page table (InOut), starts, lengths, slots, positions, free left; all i32.
+    Where the list ran out (free left's second entry), tokens whose slot is -1 are in lengths but not in the cache: the next cached leaves them out."""
     _name, _params = "page_tables", 10
 
     def __init__(self, requests, table_width, page_size, pages, tokens, free_pages):
