@@ -663,7 +663,8 @@ int mrl_run_action_timed(const mrl_spec *spec, void *const *params, const mrl_ac
  *   9  free left   i32 [2]            (Out) pages left on the list; pages that were wanting
  * The call reads nothing that it writes but columns of the page table that it leaves: run again on the same inputs it gives the
  * same.  The next step's cached are lengths, its free count free left's first entry, in buffers that take turns: a written parameter that
- * overlaps another is refused (MRL_ERR_BAD_SPEC).
+ * overlaps another is refused (MRL_ERR_BAD_SPEC).  A recorded call keeps its buffers: two recordings, one with each order of them, follow each
+ * other; one alone wants copies behind it.
  * Where pages were wanting (free left's second entry), lengths counts the tokens without a slot all the same, and columns that a step takes as cached it never
  * draws: those tokens' keys would stay hidden for good.  Of such a request the program passes as the next cached its tokens that are in the cache, cached[r] + its
  * tokens of this step whose slot is not -1 (they are its first), and the others again as new ones once there are pages; what the step's attention gave for the others counts for nothing. */
