@@ -735,7 +735,8 @@ typedef struct {
   int32_t dtype;        /* of q, keys, values and out: MRL_BF16 or MRL_F32 */
   uint32_t tokens, requests, q_heads, kv_heads, head_dim;  /* head_dim up to 1024; q_heads a multiple of kv_heads */
   uint32_t page_size, pages, table_width;
-  uint32_t max_new;     /* new tokens of any one request, where the program knows a bound (it chooses kernels; results do not depend on it); 0: tokens */
+  uint32_t max_new;     /* new tokens of any one request, where the program knows a bound: it chooses kernels (results are right whatever it says, but round differently); 0: tokens, which
+                         * puts steps of single tokens on the kernels for prompts */
   uint32_t window;
   float scale;          /* 0: 1 / sqrt(head_dim) */
   int64_t q_strides[2], out_strides[2];      /* of a token, of a head */

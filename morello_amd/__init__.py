@@ -657,7 +657,8 @@ class Rotary(_PagedOp):
 
 
 class PagedAttention(_PagedOp):
-    """Attention of each request's new tokens over its pages of keys and values (mrl_paged_attention).
+    """Attention of each request's new tokens over its pages of keys and values (mrl_paged_attention).  `max_new`: new tokens of any one request, 1 for steps
+    of single tokens; it chooses kernels, and 0 stands for `tokens`.
     Parameters: q, keys, values, page table, starts, lengths, out, workspace (workspace_bytes() bytes)."""
     _name, _params = "paged_attention", 8
 
