@@ -720,6 +720,7 @@ int mrl_rotary_plan(const mrl_rotary *op, mrl_plan *plan, mrl_plan_step *steps, 
  * What a hidden slot holds, NaN or infinity, does not matter.  Rows of q and out outside starts[0] .. starts[requests] are
  * neither read nor written.  starts do not fall (whatever they are, no row outside 0 .. tokens is touched).
  * Scores, statistics and sums are held in 32 bits; bf16: probabilities are rounded to bf16 for the product with the values.
+ * Sums are against a reference that a row's scores may outgrow by a factor of 2^40 before it moves: values past 2^64 in size may overflow them.
  * params:
  *   0  q           [tokens][q_heads][head_dim]
  *   1  keys        [pages][page_size][kv_heads][head_dim]

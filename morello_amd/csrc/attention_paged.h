@@ -10,7 +10,7 @@
 //   few tiles for the workgroups: a tile's length on the line is its request's most blocks rounded up to the share, and the share so small that the
 //     pieces are at most as many as workgroups: each has one piece;
 //   else: a tile's length is its blocks and some for what a tile costs besides.  Tile t's keys end bq / G tokens behind tile t - 1's, so lengths grow evenly up to what
-//     a window or the table allows; taken as that (at least the tile's blocks), the place of any tile is a formula, and no list of tiles is needed.
+//     a window or the table allows; taken as that (at least the tile's blocks), the place of any tile is a formula (paged_line.h), and no list of tiles is needed.
 // A workgroup's share may begin and end inside a tile: there it leaves a partial result (O, m, l: the sum of the values, the reference in the
 // exponent's base of two, the denominator) instead of the tile's rows, one for the tile it does not begin (place 0) and one for the tile it
 // begins and does not end (place 1).  Who begins a tile and does not end it describes it for a last launch, which puts the pieces together in their order.  No

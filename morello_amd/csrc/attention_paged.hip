@@ -222,8 +222,12 @@ Choice choose(const PagedAttnArgs &a) {
   paged::Work &w = c.work;
   const bool near = a.q_t < (1 << 22) && a.q_h < (1 << 28) / int64_t(a.group);   // (a tile's queries within 2 GB of its first)
   if (a.dtype == MRL_BF16 && rows > 32 && near) {
-    // Requests of few rows among others go the same way: a tile of 128 rows streams its keys at what memory delivers, too (a decoding step of 48 requests up to 16384
-    // keys that way 167 us, on tiles of 16 rows 143; 18 such requests beside 6 chunks in a launch of their own on those: 53 us, 39 together).
+    // us, on tiles of 128 rows and of 32, recorded into a graph.  48 rows: 16 requests to 16384 keys, 8 heads of 128 dims, 81 and 121; 4 requests to 2000 keys 25 and 36;
+    // 48 requests to 8000 keys, 2 heads, 48 and 62; 24 requests to 5000 keys, 2 heads of 64 dims, 23.7 and 24.1.  24 rows, the first two 76 and 79, 23.7 and 29.5; 32 rows, the last 21.4 and
+    // 27.0: of those of 17 to 32 rows that were measured the 128-row tiles are the faster, too (the border was set before).  Four rows:
+    // a decoding step of 48 requests to 16384 keys 171, on tiles of 16 rows 146.
+    // Requests of few rows among others go the same way: a tile of 128 rows streams its keys at what memory delivers, too (18 such requests beside 6 chunks in a launch
+    // of their own on tiles of 16 rows: 53 us, 39 together).
     paged::chunk_work(a, &w);
   } else {
     c.qb = rows <= 16 ? 1 : 2;
