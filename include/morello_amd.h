@@ -46,7 +46,10 @@ typedef enum {
   MRL_U32 = 4,
   MRL_I32 = 5,
   MRL_F32 = 6,
-  MRL_BF16 = 7
+  MRL_BF16 = 7,
+  /* Four bits of mantissa, four of exponent from 2^-6 to 2^8, no infinities (largest 448): of the operators on blocks
+   * and experts at this header's end alone.  No Spec has it (MRL_ERR_BAD_SPEC), and the reference does not. */
+  MRL_F8E4M3 = 8
 } mrl_dtype;
 
 /* morello/src/layout.rs:74-81 */
@@ -747,6 +750,87 @@ int mrl_paged_attention_check(const mrl_paged_attention *op);
 size_t mrl_paged_attention_workspace_bytes(const mrl_paged_attention *op);
 int mrl_run_paged_attention(const mrl_paged_attention *op, void *const *params, void *stream);
 int mrl_paged_attention_plan(const mrl_paged_attention *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
+/* ---- Feed-forward layers on weights in 8 bits ------------------------------------------------
+ * No counterpart in the reference.  What stands between two attentions of a serving program: products on tensors in e4m3 whose
+ * every 128 elements of a row (of 128 rows, for weights) share a scale in 32 bits, and layers of experts for steps of few tokens.
+ *   mrl_run_cast_blocks     bf16 or f32, behind the gate of a gated layer or not -> e4m3 and scales; weights once, activations before a product
+ *   mrl_run_matmul_blocks   the product of two such tensors
+ *   mrl_run_experts         router, choice, and the chosen experts' gated layers, on weights in bf16 or e4m3 with scales
+ * All that is said of the three operators above on streams, graphs, devices, descriptors, strides (of rows here; 0 means dense), alignment and aliasing
+ * holds for these.  An element x of a block with scale s stands for x s; the last block of a row, and the last 128 rows, may be short of elements. */
+
+/* x -> e4m3 and scales.  With a the largest size of a block's elements, at least 2^-110: scale = a / 448, element = x * (448 / a), both quotients and the product
+ * rounded to 32 bits, then to the nearest e4m3 (ties to even).  NaN stays NaN and does not count for a; in a block with an infinity every element reads back as NaN.
+ * `gated`: what is cast is silu(g) u = g / (1 + exp(-g)) u, in 32 bits, g the first `cols` elements of x's row and u the `cols` behind them.
+ * params:
+ *   0  x       [rows][cols], gated [rows][2 * cols]
+ *   1  out     e4m3 [rows][cols]                                     (Out)
+ *   2  scales  f32 [ceil(rows / block_rows)][ceil(cols / 128)]       (Out) */
+typedef struct {
+  int32_t dtype;          /* of x: MRL_BF16 or MRL_F32 */
+  uint32_t rows, cols;    /* up to 2^27 blocks of 128 elements */
+  uint32_t block_rows;    /* rows that share their scales: 1 or 128 */
+  int32_t gated;
+  int64_t x_stride, out_stride, scale_stride;   /* of a row */
+} mrl_cast_blocks;
+int mrl_cast_blocks_check(const mrl_cast_blocks *op);
+int mrl_run_cast_blocks(const mrl_cast_blocks *op, void *const *params, void *stream);
+int mrl_cast_blocks_plan(const mrl_cast_blocks *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
+/* out = a b^T: out[i][j] = sum over blocks q of K of a_scales[i][q] * b_scales[j / 128][q] * (sum over the block's k of a[i][k] * b[j][k]),
+ * sums in 32 bits, rounded once.  Where out is bf16, the matrix instruction that forms a block's sum may cut its products at 2^-13 of the largest of the 128.
+ * params:
+ *   0  a         e4m3 [m][k]
+ *   1  a scales  f32 [m][ceil(k / 128)]
+ *   2  b         e4m3 [n][k]
+ *   3  b scales  f32 [ceil(n / 128)][ceil(k / 128)]
+ *   4  out       [m][n]  (Out)
+ *   5  workspace mrl_matmul_blocks_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's */
+typedef struct {
+  int32_t out_dtype;   /* MRL_BF16 or MRL_F32 */
+  uint32_t m, n, k;    /* each up to 2^23, m * n up to 2^40 */
+  int64_t a_stride, a_scale_stride, b_stride, b_scale_stride, out_stride;   /* of a row */
+} mrl_matmul_blocks;
+int mrl_matmul_blocks_check(const mrl_matmul_blocks *op);
+size_t mrl_matmul_blocks_workspace_bytes(const mrl_matmul_blocks *op);
+int mrl_run_matmul_blocks(const mrl_matmul_blocks *op, void *const *params, void *stream);
+int mrl_matmul_blocks_plan(const mrl_matmul_blocks *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
+
+/* A layer of experts for few tokens.  For each token x: p = softmax over the experts of router x; the top_k experts of largest p are chosen (of equal ones the
+ * lowest; a logit that is NaN counts as the lowest), their shares p, or p over the sum of the chosen's with `renormalise`;
+ *     out = sum over the chosen e of share_e * down_e (silu(gate_e x) * up_e x)
+ * Logits are summed in 64 bits, all else in 32; silu(gate x) * up x is rounded to bf16 before down.  Weights of experts that no token chooses are not read.
+ * A token's results do not depend on the other tokens of the call but for their rounding.
+ * params:
+ *   0  x            bf16 [tokens][hidden]
+ *   1  router       bf16 [experts][hidden]
+ *   2  gate         [experts][inter][hidden]
+ *   3  up           [experts][inter][hidden]
+ *   4  down         [experts][hidden][inter]
+ *   5  gate scales  f32 [experts][ceil(inter / 128)][ceil(hidden / 128)]   (5, 6, 7: may be NULL for weights in bf16)
+ *   6  up scales    f32 [experts][ceil(inter / 128)][ceil(hidden / 128)]
+ *   7  down scales  f32 [experts][ceil(hidden / 128)][ceil(inter / 128)]
+ *   8  rows         i32 [1]  the first so many tokens count (taken as 0 .. tokens), rows behind them are neither read nor written: the last of a step's starts,
+ *                            say.  May be NULL: all.
+ *   9  out          bf16 [tokens][hidden]    (Out)
+ *  10  chosen       i32 [tokens][top_k]      (Out; may be NULL) experts, largest share first
+ *  11  shares       f32 [tokens][top_k]      (Out; may be NULL)
+ *  12  workspace    mrl_experts_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's */
+typedef struct {
+  int32_t weight_dtype;                  /* of gate, up and down: MRL_BF16 or MRL_F8E4M3 */
+  uint32_t tokens;                       /* up to 256 */
+  uint32_t hidden, inter;                /* up to 2^17 */
+  uint32_t experts, top_k;               /* up to 512; top_k up to 32 and at most experts */
+  int32_t renormalise;
+  int64_t x_stride, router_stride, out_stride;                                   /* of a row */
+  int64_t gate_strides[2], up_strides[2], down_strides[2];                       /* of an expert, of a row */
+  int64_t gate_scale_strides[2], up_scale_strides[2], down_scale_strides[2];     /* of an expert, of a row of blocks */
+} mrl_experts;
+int mrl_experts_check(const mrl_experts *op);
+size_t mrl_experts_workspace_bytes(const mrl_experts *op);
+int mrl_run_experts(const mrl_experts *op, void *const *params, void *stream);
+int mrl_experts_plan(const mrl_experts *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap);
 
 #ifdef __cplusplus
 }

@@ -60,6 +60,7 @@ class Dtype(enum.IntEnum):
     Sint32 = 5
     Float32 = 6
     Bfloat16 = 7
+    Float8e4m3 = 8   # of CastBlocks, MatmulBlocks and Experts; no Spec has it
 
     @property
     def size(self) -> int:
@@ -70,12 +71,12 @@ class Dtype(enum.IntEnum):
 
     @property
     def numpy(self):
-        """Storage dtype; bf16 travels as its 16-bit pattern."""
+        """Storage dtype; bf16 travels as its 16-bit pattern, e4m3 as its byte."""
         return {0: np.uint8, 1: np.int8, 2: np.uint16, 3: np.int16, 4: np.uint32, 5: np.int32,
-                6: np.float32, 7: np.uint16}[int(self)]
+                6: np.float32, 7: np.uint16, 8: np.uint8}[int(self)]
 
 
-u8, i8, u16, i16, u32, i32, f32, bf16 = (Dtype(i) for i in range(8))
+u8, i8, u16, i16, u32, i32, f32, bf16, f8e4m3 = (Dtype(i) for i in range(9))
 
 
 @dataclass(frozen=True)
@@ -581,8 +582,8 @@ class Compose:
         synchronize()
 
 
-class _PagedOp:
-    """An operator over a cache in pages: a descriptor that stays the same between steps, device pointers per call."""
+class _StepOp:
+    """An operator of a serving program: a descriptor that stays the same between steps, device pointers per call."""
     _name, _params = "", 0
 
     def check(self) -> int:
@@ -623,7 +624,7 @@ def _set_strides(c, **given):
             field[i] = v
 
 
-class PageTables(_PagedOp):
+class PageTables(_StepOp):
     """Lengths of requests -> page tables, slots and positions of a step's new tokens (mrl_page_tables).
     Parameters: cached, added, free list, free count, page table (InOut), starts, lengths, slots, positions, free left; all i32.
     Where the list ran out (free left's second entry), tokens whose slot is -1 are in lengths but not in the cache: the next cached leaves them out."""
@@ -634,7 +635,7 @@ class PageTables(_PagedOp):
         self._finish()
 
 
-class Rotary(_PagedOp):
+class Rotary(_StepOp):
     """Queries and keys turned by their tokens' positions, keys and values into their slots of a cache in pages, or (page_size 0) keys to
     a dense tensor (mrl_rotary).  `sections`: pairs of dims that follow each axis of the positions.
     Parameters: q, k, v, positions, frequencies, slots, q out, keys, values."""
@@ -656,7 +657,7 @@ class Rotary(_PagedOp):
         self._finish()
 
 
-class PagedAttention(_PagedOp):
+class PagedAttention(_StepOp):
     """Attention of each request's new tokens over its pages of keys and values (mrl_paged_attention).  `max_new`: new tokens of any one request, 1 for steps
     of single tokens; it chooses kernels, and 0 stands for `tokens`.
     Parameters: q, keys, values, page table, starts, lengths, out, workspace (workspace_bytes() bytes)."""
@@ -670,6 +671,48 @@ class PagedAttention(_PagedOp):
 
     def workspace_bytes(self) -> int:
         return int(B.load().mrl_paged_attention_workspace_bytes(C.byref(self._c)))
+
+
+class CastBlocks(_StepOp):
+    """Rows of bf16 or f32, behind a gate (silu(first half) * second half) or as they are -> e4m3 with a scale for each block of `block_rows` x 128
+    (mrl_cast_blocks): block_rows 1 for a product's left side, 128 for its right side and experts' weights.
+    Parameters: x, out, scales."""
+    _name, _params = "cast_blocks", 3
+
+    def __init__(self, dtype, rows, cols, block_rows=1, gated=False, x_stride=0, out_stride=0, scale_stride=0):
+        self._c = B.CastBlocksC(int(dtype), rows, cols, block_rows, int(gated), x_stride, out_stride, scale_stride)
+        self._finish()
+
+
+class MatmulBlocks(_StepOp):
+    """out = a b^T of a [m][k] and b [n][k] in e4m3, with scales for blocks of 1 x 128 and of 128 x 128 (mrl_matmul_blocks); out in bf16 or f32.
+    Parameters: a, a scales, b, b scales, out, workspace (workspace_bytes() bytes)."""
+    _name, _params = "matmul_blocks", 6
+
+    def __init__(self, out_dtype, m, n, k, a_stride=0, a_scale_stride=0, b_stride=0, b_scale_stride=0, out_stride=0):
+        self._c = B.MatmulBlocksC(int(out_dtype), m, n, k, a_stride, a_scale_stride, b_stride, b_scale_stride, out_stride)
+        self._finish()
+
+    def workspace_bytes(self) -> int:
+        return int(B.load().mrl_matmul_blocks_workspace_bytes(C.byref(self._c)))
+
+
+class Experts(_StepOp):
+    """A layer of experts for few tokens: router, choice of `top_k`, the chosen experts' gated layers and their sum (mrl_experts).  Weights in bf16, or in
+    e4m3 with scales for blocks of 128 x 128.
+    Parameters: x, router, gate, up, down, gate scales, up scales, down scales (None for bf16), rows (None: all tokens), out, chosen, shares (None: not wanted),
+    workspace (workspace_bytes() bytes)."""
+    _name, _params = "experts", 13
+
+    def __init__(self, weight_dtype, tokens, hidden, inter, experts, top_k, renormalise=False, x_stride=0, router_stride=0, out_stride=0,
+                 gate_strides=None, up_strides=None, down_strides=None, gate_scale_strides=None, up_scale_strides=None, down_scale_strides=None):
+        self._c = B.ExpertsC(int(weight_dtype), tokens, hidden, inter, experts, top_k, int(renormalise), x_stride, router_stride, out_stride)
+        _set_strides(self._c, gate_strides=gate_strides, up_strides=up_strides, down_strides=down_strides, gate_scale_strides=gate_scale_strides,
+                     up_scale_strides=up_scale_strides, down_scale_strides=down_scale_strides)
+        self._finish()
+
+    def workspace_bytes(self) -> int:
+        return int(B.load().mrl_experts_workspace_bytes(C.byref(self._c)))
 
 
 class PlanStep:
@@ -865,8 +908,9 @@ class Target:
 
     @staticmethod
     def kernels():
-        buf = (C.c_char_p * 64)()
-        n = B.load().mrl_target_kernels(buf, 64)
+        n = B.load().mrl_target_kernels(None, 0)
+        buf = (C.c_char_p * n)()
+        B.load().mrl_target_kernels(buf, n)
         return [buf[i].decode() for i in range(n)]
 
 

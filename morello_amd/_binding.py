@@ -123,6 +123,22 @@ class PagedAttentionC(C.Structure):
         (n, C.c_int64 * 3) for n in ("key_strides", "value_strides")]
 
 
+class CastBlocksC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_uint32), ("cols", C.c_uint32), ("block_rows", C.c_uint32), ("gated", C.c_int32)] + [
+        (n, C.c_int64) for n in ("x_stride", "out_stride", "scale_stride")]
+
+
+class MatmulBlocksC(C.Structure):
+    _fields_ = [("out_dtype", C.c_int32)] + [(n, C.c_uint32) for n in ("m", "n", "k")] + [
+        (n, C.c_int64) for n in ("a_stride", "a_scale_stride", "b_stride", "b_scale_stride", "out_stride")]
+
+
+class ExpertsC(C.Structure):
+    _fields_ = [("weight_dtype", C.c_int32)] + [(n, C.c_uint32) for n in ("tokens", "hidden", "inter", "experts", "top_k")] + [
+        ("renormalise", C.c_int32)] + [(n, C.c_int64) for n in ("x_stride", "router_stride", "out_stride")] + [
+        (n, C.c_int64 * 2) for n in ("gate_strides", "up_strides", "down_strides", "gate_scale_strides", "up_scale_strides", "down_scale_strides")]
+
+
 # name -> (restype, argtypes); every symbol include/morello_amd.h declares.
 SIGNATURES = {
     "mrl_init": (C.c_int, [C.c_int]),
@@ -207,6 +223,17 @@ SIGNATURES = {
     "mrl_run_paged_attention": (C.c_int, [C.POINTER(PagedAttentionC), C.c_void_p, C.c_void_p]),
     "mrl_paged_attention_plan": (C.c_int, [C.POINTER(PagedAttentionC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
     "mrl_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionC)]),
+    "mrl_cast_blocks_check": (C.c_int, [C.POINTER(CastBlocksC)]),
+    "mrl_run_cast_blocks": (C.c_int, [C.POINTER(CastBlocksC), C.c_void_p, C.c_void_p]),
+    "mrl_cast_blocks_plan": (C.c_int, [C.POINTER(CastBlocksC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_matmul_blocks_check": (C.c_int, [C.POINTER(MatmulBlocksC)]),
+    "mrl_run_matmul_blocks": (C.c_int, [C.POINTER(MatmulBlocksC), C.c_void_p, C.c_void_p]),
+    "mrl_matmul_blocks_plan": (C.c_int, [C.POINTER(MatmulBlocksC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_matmul_blocks_workspace_bytes": (C.c_size_t, [C.POINTER(MatmulBlocksC)]),
+    "mrl_experts_check": (C.c_int, [C.POINTER(ExpertsC)]),
+    "mrl_run_experts": (C.c_int, [C.POINTER(ExpertsC), C.c_void_p, C.c_void_p]),
+    "mrl_experts_plan": (C.c_int, [C.POINTER(ExpertsC), C.POINTER(PlanC), C.POINTER(PlanStepC), C.c_uint32]),
+    "mrl_experts_workspace_bytes": (C.c_size_t, [C.POINTER(ExpertsC)]),
 }
 
 _lib = None

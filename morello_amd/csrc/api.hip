@@ -14,6 +14,7 @@
 #include <string>
 #include <vector>
 
+#include "blocks.h"
 #include "host_stage.h"
 #include "kernels.h"
 #include "layout_factor.h"
@@ -1594,7 +1595,7 @@ uint32_t mrl_abi_version(void) { return MRL_ABI_VERSION; }
 
 size_t mrl_dtype_size(int dtype) {
   switch (dtype) {
-    case MRL_U8: case MRL_I8: return 1;
+    case MRL_U8: case MRL_I8: case MRL_F8E4M3: return 1;
     case MRL_U16: case MRL_I16: case MRL_BF16: return 2;
     case MRL_U32: case MRL_I32: case MRL_F32: return 4;
     default: return 0;
@@ -1602,8 +1603,8 @@ size_t mrl_dtype_size(int dtype) {
 }
 
 const char *mrl_dtype_name(int dtype) {
-  static const char *names[] = {"u8", "i8", "u16", "i16", "u32", "i32", "f32", "bf16"};
-  return valid_dtype(dtype) ? names[dtype] : "?";
+  static const char *names[] = {"u8", "i8", "u16", "i16", "u32", "i32", "f32", "bf16", "f8e4m3"};
+  return valid_dtype(dtype) || dtype == MRL_F8E4M3 ? names[dtype] : "?";
 }
 
 int mrl_layout_row_major(const uint32_t *shape, uint32_t rank, mrl_layout *out) {
@@ -1832,7 +1833,8 @@ uint32_t mrl_target_kernels(const char **names, uint32_t cap) {
       "k_softmax_cols",
       "k_softmax_generic", "k_softmax_cols_short", "k_parts", "k_parts_block", "k_parts_rows", "k_parts_cols", "k_broadcast", "k_broadcast_rows", "k_broadcast_fill_rows", "k_fill", "k_fill16", "k_fill_zero", "k_move_rows", "k_move_runs",
       "k_move_tiled", "k_move_tiled_as", "k_move_tiled8v", "k_move_tiled16", "k_move_tiled16v", "k_move_tiled32", "k_move_gather", "k_move_generic", "k_relayout", "k_convert4", "k_copy1",
-      "k_copy16", "k_pad_rows", "k_pad_rows_pair", "k_widen_bf16", "k_page_tables", "k_rotary", "k_paged_attn", "k_paged_attn_merge", "k_paged_attn_generic"};
+      "k_copy16", "k_pad_rows", "k_pad_rows_pair", "k_widen_bf16", "k_page_tables", "k_rotary", "k_paged_attn", "k_paged_attn_merge", "k_paged_attn_generic",
+      "k_cast_rows", "k_cast_squares", "k_product_tile", "k_product_few", "k_experts_logits", "k_experts_choose", "k_experts_up", "k_experts_down"};
   const uint32_t n = sizeof families / sizeof families[0];
   for (uint32_t i = 0; i < n && i < cap && names; i++) names[i] = families[i];
   return n;
@@ -2992,6 +2994,197 @@ int mrl_paged_attention_plan(const mrl_paged_attention *op, mrl_plan *plan, mrl_
   if (rc != MRL_OK) return rc;
   rc = plan_with(8, plan, steps, cap, [&](void *const *params, Workspace &) { return run_paged_attention(a, params, nullptr); });
   if (rc == MRL_OK) plan->scratch_bytes = mrl::paged_attn_workspace_bytes(a);
+  return rc;
+}
+
+}  // extern "C"
+
+// ---- Feed-forward layers on weights in 8 bits: checks of the descriptors, strides filled in, launches ----
+namespace {
+
+uint32_t blocks_of(uint32_t n) { return n / mrl::BLOCK + (n % mrl::BLOCK != 0); }
+
+// Rows of `inner` elements each.
+int fill_row_stride(int64_t given, uint32_t rows, uint32_t inner, bool written, const char *name, int64_t *out) {
+  return fill_strides(&given, &rows, 1, inner, written, name, out);
+}
+
+int check_workspace(const void *workspace, size_t bytes) {
+  if (!workspace && bytes) return MRL_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return bad(MRL_ERR_UNSUPPORTED, "the workspace is not 16-byte aligned");
+  return MRL_OK;
+}
+
+int cast_args(const mrl_cast_blocks *op, mrl::CastArgs *a) {
+  if (!op) return MRL_ERR_NULL;
+  if (!valid_dtype(op->dtype)) return bad(MRL_ERR_BAD_SPEC, "unknown dtype, or none that is cast");
+  if (op->dtype != MRL_BF16 && op->dtype != MRL_F32) return bad(MRL_ERR_UNSUPPORTED, "dtype is bf16 or f32");
+  if (op->rows == 0 || op->cols == 0) return bad(MRL_ERR_BAD_SPEC, "rows and cols are at least 1");
+  if (op->block_rows != 1 && op->block_rows != mrl::BLOCK) return bad(MRL_ERR_BAD_SPEC, "block_rows is 1 or 128");
+  if (op->cols > 0x7fffffffu / 2 || uint64_t(op->rows) * blocks_of(op->cols) > (1u << 27)) return bad(MRL_ERR_TOO_LARGE, "more than 2^27 blocks of 128 elements");
+  *a = {};
+  a->rows = op->rows, a->cols = op->cols, a->block_rows = op->block_rows, a->dtype = op->dtype, a->gated = op->gated != 0;
+  int rc;
+  if ((rc = fill_row_stride(op->x_stride, op->rows, op->cols * (a->gated ? 2 : 1), false, "x", &a->x_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->out_stride, op->rows, op->cols, true, "out", &a->out_s)) != MRL_OK) return rc;
+  return fill_row_stride(op->scale_stride, (op->rows + op->block_rows - 1) / op->block_rows, blocks_of(op->cols), true, "scales", &a->scale_s);
+}
+
+int run_cast(mrl::CastArgs &a, void *const *params, hipStream_t stream) {
+  for (int i = 0; i < 3; i++)
+    if (!params[i]) return MRL_ERR_NULL;
+  a.x = params[0], a.out = (uint8_t *)params[1], a.scales = (float *)params[2];
+  return launched(mrl::launch_cast_blocks(a, stream), "cast to blocks");
+}
+
+int product_args(const mrl_matmul_blocks *op, mrl::ProductArgs *p) {
+  if (!op) return MRL_ERR_NULL;
+  if (!valid_dtype(op->out_dtype)) return bad(MRL_ERR_BAD_SPEC, "unknown dtype, or none that is written");
+  if (op->out_dtype != MRL_BF16 && op->out_dtype != MRL_F32) return bad(MRL_ERR_UNSUPPORTED, "out_dtype is bf16 or f32");
+  if (op->m == 0 || op->n == 0 || op->k == 0) return bad(MRL_ERR_BAD_SPEC, "m, n and k are at least 1");
+  if (op->m > (1u << 23) || op->n > (1u << 23) || op->k > (1u << 23) || uint64_t(op->m) * op->n > (uint64_t(1) << 40))
+    return bad(MRL_ERR_TOO_LARGE, "m, n or k is past 2^23, or m * n past 2^40");
+  *p = {};
+  p->m = op->m, p->n = op->n, p->k = op->k, p->out_dtype = op->out_dtype;
+  int rc;
+  if ((rc = fill_row_stride(op->a_stride, op->m, op->k, false, "a", &p->a_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->a_scale_stride, op->m, blocks_of(op->k), false, "a scales", &p->as_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->b_stride, op->n, op->k, false, "b", &p->b_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->b_scale_stride, blocks_of(op->n), blocks_of(op->k), false, "b scales", &p->bs_s)) != MRL_OK) return rc;
+  return fill_row_stride(op->out_stride, op->m, op->n, true, "out", &p->out_s);
+}
+
+int run_product(mrl::ProductArgs &p, void *const *params, hipStream_t stream) {
+  for (int i = 0; i < 5; i++)
+    if (!params[i]) return MRL_ERR_NULL;
+  const int rc = check_workspace(params[5], mrl::product_workspace_bytes(p));
+  if (rc != MRL_OK) return rc;
+  p.a = (const uint8_t *)params[0], p.a_scales = (const float *)params[1], p.b = (const uint8_t *)params[2], p.b_scales = (const float *)params[3];
+  p.out = params[4], p.workspace = (uint8_t *)params[5];
+  return launched(mrl::launch_product(p, stream), "product of blocks");
+}
+
+int experts_args(const mrl_experts *op, mrl::ExpertsArgs *a) {
+  if (!op) return MRL_ERR_NULL;
+  if (op->weight_dtype != MRL_BF16 && op->weight_dtype != MRL_F8E4M3)
+    return bad(valid_dtype(op->weight_dtype) ? MRL_ERR_UNSUPPORTED : MRL_ERR_BAD_SPEC, "weight_dtype is bf16 or f8e4m3");
+  if (op->tokens == 0 || op->hidden == 0 || op->inter == 0 || op->experts == 0) return bad(MRL_ERR_BAD_SPEC, "tokens, hidden, inter and experts are at least 1");
+  if (op->top_k == 0 || op->top_k > op->experts) return bad(MRL_ERR_BAD_SPEC, "top_k is 1 to experts");
+  if (op->tokens > mrl::MOST_TOKENS || op->experts > mrl::MOST_EXPERTS || op->top_k > mrl::MOST_CHOSEN || op->hidden > mrl::MOST_DIMS || op->inter > mrl::MOST_DIMS)
+    return bad(MRL_ERR_TOO_LARGE, "more than 256 tokens, 512 experts or 32 chosen ones, or hidden or inter past 2^17");
+  const bool scaled = op->weight_dtype == MRL_F8E4M3;
+  *a = {};
+  a->tokens = op->tokens, a->hidden = op->hidden, a->inter = op->inter, a->experts = op->experts, a->top_k = op->top_k;
+  a->weight_dtype = op->weight_dtype, a->renormalise = op->renormalise != 0;
+  int rc;
+  if ((rc = fill_row_stride(op->x_stride, op->tokens, op->hidden, false, "x", &a->x_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->router_stride, op->experts, op->hidden, false, "router", &a->router_s)) != MRL_OK) return rc;
+  if ((rc = fill_row_stride(op->out_stride, op->tokens, op->hidden, true, "out", &a->out_s)) != MRL_OK) return rc;
+  const struct {
+    mrl::Stack *to;
+    const int64_t *strides, *scale_strides;
+    uint32_t rows, cols;
+    const char *name;
+  } stacks[3] = {{&a->gate, op->gate_strides, op->gate_scale_strides, op->inter, op->hidden, "gate"},
+                 {&a->up, op->up_strides, op->up_scale_strides, op->inter, op->hidden, "up"},
+                 {&a->down, op->down_strides, op->down_scale_strides, op->hidden, op->inter, "down"}};
+  for (const auto &s : stacks) {
+    const uint32_t dims[2] = {op->experts, s.rows}, blocks[2] = {op->experts, blocks_of(s.rows)};
+    int64_t strides[2];
+    if ((rc = fill_strides(s.strides, dims, 2, s.cols, false, s.name, strides)) != MRL_OK) return rc;
+    s.to->w_e = strides[0], s.to->w_s = strides[1];
+    if (!scaled) continue;
+    if ((rc = fill_strides(s.scale_strides, blocks, 2, blocks_of(s.cols), false, (std::string(s.name) + " scales").c_str(), strides)) != MRL_OK) return rc;
+    s.to->scales_e = strides[0], s.to->scales_s = strides[1];
+  }
+  return MRL_OK;
+}
+
+int run_experts(mrl::ExpertsArgs &a, void *const *params, hipStream_t stream) {
+  const bool scaled = a.weight_dtype == MRL_F8E4M3;
+  const bool wanted[12] = {true, true, true, true, true, scaled, scaled, scaled, false, true, false, false};
+  for (int i = 0; i < 12; i++)
+    if (wanted[i] && !params[i]) return MRL_ERR_NULL;
+  const int rc = check_workspace(params[12], mrl::experts_workspace_bytes(a));
+  if (rc != MRL_OK) return rc;
+  a.x = (const uint16_t *)params[0], a.router = (const uint16_t *)params[1];
+  mrl::Stack *const stacks[3] = {&a.gate, &a.up, &a.down};
+  for (int i = 0; i < 3; i++) stacks[i]->w = (const uint8_t *)params[2 + i], stacks[i]->scales = scaled ? (const float *)params[5 + i] : nullptr;
+  a.rows = (const int32_t *)params[8], a.out = (uint16_t *)params[9], a.chosen = (int32_t *)params[10], a.shares = (float *)params[11];
+  a.workspace = (uint8_t *)params[12];
+  return launched(mrl::launch_experts(a, stream), "experts");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mrl_cast_blocks_check(const mrl_cast_blocks *op) {
+  mrl::CastArgs a;
+  return cast_args(op, &a);
+}
+int mrl_run_cast_blocks(const mrl_cast_blocks *op, void *const *params, void *stream) {
+  mrl::CastArgs a;
+  int rc = cast_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_cast(a, params, (hipStream_t)stream);
+}
+int mrl_cast_blocks_plan(const mrl_cast_blocks *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  mrl::CastArgs a;
+  const int rc = cast_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  return plan_with(3, plan, steps, cap, [&](void *const *params, Workspace &) { return run_cast(a, params, nullptr); });
+}
+
+int mrl_matmul_blocks_check(const mrl_matmul_blocks *op) {
+  mrl::ProductArgs p;
+  return product_args(op, &p);
+}
+size_t mrl_matmul_blocks_workspace_bytes(const mrl_matmul_blocks *op) {
+  mrl::ProductArgs p;
+  return product_args(op, &p) == MRL_OK ? mrl::product_workspace_bytes(p) : 0;
+}
+int mrl_run_matmul_blocks(const mrl_matmul_blocks *op, void *const *params, void *stream) {
+  mrl::ProductArgs p;
+  int rc = product_args(op, &p);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_product(p, params, (hipStream_t)stream);
+}
+int mrl_matmul_blocks_plan(const mrl_matmul_blocks *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  mrl::ProductArgs p;
+  int rc = product_args(op, &p);
+  if (rc != MRL_OK) return rc;
+  rc = plan_with(6, plan, steps, cap, [&](void *const *params, Workspace &) { return run_product(p, params, nullptr); });
+  if (rc == MRL_OK) plan->scratch_bytes = mrl::product_workspace_bytes(p);
+  return rc;
+}
+
+int mrl_experts_check(const mrl_experts *op) {
+  mrl::ExpertsArgs a;
+  return experts_args(op, &a);
+}
+size_t mrl_experts_workspace_bytes(const mrl_experts *op) {
+  mrl::ExpertsArgs a;
+  return experts_args(op, &a) == MRL_OK ? mrl::experts_workspace_bytes(a) : 0;
+}
+int mrl_run_experts(const mrl_experts *op, void *const *params, void *stream) {
+  mrl::ExpertsArgs a;
+  int rc = experts_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  if (!params) return MRL_ERR_NULL;
+  if ((rc = on_the_device()) != MRL_OK) return rc;
+  return run_experts(a, params, (hipStream_t)stream);
+}
+int mrl_experts_plan(const mrl_experts *op, mrl_plan *plan, mrl_plan_step *steps, uint32_t cap) {
+  mrl::ExpertsArgs a;
+  int rc = experts_args(op, &a);
+  if (rc != MRL_OK) return rc;
+  rc = plan_with(13, plan, steps, cap, [&](void *const *params, Workspace &) { return run_experts(a, params, nullptr); });
+  if (rc == MRL_OK) plan->scratch_bytes = mrl::experts_workspace_bytes(a);
   return rc;
 }
 

@@ -1,0 +1,109 @@
+"""Descriptors of the operators on blocks of e4m3 and of experts: what is refused, and which kernels a call would launch.  No GPU needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import morello_amd as M
+from blocks_util import E4M3, back, cast, nearest_e4m3
+from morello_amd import _binding as B
+
+OK, UNSUPPORTED, BAD_SPEC, NULL, TOO_LARGE = 0, 1, 3, 6, 7
+
+
+def cast_op(dtype=M.bf16, **given):
+    return M.CastBlocks(dtype, **{**dict(rows=33, cols=300), **given})
+
+
+def product(dtype=M.bf16, **given):
+    return M.MatmulBlocks(dtype, **{**dict(m=33, n=200, k=300), **given})
+
+
+def experts(dtype=M.f8e4m3, **given):
+    return M.Experts(dtype, **{**dict(tokens=4, hidden=256, inter=128, experts=16, top_k=2), **given})
+
+
+def test_struct_sizes_match_the_header():
+    assert C.sizeof(B.CastBlocksC) == 6 * 4 + 3 * 8
+    assert C.sizeof(B.MatmulBlocksC) == 4 * 4 + 5 * 8
+    assert C.sizeof(B.ExpertsC) == 8 * 4 + 3 * 8 + 12 * 8
+
+
+def test_the_type_of_eight_bits():
+    assert M.f8e4m3.size == 1 and str(M.f8e4m3) == "f8e4m3"
+    assert M.Matmul([1, 4, 4, 4], [M.f8e4m3] * 3).check() == BAD_SPEC
+
+
+@pytest.mark.parametrize("given,status", [
+    (dict(), OK), (dict(dtype=M.f32), OK), (dict(dtype=M.i8), UNSUPPORTED), (dict(dtype=M.f8e4m3), BAD_SPEC), (dict(dtype=99), BAD_SPEC), (dict(rows=0), BAD_SPEC), (dict(cols=0), BAD_SPEC),
+    (dict(block_rows=128), OK), (dict(block_rows=0), BAD_SPEC), (dict(block_rows=64), BAD_SPEC), (dict(rows=1 << 27, cols=128), OK), (dict(rows=1 << 27, cols=129), TOO_LARGE),
+    (dict(rows=1, cols=0xffffffff), TOO_LARGE), (dict(rows=1, cols=(1 << 30) - 1, gated=True), OK), (dict(x_stride=7), OK), (dict(x_stride=-1), BAD_SPEC),
+    (dict(out_stride=299), BAD_SPEC), (dict(out_stride=300), OK), (dict(scale_stride=2), BAD_SPEC), (dict(scale_stride=3), OK), (dict(rows=1, out_stride=1), OK),
+    (dict(x_stride=(1 << 40) + 1), BAD_SPEC), (dict(rows=1 << 24, x_stride=1 << 40), TOO_LARGE),
+])
+def test_cast_blocks_check(given, status):
+    assert cast_op(**given).check() == status
+
+
+@pytest.mark.parametrize("given,status", [
+    (dict(), OK), (dict(dtype=M.f32), OK), (dict(dtype=M.u16), UNSUPPORTED), (dict(dtype=-1), BAD_SPEC), (dict(dtype=M.f8e4m3), BAD_SPEC), (dict(m=0), BAD_SPEC), (dict(n=0), BAD_SPEC),
+    (dict(k=0), BAD_SPEC), (dict(m=1 << 23, n=1 << 17), OK), (dict(m=1 << 23, n=(1 << 17) + 1), TOO_LARGE), (dict(m=(1 << 23) + 1), TOO_LARGE), (dict(n=(1 << 23) + 1), TOO_LARGE),
+    (dict(k=(1 << 23) + 1), TOO_LARGE), (dict(out_stride=199), BAD_SPEC), (dict(a_stride=1, a_scale_stride=1, b_stride=1, b_scale_stride=1), OK), (dict(b_stride=-5), BAD_SPEC),
+])
+def test_matmul_blocks_check(given, status):
+    op = product(**given)
+    assert op.check() == status
+    if status != OK:
+        assert op.workspace_bytes() == 0
+        with pytest.raises(M.MorelloError) as err:
+            op.plan()
+        assert err.value.status == status
+
+
+@pytest.mark.parametrize("given,status", [
+    (dict(), OK), (dict(dtype=M.bf16), OK), (dict(dtype=M.f32), UNSUPPORTED), (dict(dtype=9), BAD_SPEC), (dict(tokens=0), BAD_SPEC), (dict(tokens=256), OK), (dict(tokens=257), TOO_LARGE),
+    (dict(hidden=0), BAD_SPEC), (dict(inter=0), BAD_SPEC), (dict(experts=0), BAD_SPEC), (dict(experts=512), OK), (dict(experts=513), TOO_LARGE), (dict(top_k=0), BAD_SPEC),
+    (dict(top_k=17), BAD_SPEC), (dict(experts=64, top_k=32), OK), (dict(experts=64, top_k=33), TOO_LARGE), (dict(hidden=1 << 17), OK), (dict(hidden=(1 << 17) + 1), TOO_LARGE),
+    (dict(inter=(1 << 17) + 1), TOO_LARGE), (dict(out_stride=255), BAD_SPEC), (dict(x_stride=0, out_stride=256), OK), (dict(gate_strides=(0, 256)), OK), (dict(gate_strides=(-1, 256)), BAD_SPEC),
+    (dict(down_scale_strides=(1 << 41, 1)), BAD_SPEC), (dict(dtype=M.bf16, down_scale_strides=(1 << 41, 1)), OK),
+])
+def test_experts_check(given, status):
+    op = experts(**given)
+    assert op.check() == status
+    assert (op.workspace_bytes() > 0) == (status == OK)
+
+
+def test_null_descriptors_and_lists():
+    lib = B.load()
+    for name in ("cast_blocks", "matmul_blocks", "experts"):
+        assert getattr(lib, f"mrl_{name}_check")(None) == NULL
+        assert getattr(lib, f"mrl_run_{name}")(None, None, None) == NULL
+        assert getattr(lib, f"mrl_{name}_plan")(None, None, None, 0) == NULL
+    for op in (cast_op(), product(), experts()):
+        assert op._run(C.byref(op._c), None, None) == NULL
+        with pytest.raises(ValueError):
+            op.run_async([1, 2])
+    with pytest.raises(ValueError):
+        experts(gate_strides=(1, 2, 3))
+
+
+def test_plans():
+    families = set(M.Target.kernels())
+    for op in (cast_op(), cast_op(M.f32, gated=True, block_rows=128), product(), product(M.f32, m=4), product(m=4096, n=4096, k=4096), experts(), experts(M.bf16, tokens=256)):
+        plan = op.plan()
+        assert plan.steps and set(plan.kernels) <= families and plan.cost_ns >= 2000 * len(plan.steps), plan
+    assert product().plan().scratch_bytes == product().workspace_bytes()
+    assert experts().plan().scratch_bytes == experts().workspace_bytes()
+
+
+def test_the_oracle_of_the_casts():
+    """Every byte is its own nearest; between two numbers the nearer, halfway the even byte; a block reads back within half a step."""
+    codes = np.array([c for c in range(256) if c & 127 != 127])
+    assert np.array_equal(nearest_e4m3(E4M3[codes]), codes)
+    assert E4M3[0x7e] == 448 and E4M3[0x08] == 2.0 ** -6 and E4M3[0x01] == 2.0 ** -9 and np.isnan(E4M3[0x7f])
+    assert nearest_e4m3([17, 19, 2.0 ** -10, 1.5 * 2.0 ** -9, 447, 460, -0.0]).tolist() == [0x58, 0x5a, 0, 2, 0x7e, 0x7e, 0x80]
+    x = np.random.default_rng(1).standard_normal((130, 200)).astype(np.float32)
+    for high in (1, 128):
+        stored, scales = cast(x, high)
+        assert stored.shape == x.shape and scales.shape == (-(-130 // high), 2)
+        assert (np.abs(back(stored, scales, high) - x) <= np.abs(x) * 2.0 ** -4 * 1.001 + scales.max() * 2.0 ** -10).all()

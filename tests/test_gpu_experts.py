@@ -1,0 +1,115 @@
+"""Layers of experts for few tokens, against the same in 64 bits."""
+import numpy as np
+import pytest
+
+import morello_amd as M
+from blocks_util import POISON, Device, Layer, as_f64
+
+pytestmark = pytest.mark.gpu
+
+# tokens, hidden, inter, experts, top_k
+SIZES = [(1, 256, 128, 8, 2), (1, 1, 1, 1, 1), (1, 2048, 256, 64, 8), (2, 512, 130, 16, 4), (3, 264, 72, 60, 4), (5, 1001, 333, 7, 3), (8, 640, 384, 128, 8), (16, 512, 200, 8, 2),
+         (17, 300, 96, 4, 2), (33, 256, 256, 5, 5), (64, 384, 64, 32, 6), (100, 200, 50, 3, 1), (128, 256, 144, 256, 8), (256, 128, 40, 512, 32), (70, 130, 260, 2, 2)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", SIZES)
+def test_layer(gpu, kind, tokens, hidden, inter, experts, top_k):
+    layer = Layer(kind, tokens, hidden, inter, experts, top_k, seed=tokens + hidden, renormalise=bool(tokens % 2))
+    layer.check(layer.run())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [-3, 0, 1, 7, 20, 99])
+def test_rows_that_count(gpu, kind, rows):
+    layer = Layer(kind, 20, 256, 128, 8, 2, seed=3)
+    x = layer.x.copy()
+    layer.x[max(0, rows):] = POISON["bf16"]   # a padded batch: what lies behind is not read
+    got = layer.run(rows=rows)
+    layer.x = x
+    layer.check(got, rows)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_weights_of_experts_that_nobody_wants_do_not_matter(gpu, kind):
+    layer = Layer(kind, 3, 256, 128, 16, 2, seed=5)
+    wanted = set(layer.choice()[0].ravel().tolist())
+    for e in set(range(16)) - wanted:
+        for name in ("gate", "up", "down"):
+            layer.stored[name][e] = 0x7f if kind == "e4m3" else POISON["bf16"]
+    layer.check(layer.run())
+
+
+def test_equal_logits_go_to_the_lowest_expert(gpu):
+    layer = Layer("bf16", 9, 128, 64, 70, 4, seed=6)
+    layer.router[:] = layer.router[3]
+    layer.router64[:] = layer.router64[3]
+    got = layer.run()
+    assert (got[1] == np.arange(4)).all() and (got[2] == np.float32(1 / 70)).all()
+    layer.x[:], layer.x64[:] = 0, 0
+    got = layer.run()
+    assert (got[1] == np.arange(4)).all() and not as_f64("bf16", got[0]).any()
+
+
+def test_a_row_that_is_not_a_number(gpu):
+    """Its choice is the first experts, its results are NaN, and the other rows are what they are without it."""
+    layer = Layer("e4m3", 6, 256, 128, 8, 3, seed=7)
+    x = layer.x.copy()
+    layer.x[2, 5] = POISON["bf16"]
+    out, chosen, shares = layer.run()
+    layer.x = x
+    assert (chosen[2] == np.arange(3)).all() and np.isnan(shares[2]).all() and np.isnan(as_f64("bf16", out[2])).all()
+    want, bound, which, _ = layer.want()
+    others = np.arange(6) != 2
+    assert np.array_equal(chosen[others], which[others]) and (np.abs(as_f64("bf16", out) - want) <= bound)[others].all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_strides_and_odd_addresses(gpu, kind):
+    """gate and up behind each other in one stack, rows with gaps of NaN, and all of it off 16 bytes."""
+    layer = Layer(kind, 11, 264, 128, 6, 2, seed=8)
+    size = np.uint8 if kind == "e4m3" else np.uint16
+    poison = 0x7f if kind == "e4m3" else POISON["bf16"]
+    for gap, shift in ((0, 0), (8, 0), (3, 1)):
+        row = layer.hidden + gap
+        both = np.full(shift + 6 * 2 * 128 * row, poison, size)
+        stack = both[shift:].reshape(6, 2, 128, row)
+        stack[:, 0, :, :layer.hidden], stack[:, 1, :, :layer.hidden] = layer.stored["gate"], layer.stored["up"]
+        down_row = layer.inter + gap
+        down = np.full(shift + 6 * layer.hidden * down_row, poison, size)
+        down[shift:].reshape(6, layer.hidden, down_row)[:, :, :layer.inter] = layer.stored["down"]
+        x = np.full((11, row), POISON["bf16"], np.uint16)
+        x[:, :layer.hidden] = layer.x
+        out = np.full((11, row), POISON["bf16"], np.uint16)
+        given = dict(gate_strides=(2 * 128 * row, row), up_strides=(2 * 128 * row, row), down_strides=(layer.hidden * down_row, down_row), x_stride=row, out_stride=row)
+        scales = [None, None, None]
+        if kind == "e4m3":
+            blocks = layer.scales["gate"].shape[2]
+            given.update(gate_scale_strides=(2 * blocks, blocks), up_scale_strides=(2 * blocks, blocks))
+            scales = [np.stack([layer.scales["gate"], layer.scales["up"]], 1), None, layer.scales["down"]]
+        op = layer.op(**given)
+        with Device() as d:
+            stack_at = d.put(both, shift)
+            item = both.itemsize
+            pointers = [d.put(x), d.put(layer.router), stack_at, stack_at + 128 * row * item, d.put(down, shift)]
+            if kind == "e4m3":
+                s = d.put(scales[0])
+                pointers += [s, s + 4 * layer.scales["gate"].shape[2], d.put(scales[2])]
+            else:
+                pointers += [None, None, None]
+            pointers.append(None)
+            at = len(d.bufs)
+            pointers += [d.put(out), None, None, d.put(np.full(max(16, op.workspace_bytes()), 0xff, np.uint8))]
+            op.run_device(pointers)
+            got = d.get(at, out)
+        assert (got[:, layer.hidden:] == POISON["bf16"]).all()
+        want, bound, _, _ = layer.want()
+        assert (np.abs(as_f64("bf16", got[:, :layer.hidden]) - want) <= bound).all(), (gap, shift)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_repeats_bit_for_bit(gpu, kind):
+    layer = Layer(kind, 40, 512, 256, 16, 4, seed=9)
+    first = layer.run()
+    second = layer.run()
+    assert all(np.array_equal(a, b) for a, b in zip(first, second))
