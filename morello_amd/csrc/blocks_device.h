@@ -18,13 +18,18 @@ typedef v4f v4f_any __attribute__((aligned(4)));
 typedef v4bf v4bf_any __attribute__((aligned(2)));
 
 __device__ inline v4i chunk_at(const uint8_t *p) { return *(const v4i_any *)p; }
-// The first n bytes of sixteen, zeros behind them (n may be negative, or more).
-__device__ inline v4i chunk_up_to(const uint8_t *p, int n) {
+// The first n bytes of sixteen, zeros behind them (n may be negative, or more); `before`: bytes of the same row in front of p.
+__device__ inline v4i chunk_up_to(const uint8_t *p, int n, int before) {
   if (n >= 16) return chunk_at(p);
   v4i x = {0, 0, 0, 0};
+  if (n <= 0) return x;
+  if (n + before >= 16) {   // the row's last sixteen, moved down
+    typedef unsigned __int128 u128;
+    return __builtin_bit_cast(v4i, __builtin_bit_cast(u128, chunk_at(p + n - 16)) >> ((16 - n) * 8));
+  }
 #pragma unroll
-  for (int i = 0; i < 16; i++)
-    if (i < n) x[i / 4] |= int(uint32_t(p[i]) << (i % 4 * 8));
+  for (int d = 0; d < 4; d++)
+    for (int i = 0; i < 4 && d * 4 + i < n; i++) x[d] |= int(uint32_t(p[d * 4 + i]) << (i * 8));
   return x;
 }
 

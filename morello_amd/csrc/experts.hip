@@ -4,7 +4,7 @@
 // What bounds it is reading the wanted experts' weights, once each.  They go from memory into registers in the order in which the matrix
 // instructions take them: 16 rows of weights against up to 16 of the expert's tokens, 128 bytes of each row at a time, a lane 32 of them.
 // Each of the steps needs all of the one before, a launch each: logits; choice (with few tokens and experts every workgroup of the next launch makes it for itself);
-// gate and up to h, a workgroup to 16 rows of one expert; down, a workgroup to 16 rows of all experts, so that a token's sum over
+// gate and up to h, 16 rows of one expert at a time; down, a workgroup to some rows of all experts, so that a token's sum over
 // its experts is formed in one place and in one order.  A choice is known by its number i = token * top_k + j; no lists go through memory but the chosen experts.
 #include <algorithm>
 
@@ -57,11 +57,11 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   double sum[ROUTER_TOKENS] = {};
   for (uint32_t k = threadIdx.x * 8; k < p.hidden; k += ROUTER_THREADS * 8) {
     const int bytes = int(p.hidden - k) * 2;
-    const v4i r = chunk_up_to(from + int64_t(k) * 2, bytes);
+    const v4i r = chunk_up_to(from + int64_t(k) * 2, bytes, int(k) * 2);
 #pragma unroll
     for (int t = 0; t < ROUTER_TOKENS; t++) {
       if (t >= count) break;
-      const v4i x = chunk_up_to((const uint8_t *)(p.x + int64_t(t0 + t) * p.x_s + k), bytes);
+      const v4i x = chunk_up_to((const uint8_t *)(p.x + int64_t(t0 + t) * p.x_s + k), bytes, int(k) * 2);
 #pragma unroll
       for (int i = 0; i < 4; i++) sum[t] += double(lo_f32(r[i]) * lo_f32(x[i])), sum[t] += double(hi_f32(r[i]) * hi_f32(x[i]));
     }
@@ -81,10 +81,12 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   }
 }
 
-// ---- Choice of a token's experts by a workgroup: the j-th is the one that j others are before ----
+// ---- Choice of a token's experts by a workgroup: the j-th is the one that j others are before.  Where there are more threads than experts, an expert's threads
+// share the others. ----
 template <int THREADS>
 struct Choice {
-  double key[MOST_EXPERTS];   // logits; NaN as the lowest value
+  double key[MOST_EXPERTS];       // logits; NaN as the lowest value
+  uint32_t before[MOST_EXPERTS];
   double most;
   float sums[THREADS / 64], e[MOST_CHOSEN];
   int32_t expert[MOST_CHOSEN];
@@ -95,27 +97,36 @@ __device__ inline float choose(const ExpertsArgs &p, const Places &w, uint32_t t
   constexpr int EACH = MOST_EXPERTS / THREADS;
   static_assert(MOST_EXPERTS % THREADS == 0, "");
   const uint32_t tid = threadIdx.x;
-  double value[EACH], key[EACH];
+  double value[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
     const uint32_t e = tid + i * THREADS;
     if (e >= p.experts) break;
     value[i] = w.logits[uint64_t(token) * p.experts + e];
-    key[i] = value[i] == value[i] ? value[i] : -__builtin_inf();
-    c.key[e] = key[i];
+    c.key[e] = value[i] == value[i] ? value[i] : -__builtin_inf();
+    c.before[e] = 0;
   }
   __syncthreads();
-  uint32_t before[EACH] = {};
+  const uint32_t span = p.experts <= 64 ? 64 : 1u << (32 - __clz(p.experts - 1)), shared = span < THREADS ? THREADS / span : 1;   // (both powers of two)
+#pragma unroll
+  for (int i = 0; i < EACH; i++) {
+    const uint32_t e = (tid & (span - 1)) + i * THREADS, each = (p.experts + shared - 1) / shared;
+    if (e >= p.experts || (i > 0 && span <= THREADS)) break;
+    const uint32_t o0 = span < THREADS ? tid / span * each : 0, o1 = min(p.experts, o0 + each);
+    const double mine = c.key[e];
+    uint32_t before = 0;
+#pragma unroll 8
+    for (uint32_t o = o0; o < o1; o++) {
+      const double k = c.key[o];
+      before += (k > mine || (k == mine && o < e)) ? 1 : 0;
+    }
+    atomicAdd(&c.before[e], before);
+  }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
     const uint32_t e = tid + i * THREADS;
-    if (e >= p.experts) break;
-#pragma unroll 8
-    for (uint32_t o = 0; o < p.experts; o++) {
-      const double k = c.key[o];
-      before[i] += (k > key[i] || (k == key[i] && o < e)) ? 1 : 0;
-    }
-    if (before[i] == 0) c.most = key[i];
+    if (e < p.experts && c.before[e] == 0) c.most = c.key[e];
   }
   __syncthreads();
   float sum = 0.0f;
@@ -124,8 +135,9 @@ __device__ inline float choose(const ExpertsArgs &p, const Places &w, uint32_t t
     const uint32_t e = tid + i * THREADS;
     if (e >= p.experts) break;
     const float x = expf(float(value[i] - c.most));
+    const uint32_t before = c.before[e];
     sum += x;
-    if (before[i] < p.top_k) c.expert[before[i]] = int32_t(e), c.e[before[i]] = x;
+    if (before < p.top_k) c.expert[before] = int32_t(e), c.e[before] = x;
   }
   for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
   if (tid % 64 == 0) c.sums[tid / 64] = sum;
@@ -147,7 +159,7 @@ __device__ inline void keep(const ExpertsArgs &p, const Places &w, uint32_t toke
   if (p.chosen) p.chosen[i] = c.expert[threadIdx.x];
   if (p.shares) p.shares[i] = share;
 }
-constexpr int CHOOSE_THREADS = 256;
+constexpr int CHOOSE_THREADS = 512;
 __global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p, Places w) {
   __shared__ Choice<CHOOSE_THREADS> c;
   if (blockIdx.x >= live_rows(p)) return;
@@ -157,225 +169,344 @@ __global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p
 // ---- Products with experts' weights: 16 rows from `row` on (this lane's: row + lane % 16), steps s0 .. s1 - 1 of 128 bytes a row ----
 template <bool F8>
 struct Weights {
-  static constexpr int STEP = F8 ? 128 : 64;   // elements
-  const uint8_t *row;
-  const float *scales;
-  __device__ inline Weights(const Stack &s, uint32_t expert, uint32_t row0, uint32_t rows) {
-    const uint32_t r = min(row0 + (threadIdx.x & 15), rows - 1);
-    row = s.w + (int64_t(expert) * s.w_e + int64_t(r) * s.w_s) * (F8 ? 1 : 2);
-    scales = F8 ? s.scales + int64_t(expert) * s.scales_e + int64_t(row0 / BLOCK) * s.scales_s : nullptr;
+  static constexpr int STEP = F8 ? 128 : 64, SIZE = F8 ? 1 : 2;   // elements, bytes of one
+  const uint8_t *row;     // the lane's, from its first byte of step 0 on; nullptr: none
+  const float *scales;    // of the four rows whose sums the lane gets
+  // `height`: rows that there are from row0 on, up to sixteen.
+  __device__ inline void from(const Stack &s, uint32_t expert, uint32_t row0, uint32_t height) {
+    const uint32_t li = threadIdx.x & 15, lg = threadIdx.x >> 4 & 3;
+    row = li < height ? s.w + (int64_t(expert) * s.w_e + int64_t(row0 + li) * s.w_s) * SIZE + lg * 16 : nullptr;
+    if constexpr (F8) scales = s.scales + int64_t(expert) * s.scales_e + int64_t((row0 + (lg * 4 < height ? lg * 4 : 0)) / BLOCK) * s.scales_s;
   }
 };
-// A lane's 32 bytes of a row of weights and the x that they meet, of one step.
-template <bool F8, int N>
+// What a lane has of one step: 32 bytes of its row of each of N matrices, in two runs of 64 bytes over four lanes, and the x that they meet.
+// RAGGED: a row may end inside its last step.
+template <bool F8, int N, bool RAGGED>
 struct Step {
-  v4i q[N][2], y[F8 ? 4 : 2];
-};
-template <bool F8, int N>
-__device__ inline void multiply(v4f (&acc)[N], const Step<F8, N> &t, const Weights<F8> (&of)[N], uint32_t s) {
+  static constexpr int Y = F8 ? 2 : 1, HALF = F8 ? 64 : 32;   // chunks of x to a chunk of weights; elements of a run
+  v4i q[N][2], y[2][Y];
+  float scale[N];
+  // x: the lane's token's, from its first element of step 0 on (nullptr: zeros); k: elements of a row.
+  __device__ inline void fetch(const Weights<F8> (&of)[N], const uint16_t *x, uint32_t s, int k) {
+    typedef Weights<F8> W;
+    const uint32_t at = s * 128;   // bytes of weights
 #pragma unroll
-  for (int n = 0; n < N; n++) {
-    if constexpr (F8) {
-      v4f part = {0, 0, 0, 0};
+    for (int n = 0; n < N; n++) {
+      if constexpr (F8) scale[n] = of[n].scales[s];
+      q[n][0] = q[n][1] = v4i{0, 0, 0, 0};
+    }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        int u[4];
-        widen4(t.q[n][i / 2][i % 2 * 2], u[0], u[1]);
-        widen4(t.q[n][i / 2][i % 2 * 2 + 1], u[2], u[3]);
-        part = mma_bf16(v4i{u[0], u[1], u[2], u[3]}, t.y[i], part);
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < Y; j++) y[i][j] = v4i{0, 0, 0, 0};
+    if (!RAGGED || int(s + 1) * W::STEP <= k) {
+      if (of[0].row) {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) q[n][i] = chunk_at(of[n].row + at + i * 64);
       }
-      acc[n] += part * of[n].scales[s];
-    } else {
+      if (x) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) acc[n] = mma_bf16(t.q[n][i], t.y[i], acc[n]);
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < Y; j++) y[i][j] = chunk_at((const uint8_t *)(x + s * W::STEP + i * HALF + j * 8));
+      }
+    } else {   // the rows end inside
+      const int first = int(s) * W::STEP + int(threadIdx.x >> 4 & 3) * (HALF / 4);   // the lane's first element
+      if (of[0].row) {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) q[n][i] = chunk_up_to(of[n].row + at + i * 64, (k - first - i * HALF) * W::SIZE, (first + i * HALF) * W::SIZE);
+      }
+      if (x) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < Y; j++) y[i][j] = chunk_up_to((const uint8_t *)(x + s * W::STEP + i * HALF + j * 8), (k - first - i * HALF - j * 8) * 2, (first + i * HALF + j * 8) * 2);
+      }
     }
   }
-}
-// acc[i] += of[i]'s rows against the lane's token's x (nullptr: zeros), k elements in all.  AHEAD steps' loads are asked for together.
-template <bool F8, int N, int AHEAD>
-__device__ inline void products(v4f (&acc)[N], const Weights<F8> (&of)[N], const uint16_t *x, uint32_t s0, uint32_t s1, int k) {
-  constexpr int STEP = Weights<F8>::STEP, EACH = STEP / 4, SIZE = F8 ? 1 : 2;   // elements of a lane, bytes of one
-  const int lg = (threadIdx.x & 63) >> 4;
-  const uint32_t whole = min(s1, uint32_t(k / STEP));
-  uint32_t s = s0;
-  for (; s + AHEAD <= whole; s += AHEAD) {
-    Step<F8, N> t[AHEAD];
+  __device__ inline void multiply(v4f (&acc)[N]) const {
 #pragma unroll
-    for (int a = 0; a < AHEAD; a++) {
-      const int64_t at = int64_t(s + a) * STEP + lg * EACH;
+    for (int n = 0; n < N; n++) {
+      if constexpr (F8) {
+        v4f part = {0, 0, 0, 0};
 #pragma unroll
-      for (int n = 0; n < N; n++)
+        for (int i = 0; i < 4; i++) {
+          int u[4];
+          widen4(q[n][i / 2][i % 2 * 2], u[0], u[1]);
+          widen4(q[n][i / 2][i % 2 * 2 + 1], u[2], u[3]);
+          part = mma_bf16(v4i{u[0], u[1], u[2], u[3]}, y[i / 2][i % 2], part);
+        }
+        acc[n] += part * scale[n];
+      } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) t[a].q[n][i] = chunk_at(of[n].row + at * SIZE + i * 16);
-#pragma unroll
-      for (int i = 0; i < EACH / 8; i++) t[a].y[i] = v4i{0, 0, 0, 0};
+        for (int i = 0; i < 2; i++) acc[n] = mma_bf16(q[n][i], y[i][0], acc[n]);
+      }
     }
-    if (x) {
+  }
+};
+
+// ---- A workgroup's choices by experts: expert after expert, in parts of up to sixteen ----
+struct Part { uint16_t expert, first, count, unused; };
+constexpr uint32_t most_parts(uint32_t experts, uint32_t choices) { return (choices < experts ? choices : experts) + choices / 16; }
+// What is in LDS, for up to `choices` choices of `experts` experts by tokens of `words` times 32.
+struct Lists {
+  Part *parts;
+  uint16_t *choices;     // expert after expert, a token before the later ones
+  uint32_t *wants;       // [experts][words] a bit for each token
+  uint16_t *first_of;    // [experts]
+  int32_t *totals;       // [2][waves]
+  __device__ inline Lists(uint8_t *at, uint32_t experts, uint32_t all, uint32_t words, uint32_t waves) {
+    parts = (Part *)at, at += most_parts(experts, all) * sizeof(Part);
+    wants = (uint32_t *)at, at += experts * words * 4;
+    totals = (int32_t *)at, at += waves * 8;
+    choices = (uint16_t *)at, at += all * 2;
+    first_of = (uint16_t *)at;
+  }
+  static size_t bytes(uint32_t experts, uint32_t all, uint32_t words, uint32_t waves) { return most_parts(experts, all) * sizeof(Part) + experts * words * 4 + waves * 8 + all * 2 + experts * 2; }
+};
+// Returns the number of parts.  `all` choices, of which token i / top_k made the i-th; ends on a barrier.
+template <int THREADS>
+__device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int32_t *of_choice, uint32_t all, uint32_t words) {
+  constexpr int EACH = MOST_EXPERTS > THREADS ? MOST_EXPERTS / THREADS : 1;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (uint32_t i = tid; i < p.experts * words; i += THREADS) to.wants[i] = 0;
+  __syncthreads();
+  for (uint32_t i = tid; i < all; i += THREADS) {
+    const uint32_t t = i / p.top_k;
+    atomicOr(&to.wants[uint32_t(of_choice[i]) * words + t / 32], 1u << (t % 32));
+  }
+  __syncthreads();
+  // Choices, and parts, before each expert (a thread has EACH neighbours).
+  int32_t count[EACH], before = 0, part = 0;
 #pragma unroll
-      for (int a = 0; a < AHEAD; a++)
+  for (int k = 0; k < EACH; k++) {
+    const uint32_t e = tid * EACH + k;
+    count[k] = 0;
+    if (e < p.experts)
+      for (uint32_t j = 0; j < words; j++) count[k] += __popc(to.wants[e * words + j]);
+    before += count[k], part += (count[k] + 15) / 16;
+  }
+  const int32_t mine = before, my_parts = part;
+  for (int d = 1; d < 64; d *= 2) {
+    const int32_t x = __shfl_up(before, d), y = __shfl_up(part, d);
+    if (int(lane) >= d) before += x, part += y;
+  }
+  if (lane == 63) to.totals[wave * 2] = before, to.totals[wave * 2 + 1] = part;
+  __syncthreads();
+  uint32_t parts = 0;
 #pragma unroll
-        for (int i = 0; i < EACH / 8; i++) t[a].y[i] = chunk_at((const uint8_t *)(x + int64_t(s + a) * STEP + lg * EACH + i * 8));
+  for (uint32_t v = 0; v < THREADS / 64; v++) {
+    const int32_t x = to.totals[v * 2], y = to.totals[v * 2 + 1];
+    if (v < wave) before += x, part += y;
+    parts += y;
+  }
+  before -= mine, part -= my_parts;
+#pragma unroll
+  for (int k = 0; k < EACH; k++) {
+    const uint32_t e = tid * EACH + k;
+    if (e < p.experts) {
+      to.first_of[e] = uint16_t(before);
+      for (int32_t c = 0; c < count[k]; c += 16) to.parts[part++] = {uint16_t(e), uint16_t(before + c), uint16_t(min(16, count[k] - c)), 0};
     }
-#pragma unroll
-    for (int a = 0; a < AHEAD; a++) multiply<F8, N>(acc, t[a], of, s + a);
+    before += count[k];
   }
-  for (; s < s1; s++) {   // the steps left, and the one that holds the rows' ends
-    Step<F8, N> t;
-    const int at = int(s) * STEP + lg * EACH;
-#pragma unroll
-    for (int n = 0; n < N; n++)
-#pragma unroll
-      for (int i = 0; i < 2; i++) t.q[n][i] = chunk_up_to(of[n].row + at * SIZE + i * 16, (k - at) * SIZE - i * 16);
-#pragma unroll
-    for (int i = 0; i < EACH / 8; i++) t.y[i] = x ? chunk_up_to((const uint8_t *)(x + at + i * 8), (k - at - i * 8) * 2) : v4i{0, 0, 0, 0};
-    multiply<F8, N>(acc, t, of, s);
+  __syncthreads();
+  for (uint32_t i = tid; i < all; i += THREADS) {
+    const uint32_t t = i / p.top_k, e = uint32_t(of_choice[i]);
+    uint32_t at = to.first_of[e];
+    for (uint32_t j = 0; j < t / 32; j++) at += __popc(to.wants[e * words + j]);
+    to.choices[at + __popc(to.wants[e * words + t / 32] & ((1u << (t % 32)) - 1))] = uint16_t(i);
   }
+  __syncthreads();
+  return parts;
 }
 
-// ---- Gate and up.  blockIdx.x: an expert, or where there are fewer choices than experts a choice, which stands for its expert if no earlier one does.
-// FUSED: from logits, the choices made here. ----
-constexpr int UP_WAVES = 4;
+// ---- Gate and up.  All parts' tiles of 16 rows lie on a line, of which each workgroup has an equal run, and of a run's steps each wave; its loads run AHEAD
+// steps in front, from one tile into the next, and the waves meet behind UP_RUN tiles.  (A compute unit brings in some 23 GB/s, whatever is asked of it: all of them
+// have to have the same share.)  FUSED: from logits, the choices made here. ----
+constexpr int UP_WAVES = 4, UP_RUN = 8, UP_LOCAL = UP_RUN / UP_WAVES + 1;   // tiles that a wave has some steps of
 constexpr uint32_t FUSED_TOKENS = 4;
-template <bool F8, bool FUSED>
-__global__ __launch_bounds__(UP_WAVES * 64) void k_experts_up(ExpertsArgs p, Places w) {
-  __shared__ v4f part[UP_WAVES][2][64];
-  __shared__ uint16_t choices[MOST_TOKENS];   // of this expert, ascending
+template <bool F8, bool FUSED, bool RAGGED>
+__global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles) {
+  constexpr int AHEAD = F8 ? 3 : 4;
+  extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
+  __shared__ v4f sums[UP_WAVES][UP_LOCAL][2][64];
   __shared__ int32_t chosen[FUSED ? FUSED_TOKENS * MOST_CHOSEN : 1];
-  const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4, wave = threadIdx.x >> 6;
-  const uint32_t row0 = blockIdx.y * 16, rows = live_rows(p), all = rows * p.top_k;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t rows = live_rows(p), all = rows * p.top_k;
   if constexpr (FUSED) {
     __shared__ Choice<UP_WAVES * 64> c;
     for (uint32_t t = 0; t < rows; t++) {
       const float share = choose(p, w, t, c);
-      if (threadIdx.x < p.top_k) chosen[t * p.top_k + threadIdx.x] = c.expert[threadIdx.x];
-      if (blockIdx.x == 0 && blockIdx.y == 0) keep(p, w, t, c, share);
+      if (tid < p.top_k) chosen[t * p.top_k + tid] = c.expert[tid];
+      if (blockIdx.x == 0) keep(p, w, t, c, share);
       __syncthreads();
     }
   }
-  const int32_t *const of_choice = FUSED ? chosen : w.chosen;
-  uint32_t expert = blockIdx.x;
-  if (p.tokens * p.top_k < p.experts) {
-    if (expert >= all) return;
-    expert = uint32_t(of_choice[blockIdx.x]);
-  }
-  // Every wave goes through the choices; the first writes down the expert's.
-  uint32_t count = 0;
-  for (uint32_t i0 = 0; i0 < all; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    const bool mine = i < all && uint32_t(of_choice[i]) == expert;
-    const uint64_t mask = __ballot(mine);
-    if (mine && wave == 0) choices[count + __popcll(mask & ((1ull << lane) - 1))] = uint16_t(i);
-    count += __popcll(mask);
-  }
-  if (count == 0) return;
-  __syncthreads();
-  if (p.tokens * p.top_k < p.experts && choices[0] != blockIdx.x) return;
-  const Weights<F8> of[2] = {{p.gate, expert, row0, p.inter}, {p.up, expert, row0, p.inter}};
+  const Lists lists(dynamic, p.experts, p.tokens * p.top_k, words, UP_WAVES);
+  const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, FUSED ? chosen : w.chosen, all, words));
   const uint32_t steps = (p.hidden + Weights<F8>::STEP - 1) / Weights<F8>::STEP;
-  for (uint32_t c0 = 0; c0 < count; c0 += 16) {
-    const bool mine = c0 + li < count;
-    const uint32_t choice = choices[min(c0 + li, count - 1)];
+  const uint32_t line_end = uint32_t(uint64_t(line) * (blockIdx.x + 1) / gridDim.x);
+  for (uint32_t tile0 = uint32_t(uint64_t(line) * blockIdx.x / gridDim.x); tile0 < line_end; tile0 += UP_RUN) {
+    const uint32_t run = min(uint32_t(UP_RUN), line_end - tile0) * steps;
+    const uint32_t begin = run * wave / UP_WAVES, n = run * (wave + 1) / UP_WAVES - begin;
+    uint32_t fetch_tile = begin / steps, fetch_s = begin - fetch_tile * steps, s = fetch_s, local = 0;
+    Weights<F8> of[2];
+    const uint16_t *x = nullptr;
+    bool fresh = true;
+    Step<F8, 2, RAGGED> t[AHEAD];
+    auto fetch = [&](Step<F8, 2, RAGGED> &to) {
+      if (fresh) {
+        const uint32_t part = by_tiles.div(tile0 + fetch_tile), row0 = (tile0 + fetch_tile - part * tiles) * 16, height = min(16u, p.inter - row0);
+        const Part q = lists.parts[part];
+        const uint32_t expert = __builtin_amdgcn_readfirstlane(q.expert);
+        of[0].from(p.gate, expert, row0, height), of[1].from(p.up, expert, row0, height);
+        x = li < q.count ? p.x + int64_t(lists.choices[q.first + li] / p.top_k) * p.x_s + lg * (F8 ? 16 : 8) : nullptr;
+        fresh = false;
+      }
+      to.fetch(of, x, fetch_s, int(p.hidden));
+      if (++fetch_s == steps) fetch_s = 0, fetch_tile++, fresh = true;
+    };
     v4f acc[2] = {};
-    products<F8, 2, F8 ? 2 : 4>(acc, of, mine ? p.x + int64_t(choice / p.top_k) * p.x_s : nullptr, steps * wave / UP_WAVES, steps * (wave + 1) / UP_WAVES, int(p.hidden));
-    if (c0) __syncthreads();
-    part[wave][0][lane] = acc[0], part[wave][1][lane] = acc[1];
-    __syncthreads();
-    if (wave == 0 && mine) {
-      v4f g = part[0][0][lane], u = part[0][1][lane], h;
 #pragma unroll
-      for (int v = 1; v < UP_WAVES; v++) g += part[v][0][lane], u += part[v][1][lane];
+    for (int a = 0; a < AHEAD; a++)
+      if (uint32_t(a) < n) fetch(t[a]);
+    for (uint32_t at = 0; at < n; at += AHEAD) {
+#pragma unroll
+      for (int a = 0; a < AHEAD; a++) {
+        if (at + a >= n) break;
+        t[a].multiply(acc);
+        if (at + a + AHEAD < n) fetch(t[a]);
+        if (++s == steps || at + a + 1 == n) {
+          sums[wave][local][0][lane] = acc[0], sums[wave][local][1][lane] = acc[1];
+          acc[0] = acc[1] = v4f{0, 0, 0, 0};
+          s = 0, local++;
+        }
+      }
+    }
+    __syncthreads();
+    for (uint32_t tile = wave; tile * steps < run; tile += UP_WAVES) {
+      v4f g = {0, 0, 0, 0}, u = g, h;
+#pragma unroll
+      for (uint32_t v = 0; v < UP_WAVES; v++) {   // those that have some of the tile's steps
+        const uint32_t from = run * v / UP_WAVES, to = run * (v + 1) / UP_WAVES;
+        if (from >= (tile + 1) * steps || to <= tile * steps || from == to) continue;
+        g += sums[v][tile - from / steps][0][lane], u += sums[v][tile - from / steps][1][lane];
+      }
 #pragma unroll
       for (int i = 0; i < 4; i++) h[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
-      const uint32_t row = row0 + lg * 4;
-      if (row < p.inter) store4(w.h + uint64_t(choice) * w.h_s + row, h, int(p.inter - row));
+      const uint32_t part = by_tiles.div(tile0 + tile), row = (tile0 + tile - part * tiles) * 16 + lg * 4;
+      const Part q = lists.parts[part];
+      if (li < q.count && row < p.inter) store4(w.h + uint64_t(lists.choices[q.first + li]) * w.h_s + row, h, int(p.inter - row));
     }
+    if (tile0 + UP_RUN < line_end) __syncthreads();
   }
 }
 
-// ---- Down: blockIdx.x: 16 rows; blockIdx.y: DOWN_TOKENS tokens ----
-constexpr int DOWN_WAVES = 16, DOWN_TOKENS = 64;
-constexpr int DOWN_THREADS = DOWN_WAVES * 64;
-template <bool F8>
-__global__ __launch_bounds__(DOWN_THREADS) void k_experts_down(ExpertsArgs p, Places w, uint32_t tokens_here, uint32_t words) {
+// ---- Down: blockIdx.x: `height` rows, a multiple of four up to sixteen; blockIdx.y: DOWN_TOKENS tokens.  All parts' steps in a line, an equal share to each wave. ----
+constexpr int DOWN_TOKENS = 64;
+template <bool F8, bool RAGGED, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
+  constexpr int AHEAD = F8 ? 3 : 4, THREADS = WAVES * 64;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
-  v4f *const sums = (v4f *)dynamic;                                                       // [DOWN_WAVES][tokens_here][4]
-  uint32_t *const wants = (uint32_t *)(sums + DOWN_WAVES * tokens_here * 4);              // [experts][words] a bit for each token of this workgroup's
-  uint16_t *const choices = (uint16_t *)(wants + p.experts * words);                      // [tokens_here * top_k] expert after expert
-  __shared__ uint16_t expert_of[MOST_EXPERTS], first[MOST_EXPERTS + 1], first_of[MOST_EXPERTS];
-  __shared__ int32_t totals[2][MOST_EXPERTS / 64];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
-  const uint32_t row0 = blockIdx.x * 16, t0 = blockIdx.y * DOWN_TOKENS, rows = live_rows(p);
+  v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
+  float *const shares = (float *)(sums + WAVES * tokens_here * 4);   // [tokens_here * top_k]
+  const Lists lists((uint8_t *)(shares + (tokens_here * p.top_k + 1) / 2 * 2), p.experts, tokens_here * p.top_k, words, WAVES);
+  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t row0 = blockIdx.x * height, t0 = blockIdx.y * DOWN_TOKENS, rows = live_rows(p), rows_here = min(height, p.hidden - row0);
   if (t0 >= rows) return;
-  const uint32_t here = min(tokens_here, rows - t0), all = here * p.top_k;
-  const int32_t *const chosen = w.chosen + t0 * p.top_k;
-  for (uint32_t i = tid; i < p.experts * words; i += DOWN_THREADS) wants[i] = 0;
+  const uint32_t here = min(tokens_here, rows - t0);
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
-  __syncthreads();
-  for (uint32_t i = tid; i < all; i += DOWN_THREADS) {
-    const uint32_t t = i / p.top_k;
-    atomicOr(&wants[uint32_t(chosen[i]) * words + t / 32], 1u << (t % 32));
-  }
-  __syncthreads();
-  // Wanted experts, and choices, before each expert.
-  int32_t count = 0;
-  if (tid < p.experts)
-    for (uint32_t j = 0; j < words; j++) count += __popc(wants[tid * words + j]);
-  int32_t before = count, slot = count > 0;
-  if (tid < MOST_EXPERTS) {
-    for (int d = 1; d < 64; d *= 2) {
-      const int32_t x = __shfl_up(before, d), y = __shfl_up(slot, d);
-      if (int(lane) >= d) before += x, slot += y;
+  for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
+  const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words));
+  const uint32_t steps = (p.inter + Weights<F8>::STEP - 1) / Weights<F8>::STEP, line = parts * steps;
+  const uint32_t begin = uint32_t(uint64_t(line) * wave / WAVES), n = uint32_t(uint64_t(line) * (wave + 1) / WAVES) - begin;
+  uint32_t fetch_part = begin / steps, fetch_s = begin - fetch_part * steps, at_part = fetch_part, s = fetch_s;
+  Weights<F8> of[1];
+  const uint16_t *x = nullptr;
+  bool fresh = true;
+  Step<F8, 1, RAGGED> t[AHEAD];
+  auto fetch = [&](Step<F8, 1, RAGGED> &to) {
+    if (fresh) {
+      const Part q = lists.parts[fetch_part];
+      of[0].from(p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
+      x = li < q.count ? w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + li]) * w.h_s + lg * (F8 ? 16 : 8) : nullptr;
+      fresh = false;
     }
-    if (lane == 63) totals[0][wave] = before, totals[1][wave] = slot;
-  }
-  __syncthreads();
-  uint32_t active = 0;
-  for (uint32_t v = 0; v < MOST_EXPERTS / 64; v++) {
-    if (v < wave) before += totals[0][v], slot += totals[1][v];
-    active += totals[1][v];
-  }
-  if (tid < p.experts) {
-    first_of[tid] = uint16_t(before - count);
-    if (count > 0) expert_of[slot - 1] = uint16_t(tid), first[slot - 1] = uint16_t(before - count);
-  }
-  if (tid == 0) first[active] = uint16_t(all);
-  __syncthreads();
-  for (uint32_t i = tid; i < all; i += DOWN_THREADS) {
-    const uint32_t t = i / p.top_k, e = uint32_t(chosen[i]);
-    uint32_t at = first_of[e];
-    for (uint32_t j = 0; j < t / 32; j++) at += __popc(wants[e * words + j]);
-    choices[at + __popc(wants[e * words + t / 32] & ((1u << (t % 32)) - 1))] = uint16_t(i);
-  }
-  __syncthreads();
-  const uint32_t steps = (p.inter + Weights<F8>::STEP - 1) / Weights<F8>::STEP;
-  // All experts' steps in a line, an equal share to each wave.
-  const uint32_t line = active * steps, begin = uint32_t(uint64_t(line) * wave / DOWN_WAVES), end = uint32_t(uint64_t(line) * (wave + 1) / DOWN_WAVES);
-  for (uint32_t at = begin; at < end;) {
-    const uint32_t slot_at = at / steps, s0 = at - slot_at * steps, s1 = min(steps, s0 + (end - at));
-    at += s1 - s0;
-    const Weights<F8> of[1] = {{p.down, expert_of[slot_at], row0, p.hidden}};
-    const uint32_t last = first[slot_at + 1];
-    for (uint32_t c0 = first[slot_at]; c0 < last; c0 += 16) {
-      const bool mine = c0 + li < last;
-      const uint32_t local = choices[min(c0 + li, last - 1)], choice = t0 * p.top_k + local;
-      v4f acc[1] = {};
-      products<F8, 1, F8 ? 2 : 4>(acc, of, mine ? w.h + uint64_t(choice) * w.h_s : nullptr, s0, s1, int(p.inter));
-      if (mine) sums[(wave * tokens_here + local / p.top_k) * 4 + lg] += acc[0] * w.shares[choice];
+    to.fetch(of, x, fetch_s, int(p.inter));
+    if (++fetch_s == steps) fetch_s = 0, fetch_part++, fresh = true;
+  };
+  v4f acc[1] = {};
+#pragma unroll
+  for (int a = 0; a < AHEAD; a++)
+    if (uint32_t(a) < n) fetch(t[a]);
+  for (uint32_t at = 0; at < n; at += AHEAD) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) {
+      if (at + a >= n) break;
+      t[a].multiply(acc);
+      if (at + a + AHEAD < n) fetch(t[a]);
+      if (++s == steps || at + a + 1 == n) {
+        const Part q = lists.parts[at_part];
+        if (li < q.count) {
+          const uint32_t choice = lists.choices[q.first + li];
+          sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
+        }
+        acc[0] = v4f{0, 0, 0, 0};
+        s = 0, at_part++;
+      }
     }
   }
   __syncthreads();
-  for (uint32_t i = tid; i < here * 4; i += DOWN_THREADS) {
+  for (uint32_t i = tid; i < here * 4; i += THREADS) {
     v4f sum = sums[i];
 #pragma unroll
-    for (uint32_t v = 1; v < DOWN_WAVES; v++) sum += sums[v * tokens_here * 4 + i];
-    const uint32_t row = row0 + i % 4 * 4;
-    if (row < p.hidden) store4(p.out + int64_t(t0 + i / 4) * p.out_s + row, sum, int(p.hidden - row));
+    for (uint32_t v = 1; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i];
+    const uint32_t row = i % 4 * 4;
+    if (row < rows_here) store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
   }
 }
 
+template <bool F8, bool FUSED, bool RAGGED>
+hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  // Three workgroups to a compute unit, what their registers allow, or one to a tile.
+  const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
+  const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices)) * tiles, 3 * g_compute_units));
+  const size_t lds = Lists::bytes(a.experts, choices, words, UP_WAVES);
+  static std::atomic<uint64_t> raised{0};
+  if (lds > 32 * 1024 && !plan::recording()) {
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, FUSED, RAGGED>), 64 * 1024);
+    if (e != hipSuccess) return e;
+  }
+  MRL_LAUNCH((k_experts_up<F8, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles));
+  return plan::last_error();
+}
+template <bool F8, bool RAGGED, int WAVES>
+hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, hipStream_t stream) {
+  const uint32_t here = std::min(a.tokens, uint32_t(DOWN_TOKENS)), words = (here + 31) / 32;
+  const size_t lds = size_t(WAVES) * here * 64 + size_t(here * a.top_k + 1) / 2 * 8 + Lists::bytes(a.experts, here * a.top_k, words, WAVES);
+  static std::atomic<uint64_t> raised{0};
+  if (lds > 48 * 1024 && !plan::recording()) {
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, RAGGED, WAVES>), 96 * 1024);
+    if (e != hipSuccess) return e;
+  }
+  MRL_LAUNCH((k_experts_down<F8, RAGGED, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + DOWN_TOKENS - 1) / DOWN_TOKENS), dim3(WAVES * 64), lds, stream, a, w, height, here, words);
+  return plan::last_error();
+}
+template <bool F8, bool RAGGED>
+hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  // Rows for all compute units alike: a workgroup of sixteen waves to each where sixteen rows are enough, else several of eight.
+  const uint32_t each = (a.hidden + 16 * g_compute_units - 1) / (16 * g_compute_units), groups = each * g_compute_units;
+  const uint32_t height = std::min(16u, ((a.hidden + groups - 1) / groups + 3) / 4 * 4);
+  return each == 1 ? launch_down_waves<F8, RAGGED, 16>(a, w, height, stream) : launch_down_waves<F8, RAGGED, 8>(a, w, height, stream);
+}
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  const uint32_t choices = a.tokens * a.top_k, slots = std::min(a.experts, choices);
+  const uint32_t slots = std::min(a.experts, a.tokens * a.top_k);
   const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * slots;
   plan::work(plan::UNIT_STREAM, 0, 2.0 * (double(a.experts) + a.tokens) * a.hidden);
   MRL_LAUNCH(k_experts_logits, dim3(a.experts, (a.tokens + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(ROUTER_THREADS), 0, stream, a, w);
@@ -384,20 +515,13 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), 0, stream, a, w);
   }
+  const bool ragged_up = a.hidden % Weights<F8>::STEP != 0, ragged_down = a.inter % Weights<F8>::STEP != 0;
   plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
-  const dim3 up(slots, (a.inter + 15) / 16);
-  if (fused) MRL_LAUNCH((k_experts_up<F8, true>), up, dim3(UP_WAVES * 64), 0, stream, a, w);
-  else MRL_LAUNCH((k_experts_up<F8, false>), up, dim3(UP_WAVES * 64), 0, stream, a, w);
-  const uint32_t here = std::min(a.tokens, uint32_t(DOWN_TOKENS)), words = (here + 31) / 32;
-  const size_t lds = size_t(DOWN_WAVES) * here * 64 + size_t(a.experts) * words * 4 + size_t(here) * a.top_k * 2;
-  static std::atomic<uint64_t> raised{0};
-  if (lds > 48 * 1024 && !plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8>), 96 * 1024);
-    if (e != hipSuccess) return e;
-  }
+  const hipError_t e = fused ? ragged_up ? launch_up<F8, true, true>(a, w, stream) : launch_up<F8, true, false>(a, w, stream)
+                             : ragged_up ? launch_up<F8, false, true>(a, w, stream) : launch_up<F8, false, false>(a, w, stream);
+  if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  MRL_LAUNCH(k_experts_down<F8>, dim3((a.hidden + 15) / 16, (a.tokens + DOWN_TOKENS - 1) / DOWN_TOKENS), dim3(DOWN_THREADS), lds, stream, a, w, here, words);
-  return plan::last_error();
+  return ragged_down ? launch_down<F8, true>(a, w, stream) : launch_down<F8, false>(a, w, stream);
 }
 
 }  // namespace

@@ -44,9 +44,9 @@ __global__ __launch_bounds__(TILE_THREADS) void k_product_tile(ProductArgs p, ui
   auto fetch = [&](int step) {
     const int at = step * int(BLOCK) + chunk * 16;
 #pragma unroll
-    for (int i = 0; i < A_EACH; i++) a_reg[i] = chunk_up_to(p.a + int64_t(min(m0 + row0 + i * 32, p.m - 1)) * p.a_s + at, k - at);
+    for (int i = 0; i < A_EACH; i++) a_reg[i] = chunk_up_to(p.a + int64_t(min(m0 + row0 + i * 32, p.m - 1)) * p.a_s + at, k - at, at);
 #pragma unroll
-    for (int i = 0; i < B_EACH; i++) b_reg[i] = chunk_up_to(p.b + int64_t(min(n0 + row0 + i * 32, p.n - 1)) * p.b_s + at, k - at);
+    for (int i = 0; i < B_EACH; i++) b_reg[i] = chunk_up_to(p.b + int64_t(min(n0 + row0 + i * 32, p.n - 1)) * p.b_s + at, k - at, at);
   };
   auto keep = [&](int slot) {
 #pragma unroll
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs p) {
   }
   v4f acc[MT] = {};
   auto thirty_two = [&](const uint8_t *row, int at) {
-    const v4i lo = chunk_up_to(row + at, k - at), hi = chunk_up_to(row + at + 16, k - at - 16);
+    const v4i lo = chunk_up_to(row + at, k - at, at), hi = chunk_up_to(row + at + 16, k - at - 16, at + 16);
     return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   for (int step = wave; step < steps; step += WAVES) {
