@@ -1,0 +1,51 @@
+// What the kernels of products of blocks share (matmul_blocks.hip, matmul_blocks_wide.hip).
+#pragma once
+#include "blocks_device.h"
+
+namespace mrl {
+namespace blocks {
+
+// Results in bf16 come from products in e4m3, whose cuts they do not show (2^-9 of a result against 2^-13 of a block's largest product); results in f32 from the same numbers
+// in bf16.
+template <class OUT> struct Operand;
+template <> struct Operand<uint16_t> {
+  v8i x;
+  __device__ inline void from(v8i q) { x = q; }
+  __device__ inline v4f by(const Operand &o) const { return mma_e4m3(x, o.x); }
+};
+template <> struct Operand<float> {
+  Wide x;
+  __device__ inline void from(v8i q) { x = widen(q); }
+  __device__ inline v4f by(const Operand &o) const { return mma_wide(x, o.x); }
+};
+
+constexpr uint32_t OUTSIDE = 0x80000000u;   // an offset that no resource here holds
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ inline uint32_t lds_address(const void *p) { return uint32_t(reinterpret_cast<uintptr_t>((lds_void *)p)); }
+// 64 lanes x 16 bytes from `off` (of each lane) behind `from` into the KiB at LDS address `to`, lane l to its l-th sixteen; offsets past the resource bring zeros.  Assembly, so
+// that the compiler does not wait for it; M0 is set in the same statement.
+__device__ inline void dma16(v4i from, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(from), "s"(to) : "memory");
+}
+__device__ inline v4i resource(const void *base, uint32_t bytes) {
+  const uint64_t b = reinterpret_cast<uintptr_t>(base);
+  return v4i{int(uint32_t(b)), int(uint32_t(b >> 32)), int(bytes), 0x00020000};
+}
+// All but the newest N loads have landed, and every LDS access of this wave is done.
+template <int N>
+__device__ inline void wait_for_all_but() {
+  asm volatile("" : : : "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  asm volatile("" : : : "memory");
+}
+
+// Rows of whole 16-byte chunks, 256 of them within 2 GB.
+inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 16 == 0 && k % 16 == 0 && stride < (1 << 23);
+}
+
+}  // namespace blocks
+
+hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);
+
+}  // namespace mrl

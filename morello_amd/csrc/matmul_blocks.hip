@@ -6,25 +6,11 @@
 // has as one number.
 #include <algorithm>
 
-#include "blocks_device.h"
+#include "matmul_blocks.h"
 
 namespace mrl {
 namespace {
 using namespace blocks;
-
-// Results in bf16 come from products in e4m3, whose cuts they do not show (2^-9 of a result against 2^-13 of a block's largest product); results in f32 from the same numbers
-// in bf16.
-template <class OUT> struct Operand;
-template <> struct Operand<uint16_t> {
-  v8i x;
-  __device__ inline void from(v8i q) { x = q; }
-  __device__ inline v4f by(const Operand &o) const { return mma_e4m3(x, o.x); }
-};
-template <> struct Operand<float> {
-  Wide x;
-  __device__ inline void from(v8i q) { x = widen(q); }
-  __device__ inline v4f by(const Operand &o) const { return mma_wide(x, o.x); }
-};
 
 // ---- Tiles of BM x BN, the waves 2 x 2 ----
 constexpr int TILE_THREADS = 256;
@@ -143,6 +129,7 @@ hipError_t launch(const ProductArgs &p, hipStream_t stream) {
   plan::work(plan::UNIT_MFMA_I8, ops, bytes);
   if (p.m <= 16) MRL_LAUNCH((k_product_few<1, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
   else if (p.m <= 32) MRL_LAUNCH((k_product_few<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
+  else if (sizeof(OUT) == 2 && p.m > 512 && p.n > 512 && rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k)) return launch_product_wide(p, stream);
   else {
     const uint32_t tiles_m = (p.m + 127) / 128, tiles_n = (p.n + 127) / 128;
     MRL_LAUNCH((k_product_tile<128, 128, OUT>), dim3(tiles_m * tiles_n), dim3(TILE_THREADS), 0, stream, p, tiles_m);

@@ -53,7 +53,7 @@ class Operands:
 
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 4096, 2048), (2, 17, 129), (7, 1000, 4104), (16, 512, 512), (17, 100, 1000), (32, 64, 257), (33, 130, 384), (48, 1040, 2176),
          (64, 64, 64), (65, 300, 130), (100, 2048, 1024), (128, 128, 128), (129, 257, 640), (200, 520, 15), (300, 200, 1111), (513, 384, 2048), (1000, 1030, 1200), (257, 2000, 33),
-         (2049, 2050, 256)]
+         (2049, 2050, 256), (600, 800, 1040), (768, 520, 128), (1025, 513, 2000)]
 
 
 @pytest.mark.parametrize("out", ["bf16", "f32"])
