@@ -27,6 +27,10 @@ __device__ inline uint32_t lds_address(const void *p) { return uint32_t(reinterp
 __device__ inline void dma16(v4i from, uint32_t off, uint32_t to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(from), "s"(to) : "memory");
 }
+// The same with 4 bytes a lane: 256 bytes.
+__device__ inline void dma4(v4i from, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(from), "s"(to) : "memory");
+}
 __device__ inline v4i resource(const void *base, uint32_t bytes) {
   const uint64_t b = reinterpret_cast<uintptr_t>(base);
   return v4i{int(uint32_t(b)), int(uint32_t(b >> 32)), int(bytes), 0x00020000};
@@ -39,6 +43,13 @@ __device__ inline void wait_for_all_but() {
   asm volatile("" : : : "memory");
 }
 
+// Every LDS access of this wave is done.
+__device__ inline void wait_for_lds() {
+  asm volatile("" : : : "memory");
+  __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
+  asm volatile("" : : : "memory");
+}
+
 // Rows of whole 16-byte chunks, 256 of them within 2 GB.
 inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 16 == 0 && k % 16 == 0 && stride < (1 << 23);
@@ -47,5 +58,8 @@ inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
 }  // namespace blocks
 
 hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);
+// Up to 128 rows of a; rows of whole chunks, scales of a within 2 GB.
+constexpr uint32_t MOST_FEW = 128;
+hipError_t launch_product_few(const ProductArgs &p, hipStream_t stream);
 
 }  // namespace mrl

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_product_tile(ProductArgs p, ui
 
 // ---- Few rows: 16 of b's rows to a workgroup, whose waves share K.  Memory bounds it, so that the products are in bf16 whatever the result's type. ----
 template <int MT, int WAVES, class OUT>
-__global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs p) {
+__global__ __launch_bounds__(WAVES * 64) void k_product_few_any(ProductArgs p) {
   __shared__ v4f part[WAVES][MT][64];
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4, wave = threadIdx.x >> 6;
   const uint32_t n0 = blockIdx.x * 16;
@@ -127,9 +127,11 @@ template <class OUT>
 hipError_t launch(const ProductArgs &p, hipStream_t stream) {
   const double ops = 2.0 * p.m * double(p.n) * p.k, bytes = (double(p.m) + p.n) * p.k + double(p.m) * p.n * sizeof(OUT);
   plan::work(plan::UNIT_MFMA_I8, ops, bytes);
-  if (p.m <= 16) MRL_LAUNCH((k_product_few<1, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
-  else if (p.m <= 32) MRL_LAUNCH((k_product_few<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
-  else if (sizeof(OUT) == 2 && p.m > 512 && p.n > 512 && rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k)) return launch_product_wide(p, stream);
+  const bool chunks = rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k);
+  if (chunks && p.m <= MOST_FEW && p.as_s < (1 << 21)) return launch_product_few(p, stream);
+  if (p.m <= 16) MRL_LAUNCH((k_product_few_any<1, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
+  else if (p.m <= 32) MRL_LAUNCH((k_product_few_any<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
+  else if (sizeof(OUT) == 2 && p.m > 512 && p.n > 512 && chunks) return launch_product_wide(p, stream);
   else {
     const uint32_t tiles_m = (p.m + 127) / 128, tiles_n = (p.n + 127) / 128;
     MRL_LAUNCH((k_product_tile<128, 128, OUT>), dim3(tiles_m * tiles_n), dim3(TILE_THREADS), 0, stream, p, tiles_m);

@@ -35,7 +35,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
   const uint32_t lds0 = lds_address(lds), to0 = lds0 + (of_a ? 0 : SIDE * BLOCK) + first * BLOCK;
   const uint32_t left_in_last = p.k - (steps - 1) * BLOCK;
   auto fetch = [&](int step) {
-    const v4i from = resource(tile + step * int(BLOCK), rows * stride);   // (rows past the last bring zeros; what lies behind the last row's end is not asked for)
+    // (up to the last row's end: rows behind it bring zeros, or where rows overlap something, which nobody sees)
+    const v4i from = resource(tile + step * int(BLOCK), (rows - 1) * stride + (p.k - step * BLOCK));
     const bool last = step == steps - 1;
     const uint32_t e = last && even * 16 >= left_in_last ? OUTSIDE : off_even, o = last && odd * 16 >= left_in_last ? OUTSIDE : off_odd;
     const uint32_t to = to0 + (step & 1) * SLOT;
@@ -77,23 +78,23 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
     if (step + 1 < steps) fetch(step + 1);
     const uint8_t *const a = lds + (step & 1) * SLOT + wm * 128 * BLOCK, *const b = lds + (step & 1) * SLOT + (SIDE + wn * 64) * BLOCK;
     const float *const scale = scales + ((step / AHEAD & 1) * AHEAD * 2 + step % AHEAD * 2 + (wn >> 1)) * SIDE + wm * 128 + li;
-    v8i w[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) w[u] = fragment(b + u * 16 * BLOCK);
+    v8i w[4], x[2];
     v4f part[2][4];
     float s[2];
+    x[0] = fragment(a), s[0] = scale[0];
+#pragma unroll
+    for (int u = 0; u < 4; u++) w[u] = fragment(b + u * 16 * BLOCK);
+    // A sixteen of a's rows under the multiply-adds of the one before; its operands are read one ahead.
 #pragma unroll
     for (int t = 0; t < 9; t++) {
-      if (t < 8) {
-        const v8i x = fragment(a + t * 16 * BLOCK);
-        s[t & 1] = scale[t * 16];
+      if (t < 7) x[(t + 1) & 1] = fragment(a + (t + 1) * 16 * BLOCK);
 #pragma unroll
-        for (int u = 0; u < 4; u++) part[t & 1][u] = mma_e4m3(w[u], x);
+      for (int u = 0; u < 4; u++) {
+        if (t < 8) part[t & 1][u] = mma_e4m3(w[u], x[t & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t > 0) acc[t - 1][u] += part[(t - 1) & 1][u] * s[(t - 1) & 1];
       }
-      if (t > 0) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) acc[t - 1][u] += part[(t - 1) & 1][u] * s[(t - 1) & 1];
-      }
+      if (t < 7) s[(t + 1) & 1] = scale[(t + 1) * 16];
     }
   }
 #pragma unroll

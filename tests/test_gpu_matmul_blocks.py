@@ -51,7 +51,8 @@ class Operands:
         assert (off <= bound).all(), f"{(off / bound).max():.2f} of the bound, at {np.argwhere(~(off <= bound))[:4].tolist()}"
 
 
-SIZES = [(1, 1, 1), (1, 16, 128), (1, 4096, 2048), (2, 17, 129), (7, 1000, 4104), (16, 512, 512), (17, 100, 1000), (32, 64, 257), (33, 130, 384), (48, 1040, 2176),
+SIZES = [(20, 400, 1168), (38, 6200, 512), (50, 6160, 400), (77, 6200, 640), (90, 6150, 384), (90, 800, 1536), (72, 1000, 2048), (40, 100, 3000 + 8), (111, 250, 1024), (16, 33, 16),
+         (1, 1, 1), (1, 16, 128), (1, 4096, 2048), (2, 17, 129), (7, 1000, 4104), (16, 512, 512), (17, 100, 1000), (32, 64, 257), (33, 130, 384), (48, 1040, 2176),
          (64, 64, 64), (65, 300, 130), (100, 2048, 1024), (128, 128, 128), (129, 257, 640), (200, 520, 15), (300, 200, 1111), (513, 384, 2048), (1000, 1030, 1200), (257, 2000, 33),
          (2049, 2050, 256), (600, 800, 1040), (768, 520, 128), (1025, 513, 2000)]
 
@@ -77,6 +78,20 @@ def test_strides_and_odd_addresses(gpu, m, n, k):
                dict(a_stride=up, b_stride=k + 5, offset=8)):
         x.check(x.run("bf16", **kw), "bf16")
         x.check(x.run("f32", **kw), "f32")
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 70, 512), (60, 90, 512), (600, 530, 256)])
+def test_rows_that_overlap(gpu, m, n, k):
+    """Strides of inputs may be less than a row."""
+    x = Operands(m, n, k, 10, narrow=True)
+    flat_a, flat_b = x.a.reshape(-1)[:(m - 1) * 32 + k].copy(), x.b.reshape(-1)[:(n - 1) * 16 + k].copy()
+    x.a = np.lib.stride_tricks.as_strided(flat_a, (m, k), (32, 1))
+    x.b = np.lib.stride_tricks.as_strided(flat_b, (n, k), (16, 1))
+    op = M.MatmulBlocks(M.bf16, m, n, k, a_stride=32, b_stride=16)
+    out = np.zeros((m, n), np.uint16)
+    with Device() as d:
+        op.run_device([d.put(flat_a), d.put(x.a_scales), d.put(flat_b), d.put(x.b_scales), d.put(out), d.put(np.zeros(max(16, op.workspace_bytes()), np.uint8))])
+        x.check(d.get(4, out), "bf16")
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 40, 300), (70, 200, 500), (260, 520, 640)])
