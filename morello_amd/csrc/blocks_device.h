@@ -75,13 +75,5 @@ __device__ inline Wide widen(v8i q) {
   }
   return w;
 }
-// The same sums as mma_e4m3's at half its rate.
-__device__ inline v4f mma_wide(const Wide &a, const Wide &b) {
-  v4f c = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; i++) c = mma_bf16(a.x[i], b.x[i], c);
-  return c;
-}
-
 }  // namespace blocks
 }  // namespace mrl

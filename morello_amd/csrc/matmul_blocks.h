@@ -11,13 +11,26 @@ template <class OUT> struct Operand;
 template <> struct Operand<uint16_t> {
   v8i x;
   __device__ inline void from(v8i q) { x = q; }
-  __device__ inline v4f by(const Operand &o) const { return mma_e4m3(x, o.x); }
 };
 template <> struct Operand<float> {
   Wide x;
   __device__ inline void from(v8i q) { x = widen(q); }
-  __device__ inline v4f by(const Operand &o) const { return mma_wide(x, o.x); }
 };
+// sums[i] = a block's products of w[i] and x.  (In bf16 four instructions to a sum, each of which waits for the one before: N sums side by side.)
+template <int N>
+__device__ inline void products(v4f (&sums)[N], const Operand<uint16_t> (&w)[N], const Operand<uint16_t> &x) {
+#pragma unroll
+  for (int i = 0; i < N; i++) sums[i] = mma_e4m3(w[i].x, x.x);
+}
+template <int N>
+__device__ inline void products(v4f (&sums)[N], const Operand<float> (&w)[N], const Operand<float> &x) {
+#pragma unroll
+  for (int i = 0; i < N; i++) sums[i] = v4f{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+#pragma unroll
+    for (int i = 0; i < N; i++) sums[i] = mma_bf16(w[i].x.x[j], x.x.x[j], sums[i]);
+}
 
 constexpr uint32_t OUTSIDE = 0x80000000u;   // an offset that no resource here holds
 typedef __attribute__((address_space(3))) void lds_void;
@@ -58,6 +71,7 @@ inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
 }  // namespace blocks
 
 hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);
+hipError_t launch_product_tile(const ProductArgs &p, hipStream_t stream);
 // Up to 128 rows of a; rows of whole chunks, scales of a within 2 GB.
 constexpr uint32_t MOST_FEW = 128;
 hipError_t launch_product_few(const ProductArgs &p, hipStream_t stream);

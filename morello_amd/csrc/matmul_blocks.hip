@@ -15,7 +15,7 @@ using namespace blocks;
 // ---- Tiles of BM x BN, the waves 2 x 2 ----
 constexpr int TILE_THREADS = 256;
 template <int BM, int BN, class OUT>
-__global__ __launch_bounds__(TILE_THREADS) void k_product_tile(ProductArgs p, uint32_t tiles_m) {
+__global__ __launch_bounds__(TILE_THREADS) void k_product_tile_any(ProductArgs p, uint32_t tiles_m) {
   constexpr int A_EACH = BM * 8 / TILE_THREADS, B_EACH = BN * 8 / TILE_THREADS, MT = BM / 32, NT = BN / 32;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * BLOCK];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -66,8 +66,10 @@ __global__ __launch_bounds__(TILE_THREADS) void k_product_tile(ProductArgs p, ui
     for (int t = 0; t < MT; t++) {
       Operand<OUT> a;
       a.from(fragment(from + (wm + t * 16) * BLOCK));
+      v4f part[NT];
+      products(part, b, a);
 #pragma unroll
-      for (int u = 0; u < NT; u++) acc[t][u] += b[u].by(a) * scale[t];
+      for (int u = 0; u < NT; u++) acc[t][u] += part[u] * scale[t];
     }
   }
 #pragma unroll
@@ -83,6 +85,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_product_tile(ProductArgs p, ui
   }
 }
 
+constexpr uint32_t MOST_FEW_ANY = 32;
 // ---- Few rows: 16 of b's rows to a workgroup, whose waves share K.  Memory bounds it, so that the products are in bf16 whatever the result's type. ----
 template <int MT, int WAVES, class OUT>
 __global__ __launch_bounds__(WAVES * 64) void k_product_few_any(ProductArgs p) {
@@ -106,10 +109,16 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few_any(ProductArgs p) {
   };
   for (int step = wave; step < steps; step += WAVES) {
     const int at = step * int(BLOCK) + lg * 32;
-    const Wide x = widen(thirty_two(b, at));
+    Operand<float> x[1], y;
+    x[0].from(thirty_two(b, at));
     const float sb = b_scale[step];
 #pragma unroll
-    for (int t = 0; t < MT; t++) acc[t] += mma_wide(x, widen(thirty_two(a[t], at))) * (a_scale[t][step] * sb);
+    for (int t = 0; t < MT; t++) {
+      v4f part[1];
+      y.from(thirty_two(a[t], at));
+      products(part, x, y);
+      acc[t] += part[0] * (a_scale[t][step] * sb);
+    }
   }
 #pragma unroll
   for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
@@ -125,24 +134,69 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few_any(ProductArgs p) {
 
 template <class OUT>
 hipError_t launch(const ProductArgs &p, hipStream_t stream) {
-  const double ops = 2.0 * p.m * double(p.n) * p.k, bytes = (double(p.m) + p.n) * p.k + double(p.m) * p.n * sizeof(OUT);
-  plan::work(plan::UNIT_MFMA_I8, ops, bytes);
-  const bool chunks = rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k);
-  if (chunks && p.m <= MOST_FEW && p.as_s < (1 << 21)) return launch_product_few(p, stream);
+  plan::work(plan::UNIT_MFMA_I8, 2.0 * p.m * double(p.n) * p.k, (double(p.m) + p.n) * p.k + double(p.m) * p.n * sizeof(OUT), 0, 0, sizeof(OUT) == 2 ? 1.4 : 0.7);
+  if (rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k) && p.as_s < (1 << 21)) {
+    if (p.m <= MOST_FEW) return launch_product_few(p, stream);
+    // Tiles of 256 x 256 where the last of their rounds over the compute units is not too empty.  us, so and on the smaller ones: 2048 x 4096 x 4096 (128 tiles) 61 and 51, 2048 x 6144 x 2048
+    // (192) 38.3 and 46, 4096 x 4096 x 1024 (256) 25.9 and 32.3.
+    const uint64_t wide = uint64_t((p.m + 255) / 256) * ((p.n + 255) / 256), rounds = (wide + g_compute_units - 1) / g_compute_units;
+    return sizeof(OUT) == 2 && wide * 100 >= 62 * rounds * g_compute_units ? launch_product_wide(p, stream) : launch_product_tile(p, stream);
+  }
   if (p.m <= 16) MRL_LAUNCH((k_product_few_any<1, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
-  else if (p.m <= 32) MRL_LAUNCH((k_product_few_any<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
-  else if (sizeof(OUT) == 2 && p.m > 512 && p.n > 512 && chunks) return launch_product_wide(p, stream);
+  else if (p.m <= MOST_FEW_ANY) MRL_LAUNCH((k_product_few_any<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
   else {
     const uint32_t tiles_m = (p.m + 127) / 128, tiles_n = (p.n + 127) / 128;
-    MRL_LAUNCH((k_product_tile<128, 128, OUT>), dim3(tiles_m * tiles_n), dim3(TILE_THREADS), 0, stream, p, tiles_m);
+    MRL_LAUNCH((k_product_tile_any<128, 128, OUT>), dim3(tiles_m * tiles_n), dim3(TILE_THREADS), 0, stream, p, tiles_m);
   }
   return plan::last_error();
 }
 
+// Operands whose rows are not whole 16-byte chunks are copied into ones that are, with zeros behind K, where there are more rows than a workgroup reads b for once.
+struct Copies {
+  bool a = false, b = false;
+  uint32_t ld = 0;
+  size_t a_bytes = 0, b_bytes = 0;
+};
+Copies copies(const ProductArgs &p) {
+  Copies c;
+  if (p.m <= MOST_FEW_ANY) return c;
+  c.a = p.k % 16 != 0 || p.a_s % 16 != 0, c.b = p.k % 16 != 0 || p.b_s % 16 != 0;
+  c.ld = (p.k + 127) / 128 * 128;
+  if (c.a) c.a_bytes = size_t(p.m) * c.ld;
+  if (c.b) c.b_bytes = size_t(p.n) * c.ld;
+  if (std::max(c.a_bytes, c.b_bytes) >= (size_t(1) << 34)) return Copies();   // (numbered in chunks of 16 bytes below 2^31)
+  return c;
+}
+PadRows rows_of(const void *from, uint32_t rows, uint32_t k, int64_t stride, void *to, uint32_t ld) {
+  PadRows r = {};
+  r.src.ptr = const_cast<void *>(from), r.src.dtype = MRL_U8, r.src.rank = 3;
+  r.src.shape[0] = 1, r.src.shape[1] = rows, r.src.shape[2] = k;
+  r.src.stride[0] = 0, r.src.stride[1] = stride, r.src.stride[2] = 1;
+  r.dst = to, r.dst_ld = ld, r.dst_rows = rows, r.elem_size = 1;
+  return r;
+}
+
 }  // namespace
 
-size_t product_workspace_bytes(const ProductArgs &) { return 0; }
+size_t product_workspace_bytes(const ProductArgs &p) {
+  const Copies c = copies(p);
+  return c.a_bytes + c.b_bytes;
+}
 
-hipError_t launch_product(const ProductArgs &p, hipStream_t stream) { return p.out_dtype == MRL_BF16 ? launch<uint16_t>(p, stream) : launch<float>(p, stream); }
+hipError_t launch_product(const ProductArgs &given, hipStream_t stream) {
+  ProductArgs p = given;
+  const Copies c = copies(p);
+  // (an operand that keeps its rows has to have them at such addresses, too)
+  auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if ((c.a || c.b) && (c.a || aligned(p.a)) && (c.b || aligned(p.b))) {
+    const PadRows a = rows_of(p.a, p.m, p.k, p.a_s, p.workspace, c.ld), b = rows_of(p.b, p.n, p.k, p.b_s, p.workspace + c.a_bytes, c.ld);
+    const hipError_t e = c.a && c.b ? launch_pad_rows_pair(a, b, stream) : launch_pad_rows(c.a ? a : b, stream);
+    if (e != hipSuccess) return e;
+    if (c.a) p.a = p.workspace, p.a_s = c.ld;
+    if (c.b) p.b = p.workspace + c.a_bytes, p.b_s = c.ld;
+    p.k = (p.k + 15) / 16 * 16;
+  }
+  return p.out_dtype == MRL_BF16 ? launch<uint16_t>(p, stream) : launch<float>(p, stream);
+}
 
 }  // namespace mrl

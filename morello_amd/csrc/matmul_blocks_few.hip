@@ -74,8 +74,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs p) {
       Operand<OUT> x;
       x.from(fragment(slot + (NT + t) * 16 * BLOCK));
       const float scale = scales[t * 16 + li] * sb;
+      v4f part[NT];
+      products(part, w, x);
 #pragma unroll
-      for (int u = 0; u < NT; u++) acc[t][u] += w[u].by(x) * scale;
+      for (int u = 0; u < NT; u++) acc[t][u] += part[u] * scale;
     }
     sb = next;
     wait_for_lds();
