@@ -166,92 +166,126 @@ __global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p
   keep(p, w, blockIdx.x, c, choose(p, w, blockIdx.x, c));
 }
 
-// ---- Products with experts' weights: 16 rows from `row` on (this lane's: row + lane % 16), steps s0 .. s1 - 1 of 128 bytes a row ----
-template <bool F8>
-struct Weights {
-  static constexpr int STEP = F8 ? 128 : 64, SIZE = F8 ? 1 : 2;   // elements, bytes of one
-  const uint8_t *row;     // the lane's, from its first byte of step 0 on; nullptr: none
-  const float *scales;    // of the four rows whose sums the lane gets
-  // `height`: rows that there are from row0 on, up to sixteen.
-  __device__ inline void from(const Stack &s, uint32_t expert, uint32_t row0, uint32_t height) {
-    const uint32_t li = threadIdx.x & 15, lg = threadIdx.x >> 4 & 3;
-    row = li < height ? s.w + (int64_t(expert) * s.w_e + int64_t(row0 + li) * s.w_s) * SIZE + lg * 16 : nullptr;
-    if constexpr (F8) scales = s.scales + int64_t(expert) * s.scales_e + int64_t((row0 + (lg * 4 < height ? lg * 4 : 0)) / BLOCK) * s.scales_s;
+// ---- Products with experts' weights: 16 rows of each of N matrices against the x of a part's tokens, a step of 128 bytes of the rows at a time.  Loads take a row's 128 bytes with eight
+// lanes, x's with eight or sixteen, and LDS brings both into the order in which the matrix instructions want them: what bounds such loops else is the rate at which a compute
+// unit's address unit takes cache lines, of which a load of 16 bytes of sixteen rows next to each other has four times as many. ----
+// ROOM: tokens that a part may have, 8 or 16.
+template <bool F8, int ROOM>
+struct Shape {
+  static constexpr int STEP = F8 ? 128 : 64, SIZE = F8 ? 1 : 2;        // elements, bytes of one
+  static constexpr int X_BYTES = STEP * 2, X_CHUNKS = X_BYTES / 16;    // of a token's x
+  static constexpr int X_LOADS = ROOM * X_BYTES / 1024, X_TOKENS = 64 / X_CHUNKS;   // for all tokens; tokens of a load
+};
+constexpr int TILE_BYTES = 16 * 128;   // of LDS of a wave for each matrix
+template <bool F8, int ROOM, int N>
+struct Rows {
+  typedef Shape<F8, ROOM> S;
+  const uint8_t *row[N][2];       // of the lane: sixteen bytes of step 0 of row lane / 8, and of that row + 8 (of the last row, where there is none: its sums are not looked at)
+  const float *scale;             // of step 0: the first matrix's for the first half of the lanes, the last's for the others
+  const uint16_t *x[S::X_LOADS];  // of the lane: eight elements of step 0 of token lane / X_CHUNKS, and of those X_TOKENS behind (of the last, where there is none)
+  int x_loads;                    // that the part has tokens for
+  __device__ inline void matrix(int n, const Stack &s, uint32_t expert, uint32_t row0, uint32_t height) {   // height: rows that there are from row0 on, up to sixteen
+    const uint32_t lane = threadIdx.x & 63;
+    const uint8_t *const tile = s.w + (int64_t(expert) * s.w_e + int64_t(row0) * s.w_s) * S::SIZE + lane % 8 * 16;
+#pragma unroll
+    for (int i = 0; i < 2; i++) row[n][i] = tile + int64_t(min(lane / 8 + i * 8, height - 1)) * (s.w_s * S::SIZE);
+    if (F8 && (n == 0 || lane >= 32)) scale = s.scales + int64_t(expert) * s.scales_e + int64_t(row0 / BLOCK) * s.scales_s;
+  }
+  template <class F>
+  __device__ inline void tokens(uint32_t count, F first_of) {   // first_of(i): the i-th token's x
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < S::X_LOADS; i++) x[i] = first_of(min(lane / S::X_CHUNKS + i * S::X_TOKENS, count - 1)) + lane % S::X_CHUNKS * 8;
+    x_loads = int(count + S::X_TOKENS - 1) / S::X_TOKENS;
   }
 };
-// What a lane has of one step: 32 bytes of its row of each of N matrices, in two runs of 64 bytes over four lanes, and the x that they meet.
-// RAGGED: a row may end inside its last step.
-template <bool F8, int N, bool RAGGED>
+// What a lane has of one step.  RAGGED: a row may end inside its last step.
+template <bool F8, int ROOM, int N, bool RAGGED>
 struct Step {
-  static constexpr int Y = F8 ? 2 : 1, HALF = F8 ? 64 : 32;   // chunks of x to a chunk of weights; elements of a run
-  v4i q[N][2], y[2][Y];
-  float scale[N];
-  // x: the lane's token's, from its first element of step 0 on (nullptr: zeros); k: elements of a row.
-  __device__ inline void fetch(const Weights<F8> (&of)[N], const uint16_t *x, uint32_t s, int k) {
-    typedef Weights<F8> W;
-    const uint32_t at = s * 128;   // bytes of weights
+  typedef Shape<F8, ROOM> S;
+  v4i q[N][2], y[S::X_LOADS];
+  float scale;
+  int x_loads;
+  // k: elements of a row; half: eight rows are enough.
+  __device__ inline void fetch(const Rows<F8, ROOM, N> &of, uint32_t s, int k, bool half) {
+    const uint32_t at = s * 128, x_at = s * S::STEP;   // bytes of weights, elements of x
+    x_loads = of.x_loads;
+    if constexpr (F8) scale = of.scale[s];
+    if (!RAGGED || int(s + 1) * S::STEP <= k) {
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      if constexpr (F8) scale[n] = of[n].scales[s];
-      q[n][0] = q[n][1] = v4i{0, 0, 0, 0};
-    }
+      for (int n = 0; n < N; n++) q[n][0] = chunk_at(of.row[n][0] + at);
+      if (!half) {
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < Y; j++) y[i][j] = v4i{0, 0, 0, 0};
-    if (!RAGGED || int(s + 1) * W::STEP <= k) {
-      if (of[0].row) {
-#pragma unroll
-        for (int n = 0; n < N; n++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) q[n][i] = chunk_at(of[n].row + at + i * 64);
+        for (int n = 0; n < N; n++) q[n][1] = chunk_at(of.row[n][1] + at);
       }
-      if (x) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int j = 0; j < Y; j++) y[i][j] = chunk_at((const uint8_t *)(x + s * W::STEP + i * HALF + j * 8));
-      }
+      for (int i = 0; i < S::X_LOADS; i++)
+        if (i < x_loads) y[i] = chunk_at((const uint8_t *)(of.x[i] + x_at));
     } else {   // the rows end inside
-      const int first = int(s) * W::STEP + int(threadIdx.x >> 4 & 3) * (HALF / 4);   // the lane's first element
-      if (of[0].row) {
+      const int chunk = int(at) + int(threadIdx.x & 7) * 16, first = int(x_at) + int(threadIdx.x) % S::X_CHUNKS * 8;   // the lane's first byte of weights, element of x
 #pragma unroll
-        for (int n = 0; n < N; n++)
+      for (int n = 0; n < N; n++)
 #pragma unroll
-          for (int i = 0; i < 2; i++) q[n][i] = chunk_up_to(of[n].row + at + i * 64, (k - first - i * HALF) * W::SIZE, (first + i * HALF) * W::SIZE);
-      }
-      if (x) {
+        for (int i = 0; i < 2; i++) q[n][i] = chunk_up_to(of.row[n][i] + at, k * S::SIZE - chunk, chunk);
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int j = 0; j < Y; j++) y[i][j] = chunk_up_to((const uint8_t *)(x + s * W::STEP + i * HALF + j * 8), (k - first - i * HALF - j * 8) * 2, (first + i * HALF + j * 8) * 2);
-      }
+      for (int i = 0; i < S::X_LOADS; i++)
+        if (i < x_loads) y[i] = chunk_up_to((const uint8_t *)(of.x[i] + x_at), (k - first) * 2, first * 2);
     }
   }
-  __device__ inline void multiply(v4f (&acc)[N]) const {
+  // bounce: LDS of this wave's, N tiles and x of ROOM tokens.  Chunk c of a row of 128 bytes at c ^ (row / 2 % 8), of 256 bytes at c ^ row: sixteen lanes with a
+  // chunk of sixteen rows each reach every bank once.
+  __device__ inline void multiply(v4f (&acc)[N], uint8_t *bounce) const {
+    const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    uint8_t *const of_x = bounce + N * TILE_BYTES;
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      if constexpr (F8) {
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) *(v4i *)(bounce + n * TILE_BYTES + i * 1024 + lane / 8 * 128 + (lane % 8 ^ lane / 16 ^ i * 4) * 16) = q[n][i];
+#pragma unroll
+    for (int i = 0; i < S::X_LOADS; i++)
+      if (i < x_loads) {
+        const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS;
+        *(v4i *)(of_x + token * S::X_BYTES + (lane % S::X_CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[i];
+      }
+    const uint32_t mine = li & (ROOM - 1);
+    const uint8_t *const my_x = of_x + mine * S::X_BYTES;
+    const float scales[2] = {F8 ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))) : 0.0f, F8 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32)) : 0.0f};
+    if constexpr (F8) {
+      v4i u[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) u[i][j] = *(const v4i *)(my_x + ((i * 8 + lg * 2 + j) ^ mine) * 16);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
         v4f part = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          int u[4];
-          widen4(q[n][i / 2][i % 2 * 2], u[0], u[1]);
-          widen4(q[n][i / 2][i % 2 * 2 + 1], u[2], u[3]);
-          part = mma_bf16(v4i{u[0], u[1], u[2], u[3]}, y[i / 2][i % 2], part);
-        }
-        acc[n] += part * scale[n];
-      } else {
+        for (int i = 0; i < 2; i++) {
+          const v4i w = *(const v4i *)(bounce + n * TILE_BYTES + li * 128 + ((i * 4 + lg) ^ (li >> 1)) * 16);
 #pragma unroll
-        for (int i = 0; i < 2; i++) acc[n] = mma_bf16(q[n][i], y[i][0], acc[n]);
+          for (int j = 0; j < 2; j++) {
+            int b[4];
+            widen4(w[2 * j], b[0], b[1]);
+            widen4(w[2 * j + 1], b[2], b[3]);
+            part = mma_bf16(v4i{b[0], b[1], b[2], b[3]}, u[i][j], part);
+          }
+        }
+        acc[n] += part * scales[n];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const v4i u = *(const v4i *)(my_x + ((i * 4 + lg) ^ (mine >> 1)) * 16);
+#pragma unroll
+        for (int n = 0; n < N; n++) acc[n] = mma_bf16(*(const v4i *)(bounce + n * TILE_BYTES + li * 128 + ((i * 4 + lg) ^ (li >> 1)) * 16), u, acc[n]);
       }
     }
   }
 };
 
-// ---- A workgroup's choices by experts: expert after expert, in parts of up to sixteen ----
+// ---- A workgroup's choices by experts: expert after expert, in parts of up to `room` (8 or 16) ----
 struct Part { uint16_t expert, first, count, unused; };
-constexpr uint32_t most_parts(uint32_t experts, uint32_t choices) { return (choices < experts ? choices : experts) + choices / 16; }
+constexpr uint32_t most_parts(uint32_t experts, uint32_t choices, uint32_t room) { return (choices < experts ? choices : experts) + choices / room; }
 // What is in LDS, for up to `choices` choices of `experts` experts by tokens of `words` times 32.
 struct Lists {
   Part *parts;
@@ -259,18 +293,18 @@ struct Lists {
   uint32_t *wants;       // [experts][words] a bit for each token
   uint16_t *first_of;    // [experts]
   int32_t *totals;       // [2][waves]
-  __device__ inline Lists(uint8_t *at, uint32_t experts, uint32_t all, uint32_t words, uint32_t waves) {
-    parts = (Part *)at, at += most_parts(experts, all) * sizeof(Part);
+  __device__ inline Lists(uint8_t *at, uint32_t experts, uint32_t all, uint32_t words, uint32_t room, uint32_t waves) {
+    parts = (Part *)at, at += most_parts(experts, all, room) * sizeof(Part);
     wants = (uint32_t *)at, at += experts * words * 4;
     totals = (int32_t *)at, at += waves * 8;
     choices = (uint16_t *)at, at += all * 2;
     first_of = (uint16_t *)at;
   }
-  static size_t bytes(uint32_t experts, uint32_t all, uint32_t words, uint32_t waves) { return most_parts(experts, all) * sizeof(Part) + experts * words * 4 + waves * 8 + all * 2 + experts * 2; }
+  static size_t bytes(uint32_t experts, uint32_t all, uint32_t words, uint32_t room, uint32_t waves) { return most_parts(experts, all, room) * sizeof(Part) + experts * words * 4 + waves * 8 + all * 2 + experts * 2; }
 };
 // Returns the number of parts.  `all` choices, of which token i / top_k made the i-th; ends on a barrier.
 template <int THREADS>
-__device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int32_t *of_choice, uint32_t all, uint32_t words) {
+__device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int32_t *of_choice, uint32_t all, uint32_t words, uint32_t room) {
   constexpr int EACH = MOST_EXPERTS > THREADS ? MOST_EXPERTS / THREADS : 1;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (uint32_t i = tid; i < p.experts * words; i += THREADS) to.wants[i] = 0;
@@ -288,7 +322,7 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
     count[k] = 0;
     if (e < p.experts)
       for (uint32_t j = 0; j < words; j++) count[k] += __popc(to.wants[e * words + j]);
-    before += count[k], part += (count[k] + 15) / 16;
+    before += count[k], part += (count[k] + room - 1) / room;
   }
   const int32_t mine = before, my_parts = part;
   for (int d = 1; d < 64; d *= 2) {
@@ -310,7 +344,7 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
     const uint32_t e = tid * EACH + k;
     if (e < p.experts) {
       to.first_of[e] = uint16_t(before);
-      for (int32_t c = 0; c < count[k]; c += 16) to.parts[part++] = {uint16_t(e), uint16_t(before + c), uint16_t(min(16, count[k] - c)), 0};
+      for (int32_t c = 0; c < count[k]; c += room) to.parts[part++] = {uint16_t(e), uint16_t(before + c), uint16_t(min(int32_t(room), count[k] - c)), 0};
     }
     before += count[k];
   }
@@ -328,9 +362,9 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
 // ---- Gate and up.  All parts' tiles of 16 rows lie on a line, of which each workgroup has an equal run, and of a run's steps each wave; its loads run AHEAD
 // steps in front, from one tile into the next, and the waves meet behind UP_RUN tiles.  (A compute unit brings in some 23 GB/s, whatever is asked of it: all of them
 // have to have the same share.)  FUSED: from logits, the choices made here. ----
-constexpr int UP_WAVES = 4, UP_RUN = 8, UP_LOCAL = UP_RUN / UP_WAVES + 1;   // tiles that a wave has some steps of
+constexpr int UP_WAVES = 4, UP_RUN = 4, UP_LOCAL = UP_RUN / UP_WAVES + 1;   // tiles that a wave has some steps of
 constexpr uint32_t FUSED_TOKENS = 4;
-template <bool F8, bool FUSED, bool RAGGED>
+template <bool F8, int ROOM, bool FUSED, bool RAGGED>
 __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles) {
   constexpr int AHEAD = F8 ? 3 : 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
@@ -347,28 +381,29 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
       __syncthreads();
     }
   }
-  const Lists lists(dynamic, p.experts, p.tokens * p.top_k, words, UP_WAVES);
-  const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, FUSED ? chosen : w.chosen, all, words));
-  const uint32_t steps = (p.hidden + Weights<F8>::STEP - 1) / Weights<F8>::STEP;
+  const uint32_t bounce_bytes = 2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES;
+  uint8_t *const bounce = dynamic + wave * bounce_bytes;
+  const Lists lists(dynamic + UP_WAVES * bounce_bytes, p.experts, p.tokens * p.top_k, words, ROOM, UP_WAVES);
+  const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, FUSED ? chosen : w.chosen, all, words, ROOM));
+  const uint32_t steps = (p.hidden + Shape<F8, ROOM>::STEP - 1) / Shape<F8, ROOM>::STEP;
   const uint32_t line_end = uint32_t(uint64_t(line) * (blockIdx.x + 1) / gridDim.x);
   for (uint32_t tile0 = uint32_t(uint64_t(line) * blockIdx.x / gridDim.x); tile0 < line_end; tile0 += UP_RUN) {
     const uint32_t run = min(uint32_t(UP_RUN), line_end - tile0) * steps;
     const uint32_t begin = run * wave / UP_WAVES, n = run * (wave + 1) / UP_WAVES - begin;
     uint32_t fetch_tile = begin / steps, fetch_s = begin - fetch_tile * steps, s = fetch_s, local = 0;
-    Weights<F8> of[2];
-    const uint16_t *x = nullptr;
+    Rows<F8, ROOM, 2> of;
     bool fresh = true;
-    Step<F8, 2, RAGGED> t[AHEAD];
-    auto fetch = [&](Step<F8, 2, RAGGED> &to) {
+    Step<F8, ROOM, 2, RAGGED> t[AHEAD] = {};
+    auto fetch = [&](Step<F8, ROOM, 2, RAGGED> &to) {
       if (fresh) {
         const uint32_t part = by_tiles.div(tile0 + fetch_tile), row0 = (tile0 + fetch_tile - part * tiles) * 16, height = min(16u, p.inter - row0);
         const Part q = lists.parts[part];
         const uint32_t expert = __builtin_amdgcn_readfirstlane(q.expert);
-        of[0].from(p.gate, expert, row0, height), of[1].from(p.up, expert, row0, height);
-        x = li < q.count ? p.x + int64_t(lists.choices[q.first + li] / p.top_k) * p.x_s + lg * (F8 ? 16 : 8) : nullptr;
+        of.matrix(0, p.gate, expert, row0, height), of.matrix(1, p.up, expert, row0, height);
+        of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return p.x + int64_t(lists.choices[q.first + i] / p.top_k) * p.x_s; });
         fresh = false;
       }
-      to.fetch(of, x, fetch_s, int(p.hidden));
+      to.fetch(of, fetch_s, int(p.hidden), false);
       if (++fetch_s == steps) fetch_s = 0, fetch_tile++, fresh = true;
     };
     v4f acc[2] = {};
@@ -379,7 +414,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
 #pragma unroll
       for (int a = 0; a < AHEAD; a++) {
         if (at + a >= n) break;
-        t[a].multiply(acc);
+        t[a].multiply(acc, bounce);
         if (at + a + AHEAD < n) fetch(t[a]);
         if (++s == steps || at + a + 1 == n) {
           sums[wave][local][0][lane] = acc[0], sums[wave][local][1][lane] = acc[1];
@@ -407,37 +442,37 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
   }
 }
 
-// ---- Down: blockIdx.x: `height` rows, a multiple of four up to sixteen; blockIdx.y: DOWN_TOKENS tokens.  All parts' steps in a line, an equal share to each wave. ----
-constexpr int DOWN_TOKENS = 64;
-template <bool F8, bool RAGGED, int WAVES>
+// ---- Down: blockIdx.x: `height` rows, 4, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, an equal share to each wave. ----
+template <bool F8, int ROOM, bool RAGGED, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
   constexpr int AHEAD = F8 ? 3 : 4, THREADS = WAVES * 64;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
   float *const shares = (float *)(sums + WAVES * tokens_here * 4);   // [tokens_here * top_k]
-  const Lists lists((uint8_t *)(shares + (tokens_here * p.top_k + 1) / 2 * 2), p.experts, tokens_here * p.top_k, words, WAVES);
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t row0 = blockIdx.x * height, t0 = blockIdx.y * DOWN_TOKENS, rows = live_rows(p), rows_here = min(height, p.hidden - row0);
+  const uint32_t bounce_bytes = TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES;
+  uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * bounce_bytes;
+  const Lists lists(bounces + WAVES * bounce_bytes, p.experts, tokens_here * p.top_k, words, ROOM, WAVES);
+  const uint32_t row0 = blockIdx.x * height, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(height, p.hidden - row0);
   if (t0 >= rows) return;
   const uint32_t here = min(tokens_here, rows - t0);
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
   for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
-  const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words));
-  const uint32_t steps = (p.inter + Weights<F8>::STEP - 1) / Weights<F8>::STEP, line = parts * steps;
+  const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, ROOM));
+  const uint32_t steps = (p.inter + Shape<F8, ROOM>::STEP - 1) / Shape<F8, ROOM>::STEP, line = parts * steps;
   const uint32_t begin = uint32_t(uint64_t(line) * wave / WAVES), n = uint32_t(uint64_t(line) * (wave + 1) / WAVES) - begin;
   uint32_t fetch_part = begin / steps, fetch_s = begin - fetch_part * steps, at_part = fetch_part, s = fetch_s;
-  Weights<F8> of[1];
-  const uint16_t *x = nullptr;
+  Rows<F8, ROOM, 1> of;
   bool fresh = true;
-  Step<F8, 1, RAGGED> t[AHEAD];
-  auto fetch = [&](Step<F8, 1, RAGGED> &to) {
+  Step<F8, ROOM, 1, RAGGED> t[AHEAD] = {};
+  auto fetch = [&](Step<F8, ROOM, 1, RAGGED> &to) {
     if (fresh) {
       const Part q = lists.parts[fetch_part];
-      of[0].from(p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
-      x = li < q.count ? w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + li]) * w.h_s + lg * (F8 ? 16 : 8) : nullptr;
+      of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
+      of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + i]) * w.h_s; });
       fresh = false;
     }
-    to.fetch(of, x, fetch_s, int(p.inter));
+    to.fetch(of, fetch_s, int(p.inter), height <= 8);
     if (++fetch_s == steps) fetch_s = 0, fetch_part++, fresh = true;
   };
   v4f acc[1] = {};
@@ -448,7 +483,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
 #pragma unroll
     for (int a = 0; a < AHEAD; a++) {
       if (at + a >= n) break;
-      t[a].multiply(acc);
+      t[a].multiply(acc, bounce);
       if (at + a + AHEAD < n) fetch(t[a]);
       if (++s == steps || at + a + 1 == n) {
         const Part q = lists.parts[at_part];
@@ -471,43 +506,59 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   }
 }
 
-template <bool F8, bool FUSED, bool RAGGED>
+template <bool F8, int ROOM, bool FUSED, bool RAGGED>
 hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   // Three workgroups to a compute unit, what their registers allow, or one to a tile.
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
-  const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices)) * tiles, 3 * g_compute_units));
-  const size_t lds = Lists::bytes(a.experts, choices, words, UP_WAVES);
+  const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 3 * g_compute_units));
+  const size_t lds = UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
-  if (lds > 32 * 1024 && !plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, FUSED, RAGGED>), 64 * 1024);
+  if (!plan::recording()) {
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, RAGGED>), 96 * 1024);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_up<F8, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles));
+  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles));
   return plan::last_error();
 }
-template <bool F8, bool RAGGED, int WAVES>
-hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, hipStream_t stream) {
-  const uint32_t here = std::min(a.tokens, uint32_t(DOWN_TOKENS)), words = (here + 31) / 32;
-  const size_t lds = size_t(WAVES) * here * 64 + size_t(here * a.top_k + 1) / 2 * 8 + Lists::bytes(a.experts, here * a.top_k, words, WAVES);
+template <bool F8, int ROOM, bool RAGGED, int WAVES>
+hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, uint32_t here, hipStream_t stream) {
+  const uint32_t words = (here + 31) / 32;
+  const size_t lds = size_t(WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + WAVES * (TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, here * a.top_k, words, ROOM, WAVES);
   static std::atomic<uint64_t> raised{0};
-  if (lds > 48 * 1024 && !plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, RAGGED, WAVES>), 96 * 1024);
+  if (!plan::recording()) {
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, RAGGED, WAVES>), 160 * 1024);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_down<F8, RAGGED, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + DOWN_TOKENS - 1) / DOWN_TOKENS), dim3(WAVES * 64), lds, stream, a, w, height, here, words);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, RAGGED, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + here - 1) / here), dim3(WAVES * 64), lds, stream, a, w, height, here, words);
   return plan::last_error();
 }
-template <bool F8, bool RAGGED>
+template <bool F8, int ROOM, bool RAGGED>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  // Rows for all compute units alike: a workgroup of sixteen waves to each where sixteen rows are enough, else several of eight.
-  const uint32_t each = (a.hidden + 16 * g_compute_units - 1) / (16 * g_compute_units), groups = each * g_compute_units;
-  const uint32_t height = std::min(16u, ((a.hidden + groups - 1) / groups + 3) / 4 * 4);
-  return each == 1 ? launch_down_waves<F8, RAGGED, 16>(a, w, height, stream) : launch_down_waves<F8, RAGGED, 8>(a, w, height, stream);
+  // Rows for all compute units alike: a workgroup of sixteen waves to each where sixteen rows are enough and its sums of all tokens fit LDS, else several of eight.
+  const uint32_t each = (a.hidden + 16 * g_compute_units - 1) / (16 * g_compute_units), rows = (a.hidden + each * g_compute_units - 1) / (each * g_compute_units);
+  const uint32_t height = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  return each == 1 && a.tokens <= 32 ? launch_down_waves<F8, ROOM, RAGGED, 16>(a, w, height, a.tokens, stream)
+                                     : launch_down_waves<F8, ROOM, RAGGED, 8>(a, w, height, std::min(a.tokens, 96u), stream);
+}
+template <bool F8, int ROOM>
+hipError_t launch_products(const ExpertsArgs &a, const Places &w, bool fused, hipStream_t stream) {
+  constexpr uint32_t STEP = Shape<F8, ROOM>::STEP;
+  const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * std::min(a.experts, a.tokens * a.top_k);
+  const bool ragged = a.hidden % STEP != 0;
+  plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
+  hipError_t e;
+  if constexpr (ROOM == 8) {
+    if (fused) e = ragged ? launch_up<F8, ROOM, true, true>(a, w, stream) : launch_up<F8, ROOM, true, false>(a, w, stream);
+    else e = ragged ? launch_up<F8, ROOM, false, true>(a, w, stream) : launch_up<F8, ROOM, false, false>(a, w, stream);
+  } else {
+    e = ragged ? launch_up<F8, ROOM, false, true>(a, w, stream) : launch_up<F8, ROOM, false, false>(a, w, stream);
+  }
+  if (e != hipSuccess) return e;
+  plan::work(plan::UNIT_STREAM, 0, weight / 3);
+  return a.inter % STEP ? launch_down<F8, ROOM, true>(a, w, stream) : launch_down<F8, ROOM, false>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  const uint32_t slots = std::min(a.experts, a.tokens * a.top_k);
-  const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * slots;
   plan::work(plan::UNIT_STREAM, 0, 2.0 * (double(a.experts) + a.tokens) * a.hidden);
   MRL_LAUNCH(k_experts_logits, dim3(a.experts, (a.tokens + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(ROUTER_THREADS), 0, stream, a, w);
   const bool fused = a.tokens <= FUSED_TOKENS && a.tokens * a.experts * a.experts <= 1u << 16;
@@ -515,13 +566,8 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), 0, stream, a, w);
   }
-  const bool ragged_up = a.hidden % Weights<F8>::STEP != 0, ragged_down = a.inter % Weights<F8>::STEP != 0;
-  plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
-  const hipError_t e = fused ? ragged_up ? launch_up<F8, true, true>(a, w, stream) : launch_up<F8, true, false>(a, w, stream)
-                             : ragged_up ? launch_up<F8, false, true>(a, w, stream) : launch_up<F8, false, false>(a, w, stream);
-  if (e != hipSuccess) return e;
-  plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  return ragged_down ? launch_down<F8, true>(a, w, stream) : launch_down<F8, false>(a, w, stream);
+  // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.
+  return a.tokens > 8 && a.tokens * a.top_k > 6 * a.experts ? launch_products<F8, 16>(a, w, fused, stream) : launch_products<F8, 8>(a, w, fused, stream);
 }
 
 }  // namespace
