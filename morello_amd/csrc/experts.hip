@@ -359,16 +359,17 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
   return parts;
 }
 
-// ---- Gate and up.  All parts' tiles of 16 rows lie on a line, of which each workgroup has an equal run, and of a run's steps each wave; its loads run AHEAD
-// steps in front, from one tile into the next, and the waves meet behind UP_RUN tiles.  (A compute unit brings in some 23 GB/s, whatever is asked of it: all of them
-// have to have the same share.)  FUSED: from logits, the choices made here. ----
-constexpr int UP_WAVES = 4, UP_RUN = 4, UP_LOCAL = UP_RUN / UP_WAVES + 1;   // tiles that a wave has some steps of
+// ---- Gate and up.  All parts' tiles of 16 rows lie on a line, of which workgroup b has the tiles b, b + gridDim.x, ..: what is under way at a time lies close together (equal runs of the line for each
+// took 10 % longer over 1.9 GB).  The waves share a tile's steps; their loads run AHEAD steps in front, from one tile into the next, and the
+// waves' sums meet behind each.  FUSED: from logits, the choices made here. ----
+constexpr int UP_WAVES = 4;
 constexpr uint32_t FUSED_TOKENS = 4;
 template <bool F8, int ROOM, bool FUSED, bool RAGGED>
 __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles) {
-  constexpr int AHEAD = F8 ? 3 : 4;
+  constexpr int AHEAD = F8 ? ROOM == 16 ? 2 : 3 : 4;
+  typedef Shape<F8, ROOM> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
-  __shared__ v4f sums[UP_WAVES][UP_LOCAL][2][64];
+  __shared__ v4f sums[2][UP_WAVES][2][64];
   __shared__ int32_t chosen[FUSED ? FUSED_TOKENS * MOST_CHOSEN : 1];
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t rows = live_rows(p), all = rows * p.top_k;
@@ -381,118 +382,114 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
       __syncthreads();
     }
   }
-  const uint32_t bounce_bytes = 2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES;
-  uint8_t *const bounce = dynamic + wave * bounce_bytes;
-  const Lists lists(dynamic + UP_WAVES * bounce_bytes, p.experts, p.tokens * p.top_k, words, ROOM, UP_WAVES);
+  constexpr uint32_t BOUNCE = 2 * TILE_BYTES + ROOM * S::X_BYTES;
+  uint8_t *const bounce = dynamic + wave * BOUNCE;
+  const Lists lists(dynamic + UP_WAVES * BOUNCE, p.experts, p.tokens * p.top_k, words, ROOM, UP_WAVES);
   const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, FUSED ? chosen : w.chosen, all, words, ROOM));
-  const uint32_t steps = (p.hidden + Shape<F8, ROOM>::STEP - 1) / Shape<F8, ROOM>::STEP;
-  const uint32_t line_end = uint32_t(uint64_t(line) * (blockIdx.x + 1) / gridDim.x);
-  for (uint32_t tile0 = uint32_t(uint64_t(line) * blockIdx.x / gridDim.x); tile0 < line_end; tile0 += UP_RUN) {
-    const uint32_t run = min(uint32_t(UP_RUN), line_end - tile0) * steps;
-    const uint32_t begin = run * wave / UP_WAVES, n = run * (wave + 1) / UP_WAVES - begin;
-    uint32_t fetch_tile = begin / steps, fetch_s = begin - fetch_tile * steps, s = fetch_s, local = 0;
-    Rows<F8, ROOM, 2> of;
-    bool fresh = true;
-    Step<F8, ROOM, 2, RAGGED> t[AHEAD] = {};
-    auto fetch = [&](Step<F8, ROOM, 2, RAGGED> &to) {
-      if (fresh) {
-        const uint32_t part = by_tiles.div(tile0 + fetch_tile), row0 = (tile0 + fetch_tile - part * tiles) * 16, height = min(16u, p.inter - row0);
-        const Part q = lists.parts[part];
-        const uint32_t expert = __builtin_amdgcn_readfirstlane(q.expert);
-        of.matrix(0, p.gate, expert, row0, height), of.matrix(1, p.up, expert, row0, height);
-        of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return p.x + int64_t(lists.choices[q.first + i] / p.top_k) * p.x_s; });
-        fresh = false;
-      }
-      to.fetch(of, fetch_s, int(p.hidden), false);
-      if (++fetch_s == steps) fetch_s = 0, fetch_tile++, fresh = true;
-    };
-    v4f acc[2] = {};
+  const uint32_t steps = (p.hidden + S::STEP - 1) / S::STEP, s0 = steps * wave / UP_WAVES, n = steps * (wave + 1) / UP_WAVES - s0;   // this wave's steps of each tile
+  Rows<F8, ROOM, 2> of;
+  Step<F8, ROOM, 2, RAGGED> t[AHEAD] = {};
+  auto go_to = [&](uint32_t tile) {
+    const uint32_t part = by_tiles.div(tile), row0 = (tile - part * tiles) * 16, height = min(16u, p.inter - row0);
+    const Part q = lists.parts[part];
+    const uint32_t expert = __builtin_amdgcn_readfirstlane(q.expert);
+    of.matrix(0, p.gate, expert, row0, height), of.matrix(1, p.up, expert, row0, height);
+    of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return p.x + int64_t(lists.choices[q.first + i] / p.top_k) * p.x_s; });
+  };
+  if (blockIdx.x < line) {
+    go_to(blockIdx.x);
 #pragma unroll
     for (int a = 0; a < AHEAD; a++)
-      if (uint32_t(a) < n) fetch(t[a]);
+      if (uint32_t(a) < n) t[a].fetch(of, s0 + a, int(p.hidden), false);
+  }
+  uint32_t turn = 0;
+  for (uint32_t tile = blockIdx.x; tile < line; tile += gridDim.x, turn ^= 1) {
+    v4f acc[2] = {};
     for (uint32_t at = 0; at < n; at += AHEAD) {
+      const bool last = at + AHEAD >= n, more = tile + gridDim.x < line;
+      if (last && more) go_to(tile + gridDim.x);
 #pragma unroll
       for (int a = 0; a < AHEAD; a++) {
-        if (at + a >= n) break;
-        t[a].multiply(acc, bounce);
-        if (at + a + AHEAD < n) fetch(t[a]);
-        if (++s == steps || at + a + 1 == n) {
-          sums[wave][local][0][lane] = acc[0], sums[wave][local][1][lane] = acc[1];
-          acc[0] = acc[1] = v4f{0, 0, 0, 0};
-          s = 0, local++;
-        }
+        if (at + a < n) t[a].multiply(acc, bounce);
+        const uint32_t next = last ? uint32_t(a) : at + a + AHEAD;
+        if (next < n && (!last || more)) t[a].fetch(of, s0 + next, int(p.hidden), false);
       }
     }
-    __syncthreads();
-    for (uint32_t tile = wave; tile * steps < run; tile += UP_WAVES) {
-      v4f g = {0, 0, 0, 0}, u = g, h;
+    v4f(&here)[UP_WAVES][2][64] = sums[turn];
+    here[wave][0][lane] = acc[0], here[wave][1][lane] = acc[1];
+    __syncthreads();   // (the tile before the last has been read: its readers are here)
+    if (wave == tile / gridDim.x % UP_WAVES) {
+      v4f g = here[0][0][lane], u = here[0][1][lane], h;
 #pragma unroll
-      for (uint32_t v = 0; v < UP_WAVES; v++) {   // those that have some of the tile's steps
-        const uint32_t from = run * v / UP_WAVES, to = run * (v + 1) / UP_WAVES;
-        if (from >= (tile + 1) * steps || to <= tile * steps || from == to) continue;
-        g += sums[v][tile - from / steps][0][lane], u += sums[v][tile - from / steps][1][lane];
-      }
+      for (uint32_t v = 1; v < UP_WAVES; v++) g += here[v][0][lane], u += here[v][1][lane];
 #pragma unroll
       for (int i = 0; i < 4; i++) h[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
-      const uint32_t part = by_tiles.div(tile0 + tile), row = (tile0 + tile - part * tiles) * 16 + lg * 4;
+      const uint32_t part = by_tiles.div(tile), row = (tile - part * tiles) * 16 + lg * 4;
       const Part q = lists.parts[part];
       if (li < q.count && row < p.inter) store4(w.h + uint64_t(lists.choices[q.first + li]) * w.h_s + row, h, int(p.inter - row));
     }
-    if (tile0 + UP_RUN < line_end) __syncthreads();
   }
 }
 
-// ---- Down: blockIdx.x: `height` rows, 4, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, an equal share to each wave. ----
+// ---- Down: blockIdx.x: `height` rows, 4, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to eight steps of a part, of which a wave has every
+// WAVES-th: a workgroup's waves go through the same rows together. ----
 template <bool F8, int ROOM, bool RAGGED, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
-  constexpr int AHEAD = F8 ? 3 : 4, THREADS = WAVES * 64;
+  constexpr int AHEAD = F8 ? ROOM == 16 ? 2 : 3 : 4, THREADS = WAVES * 64;
+  typedef Shape<F8, ROOM> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
   float *const shares = (float *)(sums + WAVES * tokens_here * 4);   // [tokens_here * top_k]
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t bounce_bytes = TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES;
-  uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * bounce_bytes;
-  const Lists lists(bounces + WAVES * bounce_bytes, p.experts, tokens_here * p.top_k, words, ROOM, WAVES);
+  constexpr uint32_t BOUNCE = TILE_BYTES + ROOM * S::X_BYTES;
+  uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * BOUNCE;
+  const Lists lists(bounces + WAVES * BOUNCE, p.experts, tokens_here * p.top_k, words, ROOM, WAVES);
   const uint32_t row0 = blockIdx.x * height, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(height, p.hidden - row0);
   if (t0 >= rows) return;
   const uint32_t here = min(tokens_here, rows - t0);
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
   for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
   const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, ROOM));
-  const uint32_t steps = (p.inter + Shape<F8, ROOM>::STEP - 1) / Shape<F8, ROOM>::STEP, line = parts * steps;
-  const uint32_t begin = uint32_t(uint64_t(line) * wave / WAVES), n = uint32_t(uint64_t(line) * (wave + 1) / WAVES) - begin;
-  uint32_t fetch_part = begin / steps, fetch_s = begin - fetch_part * steps, at_part = fetch_part, s = fetch_s;
+  // At least four pieces for each wave, where there are steps for them.
+  const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP, want = max((steps + 7) / 8, min(steps, (4 * WAVES + parts - 1) / parts));
+  const uint32_t size = (steps + want - 1) / want, of_part = (steps + size - 1) / size, pieces = parts * of_part;
+  // The piece to fetch from, and the one to multiply.
+  uint32_t fetch_piece = wave, fetch_s = 0, fetch_end = 0, piece = wave, s = 0, end = 0;
   Rows<F8, ROOM, 1> of;
-  bool fresh = true;
   Step<F8, ROOM, 1, RAGGED> t[AHEAD] = {};
   auto fetch = [&](Step<F8, ROOM, 1, RAGGED> &to) {
-    if (fresh) {
-      const Part q = lists.parts[fetch_part];
+    if (fetch_s == fetch_end) {
+      const uint32_t part = fetch_piece / of_part;
+      const Part q = lists.parts[part];
+      fetch_s = (fetch_piece - part * of_part) * size, fetch_end = min(steps, fetch_s + size);
       of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
       of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + i]) * w.h_s; });
-      fresh = false;
     }
     to.fetch(of, fetch_s, int(p.inter), height <= 8);
-    if (++fetch_s == steps) fetch_s = 0, fetch_part++, fresh = true;
+    if (++fetch_s == fetch_end) fetch_piece += WAVES;
   };
   v4f acc[1] = {};
 #pragma unroll
   for (int a = 0; a < AHEAD; a++)
-    if (uint32_t(a) < n) fetch(t[a]);
-  for (uint32_t at = 0; at < n; at += AHEAD) {
+    if (fetch_piece < pieces) fetch(t[a]);
+  while (piece < pieces) {
 #pragma unroll
     for (int a = 0; a < AHEAD; a++) {
-      if (at + a >= n) break;
+      if (piece >= pieces) break;
+      if (s == end) {
+        const uint32_t part = piece / of_part;
+        s = (piece - part * of_part) * size, end = min(steps, s + size);
+      }
       t[a].multiply(acc, bounce);
-      if (at + a + AHEAD < n) fetch(t[a]);
-      if (++s == steps || at + a + 1 == n) {
-        const Part q = lists.parts[at_part];
+      if (fetch_piece < pieces) fetch(t[a]);
+      if (++s == end) {
+        const Part q = lists.parts[piece / of_part];
         if (li < q.count) {
           const uint32_t choice = lists.choices[q.first + li];
           sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
         }
         acc[0] = v4f{0, 0, 0, 0};
-        s = 0, at_part++;
+        piece += WAVES;
       }
     }
   }
