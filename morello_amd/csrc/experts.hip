@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "blocks_device.h"
+#include "paged.h"
 
 namespace mrl {
 namespace {
@@ -45,35 +46,47 @@ __device__ inline uint32_t live_rows(const ExpertsArgs &p) { return p.rows ? uin
 __device__ inline float lo_f32(int x) { return __uint_as_float(uint32_t(x) << 16); }
 __device__ inline float hi_f32(int x) { return __uint_as_float(uint32_t(x) & 0xffff0000u); }
 
-// ---- Logits: a workgroup to an expert and ROUTER_TOKENS tokens, in 64 bits (a product of two bf16 numbers is exact in 32), so that which experts are chosen
+// ---- Logits: a workgroup to an expert and TOKENS tokens, in 64 bits (a product of two bf16 numbers is exact in 32), so that which experts are chosen
 // does not hang on the order of a sum. ----
-constexpr int ROUTER_TOKENS = 4, ROUTER_THREADS = 256;
+constexpr int ROUTER_THREADS = 256;
+template <int TOKENS>
 __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p, Places w) {
-  __shared__ double part[ROUTER_THREADS / 64][ROUTER_TOKENS];
-  const uint32_t lane = threadIdx.x & 63, expert = blockIdx.x, t0 = blockIdx.y * ROUTER_TOKENS, rows = live_rows(p);
+  __shared__ double part[ROUTER_THREADS / 64][TOKENS];
+  const uint32_t lane = threadIdx.x & 63, expert = blockIdx.x, t0 = blockIdx.y * TOKENS, rows = live_rows(p);
   if (t0 >= rows) return;
-  const uint8_t *from = (const uint8_t *)(p.router + int64_t(expert) * p.router_s);
-  const int count = int(min(uint32_t(ROUTER_TOKENS), rows - t0));
-  double sum[ROUTER_TOKENS] = {};
-  for (uint32_t k = threadIdx.x * 8; k < p.hidden; k += ROUTER_THREADS * 8) {
+  const uint8_t *const from = (const uint8_t *)(p.router + int64_t(expert) * p.router_s), *x[TOKENS];
+#pragma unroll
+  for (int t = 0; t < TOKENS; t++) x[t] = (const uint8_t *)(p.x + int64_t(min(t0 + t, rows - 1)) * p.x_s);   // (the last again, behind it)
+  double sum[TOKENS] = {};
+  auto add = [&](v4i r, const v4i (&y)[TOKENS]) {
+#pragma unroll
+    for (int t = 0; t < TOKENS; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[t] += double(lo_f32(r[i]) * lo_f32(y[t][i])), sum[t] += double(hi_f32(r[i]) * hi_f32(y[t][i]));
+  };
+  uint32_t k = threadIdx.x * 8;
+  for (; k + 8 <= p.hidden; k += ROUTER_THREADS * 8) {
+    v4i y[TOKENS];
+    const v4i r = chunk_at(from + k * 2);
+#pragma unroll
+    for (int t = 0; t < TOKENS; t++) y[t] = chunk_at(x[t] + k * 2);
+    add(r, y);
+  }
+  if (k < p.hidden) {
+    v4i y[TOKENS];
     const int bytes = int(p.hidden - k) * 2;
-    const v4i r = chunk_up_to(from + int64_t(k) * 2, bytes, int(k) * 2);
+    const v4i r = chunk_up_to(from + k * 2, bytes, int(k) * 2);
 #pragma unroll
-    for (int t = 0; t < ROUTER_TOKENS; t++) {
-      if (t >= count) break;
-      const v4i x = chunk_up_to((const uint8_t *)(p.x + int64_t(t0 + t) * p.x_s + k), bytes, int(k) * 2);
-#pragma unroll
-      for (int i = 0; i < 4; i++) sum[t] += double(lo_f32(r[i]) * lo_f32(x[i])), sum[t] += double(hi_f32(r[i]) * hi_f32(x[i]));
-    }
+    for (int t = 0; t < TOKENS; t++) y[t] = chunk_up_to(x[t] + k * 2, bytes, int(k) * 2);
+    add(r, y);
   }
 #pragma unroll
-  for (int t = 0; t < ROUTER_TOKENS; t++) {
-    if (t >= count) break;
+  for (int t = 0; t < TOKENS; t++) {
     for (int d = 32; d; d /= 2) sum[t] += __shfl_xor(sum[t], d);
     if (lane == 0) part[threadIdx.x / 64][t] = sum[t];
   }
   __syncthreads();
-  if (int(threadIdx.x) < count) {
+  if (threadIdx.x < TOKENS && t0 + threadIdx.x < rows) {
     double all = 0;
 #pragma unroll
     for (int v = 0; v < ROUTER_THREADS / 64; v++) all += part[v][threadIdx.x];
@@ -307,6 +320,11 @@ template <int THREADS>
 __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int32_t *of_choice, uint32_t all, uint32_t words, uint32_t room) {
   constexpr int EACH = MOST_EXPERTS > THREADS ? MOST_EXPERTS / THREADS : 1;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (all <= p.top_k) {   // one token: its experts differ
+    if (tid < all) to.parts[tid] = {uint16_t(of_choice[tid]), uint16_t(tid), 1, 0}, to.choices[tid] = uint16_t(tid);
+    __syncthreads();
+    return all;
+  }
   for (uint32_t i = tid; i < p.experts * words; i += THREADS) to.wants[i] = 0;
   __syncthreads();
   for (uint32_t i = tid; i < all; i += THREADS) {
@@ -314,39 +332,35 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
     atomicOr(&to.wants[uint32_t(of_choice[i]) * words + t / 32], 1u << (t % 32));
   }
   __syncthreads();
-  // Choices, and parts, before each expert (a thread has EACH neighbours).
-  int32_t count[EACH], before = 0, part = 0;
+  // Choices (below 2^14), and parts of them, before each expert, in one number (a thread has EACH neighbours).
+  uint32_t count[EACH], mine = 0;
 #pragma unroll
   for (int k = 0; k < EACH; k++) {
     const uint32_t e = tid * EACH + k;
     count[k] = 0;
     if (e < p.experts)
       for (uint32_t j = 0; j < words; j++) count[k] += __popc(to.wants[e * words + j]);
-    before += count[k], part += (count[k] + room - 1) / room;
+    mine += count[k] << 16 | (count[k] + room - 1) / room;
   }
-  const int32_t mine = before, my_parts = part;
-  for (int d = 1; d < 64; d *= 2) {
-    const int32_t x = __shfl_up(before, d), y = __shfl_up(part, d);
-    if (int(lane) >= d) before += x, part += y;
-  }
-  if (lane == 63) to.totals[wave * 2] = before, to.totals[wave * 2 + 1] = part;
+  uint32_t before = paged::over_lanes_up_to(mine, [](uint32_t x, auto ctrl, auto rows) { return x + uint32_t(paged::moved<ctrl(), rows()>(int32_t(x), 0)); });
+  if (lane == 63) to.totals[wave] = int32_t(before);
   __syncthreads();
+  before -= mine;
   uint32_t parts = 0;
 #pragma unroll
   for (uint32_t v = 0; v < THREADS / 64; v++) {
-    const int32_t x = to.totals[v * 2], y = to.totals[v * 2 + 1];
-    if (v < wave) before += x, part += y;
-    parts += y;
+    const uint32_t x = uint32_t(to.totals[v]);
+    if (v < wave) before += x;
+    parts += x & 0xffff;
   }
-  before -= mine, part -= my_parts;
 #pragma unroll
   for (int k = 0; k < EACH; k++) {
     const uint32_t e = tid * EACH + k;
     if (e < p.experts) {
-      to.first_of[e] = uint16_t(before);
-      for (int32_t c = 0; c < count[k]; c += room) to.parts[part++] = {uint16_t(e), uint16_t(before + c), uint16_t(min(int32_t(room), count[k] - c)), 0};
+      to.first_of[e] = uint16_t(before >> 16);
+      for (uint32_t c = 0; c < count[k]; c += room) to.parts[before++ & 0xffff] = {uint16_t(e), uint16_t(to.first_of[e] + c), uint16_t(min(room, count[k] - c)), 0};
     }
-    before += count[k];
+    before += count[k] << 16;
   }
   __syncthreads();
   for (uint32_t i = tid; i < all; i += THREADS) {
@@ -450,9 +464,13 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
   for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
   const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, ROOM));
-  // At least four pieces for each wave, where there are steps for them.
-  const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP, want = max((steps + 7) / 8, min(steps, (4 * WAVES + parts - 1) / parts));
-  const uint32_t size = (steps + want - 1) / want, of_part = (steps + size - 1) / size, pieces = parts * of_part;
+  // Pieces of eight steps, or fewer where a seventh of the waves' last turn would be idle.
+  const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP;
+  uint32_t size = 8, of_part, pieces;
+  for (;; size /= 2) {
+    of_part = (steps + size - 1) / size, pieces = parts * of_part;
+    if (size == 1 || pieces * 7 >= (pieces + WAVES - 1) / WAVES * WAVES * 6) break;
+  }
   // The piece to fetch from, and the one to multiply.
   uint32_t fetch_piece = wave, fetch_s = 0, fetch_end = 0, piece = wave, s = 0, end = 0;
   Rows<F8, ROOM, 1> of;
@@ -557,7 +575,9 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, bool fused, hi
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   plan::work(plan::UNIT_STREAM, 0, 2.0 * (double(a.experts) + a.tokens) * a.hidden);
-  MRL_LAUNCH(k_experts_logits, dim3(a.experts, (a.tokens + ROUTER_TOKENS - 1) / ROUTER_TOKENS), dim3(ROUTER_THREADS), 0, stream, a, w);
+  // (a token to a workgroup while these still run side by side)
+  if (a.experts * a.tokens <= 8 * g_compute_units) MRL_LAUNCH(k_experts_logits<1>, dim3(a.experts, a.tokens), dim3(ROUTER_THREADS), 0, stream, a, w);
+  else MRL_LAUNCH(k_experts_logits<4>, dim3(a.experts, (a.tokens + 3) / 4), dim3(ROUTER_THREADS), 0, stream, a, w);
   const bool fused = a.tokens <= FUSED_TOKENS && a.tokens * a.experts * a.experts <= 1u << 16;
   if (!fused) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
