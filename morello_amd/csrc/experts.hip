@@ -43,6 +43,18 @@ size_t places(const ExpertsArgs &a, Places *to) {
 
 __device__ inline uint32_t live_rows(const ExpertsArgs &p) { return p.rows ? uint32_t(min(max(*p.rows, 0), int32_t(p.tokens))) : p.tokens; }
 
+// Over the lanes of a wave, in the last one (the same order whatever the kernel).
+__device__ inline double sum_over_wave(double x) {
+  return paged::over_lanes_up_to(x, [](double y, auto ctrl, auto rows) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, y);
+    const uint32_t lo = uint32_t(paged::moved<ctrl(), rows()>(int32_t(uint32_t(bits)), 0)), hi = uint32_t(paged::moved<ctrl(), rows()>(int32_t(uint32_t(bits >> 32)), 0));
+    return y + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+  });
+}
+__device__ inline float sum_over_wave(float x) {
+  return paged::over_lanes_up_to(x, [](float y, auto ctrl, auto rows) { return y + __int_as_float(paged::moved<ctrl(), rows()>(__float_as_int(y), 0)); });
+}
+
 __device__ inline float lo_f32(int x) { return __uint_as_float(uint32_t(x) << 16); }
 __device__ inline float hi_f32(int x) { return __uint_as_float(uint32_t(x) & 0xffff0000u); }
 
@@ -82,8 +94,8 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   }
 #pragma unroll
   for (int t = 0; t < TOKENS; t++) {
-    for (int d = 32; d; d /= 2) sum[t] += __shfl_xor(sum[t], d);
-    if (lane == 0) part[threadIdx.x / 64][t] = sum[t];
+    const double all = sum_over_wave(sum[t]);
+    if (lane == 63) part[threadIdx.x / 64][t] = all;
   }
   __syncthreads();
   if (threadIdx.x < TOKENS && t0 + threadIdx.x < rows) {
@@ -152,8 +164,8 @@ __device__ inline float choose(const ExpertsArgs &p, const Places &w, uint32_t t
     sum += x;
     if (before < p.top_k) c.expert[before] = int32_t(e), c.e[before] = x;
   }
-  for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-  if (tid % 64 == 0) c.sums[tid / 64] = sum;
+  sum = sum_over_wave(sum);
+  if (tid % 64 == 63) c.sums[tid / 64] = sum;
   __syncthreads();
   sum = 0.0f;
   if (p.renormalise) {
@@ -194,7 +206,7 @@ template <bool F8, int ROOM, int N>
 struct Rows {
   typedef Shape<F8, ROOM> S;
   const uint8_t *row[N][2];       // of the lane: sixteen bytes of step 0 of row lane / 8, and of that row + 8 (of the last row, where there is none: its sums are not looked at)
-  const float *scale;             // of step 0: the first matrix's for the first half of the lanes, the last's for the others
+  const float *scale;             // of step 0: the first matrix's for the first half of the lanes, the last's for the others (a tile's rows are of one block of 128)
   const uint16_t *x[S::X_LOADS];  // of the lane: eight elements of step 0 of token lane / X_CHUNKS, and of those X_TOKENS behind (of the last, where there is none)
   int x_loads;                    // that the part has tokens for
   __device__ inline void matrix(int n, const Stack &s, uint32_t expert, uint32_t row0, uint32_t height) {   // height: rows that there are from row0 on, up to sixteen
@@ -262,7 +274,8 @@ struct Step {
       }
     const uint32_t mine = li & (ROOM - 1);
     const uint8_t *const my_x = of_x + mine * S::X_BYTES;
-    const float scales[2] = {F8 ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))) : 0.0f, F8 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32)) : 0.0f};
+    float scales[2] = {0, 0};
+    if constexpr (F8) scales[0] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))), scales[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32));
     if constexpr (F8) {
       v4i u[2][2];
 #pragma unroll
@@ -445,7 +458,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
   }
 }
 
-// ---- Down: blockIdx.x: `height` rows, 4, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to eight steps of a part, of which a wave has every
+// ---- Down: blockIdx.x: `height` rows, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to eight steps of a part, of which a wave has every
 // WAVES-th: a workgroup's waves go through the same rows together. ----
 template <bool F8, int ROOM, bool RAGGED, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
@@ -549,11 +562,12 @@ hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t hei
 }
 template <bool F8, int ROOM, bool RAGGED>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  // Rows for all compute units alike: a workgroup of sixteen waves to each where sixteen rows are enough and its sums of all tokens fit LDS, else several of eight.
-  const uint32_t each = (a.hidden + 16 * g_compute_units - 1) / (16 * g_compute_units), rows = (a.hidden + each * g_compute_units - 1) / (each * g_compute_units);
-  const uint32_t height = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  return each == 1 && a.tokens <= 32 ? launch_down_waves<F8, ROOM, RAGGED, 16>(a, w, height, a.tokens, stream)
-                                     : launch_down_waves<F8, ROOM, RAGGED, 8>(a, w, height, std::min(a.tokens, 96u), stream);
+  // Eight rows where these leave the compute unit with the most of them fewer; a workgroup of sixteen waves to each unit where one is enough and its sums of all tokens fit LDS, else
+  // several of eight.
+  auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
+  const uint32_t height = most_rows(8) < most_rows(16) ? 8 : 16;
+  return most_rows(height) <= height && a.tokens <= 32 ? launch_down_waves<F8, ROOM, RAGGED, 16>(a, w, height, a.tokens, stream)
+                                                       : launch_down_waves<F8, ROOM, RAGGED, 8>(a, w, height, std::min(a.tokens, 96u), stream);
 }
 template <bool F8, int ROOM>
 hipError_t launch_products(const ExpertsArgs &a, const Places &w, bool fused, hipStream_t stream) {
