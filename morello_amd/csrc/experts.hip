@@ -106,90 +106,87 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   }
 }
 
-// ---- Choice of a token's experts by a workgroup: the j-th is the one that j others are before.  Where there are more threads than experts, an expert's threads
+// ---- Choice of experts, of some tokens by a workgroup: a token's j-th is the one that j others are before.  Where there are more threads than logits, a logit's threads
 // share the others. ----
-template <int THREADS>
-struct Choice {
-  double key[MOST_EXPERTS];       // logits; NaN as the lowest value
-  uint32_t before[MOST_EXPERTS];
-  double most;
-  float sums[THREADS / 64], e[MOST_CHOSEN];
-  int32_t expert[MOST_CHOSEN];
+struct Choice {          // in LDS, for `tokens` tokens
+  double *key;           // [tokens][experts] logits; NaN as the lowest value
+  double *most;          // [tokens]
+  uint32_t *before;      // [tokens][experts]
+  int32_t *expert;       // [tokens][top_k]
+  float *share;          // [tokens][top_k]
+  __device__ inline Choice(uint8_t *at, const ExpertsArgs &p, uint32_t tokens) {
+    key = (double *)at, at += tokens * p.experts * 8;
+    most = (double *)at, at += tokens * 8;
+    before = (uint32_t *)at, at += tokens * p.experts * 4;
+    expert = (int32_t *)at, at += tokens * p.top_k * 4;
+    share = (float *)at;
+  }
+  static size_t bytes(uint32_t experts, uint32_t top_k, uint32_t tokens) { return tokens * (experts * 12 + 8 + top_k * 8); }
 };
-// Ends on a barrier: expert[0 .. top_k) are there; returns their number tid's share (for tid < top_k).
+// Tokens t0 .. t0 + tokens - 1.  Ends on a barrier.
 template <int THREADS>
-__device__ inline float choose(const ExpertsArgs &p, const Places &w, uint32_t token, Choice<THREADS> &c) {
-  constexpr int EACH = MOST_EXPERTS / THREADS;
-  static_assert(MOST_EXPERTS % THREADS == 0, "");
-  const uint32_t tid = threadIdx.x;
-  double value[EACH];
-#pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const uint32_t e = tid + i * THREADS;
-    if (e >= p.experts) break;
-    value[i] = w.logits[uint64_t(token) * p.experts + e];
-    c.key[e] = value[i] == value[i] ? value[i] : -__builtin_inf();
-    c.before[e] = 0;
+__device__ inline void choose(const ExpertsArgs &p, const Places &w, uint32_t t0, uint32_t tokens, const FastDiv &by_experts, const Choice &c) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = tokens * p.experts;
+  const double *const logits = w.logits + uint64_t(t0) * p.experts;
+  for (uint32_t i = tid; i < all; i += THREADS) {
+    const double x = logits[i];
+    c.key[i] = x == x ? x : -__builtin_inf();
+    c.before[i] = 0;
   }
   __syncthreads();
-  const uint32_t span = p.experts <= 64 ? 64 : 1u << (32 - __clz(p.experts - 1)), shared = span < THREADS ? THREADS / span : 1;   // (both powers of two)
-#pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const uint32_t e = (tid & (span - 1)) + i * THREADS, each = (p.experts + shared - 1) / shared;
-    if (e >= p.experts || (i > 0 && span <= THREADS)) break;
-    const uint32_t o0 = span < THREADS ? tid / span * each : 0, o1 = min(p.experts, o0 + each);
-    const double mine = c.key[e];
+  const uint32_t span = all <= 64 ? 64 : 1u << (32 - __clz(all - 1)), shared = span < THREADS ? THREADS / span : 1, each = (p.experts + shared - 1) / shared;   // (span: a power of two)
+  for (uint32_t i = tid & (span - 1); i < all; i += THREADS) {   // (span below THREADS: one turn, tid / span below shared)
+    const uint32_t t = by_experts.div(i), e = i - t * p.experts, o0 = span < THREADS ? tid / span * each : 0, o1 = min(p.experts, o0 + each);
+    const double mine = c.key[i], *const others = c.key + t * p.experts;
     uint32_t before = 0;
 #pragma unroll 8
     for (uint32_t o = o0; o < o1; o++) {
-      const double k = c.key[o];
+      const double k = others[o];
       before += (k > mine || (k == mine && o < e)) ? 1 : 0;
     }
-    atomicAdd(&c.before[e], before);
+    atomicAdd(&c.before[i], before);
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const uint32_t e = tid + i * THREADS;
-    if (e < p.experts && c.before[e] == 0) c.most = c.key[e];
+  for (uint32_t i = tid; i < all; i += THREADS) {
+    const uint32_t t = by_experts.div(i), before = c.before[i];
+    if (before == 0) c.most[t] = c.key[i];
+    if (before < p.top_k) c.expert[t * p.top_k + before] = int32_t(i - t * p.experts);
   }
   __syncthreads();
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const uint32_t e = tid + i * THREADS;
-    if (e >= p.experts) break;
-    const float x = expf(float(value[i] - c.most));
-    const uint32_t before = c.before[e];
-    sum += x;
-    if (before < p.top_k) c.expert[before] = int32_t(e), c.e[before] = x;
+  for (uint32_t t = wave; t < tokens; t += THREADS / 64) {   // (logits again: a NaN makes all shares of its token NaN)
+    const double most = c.most[t], *const of_token = logits + t * p.experts;
+    float sum = 0.0f, mine = 0.0f;
+    if (lane < p.top_k) mine = expf(float(of_token[c.expert[t * p.top_k + lane]] - most));
+    if (p.renormalise) {
+      sum = mine;
+    } else {
+      for (uint32_t e = lane; e < p.experts; e += 64) sum += expf(float(of_token[e] - most));
+    }
+    sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_over_wave(sum)), 63));
+    if (lane < p.top_k) c.share[t * p.top_k + lane] = mine / sum;
   }
-  sum = sum_over_wave(sum);
-  if (tid % 64 == 63) c.sums[tid / 64] = sum;
   __syncthreads();
-  sum = 0.0f;
-  if (p.renormalise) {
-    for (uint32_t j = 0; j < p.top_k; j++) sum += c.e[j];
-  } else {
-#pragma unroll
-    for (int v = 0; v < THREADS / 64; v++) sum += c.sums[v];
-  }
-  return tid < p.top_k ? c.e[tid] / sum : 0.0f;
 }
 template <int THREADS>
-__device__ inline void keep(const ExpertsArgs &p, const Places &w, uint32_t token, const Choice<THREADS> &c, float share) {
-  if (threadIdx.x >= p.top_k) return;
-  const uint32_t i = token * p.top_k + threadIdx.x;
-  w.chosen[i] = c.expert[threadIdx.x], w.shares[i] = share;
-  if (p.chosen) p.chosen[i] = c.expert[threadIdx.x];
-  if (p.shares) p.shares[i] = share;
+__device__ inline void keep(const ExpertsArgs &p, const Places &w, uint32_t t0, uint32_t tokens, const Choice &c) {
+  for (uint32_t i = threadIdx.x; i < tokens * p.top_k; i += THREADS) {
+    const uint32_t to = t0 * p.top_k + i;
+    w.chosen[to] = c.expert[i], w.shares[to] = c.share[i];
+    if (p.chosen) p.chosen[to] = c.expert[i];
+    if (p.shares) p.shares[to] = c.share[i];
+  }
 }
 constexpr int CHOOSE_THREADS = 512;
-__global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p, Places w) {
-  __shared__ Choice<CHOOSE_THREADS> c;
+__global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p, Places w, FastDiv by_experts) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   if (blockIdx.x >= live_rows(p)) return;
-  keep(p, w, blockIdx.x, c, choose(p, w, blockIdx.x, c));
+  const Choice c(dynamic, p, 1);
+  choose<CHOOSE_THREADS>(p, w, blockIdx.x, 1, by_experts, c);
+  keep<CHOOSE_THREADS>(p, w, blockIdx.x, 1, c);
 }
+// Whether a workgroup of another kernel's makes all choices for itself: some hundred comparisons a thread (a launch takes 5 us).
+constexpr uint32_t MOST_FUSED = 1024;   // logits
+bool fused_choice(const ExpertsArgs &a) { return a.tokens * a.experts <= MOST_FUSED && a.tokens * a.experts * a.experts <= 1u << 15 && a.tokens <= 32 && a.tokens * a.top_k <= 512; }
 
 // ---- Products with experts' weights: 16 rows of each of N matrices against the x of a part's tokens, a step of 128 bytes of the rows at a time.  Loads take a row's 128 bytes with eight
 // lanes, x's with eight or sixteen, and LDS brings both into the order in which the matrix instructions want them: what bounds such loops else is the rate at which a compute
@@ -390,29 +387,25 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
 // took 10 % longer over 1.9 GB).  The waves share a tile's steps; their loads run AHEAD steps in front, from one tile into the next, and the
 // waves' sums meet behind each.  FUSED: from logits, the choices made here. ----
 constexpr int UP_WAVES = 4;
-constexpr uint32_t FUSED_TOKENS = 4;
 template <bool F8, int ROOM, bool FUSED, bool RAGGED>
-__global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles) {
-  constexpr int AHEAD = F8 ? ROOM == 16 ? 2 : 3 : 4;
+__global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles, FastDiv by_experts) {
+  constexpr int AHEAD = 2;   // (us, 2, 3 and 4: 32 tokens through 128 experts of 2048 x 768 in e4m3 63, 68, 87; one through 64 of 2048 x 1024 in bf16 14.6, 15.4, 15.3)
   typedef Shape<F8, ROOM> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   __shared__ v4f sums[2][UP_WAVES][2][64];
-  __shared__ int32_t chosen[FUSED ? FUSED_TOKENS * MOST_CHOSEN : 1];
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t rows = live_rows(p), all = rows * p.top_k;
-  if constexpr (FUSED) {
-    __shared__ Choice<UP_WAVES * 64> c;
-    for (uint32_t t = 0; t < rows; t++) {
-      const float share = choose(p, w, t, c);
-      if (tid < p.top_k) chosen[t * p.top_k + tid] = c.expert[tid];
-      if (blockIdx.x == 0) keep(p, w, t, c, share);
-      __syncthreads();
-    }
-  }
   constexpr uint32_t BOUNCE = 2 * TILE_BYTES + ROOM * S::X_BYTES;
   uint8_t *const bounce = dynamic + wave * BOUNCE;
   const Lists lists(dynamic + UP_WAVES * BOUNCE, p.experts, p.tokens * p.top_k, words, ROOM, UP_WAVES);
-  const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, FUSED ? chosen : w.chosen, all, words, ROOM));
+  const int32_t *chosen = w.chosen;
+  if constexpr (FUSED) {
+    const Choice c(dynamic, p, p.tokens);   // (where the waves' tiles will be)
+    choose<UP_WAVES * 64>(p, w, 0, rows, by_experts, c);
+    if (blockIdx.x == 0) keep<UP_WAVES * 64>(p, w, 0, rows, c);
+    chosen = c.expert;
+  }
+  const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, chosen, all, words, ROOM));
   const uint32_t steps = (p.hidden + S::STEP - 1) / S::STEP, s0 = steps * wave / UP_WAVES, n = steps * (wave + 1) / UP_WAVES - s0;   // this wave's steps of each tile
   Rows<F8, ROOM, 2> of;
   Step<F8, ROOM, 2, RAGGED> t[AHEAD] = {};
@@ -539,13 +532,14 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   // Three workgroups to a compute unit, what their registers allow, or one to a tile.
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
   const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 3 * g_compute_units));
+  static_assert(!FUSED || MOST_FUSED * 12 + 32 * 8 + 512 * 8 <= UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES), "");
   const size_t lds = UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
     const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, RAGGED>), 96 * 1024);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles));
+  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles), FastDiv(a.experts));
   return plan::last_error();
 }
 template <bool F8, int ROOM, bool RAGGED, int WAVES>
@@ -592,13 +586,13 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   // (a token to a workgroup while these still run side by side)
   if (a.experts * a.tokens <= 8 * g_compute_units) MRL_LAUNCH(k_experts_logits<1>, dim3(a.experts, a.tokens), dim3(ROUTER_THREADS), 0, stream, a, w);
   else MRL_LAUNCH(k_experts_logits<4>, dim3(a.experts, (a.tokens + 3) / 4), dim3(ROUTER_THREADS), 0, stream, a, w);
-  const bool fused = a.tokens <= FUSED_TOKENS && a.tokens * a.experts * a.experts <= 1u << 16;
+  const bool few = !(a.tokens > 8 && a.tokens * a.top_k > 6 * a.experts), fused = few && fused_choice(a);
   if (!fused) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
-    MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), 0, stream, a, w);
+    MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), Choice::bytes(a.experts, a.top_k, 1), stream, a, w, FastDiv(a.experts));
   }
   // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.
-  return a.tokens > 8 && a.tokens * a.top_k > 6 * a.experts ? launch_products<F8, 16>(a, w, fused, stream) : launch_products<F8, 8>(a, w, fused, stream);
+  return few ? launch_products<F8, 8>(a, w, fused, stream) : launch_products<F8, 16>(a, w, fused, stream);
 }
 
 }  // namespace
