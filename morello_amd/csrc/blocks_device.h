@@ -18,15 +18,17 @@ typedef v4f v4f_any __attribute__((aligned(4)));
 typedef v4bf v4bf_any __attribute__((aligned(2)));
 
 __device__ inline v4i chunk_at(const uint8_t *p) { return *(const v4i_any *)p; }
+// A row's last sixteen bytes moved down to where its last n of them belong, zeros behind them (n: 0 or less: zeros; 16 and more: as they are).
+__device__ inline v4i last_of_row(v4i x, int n) {
+  typedef unsigned __int128 u128;
+  return n >= 16 ? x : n <= 0 ? v4i{0, 0, 0, 0} : __builtin_bit_cast(v4i, __builtin_bit_cast(u128, x) >> ((16 - n) * 8));
+}
 // The first n bytes of sixteen, zeros behind them (n may be negative, or more); `before`: bytes of the same row in front of p.
 __device__ inline v4i chunk_up_to(const uint8_t *p, int n, int before) {
   if (n >= 16) return chunk_at(p);
   v4i x = {0, 0, 0, 0};
   if (n <= 0) return x;
-  if (n + before >= 16) {   // the row's last sixteen, moved down
-    typedef unsigned __int128 u128;
-    return __builtin_bit_cast(v4i, __builtin_bit_cast(u128, chunk_at(p + n - 16)) >> ((16 - n) * 8));
-  }
+  if (n + before >= 16) return last_of_row(chunk_at(p + n - 16), n);
 #pragma unroll
   for (int d = 0; d < 4; d++)
     for (int i = 0; i < 4 && d * 4 + i < n; i++) x[d] |= int(uint32_t(p[d * 4 + i]) << (i * 8));

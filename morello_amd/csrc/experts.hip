@@ -221,43 +221,60 @@ struct Rows {
     x_loads = int(count + S::X_TOKENS - 1) / S::X_TOKENS;
   }
 };
-// What a lane has of one step.  RAGGED: a row may end inside its last step.
-template <bool F8, int ROOM, int N, bool RAGGED>
+// Where rows end.  INSIDE a step: its chunks that the end cuts, or that lie behind it, come from the row's last sixteen bytes and are put right before they are used, so that all steps have
+// the same loads, without branches; SHORT: rows of weights or of x below sixteen bytes, byte by byte.
+enum Tail { WHOLE = 0, INSIDE = 1, SHORT = 2 };
+// What a lane has of one step.
+template <bool F8, int ROOM, int N, int TAIL>
 struct Step {
   typedef Shape<F8, ROOM> S;
   v4i q[N][2], y[S::X_LOADS];
   float scale;
   int x_loads;
+  int left, x_left;   // INSIDE: bytes of a row from the lane's chunk on
   // k: elements of a row; half: eight rows are enough.
   __device__ inline void fetch(const Rows<F8, ROOM, N> &of, uint32_t s, int k, bool half) {
-    const uint32_t at = s * 128, x_at = s * S::STEP;   // bytes of weights, elements of x
+    const int at = int(s) * 128, x_at = int(s) * S::STEP * 2;   // bytes
     x_loads = of.x_loads;
     if constexpr (F8) scale = of.scale[s];
-    if (!RAGGED || int(s + 1) * S::STEP <= k) {
+    const int chunk = at + int(threadIdx.x & 7) * 16, x_chunk = x_at + int(threadIdx.x) % S::X_CHUNKS * 16;   // the lane's
+    if constexpr (TAIL != SHORT) {
+      int back = at, x_back = x_at;
+      if constexpr (TAIL == INSIDE) {
+        left = k * S::SIZE - chunk, x_left = k * 2 - x_chunk;
+        back += min(left - 16, 0), x_back += min(x_left - 16, 0);
+      }
 #pragma unroll
-      for (int n = 0; n < N; n++) q[n][0] = chunk_at(of.row[n][0] + at);
+      for (int n = 0; n < N; n++) q[n][0] = chunk_at(of.row[n][0] + back);
       if (!half) {
 #pragma unroll
-        for (int n = 0; n < N; n++) q[n][1] = chunk_at(of.row[n][1] + at);
+        for (int n = 0; n < N; n++) q[n][1] = chunk_at(of.row[n][1] + back);
       }
 #pragma unroll
       for (int i = 0; i < S::X_LOADS; i++)
-        if (i < x_loads) y[i] = chunk_at((const uint8_t *)(of.x[i] + x_at));
-    } else {   // the rows end inside
-      const int chunk = int(at) + int(threadIdx.x & 7) * 16, first = int(x_at) + int(threadIdx.x) % S::X_CHUNKS * 8;   // the lane's first byte of weights, element of x
+        if (i < x_loads) y[i] = chunk_at((const uint8_t *)of.x[i] + x_back);
+    } else {
 #pragma unroll
       for (int n = 0; n < N; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) q[n][i] = chunk_up_to(of.row[n][i] + at, k * S::SIZE - chunk, chunk);
 #pragma unroll
       for (int i = 0; i < S::X_LOADS; i++)
-        if (i < x_loads) y[i] = chunk_up_to((const uint8_t *)(of.x[i] + x_at), (k - first) * 2, first * 2);
+        if (i < x_loads) y[i] = chunk_up_to((const uint8_t *)of.x[i] + x_at, k * 2 - x_chunk, x_chunk);
     }
   }
   // bounce: LDS of this wave's, N tiles and x of ROOM tokens.  Chunk c of a row of 128 bytes at c ^ (row / 2 % 8), of 256 bytes at c ^ row: sixteen lanes with a
   // chunk of sixteen rows each reach every bank once.
-  __device__ inline void multiply(v4f (&acc)[N], uint8_t *bounce) const {
+  __device__ inline void multiply(v4f (&acc)[N], uint8_t *bounce) {
     const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    if (TAIL == INSIDE && __any(left < 16 || x_left < 16)) {
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) q[n][i] = last_of_row(q[n][i], left);
+#pragma unroll
+      for (int i = 0; i < S::X_LOADS; i++) y[i] = last_of_row(y[i], x_left);
+    }
     uint8_t *const of_x = bounce + N * TILE_BYTES;
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -387,9 +404,9 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
 // took 10 % longer over 1.9 GB).  The waves share a tile's steps; their loads run AHEAD steps in front, from one tile into the next, and the
 // waves' sums meet behind each.  FUSED: from logits, the choices made here. ----
 constexpr int UP_WAVES = 4;
-template <bool F8, int ROOM, bool FUSED, bool RAGGED>
-__global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles, FastDiv by_experts) {
-  constexpr int AHEAD = 2;   // (us, 2, 3 and 4: 32 tokens through 128 experts of 2048 x 768 in e4m3 63, 68, 87; one through 64 of 2048 x 1024 in bf16 14.6, 15.4, 15.3)
+template <bool F8, int ROOM, bool FUSED, int TAIL>
+__global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles, FastDiv by_experts) {
+  constexpr int AHEAD = 3;
   typedef Shape<F8, ROOM> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   __shared__ v4f sums[2][UP_WAVES][2][64];
@@ -408,7 +425,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
   const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, chosen, all, words, ROOM));
   const uint32_t steps = (p.hidden + S::STEP - 1) / S::STEP, s0 = steps * wave / UP_WAVES, n = steps * (wave + 1) / UP_WAVES - s0;   // this wave's steps of each tile
   Rows<F8, ROOM, 2> of;
-  Step<F8, ROOM, 2, RAGGED> t[AHEAD] = {};
+  Step<F8, ROOM, 2, TAIL> t[AHEAD] = {};
   auto go_to = [&](uint32_t tile) {
     const uint32_t part = by_tiles.div(tile), row0 = (tile - part * tiles) * 16, height = min(16u, p.inter - row0);
     const Part q = lists.parts[part];
@@ -453,9 +470,9 @@ __global__ __launch_bounds__(UP_WAVES * 64, 3) void k_experts_up(ExpertsArgs p, 
 
 // ---- Down: blockIdx.x: `height` rows, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to eight steps of a part, of which a wave has every
 // WAVES-th: a workgroup's waves go through the same rows together. ----
-template <bool F8, int ROOM, bool RAGGED, int WAVES>
+template <bool F8, int ROOM, int TAIL, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
-  constexpr int AHEAD = F8 ? ROOM == 16 ? 2 : 3 : 4, THREADS = WAVES * 64;
+  constexpr int AHEAD = WAVES == 8 ? 6 : F8 ? ROOM == 16 ? 2 : 3 : 4, THREADS = WAVES * 64;
   typedef Shape<F8, ROOM> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
@@ -480,8 +497,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   // The piece to fetch from, and the one to multiply.
   uint32_t fetch_piece = wave, fetch_s = 0, fetch_end = 0, piece = wave, s = 0, end = 0;
   Rows<F8, ROOM, 1> of;
-  Step<F8, ROOM, 1, RAGGED> t[AHEAD] = {};
-  auto fetch = [&](Step<F8, ROOM, 1, RAGGED> &to) {
+  Step<F8, ROOM, 1, TAIL> t[AHEAD] = {};
+  auto fetch = [&](Step<F8, ROOM, 1, TAIL> &to) {
     if (fetch_s == fetch_end) {
       const uint32_t part = fetch_piece / of_part;
       const Part q = lists.parts[part];
@@ -527,58 +544,65 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   }
 }
 
-template <bool F8, int ROOM, bool FUSED, bool RAGGED>
+template <bool F8, int ROOM, bool FUSED, int TAIL>
 hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  // Three workgroups to a compute unit, what their registers allow, or one to a tile.
+  // Two workgroups to a compute unit, what their registers allow, or one to a tile.  (us, two with three steps ahead and three with two: 128 tokens through 128 experts of 2048 x 768 in e4m3 155 and
+  // 180, 32 tokens 110 and 112, 16 through 8 of 4096 x 14336 254 and 253.)
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
-  const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 3 * g_compute_units));
+  const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 2 * g_compute_units));
   static_assert(!FUSED || MOST_FUSED * 12 + 32 * 8 + 512 * 8 <= UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES), "");
   const size_t lds = UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, RAGGED>), 96 * 1024);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, TAIL>), 96 * 1024);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, RAGGED>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles), FastDiv(a.experts));
+  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, TAIL>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles), FastDiv(a.experts));
   return plan::last_error();
 }
-template <bool F8, int ROOM, bool RAGGED, int WAVES>
-hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, uint32_t here, hipStream_t stream) {
-  const uint32_t words = (here + 31) / 32;
-  const size_t lds = size_t(WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + WAVES * (TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, here * a.top_k, words, ROOM, WAVES);
+constexpr size_t MOST_LDS = 160 * 1024;
+template <bool F8, int ROOM, int TAIL, int WAVES>
+size_t down_lds(const ExpertsArgs &a, uint32_t here) {
+  return size_t(WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + WAVES * (TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, ROOM, WAVES);
+}
+template <bool F8, int ROOM, int TAIL, int WAVES>
+hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, hipStream_t stream) {
+  uint32_t here = a.tokens;   // of a workgroup: all, or as many as its sums have place for
+  while (down_lds<F8, ROOM, TAIL, WAVES>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, RAGGED, WAVES>), 160 * 1024);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, WAVES>), MOST_LDS);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_down<F8, ROOM, RAGGED, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + here - 1) / here), dim3(WAVES * 64), lds, stream, a, w, height, here, words);
+  const size_t lds = down_lds<F8, ROOM, TAIL, WAVES>(a, here);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + here - 1) / here), dim3(WAVES * 64), lds, stream, a, w, height, here, (here + 31) / 32);
   return plan::last_error();
 }
-template <bool F8, int ROOM, bool RAGGED>
+template <bool F8, int ROOM, int TAIL>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   // Eight rows where these leave the compute unit with the most of them fewer; a workgroup of sixteen waves to each unit where one is enough and its sums of all tokens fit LDS, else
   // several of eight.
   auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
   const uint32_t height = most_rows(8) < most_rows(16) ? 8 : 16;
-  return most_rows(height) <= height && a.tokens <= 32 ? launch_down_waves<F8, ROOM, RAGGED, 16>(a, w, height, a.tokens, stream)
-                                                       : launch_down_waves<F8, ROOM, RAGGED, 8>(a, w, height, std::min(a.tokens, 96u), stream);
-}
-template <bool F8, int ROOM>
-hipError_t launch_products(const ExpertsArgs &a, const Places &w, bool fused, hipStream_t stream) {
-  constexpr uint32_t STEP = Shape<F8, ROOM>::STEP;
-  const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * std::min(a.experts, a.tokens * a.top_k);
-  const bool ragged = a.hidden % STEP != 0;
-  plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
-  hipError_t e;
-  if constexpr (ROOM == 8) {
-    if (fused) e = ragged ? launch_up<F8, ROOM, true, true>(a, w, stream) : launch_up<F8, ROOM, true, false>(a, w, stream);
-    else e = ragged ? launch_up<F8, ROOM, false, true>(a, w, stream) : launch_up<F8, ROOM, false, false>(a, w, stream);
-  } else {
-    e = ragged ? launch_up<F8, ROOM, false, true>(a, w, stream) : launch_up<F8, ROOM, false, false>(a, w, stream);
+  if constexpr (TAIL != SHORT) {
+    if (most_rows(height) <= height && a.tokens <= 32) return launch_down_waves<F8, ROOM, TAIL, 16>(a, w, height, stream);
   }
+  return launch_down_waves<F8, ROOM, TAIL, 8>(a, w, height, stream);
+}
+// How rows of k elements end.
+template <bool F8>
+Tail tail_of(uint32_t k) { return k * (F8 ? 1 : 2) < 16 || k * 2 < 16 ? SHORT : k % (F8 ? 128 : 64) ? INSIDE : WHOLE; }
+template <bool F8, int ROOM, bool FUSED>
+hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * std::min(a.experts, a.tokens * a.top_k);
+  const Tail up = tail_of<F8>(a.hidden), down = tail_of<F8>(a.inter);
+  plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
+  const hipError_t e = up == WHOLE    ? launch_up<F8, ROOM, FUSED, WHOLE>(a, w, stream)
+                       : up == INSIDE ? launch_up<F8, ROOM, FUSED, INSIDE>(a, w, stream)
+                                      : launch_up<F8, ROOM, FUSED, SHORT>(a, w, stream);
   if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  return a.inter % STEP ? launch_down<F8, ROOM, true>(a, w, stream) : launch_down<F8, ROOM, false>(a, w, stream);
+  return down == WHOLE ? launch_down<F8, ROOM, WHOLE>(a, w, stream) : down == INSIDE ? launch_down<F8, ROOM, INSIDE>(a, w, stream) : launch_down<F8, ROOM, SHORT>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
@@ -592,7 +616,7 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), Choice::bytes(a.experts, a.top_k, 1), stream, a, w, FastDiv(a.experts));
   }
   // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.
-  return few ? launch_products<F8, 8>(a, w, fused, stream) : launch_products<F8, 16>(a, w, fused, stream);
+  return !few ? launch_products<F8, 16, false>(a, w, stream) : fused ? launch_products<F8, 8, true>(a, w, stream) : launch_products<F8, 8, false>(a, w, stream);
 }
 
 }  // namespace
