@@ -72,8 +72,8 @@ inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
 
 hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);
 hipError_t launch_product_tile(const ProductArgs &p, hipStream_t stream);
-// Up to 128 rows of a; rows of whole chunks, scales of a within 2 GB.
-constexpr uint32_t MOST_FEW = 128;
+// Rows of whole chunks, scales of a within 2 GB.  (us, so and on tiles: 80 x 8192 x 8192 19.4 and 20.4, 96 x 4096 x 4096 10.4 and 11.8, 128 x 8192 x 8192 41.8 and 21.3, 128 x 4096 x 4096 13.4 and 12.0.)
+constexpr uint32_t MOST_FEW = 96;
 hipError_t launch_product_few(const ProductArgs &p, hipStream_t stream);
 
 }  // namespace mrl

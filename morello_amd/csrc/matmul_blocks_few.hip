@@ -1,4 +1,4 @@
-// The product of blocks (matmul_blocks.hip) for up to 128 rows of a, of whole 16-byte chunks.
+// The product of blocks (matmul_blocks.hip) for up to 96 rows of a, of whole 16-byte chunks.
 //
 // What bounds it is reading b once.  A workgroup has 16 NT of b's rows and all of a's (16 MT), its waves every WAVES-th block of K each: a block's 128 bytes
 // of all these rows, and a's scales, go straight from memory into a ring of DEPTH blocks in LDS that is the wave's own, so that no wave waits for another
@@ -118,9 +118,8 @@ hipError_t choose(const ProductArgs &p, hipStream_t stream) {
     case 2: return launch<2, 1, 8, 3, OUT>(p, stream);
     case 3: return pairs ? launch<3, 2, 4, 3, OUT>(p, stream) : launch<3, 1, 8, 2, OUT>(p, stream);
     case 4: return pairs ? launch<4, 2, 4, 3, OUT>(p, stream) : launch<4, 1, 4, 3, OUT>(p, stream);
-    case 5: return pairs ? launch<5, 2, 4, 2, OUT>(p, stream) : launch<5, 1, 4, 3, OUT>(p, stream);
-    case 6: return pairs ? launch<6, 2, 4, 2, OUT>(p, stream) : launch<6, 1, 4, 2, OUT>(p, stream);
-    default: return launch<8, 1, 4, 2, OUT>(p, stream);
+    case 5: return pairs ? launch<5, 2, 4, 2, OUT>(p, stream) : launch<5, 1, 6, 2, OUT>(p, stream);
+    default: return pairs ? launch<6, 2, 4, 2, OUT>(p, stream) : launch<6, 1, 4, 2, OUT>(p, stream);
   }
 }
 
