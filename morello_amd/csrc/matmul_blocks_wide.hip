@@ -3,19 +3,22 @@
 // Eight waves of 128 rows of a by 64 of b: 128 sums a lane.  (Four waves of 128 x 128 would read a third less from LDS, but their 256 sums leave a wave's vector
 // instructions, which reach 256 registers, nothing to work with: every sum takes one of them per block.)  Per block of K a wave has 32 matrix
 // instructions of 32 cycles and 128 multiply-adds of 4, in the shadow of the other wave's matrix instructions on the same SIMD.  Operands go
-// straight from memory into LDS, two blocks of 64 KiB, the next under this one's products; chunk c of a row at c ^ (row / 2 % 8), so that sixteen lanes with
-// a chunk of sixteen rows each reach every bank once.  The products of both scales are formed four blocks ahead by all threads, and lie in LDS by rows of a.
+// straight from memory into LDS, which holds two blocks of 64 KiB; chunk c of a row at c ^ (row / 2 % 8), so that sixteen lanes with
+// a chunk of sixteen rows each reach every bank once.  What bounds it is the way of 64 KiB into each compute unit, some 3500 cycles from the first load to the last byte where the products take
+// 2048: a block's last operands are read into registers halfway through its products, and the block after the next is asked for then, over it.
 #include "matmul_blocks.h"
 
 namespace mrl {
 namespace {
 using namespace blocks;
 
-constexpr int SIDE = 256, THREADS = 512, AHEAD = 4;            // AHEAD: blocks whose scales are formed together
-constexpr int SLOT = 2 * SIDE * int(BLOCK), SCALES = AHEAD * 2 * SIDE * 4;
+constexpr int SIDE = 256, THREADS = 512;
+constexpr int SLOT = 2 * SIDE * int(BLOCK), LOADS = 8;          // a's rows and b's; a wave's loads, a step
+constexpr int GROUP = 8, SCALES = GROUP * SIDE * 4;             // a's scales, of a group of steps
 constexpr int LDS_BYTES = 2 * SLOT + 2 * SCALES;
 constexpr int HIGH = 4;                                         // tiles of m that go together
 
+template <bool CHUNKS>   // a's scales are whole 16-byte chunks
 __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint32_t tiles_m, uint32_t tiles_n) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -34,31 +37,32 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
   const uint32_t off_even = (first + row8) * stride + even * 16, off_odd = (first + 8 + row8) * stride + odd * 16;
   const uint32_t lds0 = lds_address(lds), to0 = lds0 + (of_a ? 0 : SIDE * BLOCK) + first * BLOCK;
   const uint32_t left_in_last = p.k - (steps - 1) * BLOCK;
-  auto fetch = [&](int step) {
-    // (up to the last row's end: rows behind it bring zeros, or where rows overlap something, which nobody sees)
-    const v4i from = resource(tile + step * int(BLOCK), (rows - 1) * stride + (p.k - step * BLOCK));
-    const bool last = step == steps - 1;
-    const uint32_t e = last && even * 16 >= left_in_last ? OUTSIDE : off_even, o = last && odd * 16 >= left_in_last ? OUTSIDE : off_odd;
-    const uint32_t to = to0 + (step & 1) * SLOT;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      dma16(from, e + i * 8 * stride, to + i * 1024);
-      dma16(from, o + i * 8 * stride, to + (i + 1) * 1024);
+  // a's scales of a group of steps, with the first of them: 32 rows from each wave, two lanes to a row's 32 bytes, to [row][step]; where they are not whole chunks four bytes of a row at a time, from the
+  // first four waves 64 rows each, to [step][row].
+  const uint32_t a_rows = min(uint32_t(SIDE), p.m - m0);
+  const uint32_t scale_row = CHUNKS ? wave * 32 + lane / 2 : (wave & 3) * 64 + lane, scale_off = scale_row < a_rows ? scale_row * uint32_t(p.as_s) * 4 + (CHUNKS ? lane % 2 * 16 : 0) : OUTSIDE;
+  const float *const a_scales = p.a_scales + int64_t(m0) * p.as_s;
+  auto fetch_scales = [&](int step) {
+    const uint32_t to = lds0 + 2 * SLOT + (step / GROUP & 1) * SCALES;
+    if constexpr (CHUNKS) {
+      dma16(resource(a_scales + step, 0x7fffffff), step + lane % 2 * 4 < steps ? scale_off : OUTSIDE, to + wave * 1024);
+    } else if (wave < 4) {
+      for (int i = 0; i < GROUP && step + i < steps; i++) dma4(resource(a_scales + step + i, 0x7fffffff), scale_off, to + i * (SIDE * 4) + wave * 256);
     }
   };
-  // The products of scales of AHEAD steps: [slot][step][half of n][row of a].
-  float *const scales = (float *)(lds + 2 * SLOT);
-  const float *const a_scale = p.a_scales + int64_t(min(m0 + (tid & 255), p.m - 1)) * p.as_s;
-  const float *const b_scale = p.b_scales + int64_t(min(n0 / BLOCK + (tid >> 8), (p.n - 1) / BLOCK)) * p.bs_s;
-  float sa[AHEAD], sb[AHEAD];
-  auto fetch_scales = [&](int step) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) sa[i] = a_scale[min(step + i, steps - 1)], sb[i] = b_scale[min(step + i, steps - 1)];
+  // What of the others depends on the step; the i-th of them.  (Behind the last step: zeros that nobody reads, rather than branches.)
+  v4i from;
+  uint32_t even_off, odd_off, slot_in;
+  auto begin_fetch = [&](int step) {
+    // (up to the last row's end: rows behind it bring zeros, or where rows overlap something, which nobody sees)
+    from = resource(tile + step * int(BLOCK), step < steps ? (rows - 1) * stride + (p.k - step * BLOCK) : 0);
+    const bool last = step == steps - 1;
+    even_off = last && even * 16 >= left_in_last ? OUTSIDE : off_even, odd_off = last && odd * 16 >= left_in_last ? OUTSIDE : off_odd;
+    slot_in = (step & 1) * SLOT;
   };
-  auto keep_scales = [&](int slot) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) scales[((slot * AHEAD + i) * 2 + (tid >> 8)) * SIDE + (tid & 255)] = sa[i] * sb[i];
-  };
+  auto fetch = [&](int i) { dma16(from, (i & 1 ? odd_off : even_off) + (i & ~1) * 8 * stride, to0 + slot_in + i * 1024); };
+  typedef const __attribute__((address_space(4))) float const_float;   // (scalar loads: vector ones would be counted with those above)
+  const_float *const b_scale = (const_float *)(p.b_scales + int64_t(min(n0 + wn * 64, p.n - 1) / BLOCK) * p.bs_s);
   auto fragment = [&](const uint8_t *row) {   // (rows of a fragment start at a multiple of 16)
     const uint8_t *const mine = row + li * BLOCK;
     const v4i lo = *(const v4i *)(mine + (lg ^ (li >> 1)) * 16), hi = *(const v4i *)(mine + ((lg + 4) ^ (li >> 1)) * 16);
@@ -66,37 +70,55 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
   };
 
   v4f acc[8][4] = {};
-  fetch_scales(0);
-  fetch(0);
-  keep_scales(0);
+#pragma unroll
+  for (int ahead = 0; ahead < 2; ahead++) {
+    if (ahead == 0) fetch_scales(0);
+    begin_fetch(ahead);
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) fetch(i);
+  }
+  float sb = b_scale[0];
   for (int step = 0; step < steps; step++) {
-    wait_for_all_but<0>();
-    if (step % AHEAD == 1 && step + AHEAD - 1 < steps) keep_scales((step / AHEAD + 1) & 1);   // (asked for a step ago)
+    wait_for_all_but<LOADS>();   // (those of the step behind this one; scales are asked for in front of them)
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
-    if (step % AHEAD == 0 && step + AHEAD < steps) fetch_scales(step + AHEAD);
-    if (step + 1 < steps) fetch(step + 1);
-    const uint8_t *const a = lds + (step & 1) * SLOT + wm * 128 * BLOCK, *const b = lds + (step & 1) * SLOT + (SIDE + wn * 64) * BLOCK;
-    const float *const scale = scales + ((step / AHEAD & 1) * AHEAD * 2 + step % AHEAD * 2 + (wn >> 1)) * SIDE + wm * 128 + li;
-    v8i w[4], x[2];
+    if ((step + 1) % GROUP == 0 && step + 1 < steps) fetch_scales(step + 1);
+    const uint8_t *const slot = lds + (step & 1) * SLOT, *const a = slot + wm * 128 * BLOCK, *const b = slot + (SIDE + wn * 64) * BLOCK;
+    const float *const scale = (const float *)(lds + 2 * SLOT + (step / GROUP & 1) * SCALES) + (CHUNKS ? (wm * 128 + li) * GROUP + step % GROUP : step % GROUP * SIDE + wm * 128 + li);
+    const float next = b_scale[min(step + 1, steps - 1)];
+    // A sixteen of a's rows under the multiply-adds of the one before; its operands are read three ahead.
+    v8i w[4], x[4];
     v4f part[2][4];
-    float s[2];
-    x[0] = fragment(a), s[0] = scale[0];
+    float s[8];
+    x[0] = fragment(a);
 #pragma unroll
     for (int u = 0; u < 4; u++) w[u] = fragment(b + u * 16 * BLOCK);
-    // A sixteen of a's rows under the multiply-adds of the one before; its operands are read one ahead.
+#pragma unroll
+    for (int t = 1; t < 3; t++) x[t] = fragment(a + t * 16 * BLOCK);
+#pragma unroll
+    for (int t = 0; t < 8; t++) s[t] = scale[t * 16 * (CHUNKS ? GROUP : 1)];
 #pragma unroll
     for (int t = 0; t < 9; t++) {
-      if (t < 7) x[(t + 1) & 1] = fragment(a + (t + 1) * 16 * BLOCK);
+      if (t < 5) x[(t + 3) & 3] = fragment(a + (t + 3) * 16 * BLOCK);
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        if (t < 8) part[t & 1][u] = mma_e4m3(w[u], x[t & 1]);
+        if (t < 8) part[t & 1][u] = mma_e4m3(w[u], x[t & 3]);
         __builtin_amdgcn_sched_barrier(0);
-        if (t > 0) acc[t - 1][u] += part[(t - 1) & 1][u] * s[(t - 1) & 1];
+        if (t > 0) acc[t - 1][u] += part[(t - 1) & 1][u] * (s[t - 1] * sb);
       }
-      if (t < 7) s[(t + 1) & 1] = scale[(t + 1) * 16];
+      if (t == 4) {   // the slot has been read
+        wait_for_lds();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" : : : "memory");
+        begin_fetch(step + 2);
+      }
+#pragma unroll
+      for (int i = 0; i < 3; i++)
+        if (t >= 5 && t < 8 && (t - 5) * 3 + i < LOADS) fetch((t - 5) * 3 + i);
     }
+    sb = next;
   }
+  wait_for_all_but<0>();   // (what is under way goes into this workgroup's LDS)
 #pragma unroll
   for (int t = 0; t < 8; t++) {
     const uint32_t row = m0 + wm * 128 + t * 16 + li;
@@ -110,17 +132,23 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
   }
 }
 
-}  // namespace
 
-hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream) {
+template <bool CHUNKS>
+hipError_t launch(const ProductArgs &p, hipStream_t stream) {
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_product_wide), LDS_BYTES);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_product_wide<CHUNKS>), LDS_BYTES);
     if (e != hipSuccess) return e;
   }
   const uint32_t tiles_m = (p.m + SIDE - 1) / SIDE, tiles_n = (p.n + SIDE - 1) / SIDE;
-  MRL_LAUNCH(k_product_wide, dim3(tiles_m * tiles_n), dim3(THREADS), LDS_BYTES, stream, p, tiles_m, tiles_n);
+  MRL_LAUNCH(k_product_wide<CHUNKS>, dim3(tiles_m * tiles_n), dim3(THREADS), LDS_BYTES, stream, p, tiles_m, tiles_n);
   return plan::last_error();
+}
+
+}  // namespace
+
+hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream) {
+  return (reinterpret_cast<uintptr_t>(p.a_scales) & 15) == 0 && p.as_s % 4 == 0 && (p.k + BLOCK - 1) / BLOCK % 4 == 0 ? launch<true>(p, stream) : launch<false>(p, stream);
 }
 
 }  // namespace mrl
