@@ -119,19 +119,29 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
     sb = next;
   }
   wait_for_all_but<0>();   // (what is under way goes into this workgroup's LDS)
+  __syncthreads();
+  // Through LDS, where a wave's sums take 16 KiB, into whole rows of 128 bytes: eight columns, which are sixteen bytes, at c ^ (row % 8).
+  uint8_t *const mine = lds + wave * 16384;
 #pragma unroll
-  for (int t = 0; t < 8; t++) {
-    const uint32_t row = m0 + wm * 128 + t * 16 + li;
-    if (row >= p.m) continue;
-    uint16_t *const out = (uint16_t *)p.out + int64_t(row) * p.out_s;
+  for (int t = 0; t < 8; t++)
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const uint32_t col = n0 + wn * 64 + u * 16 + lg * 4;
-      store4(out + col, acc[t][u], int(p.n) - int(col));
+      const v4f &x = acc[t][u];
+      *(v4bf *)(mine + (t * 16 + li) * 128 + ((u * 2 + lg / 2) ^ (li & 7)) * 16 + lg % 2 * 8) = v4bf{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+    }
+  const uint32_t col = n0 + wn * 64 + (lane & 7) * 8, row_end = min(128u, p.m - min(p.m, m0 + wm * 128));
+  uint16_t *const out = (uint16_t *)p.out + int64_t(m0 + wm * 128) * p.out_s + col;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const uint32_t row = i * 8 + row8;
+    const v4i x = *(const v4i *)(mine + row * 128 + ((lane & 7) ^ row8) * 16);
+    if (row < row_end && col < p.n) {
+      if (col + 8 <= p.n) *(v4i_any *)(out + int64_t(row) * p.out_s) = x;
+      else
+        for (uint32_t e = 0; e < p.n - col; e++) out[int64_t(row) * p.out_s + e] = uint16_t(uint32_t(x[e / 2]) >> (e % 2 * 16));
     }
   }
 }
-
 
 template <bool CHUNKS>
 hipError_t launch(const ProductArgs &p, hipStream_t stream) {
