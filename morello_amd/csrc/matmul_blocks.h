@@ -68,6 +68,41 @@ inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 16 == 0 && k % 16 == 0 && stride < (1 << 23);
 }
 
+// A wave's sums of MT x NT sixteens, the first of row `row0` and column `col0`, through `lds` (16 * MT * 16 * NT elements) into whole rows: chunk c of a row at c ^ row.
+template <int MT, int NT, class OUT>
+__device__ inline void store_sums(uint8_t *lds, const v4f (&acc)[MT][NT], const ProductArgs &p, uint32_t row0, uint32_t col0) {
+  constexpr int SIZE = sizeof(OUT), EACH = 16 / SIZE, ROW = NT * 16 * SIZE, CHUNKS = ROW / 16, ROWS = 64 / CHUNKS;
+  const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < MT; t++)
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+      const v4f &x = acc[t][u];
+      const uint32_t byte = (u * 16 + lg * 4) * SIZE;
+      uint8_t *const to = lds + (t * 16 + li) * ROW + (byte / 16 ^ (li & (CHUNKS - 1))) * 16 + byte % 16;
+      if constexpr (SIZE == 2) *(v4bf *)to = v4bf{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+      else *(v4f *)to = x;
+    }
+  const uint32_t chunk = lane % CHUNKS, first = lane / CHUNKS, col = col0 + chunk * EACH, row_end = p.m - min(p.m, row0);
+  OUT *const out = (OUT *)p.out + int64_t(row0) * p.out_s + col;
+#pragma unroll
+  for (int i = 0; i < MT * 16 / ROWS; i++) {
+    const uint32_t row = i * ROWS + first;
+    const v4i x = *(const v4i *)(lds + row * ROW + (chunk ^ (row & (CHUNKS - 1))) * 16);
+    if (row < row_end && col < p.n) {
+      OUT *const to = out + int64_t(row) * p.out_s;
+      if (col + EACH <= p.n) *(v4i_any *)to = x;
+      else
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+          if (col + e < p.n) {
+            if constexpr (SIZE == 2) to[e] = uint16_t(uint32_t(x[e / 2]) >> (e % 2 * 16));
+            else to[e] = __int_as_float(x[e]);
+          }
+    }
+  }
+}
+
 }  // namespace blocks
 
 hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);

@@ -111,17 +111,9 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
 #pragma unroll
         for (int u = 0; u < NT; u++) acc[t][u] += parts[(g * 4 * MT * NT + t * NT + u) * 64];
   }
-#pragma unroll
-  for (int t = 0; t < MT; t++) {
-    const uint32_t row = m0 + wm + t * 16 + li;
-    if (row >= p.m) continue;
-    OUT *const out = (OUT *)p.out + int64_t(row) * p.out_s;
-#pragma unroll
-    for (int u = 0; u < NT; u++) {
-      const uint32_t col = n0 + wn + u * 16 + lg * 4;
-      store4(out + col, acc[t][u], int(p.n) - int(col));
-    }
-  }
+  if constexpr (GROUPS == 1) __syncthreads();   // (all waves have read their operands)
+  else wait_for_lds();                          // (the sums of the others are in; each wave's lie where its own have been)
+  store_sums<MT, NT, OUT>(lds + wave * (MT * NT * 1024), acc, p, m0 + wm, n0 + wn);
 }
 
 template <int BM, int BN, int GROUPS, int DEPTH, class OUT>
