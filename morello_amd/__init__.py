@@ -20,7 +20,7 @@ import numpy as np
 from . import _binding as B
 
 
-_PAGED_CALLS = ("mrl_run_page_tables", "mrl_run_rotary", "mrl_run_paged_attention", "mrl_page_tables_plan", "mrl_rotary_plan", "mrl_paged_attention_plan")
+_DETAILED_CALLS = tuple(c for n in ("page_tables", "rotary", "paged_attention", "cast_blocks", "matmul_blocks", "experts") for c in (f"mrl_run_{n}", f"mrl_{n}_plan"))
 
 
 class MorelloError(RuntimeError):
@@ -29,7 +29,7 @@ class MorelloError(RuntimeError):
         msg = lib.mrl_status_string(status).decode()
         detail = lib.mrl_last_error().decode()
         # the calls that set the detail they fail with
-        with_detail = status == 4 or where == "mrl_run_noalloc" or (status != 6 and where in _PAGED_CALLS)
+        with_detail = status == 4 or where == "mrl_run_noalloc" or (status != 6 and where in _DETAILED_CALLS)
         super().__init__(f"{where}: {msg}" + (f" ({detail})" if detail and with_detail else ""))
         self.status = status
 
