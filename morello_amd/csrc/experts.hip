@@ -184,9 +184,10 @@ __global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p
   choose<CHOOSE_THREADS>(p, w, blockIdx.x, 1, by_experts, c);
   keep<CHOOSE_THREADS>(p, w, blockIdx.x, 1, c);
 }
-// Whether a workgroup of another kernel's makes all choices for itself: some hundred comparisons a thread (a launch takes 5 us).
-constexpr uint32_t MOST_FUSED = 1024;   // logits
-bool fused_choice(const ExpertsArgs &a) { return a.tokens * a.experts <= MOST_FUSED && a.tokens * a.experts * a.experts <= 1u << 15 && a.tokens <= 32 && a.tokens * a.top_k <= 512; }
+// Whether every workgroup of the next launch makes all choices for itself: up to 64 comparisons a thread.  (us of the layer in a graph, so and with a launch for them, 2048 x 512 and experts: 1 token 64 16.3
+// and 17.3, 128 20.6 and 21.4, 160 28.5 and 28.3; 4 tokens 32 22.0 and 23.4, 64 24.1 and 23.8; 8 tokens 32 27.1 and 27.7, 128 84.9 and 74.8; 32 tokens 16 26.9 and 24.7.  Outside of graphs a launch is some 4 more.)
+constexpr uint32_t MOST_FUSED_TOKENS = 8, MOST_FUSED = 384;   // (logits: the root of 2^17 at most)
+bool fused_choice(const ExpertsArgs &a) { return a.tokens <= MOST_FUSED_TOKENS && a.tokens * a.experts * a.experts <= 1u << 14; }
 
 // ---- Products with experts' weights: 16 rows of each of N matrices against the x of a part's tokens, a step of 128 bytes of the rows at a time.  Loads take a row's 128 bytes with eight
 // lanes, x's with eight or sixteen, and LDS brings both into the order in which the matrix instructions want them: what bounds such loops else is the rate at which a compute
@@ -550,7 +551,7 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   // 180, 32 tokens 110 and 112, 16 through 8 of 4096 x 14336 254 and 253.)
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
   const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 2 * g_compute_units));
-  static_assert(!FUSED || MOST_FUSED * 12 + 32 * 8 + 512 * 8 <= UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES), "");
+  static_assert(!FUSED || MOST_FUSED * 12 + MOST_FUSED_TOKENS * (8 + MOST_CHOSEN * 8) <= UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES), "");
   const size_t lds = UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
@@ -580,12 +581,13 @@ hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t hei
 }
 template <bool F8, int ROOM, int TAIL>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  // Eight rows where these leave the compute unit with the most of them fewer; a workgroup of sixteen waves to each unit where one is enough and its sums of all tokens fit LDS, else
-  // several of eight.
-  auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
-  const uint32_t height = most_rows(8) < most_rows(16) ? 8 : 16;
-  if constexpr (TAIL != SHORT) {
-    if (most_rows(height) <= height && a.tokens <= 32) return launch_down_waves<F8, ROOM, TAIL, 16>(a, w, height, stream);
+  // Eight rows where sixteen would leave half of the compute units without any.  (us of the layer, 8 and 16, in bf16 through 64 experts of 768, 8 chosen: 32 tokens of 2048 124.7 and 133.1, 8 of 1024 65.5 and 68.1,
+  // 8 of 2880 123.9 and 116.7, 1 of 5120 54.0 and 50.9; in e4m3 32 of 2048 76 and 81, 8 of 2880 88 and 71.)
+  const uint32_t height = a.hidden <= 8 * g_compute_units ? 8 : 16;
+  // A workgroup of sixteen waves to each unit where one is enough and its tokens are few enough for deep lookahead, else several of eight.  (us, 16 and 8 waves, 128 experts of 2048 x 768, 8 chosen, in bf16: 1 token 26.2 and 28.2,
+  // 32 204 and 221, 64 237 and 256, 128 323 and 276; in e4m3 64 132 and 147, 128 232 and 157, in parts of sixteen 64 tokens through 32 experts 61 and 55.)
+  if constexpr (TAIL != SHORT && !(F8 && ROOM == 16)) {
+    if (a.hidden <= height * g_compute_units && a.tokens <= 64) return launch_down_waves<F8, ROOM, TAIL, 16>(a, w, height, stream);
   }
   return launch_down_waves<F8, ROOM, TAIL, 8>(a, w, height, stream);
 }
@@ -607,15 +609,16 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t st
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   plan::work(plan::UNIT_STREAM, 0, 2.0 * (double(a.experts) + a.tokens) * a.hidden);
-  // (a token to a workgroup while these still run side by side)
+  // (a token to a workgroup while these still run side by side: the layer takes 31.5 us so and 32.3 with four for 1 token and 512 experts, 33 and 33 for 16 and 128, 202 and 185 for 200 and 256)
   if (a.experts * a.tokens <= 8 * g_compute_units) MRL_LAUNCH(k_experts_logits<1>, dim3(a.experts, a.tokens), dim3(ROUTER_THREADS), 0, stream, a, w);
   else MRL_LAUNCH(k_experts_logits<4>, dim3(a.experts, (a.tokens + 3) / 4), dim3(ROUTER_THREADS), 0, stream, a, w);
-  const bool few = !(a.tokens > 8 && a.tokens * a.top_k > 6 * a.experts), fused = few && fused_choice(a);
+  const bool few = !(a.tokens > 8 && a.tokens * a.top_k >= 6 * a.experts), fused = few && fused_choice(a);
   if (!fused) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), Choice::bytes(a.experts, a.top_k, 1), stream, a, w, FastDiv(a.experts));
   }
-  // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.
+  // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.  (us, 16 and 8, choices an expert: 2 113.6 and 111.6,
+  // 4 33.3 and 31.5, 6 149.2 and 150.5, 137 and 145, 8 156 and 172, 91 and 101.)
   return !few ? launch_products<F8, 16, false>(a, w, stream) : fused ? launch_products<F8, 8, true>(a, w, stream) : launch_products<F8, 8, false>(a, w, stream);
 }
 

@@ -112,7 +112,9 @@ hipError_t launch(const ProductArgs &p, hipStream_t stream) {
 
 template <class OUT>
 hipError_t choose(const ProductArgs &p, hipStream_t stream) {
-  const bool pairs = p.n >= 32 * g_compute_units * 3 / 4;   // 32 of b's rows to a workgroup still keep three in four compute units busy
+  // 32 of b's rows to a workgroup where these still keep three in four compute units busy.  (us, 16 and 32: 48 x 4096 x 4096 7.5 and 7.7, 96 x 4096 x 4096 10.4 and 11.0, 48 x 6144 x 4096 11.5 and 8.2,
+  // 96 x 6144 x 4096 18.0 and 11.6.)
+  const bool pairs = p.n >= 32 * g_compute_units * 3 / 4;
   switch ((p.m + 15) / 16) {
     case 1: return launch<1, 1, 8, 4, OUT>(p, stream);
     case 2: return launch<2, 1, 8, 3, OUT>(p, stream);

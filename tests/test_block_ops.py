@@ -96,6 +96,31 @@ def test_plans():
     assert experts().plan().scratch_bytes == experts().workspace_bytes()
 
 
+ODD = dict(a_stride=4097)
+
+
+@pytest.mark.parametrize("m,n,k,out,strides,kernel,copied", [
+    (1, 4096, 4096, M.bf16, {}, "k_product_few", 0), (96, 4096, 4096, M.f32, {}, "k_product_few", 0), (97, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
+    (4096, 4096, 4096, M.bf16, {}, "k_product_wide", 0), (4096, 4096, 4096, M.f32, {}, "k_product_tile", 0), (2048, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
+    (2048, 6144, 4096, M.bf16, {}, "k_product_wide", 0), (32, 100, 4095, M.bf16, {}, "k_product_few_any", 0), (33, 100, 4095, M.bf16, {}, "k_product_few", 133 * 4096),
+    (40, 100, 4096, M.bf16, ODD, "k_product_few", 40 * 4096), (40, 100, 4096, M.bf16, dict(b_stride=4100), "k_product_few", 100 * 4096),
+    (100, 1 << 23, 2049, M.bf16, {}, "k_product_tile_any", 0), (300, 100, 256, M.f32, dict(a_scale_stride=1 << 21), "k_product_tile_any", 0),
+])
+def test_which_kernel_a_product_takes(m, n, k, out, strides, kernel, copied):
+    op = M.MatmulBlocks(out, m, n, k, **strides)
+    assert op.workspace_bytes() == copied
+    steps = op.plan().steps
+    assert [s.family for s in steps][-1] == kernel and len(steps) == 1 + (copied > 0)
+
+
+@pytest.mark.parametrize("tokens,hidden,experts_,top_k,launches", [
+    (1, 2048, 128, 8, 3), (1, 2048, 129, 8, 4), (8, 2048, 45, 8, 3), (8, 2048, 46, 8, 4), (9, 2048, 8, 2, 4), (256, 2048, 512, 32, 4)])
+def test_which_kernels_a_layer_of_experts_takes(tokens, hidden, experts_, top_k, launches):
+    for dtype in (M.bf16, M.f8e4m3):
+        families = [s.family for s in M.Experts(dtype, tokens, hidden, 768, experts_, top_k).plan().steps]
+        assert families == ["k_experts_logits"] + ["k_experts_choose"] * (launches == 4) + ["k_experts_up", "k_experts_down"]
+
+
 def test_the_oracle_of_the_casts():
     """Every byte is its own nearest; between two numbers the nearer, halfway the even byte; a block reads back within half a step."""
     codes = np.array([c for c in range(256) if c & 127 != 127])

@@ -11,7 +11,11 @@ pytestmark = pytest.mark.gpu
 SIZES = [(1, 256, 128, 8, 2), (1, 1, 1, 1, 1), (1, 2048, 256, 64, 8), (2, 512, 130, 16, 4), (3, 264, 72, 60, 4), (5, 1001, 333, 7, 3), (8, 640, 384, 128, 8), (16, 512, 200, 8, 2),
          (17, 300, 96, 4, 2), (33, 256, 256, 5, 5), (64, 384, 64, 32, 6), (100, 200, 50, 3, 1), (128, 256, 144, 256, 8), (256, 128, 40, 512, 32), (70, 130, 260, 2, 2),
          # logits of all tokens below, at and past the threads that choose; the last that one workgroup chooses for all, and one more
-         (5, 264, 72, 60, 4), (2, 128, 64, 127, 5), (2, 128, 64, 128, 5), (3, 128, 64, 104, 7), (16, 136, 40, 45, 3), (32, 64, 48, 32, 4), (31, 64, 48, 32, 16), (33, 64, 48, 31, 4), (1, 64, 48, 181, 32)]
+         (5, 264, 72, 60, 4), (2, 128, 64, 127, 5), (2, 128, 64, 128, 5), (3, 128, 64, 104, 7), (16, 136, 40, 45, 3), (32, 64, 48, 32, 4), (31, 64, 48, 32, 16), (33, 64, 48, 31, 4), (1, 64, 48, 181, 32),
+         # the largest of whose choices every workgroup makes all, and those behind them
+         (8, 72, 40, 45, 32), (8, 72, 40, 46, 32), (4, 136, 64, 64, 6), (1, 136, 64, 128, 32), (1, 136, 64, 129, 32), (9, 64, 48, 8, 2),
+         # sixteen waves for the products with down, and one token more
+         (64, 300, 136, 128, 8), (65, 300, 136, 128, 8), (64, 2050, 64, 40, 3), (64, 264, 128, 300, 32), (33, 4096, 48, 6, 2), (40, 4100, 48, 64, 2)]
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
