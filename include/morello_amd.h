@@ -47,8 +47,8 @@ typedef enum {
   MRL_I32 = 5,
   MRL_F32 = 6,
   MRL_BF16 = 7,
-  /* Four bits of mantissa, four of exponent from 2^-6 to 2^8, no infinities (largest 448): of the operators on blocks
-   * and experts at this header's end alone.  No Spec has it (MRL_ERR_BAD_SPEC), and the reference does not. */
+  /* A byte: sign, four bits of exponent (2^-6 to 2^8), three of fraction; sizes below 2^-6 in steps of 2^-9, largest 448, no infinities, NaN 0x7f and 0xff.
+   * Of the operators on blocks and experts at this header's end alone: no Spec has it (MRL_ERR_BAD_SPEC), and the reference does not. */
   MRL_F8E4M3 = 8
 } mrl_dtype;
 
@@ -762,7 +762,8 @@ int mrl_paged_attention_plan(const mrl_paged_attention *op, mrl_plan *plan, mrl_
 
 /* x -> e4m3 and scales.  With a the largest size of a block's elements, at least 2^-110: scale = a / 448, element = x * (448 / a), both quotients and the product
  * rounded to 32 bits, then to the nearest e4m3 (ties to even).  NaN stays NaN and does not count for a; in a block with an infinity every element reads back as NaN.
- * `gated`: what is cast is silu(g) u = g / (1 + exp(-g)) u, in 32 bits, g the first `cols` elements of x's row and u the `cols` behind them.
+ * `gated`: what is cast is silu(g) u = g / (1 + exp(-g)) u, in 32 bits, g the first `cols` elements of x's row and u the `cols` behind them (below g = -87,
+ * where g / (1 + exp(-g)) is less than 2^-119 in size, it may be taken as 0).
  * params:
  *   0  x       [rows][cols], gated [rows][2 * cols]
  *   1  out     e4m3 [rows][cols]                                     (Out)
@@ -786,7 +787,8 @@ int mrl_cast_blocks_plan(const mrl_cast_blocks *op, mrl_plan *plan, mrl_plan_ste
  *   2  b         e4m3 [n][k]
  *   3  b scales  f32 [ceil(n / 128)][ceil(k / 128)]
  *   4  out       [m][n]  (Out)
- *   5  workspace mrl_matmul_blocks_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's */
+ *   5  workspace mrl_matmul_blocks_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's: 0 where a's and b's rows lie 16 bytes apart or a multiple of that and k is one, and for the
+ *                smallest products; else room for copies of a, b or both whose rows do, which every call makes anew.  (Weights whose rows do are read where they lie.) */
 typedef struct {
   int32_t out_dtype;   /* MRL_BF16 or MRL_F32 */
   uint32_t m, n, k;    /* each up to 2^23, m * n up to 2^40 */

@@ -102,7 +102,8 @@ ODD = dict(a_stride=4097)
 @pytest.mark.parametrize("m,n,k,out,strides,kernel,copied", [
     (1, 4096, 4096, M.bf16, {}, "k_product_few", 0), (96, 4096, 4096, M.f32, {}, "k_product_few", 0), (97, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
     (4096, 4096, 4096, M.bf16, {}, "k_product_wide", 0), (4096, 4096, 4096, M.f32, {}, "k_product_tile", 0), (2048, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
-    (2048, 6144, 4096, M.bf16, {}, "k_product_wide", 0), (32, 100, 4095, M.bf16, {}, "k_product_few_any", 0), (33, 100, 4095, M.bf16, {}, "k_product_few", 133 * 4096),
+    (2048, 6144, 4096, M.bf16, {}, "k_product_wide", 0), (16, 100, 4095, M.bf16, {}, "k_product_few_any", 0), (17, 100, 4095, M.bf16, {}, "k_product_few", 117 * 4096),
+    (2, 4000, 4095, M.f32, {}, "k_product_few_any", 0), (3, 4000, 4095, M.f32, {}, "k_product_few", 4003 * 4096),
     (40, 100, 4096, M.bf16, ODD, "k_product_few", 40 * 4096), (40, 100, 4096, M.bf16, dict(b_stride=4100), "k_product_few", 100 * 4096),
     (100, 1 << 23, 2049, M.bf16, {}, "k_product_tile_any", 0), (300, 100, 256, M.f32, dict(a_scale_stride=1 << 21), "k_product_tile_any", 0),
 ])

@@ -120,3 +120,14 @@ def test_repeats_bit_for_bit(gpu):
         x = Operands(m, n, k, 6)
         first = x.run("f32")
         assert np.array_equal(first, x.run("f32"))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 100, 2064), (2, 3000, 1001), (3, 3000, 1001), (16, 130, 1000), (17, 77, 384), (32, 200, 1040), (33, 130, 272), (150, 300, 400)])
+def test_whole_chunks_at_odd_addresses(gpu, m, n, k):
+    """Strides that say whole chunks of addresses that are not: the sizes alone decide on the workspace."""
+    x = Operands(m, n, k, 11, narrow=True)
+    up = -(-k // 16) * 16
+    for offset in (1, 8):
+        for kw in (dict(a_stride=up, b_stride=up), dict(a_stride=up, b_stride=up + 3), dict(a_stride=k + 1, b_stride=up)):
+            for out in ("bf16", "f32"):
+                x.check(x.run(out, offset=offset, **kw), out)
