@@ -68,10 +68,11 @@ inline bool rows_of_chunks(const void *p, int64_t stride, uint32_t k) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 16 == 0 && k % 16 == 0 && stride < (1 << 23);
 }
 
-// A wave's sums of MT x NT sixteens, the first of row `row0` and column `col0`, through `lds` (16 * MT * 16 * NT elements) into whole rows: chunk c of a row at c ^ row.
+// A wave's sums of MT x NT sixteens, the first of row `row0` and column `col0`, through `lds` (16 * MT * 16 * NT elements) into whole rows: chunk c of a row at c ^ row, as far as
+// that stays in the row.
 template <int MT, int NT, class OUT>
 __device__ inline void store_sums(uint8_t *lds, const v4f (&acc)[MT][NT], const ProductArgs &p, uint32_t row0, uint32_t col0) {
-  constexpr int SIZE = sizeof(OUT), EACH = 16 / SIZE, ROW = NT * 16 * SIZE, CHUNKS = ROW / 16, ROWS = 64 / CHUNKS;
+  constexpr int SIZE = sizeof(OUT), EACH = 16 / SIZE, ROW = NT * 16 * SIZE, CHUNKS = ROW / 16, TURNED = (CHUNKS & -CHUNKS) - 1, ALL = MT * 16 * CHUNKS;
   const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
 #pragma unroll
   for (int t = 0; t < MT; t++)
@@ -79,18 +80,18 @@ __device__ inline void store_sums(uint8_t *lds, const v4f (&acc)[MT][NT], const 
     for (int u = 0; u < NT; u++) {
       const v4f &x = acc[t][u];
       const uint32_t byte = (u * 16 + lg * 4) * SIZE;
-      uint8_t *const to = lds + (t * 16 + li) * ROW + (byte / 16 ^ (li & (CHUNKS - 1))) * 16 + byte % 16;
+      uint8_t *const to = lds + (t * 16 + li) * ROW + (byte / 16 ^ (li & TURNED)) * 16 + byte % 16;
       if constexpr (SIZE == 2) *(v4bf *)to = v4bf{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
       else *(v4f *)to = x;
     }
-  const uint32_t chunk = lane % CHUNKS, first = lane / CHUNKS, col = col0 + chunk * EACH, row_end = p.m - min(p.m, row0);
-  OUT *const out = (OUT *)p.out + int64_t(row0) * p.out_s + col;
+  const uint32_t row_end = p.m - min(p.m, row0);
+  OUT *const out = (OUT *)p.out + int64_t(row0) * p.out_s + col0;
 #pragma unroll
-  for (int i = 0; i < MT * 16 / ROWS; i++) {
-    const uint32_t row = i * ROWS + first;
-    const v4i x = *(const v4i *)(lds + row * ROW + (chunk ^ (row & (CHUNKS - 1))) * 16);
-    if (row < row_end && col < p.n) {
-      OUT *const to = out + int64_t(row) * p.out_s;
+  for (int i = 0; i < (ALL + 63) / 64; i++) {
+    const uint32_t at = i * 64 + lane, row = at / CHUNKS, chunk = at % CHUNKS, col = col0 + chunk * EACH;
+    if ((ALL % 64 == 0 || at < ALL) && row < row_end && col < p.n) {
+      const v4i x = *(const v4i *)(lds + row * ROW + (chunk ^ (row & TURNED)) * 16);
+      OUT *const to = out + int64_t(row) * p.out_s + chunk * EACH;
       if (col + EACH <= p.n) *(v4i_any *)to = x;
       else
 #pragma unroll

@@ -13,7 +13,8 @@ using namespace blocks;
 template <int BM, int BN, int GROUPS, int DEPTH, class OUT>
 __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, uint32_t tiles_m, uint32_t tiles_n, uint32_t high) {
   constexpr int MT = BM / 32, NT = BN / 32, A_LOADS = BM / 32, B_LOADS = BN / 32, LOADS = A_LOADS + B_LOADS + 1;   // a wave's, a step
-  constexpr int SLOT = (BM + BN) * int(BLOCK) + 4 * 256;   // (a's scales: 256 bytes from each wave, two waves' the same where BM is 128)
+  constexpr int SLOT = (BM + BN) * int(BLOCK) + 4 * 256;   // (a's scales: 256 bytes from each wave, BM of them what is wanted)
+  constexpr int SCALES = BLOCK % BN == 0 ? 1 : NT;                 // of b, for a wave's sums: one, or one for each sixteen of b's rows
   static_assert((DEPTH - 2) * LOADS < 64 && GROUPS * DEPTH * SLOT <= 160 * 1024 && (GROUPS - 1) * BM * BN * 4 <= GROUPS * DEPTH * SLOT, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
@@ -23,8 +24,9 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
   const uint32_t tile_n = in_group / here, tile_m = group * high + in_group - tile_n * here;
   const uint32_t m0 = tile_m * BM, n0 = tile_n * BN, wm = wave / 2 * (BM / 2), wn = wave % 2 * (BN / 2);
   const int steps = int((p.k + BLOCK - 1) / BLOCK), turns = (steps + GROUPS - 1) / GROUPS, mine = steps > my_group ? (steps - my_group + GROUPS - 1) / GROUPS : 0;   // mine: turns or one less
-  // This wave's loads of a step, eight rows to each: BM / 4 rows of a, BN / 4 of b.
-  const uint32_t row8 = lane >> 3, even = (lane & 7) ^ (row8 >> 1), odd = even ^ 4, a_s = uint32_t(p.a_s), b_s = uint32_t(p.b_s);
+  // This wave's loads of a step: every fourth eight rows of a and of b, from the wave-th on.  Chunk c of a row at c ^ (row / 2 % 8) of its 128 bytes.
+  const uint32_t row0 = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ (row0 >> 1 & 7), a_s = uint32_t(p.a_s), b_s = uint32_t(p.b_s);
+  const uint32_t a_off = row0 * a_s + chunk * 16, b_off = row0 * b_s + chunk * 16;
   const uint32_t a_rows = min(uint32_t(BM), p.m - m0), b_rows = min(uint32_t(BN), p.n - n0), left_in_last = p.k - (steps - 1) * BLOCK;
   const uint8_t *const a = p.a + int64_t(m0) * p.a_s, *const b = p.b + int64_t(n0) * p.b_s;
   const uint32_t scale_row = (wave * 64 + lane) % BM, scale_off = scale_row < a_rows ? scale_row * uint32_t(p.as_s) * 4 : OUTSIDE;
@@ -34,27 +36,22 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
   uint32_t slot_in = 0;   // where the next step goes
   auto fetch = [&](int turn) {
     const int step = turn * GROUPS + my_group;
-    const bool last = step == steps - 1;
-    const bool no_even = last && even * 16 >= left_in_last, no_odd = last && odd * 16 >= left_in_last;
+    const bool none = step == steps - 1 && chunk * 16 >= left_in_last;
     // (up to the last row's end: rows behind it bring zeros, or where rows overlap something, which nobody sees)
     const uint32_t left = p.k - step * BLOCK;
     const v4i from_a = resource(a + step * int(BLOCK), (a_rows - 1) * a_s + left), from_b = resource(b + step * int(BLOCK), (b_rows - 1) * b_s + left);
     const uint32_t to = lds0 + slot_in * SLOT;
     slot_in = slot_in + 1 == DEPTH ? 0 : slot_in + 1;
 #pragma unroll
-    for (int i = 0; i < A_LOADS; i++) {
-      const uint32_t row = wave * (BM / 4) + i * 8;
-      dma16(from_a, (i & 1 ? no_odd : no_even) ? OUTSIDE : (row + row8) * a_s + (i & 1 ? odd : even) * 16, to + row * BLOCK);
-    }
+    for (int i = 0; i < A_LOADS; i++) dma16(from_a, none ? OUTSIDE : a_off + i * 32 * a_s, to + (i * 32 + wave * 8) * BLOCK);
 #pragma unroll
-    for (int i = 0; i < B_LOADS; i++) {
-      const uint32_t row = wave * (BN / 4) + i * 8;
-      dma16(from_b, (i & 1 ? no_odd : no_even) ? OUTSIDE : (row + row8) * b_s + (i & 1 ? odd : even) * 16, to + (BM + row) * BLOCK);
-    }
+    for (int i = 0; i < B_LOADS; i++) dma16(from_b, none ? OUTSIDE : b_off + i * 32 * b_s, to + (BM + i * 32 + wave * 8) * BLOCK);
     dma4(resource(a_scales + step, 0x7fffffff), scale_off, to + (BM + BN) * BLOCK + wave * 256);
   };
   typedef const __attribute__((address_space(4))) float const_float;   // (scalar loads: vector ones would be counted with those above)
-  const_float *const b_scale = (const_float *)(p.b_scales + int64_t(min(n0 + wn, p.n - 1) / BLOCK) * p.bs_s);
+  const_float *b_scale[SCALES];
+#pragma unroll
+  for (int u = 0; u < SCALES; u++) b_scale[u] = (const_float *)(p.b_scales + int64_t(min(n0 + wn + u * 16, p.n - 1) / BLOCK) * p.bs_s);
   auto fragment = [&](const uint8_t *row) {   // (rows of a fragment start at a multiple of 16)
     const uint8_t *const mine = row + li * BLOCK;
     const v4i lo = *(const v4i *)(mine + (lg ^ (li >> 1)) * 16), hi = *(const v4i *)(mine + ((lg + 4) ^ (li >> 1)) * 16);
@@ -64,7 +61,9 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
 #pragma unroll
   for (int i = 0; i < DEPTH - 1; i++)
     if (i < mine) fetch(i);
-  float sb = b_scale[min(my_group, steps - 1)];
+  float sb[SCALES];
+#pragma unroll
+  for (int u = 0; u < SCALES; u++) sb[u] = b_scale[u][min(my_group, steps - 1)];
   uint32_t slot = 0;
   for (int turn = 0; turn < turns; turn++) {
     if (turn + DEPTH - 1 <= mine) wait_for_all_but<(DEPTH - 2) * LOADS>();   // (DEPTH - 2 steps behind this one are under way)
@@ -73,7 +72,9 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
     asm volatile("" : : : "memory");
     if (turn + DEPTH - 1 < mine) fetch(turn + DEPTH - 1);   // (over the step before this one, which all waves are done with)
     if (GROUPS > 1 && turn >= mine) break;                  // (the last turn, and no barrier behind it in the loop)
-    const float next = b_scale[min((turn + 1) * GROUPS + my_group, steps - 1)];
+    float next[SCALES];
+#pragma unroll
+    for (int u = 0; u < SCALES; u++) next[u] = b_scale[u][min((turn + 1) * GROUPS + my_group, steps - 1)];
     const uint8_t *const from = ring + slot * SLOT;
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
     const float *const scales = (const float *)(from + (BM + BN) * BLOCK) + wm + li;
@@ -84,13 +85,14 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
     for (int t = 0; t < MT; t++) {
       Operand<OUT> x;
       x.from(fragment(from + (wm + t * 16) * BLOCK));
-      const float scale = scales[t * 16] * sb;
+      const float scale = scales[t * 16];
       v4f part[NT];
       products(part, w, x);
 #pragma unroll
-      for (int u = 0; u < NT; u++) acc[t][u] += part[u] * scale;
+      for (int u = 0; u < NT; u++) acc[t][u] += part[u] * (scale * sb[SCALES == 1 ? 0 : u]);
     }
-    sb = next;
+#pragma unroll
+    for (int u = 0; u < SCALES; u++) sb[u] = next[u];
   }
   if constexpr (GROUPS > 1) {
     // The groups' sums in their order.
@@ -133,11 +135,15 @@ template <class OUT>
 hipError_t choose(const ProductArgs &p, hipStream_t stream) {
   auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
   // The smallest tiles that the compute units take in one round, each with a workgroup of several groups; past a round of the largest, two workgroups of one to a unit.  us as 64 x 64
-  // in 3 groups, 128 x 64 in 2, 128 x 128 in 2 and in 1, bf16: 1024 x 1024 x 4096 (256 tiles of 64 x 64) 12.6, 18.4, 24.4, 28.0; 1024 x 1536 x 4096 22.4, 18.9, 24.5, 28.4;
-  // 1500 x 1500 x 2048 19.8, 19.2, 14.4, 16.3; 1500 x 3500 x 2048 (336 of 128 x 128) 37, 28, 26.8, 24.0; f32: 600 x 600 x 4096 14.7, 23.6, 32.6, 41.7; 1300 x 2600 x 2048 33.5, 26.6,
-  // 22.1, 26.3; 2048 x 4096 x 1024 43, 32.7, 26.6, 24.8.
+  // in 3 groups, 64 x 96, 128 x 64, 96 x 96, 128 x 96 and 128 x 128 in 2, and 128 x 128 in 1, bf16: 1024 x 1024 x 4096 (256 tiles of 64 x 64) 12.1, .., 18.4, .., .., 24.4, 28; 1024 x 1536 x 4096 22.4,
+  // 15.3, 17.7, 18.7, 21.9, 23.6, 27.2; 1500 x 1500 x 2048 19.8, 16.6, 18.7, 12.0, 13.5, 14.8, 16.9; 1300 x 2600 x 2048 .., 23.3, 18.7, 20.6, 23.4, 14.6, 16.3; f32: 1001 x 2050 x 4432 .., 47.9, 58, 35,
+  // 40, 44, 53; 1500 x 1500 x 2048 .., 22.6, 26.9, 16.2, 18.5, 20.7, 24.6; 1500 x 3500 x 2048 .., 42.6, 38.8, 41.5, 34.2, 38.4, 35.4.
   if (tiles(64, 64) <= g_compute_units) return launch<64, 64, 3, 3, OUT>(p, stream);
+  if (tiles(64, 96) <= g_compute_units) return launch<64, 96, 2, 3, OUT>(p, stream);
+  if (tiles(96, 64) <= g_compute_units) return launch<96, 64, 2, 3, OUT>(p, stream);
   if (tiles(128, 64) <= g_compute_units) return launch<128, 64, 2, 3, OUT>(p, stream);
+  if (tiles(96, 96) <= g_compute_units) return launch<96, 96, 2, 3, OUT>(p, stream);
+  if (tiles(128, 96) <= g_compute_units) return launch<128, 96, 2, 2, OUT>(p, stream);
   if (tiles(128, 128) <= g_compute_units) return launch<128, 128, 2, 2, OUT>(p, stream);
   return launch<128, 128, 1, 2, OUT>(p, stream);
 }

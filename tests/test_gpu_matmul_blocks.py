@@ -54,7 +54,9 @@ class Operands:
 SIZES = [(20, 400, 1168), (38, 6200, 512), (50, 6160, 400), (77, 6200, 640), (90, 6150, 384), (90, 800, 1536), (72, 1000, 2048), (40, 100, 3000 + 8), (111, 250, 1024), (16, 33, 16),
          (1, 1, 1), (1, 16, 128), (1, 4096, 2048), (2, 17, 129), (7, 1000, 4104), (16, 512, 512), (17, 100, 1000), (32, 64, 257), (33, 130, 384), (48, 1040, 2176),
          (64, 64, 64), (65, 300, 130), (100, 2048, 1024), (128, 128, 128), (129, 257, 640), (200, 520, 15), (300, 200, 1111), (513, 384, 2048), (1000, 1030, 1200), (257, 2000, 33),
-         (2049, 2050, 256), (600, 800, 1040), (768, 520, 128), (1025, 513, 2000)]
+         (2049, 2050, 256), (600, 800, 1040),
+         # tiles of 64 x 96, 96 x 64, 96 x 96 and 128 x 96, whole ones and ones that the sizes cut
+         (1024, 1536, 400), (200, 6100, 272), (1536, 1024, 256), (1500, 1020, 1040), (1500, 1500, 528), (1001, 2050, 657), (1536, 1536, 128), (1537, 2000, 384), (2001, 1501, 1300), (768, 520, 128), (1025, 513, 2000)]
 
 
 @pytest.mark.parametrize("out", ["bf16", "f32"])
