@@ -184,34 +184,42 @@ __global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p
   choose<CHOOSE_THREADS>(p, w, blockIdx.x, 1, by_experts, c);
   keep<CHOOSE_THREADS>(p, w, blockIdx.x, 1, c);
 }
-// Whether every workgroup of the next launch makes all choices for itself: up to 64 comparisons a thread.  (us of the layer in a graph, so and with a launch for them, 2048 x 512 and experts: 1 token 64 16.3
-// and 17.3, 128 20.6 and 21.4, 160 28.5 and 28.3; 4 tokens 32 22.0 and 23.4, 64 24.1 and 23.8; 8 tokens 32 27.1 and 27.7, 128 84.9 and 74.8; 32 tokens 16 26.9 and 24.7.  Outside of graphs a launch is some 4 more.)
-constexpr uint32_t MOST_FUSED_TOKENS = 8, MOST_FUSED = 384;   // (logits: the root of 2^17 at most)
-bool fused_choice(const ExpertsArgs &a) { return a.tokens <= MOST_FUSED_TOKENS && a.tokens * a.experts * a.experts <= 1u << 14; }
+// Whether every workgroup of the next launch makes all choices for itself: up to 128 comparisons a thread.  (us of the layer in a graph, so and with a launch for them, 2048 x 512, tokens and experts: 1 and 64 16.3
+// and 17.3, 1 and 128 20.6 and 21.4, 1 and 160 28.5 and 28.3, 1 and 512 49.8 and 38.1, 4 and 32 22.0 and 23.4, 4 and 64 24.1 and 23.8, 8 and 32 27.1 and 27.7, 8 and 128 84.9 and 74.8, 16 and 16 24.0 and 24.2,
+// 16 and 32 48.5 and 47.6, 32 and 8 20.5 and 20.7, 32 and 16 26.9 and 24.7.  Outside of graphs a launch is some 4 more.)
+constexpr uint32_t MOST_FUSED_TOKENS = 32, MOST_FUSED = 256;   // (logits, and so choices)
+bool fused_choice(const ExpertsArgs &a) { return a.tokens <= MOST_FUSED_TOKENS && a.tokens * a.experts <= MOST_FUSED && a.tokens * a.experts * a.experts <= 1u << 15; }
 
 // ---- Products with experts' weights: 16 rows of each of N matrices against the x of a part's tokens, a step of 128 bytes of the rows at a time.  Loads take a row's 128 bytes with eight
 // lanes, x's with eight or sixteen, and LDS brings both into the order in which the matrix instructions want them: what bounds such loops else is the rate at which a compute
 // unit's address unit takes cache lines, of which a load of 16 bytes of sixteen rows next to each other has four times as many. ----
-// ROOM: tokens that a part may have, 8 or 16.
-template <bool F8, int ROOM>
+// ROOM: tokens that a part may have, 8 or 16.  HOW a step fills an instruction: FULL as above; HALF: with eight rows, and nothing for the others; PAIRED, of parts of eight: eight rows and tokens, 256 bytes of the
+// rows, whose second 128 go where rows and tokens 8 to 15 would be: the instruction's sums of rows 0 to 7 with tokens 0 to 7, and of 8 to 15 with 8 to 15, are what is wanted.
+enum How { FULL = 0, HALF = 1, PAIRED = 2 };
+template <bool F8, int ROOM, int HOW>
 struct Shape {
-  static constexpr int STEP = F8 ? 128 : 64, SIZE = F8 ? 1 : 2;        // elements, bytes of one
-  static constexpr int X_BYTES = STEP * 2, X_CHUNKS = X_BYTES / 16;    // of a token's x
-  static constexpr int X_LOADS = ROOM * X_BYTES / 1024, X_TOKENS = 64 / X_CHUNKS;   // for all tokens; tokens of a load
+  static constexpr int PAIR = HOW == PAIRED ? 2 : 1, SIZE = F8 ? 1 : 2;                 // runs of 128 bytes of a row in a step; bytes of an element
+  static constexpr int STEP = (F8 ? 128 : 64) * PAIR, BYTES = 128 * PAIR;               // of a row in a step: elements, bytes
+  static constexpr int LANES = BYTES / 16, LOADS = HOW == HALF ? 1 : 2;                 // of a row in a load; loads for all rows
+  static constexpr int X_BYTES = STEP * 2, X_CHUNKS = X_BYTES / 16;                     // of a token's x
+  static constexpr int X_LOADS = ROOM * X_BYTES / 1024, X_TOKENS = 64 / X_CHUNKS;       // for all tokens; tokens of a load
+  static constexpr int IN_LDS = ROOM * PAIR, ROW_BYTES = X_BYTES / PAIR;                // tokens as the instruction has them, and of one of these
+  static constexpr int BOUNCE = IN_LDS * ROW_BYTES;
+  static_assert(HOW != PAIRED || ROOM == 8, "");
 };
 constexpr int TILE_BYTES = 16 * 128;   // of LDS of a wave for each matrix
-template <bool F8, int ROOM, int N>
+template <bool F8, int ROOM, int N, int HOW>
 struct Rows {
-  typedef Shape<F8, ROOM> S;
-  const uint8_t *row[N][2];       // of the lane: sixteen bytes of step 0 of row lane / 8, and of that row + 8 (of the last row, where there is none: its sums are not looked at)
-  const float *scale;             // of step 0: the first matrix's for the first half of the lanes, the last's for the others (a tile's rows are of one block of 128)
+  typedef Shape<F8, ROOM, HOW> S;
+  const uint8_t *row[N][S::LOADS];   // of the lane: sixteen bytes of step 0 of row lane / LANES, and of that row + 64 / LANES (of the last row, where there is none: its sums are not looked at)
+  const float *scale;             // of step 0: the first matrix's for the first half of the lanes, the last's for the others (a tile's rows are of one block of 128); PAIRED: all lanes the one's
   const uint16_t *x[S::X_LOADS];  // of the lane: eight elements of step 0 of token lane / X_CHUNKS, and of those X_TOKENS behind (of the last, where there is none)
   int x_loads;                    // that the part has tokens for
   __device__ inline void matrix(int n, const Stack &s, uint32_t expert, uint32_t row0, uint32_t height) {   // height: rows that there are from row0 on, up to sixteen
     const uint32_t lane = threadIdx.x & 63;
-    const uint8_t *const tile = s.w + (int64_t(expert) * s.w_e + int64_t(row0) * s.w_s) * S::SIZE + lane % 8 * 16;
+    const uint8_t *const tile = s.w + (int64_t(expert) * s.w_e + int64_t(row0) * s.w_s) * S::SIZE + lane % S::LANES * 16;
 #pragma unroll
-    for (int i = 0; i < 2; i++) row[n][i] = tile + int64_t(min(lane / 8 + i * 8, height - 1)) * (s.w_s * S::SIZE);
+    for (int i = 0; i < S::LOADS; i++) row[n][i] = tile + int64_t(min(lane / S::LANES + i * (64 / S::LANES), height - 1)) * (s.w_s * S::SIZE);
     if (F8 && (n == 0 || lane >= 32)) scale = s.scales + int64_t(expert) * s.scales_e + int64_t(row0 / BLOCK) * s.scales_s;
   }
   template <class F>
@@ -226,19 +234,20 @@ struct Rows {
 // the same loads, without branches; SHORT: rows of weights or of x below sixteen bytes, byte by byte.
 enum Tail { WHOLE = 0, INSIDE = 1, SHORT = 2 };
 // What a lane has of one step.
-template <bool F8, int ROOM, int N, int TAIL>
+template <bool F8, int ROOM, int N, int TAIL, int HOW>
 struct Step {
-  typedef Shape<F8, ROOM> S;
-  v4i q[N][2], y[S::X_LOADS];
+  typedef Shape<F8, ROOM, HOW> S;
+  v4i q[N][S::LOADS], y[S::X_LOADS];
   float scale;
   int x_loads;
   int left, x_left;   // INSIDE: bytes of a row from the lane's chunk on
-  // k: elements of a row; half: eight rows are enough.
-  __device__ inline void fetch(const Rows<F8, ROOM, N> &of, uint32_t s, int k, bool half) {
-    const int at = int(s) * 128, x_at = int(s) * S::STEP * 2;   // bytes
+  // k: elements of a row.
+  __device__ inline void fetch(const Rows<F8, ROOM, N, HOW> &of, uint32_t s, int k) {
+    const int at = int(s) * S::BYTES, x_at = int(s) * S::X_BYTES;   // bytes
     x_loads = of.x_loads;
-    if constexpr (F8) scale = of.scale[s];
-    const int chunk = at + int(threadIdx.x & 7) * 16, x_chunk = x_at + int(threadIdx.x) % S::X_CHUNKS * 16;   // the lane's
+    // (PAIRED: the first half of the lanes has the sums with the step's first block, the others those with its second; the row's last block again, where that is behind it)
+    if constexpr (F8) scale = of.scale[HOW == PAIRED ? min(int(s) * 2 + int(threadIdx.x >> 5 & 1), (k - 1) / int(BLOCK)) : int(s)];
+    const int chunk = at + int(threadIdx.x) % S::LANES * 16, x_chunk = x_at + int(threadIdx.x) % S::X_CHUNKS * 16;   // the lane's
     if constexpr (TAIL != SHORT) {
       int back = at, x_back = x_at;
       if constexpr (TAIL == INSIDE) {
@@ -246,11 +255,9 @@ struct Step {
         back += min(left - 16, 0), x_back += min(x_left - 16, 0);
       }
 #pragma unroll
-      for (int n = 0; n < N; n++) q[n][0] = chunk_at(of.row[n][0] + back);
-      if (!half) {
+      for (int i = 0; i < S::LOADS; i++)
 #pragma unroll
-        for (int n = 0; n < N; n++) q[n][1] = chunk_at(of.row[n][1] + back);
-      }
+        for (int n = 0; n < N; n++) q[n][i] = chunk_at(of.row[n][i] + back);
 #pragma unroll
       for (int i = 0; i < S::X_LOADS; i++)
         if (i < x_loads) y[i] = chunk_at((const uint8_t *)of.x[i] + x_back);
@@ -258,13 +265,13 @@ struct Step {
 #pragma unroll
       for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) q[n][i] = chunk_up_to(of.row[n][i] + at, k * S::SIZE - chunk, chunk);
+        for (int i = 0; i < S::LOADS; i++) q[n][i] = chunk_up_to(of.row[n][i] + at, k * S::SIZE - chunk, chunk);
 #pragma unroll
       for (int i = 0; i < S::X_LOADS; i++)
         if (i < x_loads) y[i] = chunk_up_to((const uint8_t *)of.x[i] + x_at, k * 2 - x_chunk, x_chunk);
     }
   }
-  // bounce: LDS of this wave's, N tiles and x of ROOM tokens.  Chunk c of a row of 128 bytes at c ^ (row / 2 % 8), of 256 bytes at c ^ row: sixteen lanes with a
+  // bounce: LDS of this wave's, N tiles and x of IN_LDS tokens.  Chunk c of a row of 128 bytes at c ^ (row / 2 % 8), of 256 bytes at c ^ row: sixteen lanes with a
   // chunk of sixteen rows each reach every bank once.
   __device__ inline void multiply(v4f (&acc)[N], uint8_t *bounce) {
     const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
@@ -272,25 +279,31 @@ struct Step {
 #pragma unroll
       for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) q[n][i] = last_of_row(q[n][i], left);
+        for (int i = 0; i < S::LOADS; i++) q[n][i] = last_of_row(q[n][i], left);
 #pragma unroll
       for (int i = 0; i < S::X_LOADS; i++) y[i] = last_of_row(y[i], x_left);
+      if (F8 && HOW == PAIRED && left + int(lane % S::LANES) * 16 <= int(lane / 32) * 128) scale = 0;   // (no such block; the last one's may be infinite)
     }
     uint8_t *const of_x = bounce + N * TILE_BYTES;
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
-      for (int i = 0; i < 2; i++) *(v4i *)(bounce + n * TILE_BYTES + i * 1024 + lane / 8 * 128 + (lane % 8 ^ lane / 16 ^ i * 4) * 16) = q[n][i];
+      for (int i = 0; i < S::LOADS; i++) {
+        const uint32_t row = lane / S::LANES + i * (64 / S::LANES) + lane % S::LANES / 8 * 8;
+        *(v4i *)(bounce + n * TILE_BYTES + row * 128 + (lane % 8 ^ (row / 2 & 7)) * 16) = q[n][i];
+      }
 #pragma unroll
     for (int i = 0; i < S::X_LOADS; i++)
       if (i < x_loads) {
-        const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS;
-        *(v4i *)(of_x + token * S::X_BYTES + (lane % S::X_CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[i];
+        constexpr uint32_t CHUNKS = S::ROW_BYTES / 16;
+        const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS + lane % S::X_CHUNKS / CHUNKS * 8;
+        *(v4i *)(of_x + token * S::ROW_BYTES + (lane % CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[i];
       }
-    const uint32_t mine = li & (ROOM - 1);
-    const uint8_t *const my_x = of_x + mine * S::X_BYTES;
+    const uint32_t mine = li & (S::IN_LDS - 1);
+    const uint8_t *const my_x = of_x + mine * S::ROW_BYTES;
     float scales[2] = {0, 0};
-    if constexpr (F8) scales[0] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))), scales[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32));
+    if constexpr (F8 && HOW == PAIRED) scales[0] = scale;
+    else if constexpr (F8) scales[0] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))), scales[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32));
     if constexpr (F8) {
       v4i u[2][2];
 #pragma unroll
@@ -408,12 +421,12 @@ constexpr int UP_WAVES = 4;
 template <bool F8, int ROOM, bool FUSED, int TAIL>
 __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles, FastDiv by_experts) {
   constexpr int AHEAD = 3;
-  typedef Shape<F8, ROOM> S;
+  typedef Shape<F8, ROOM, FULL> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   __shared__ v4f sums[2][UP_WAVES][2][64];
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t rows = live_rows(p), all = rows * p.top_k;
-  constexpr uint32_t BOUNCE = 2 * TILE_BYTES + ROOM * S::X_BYTES;
+  constexpr uint32_t BOUNCE = 2 * TILE_BYTES + S::BOUNCE;
   uint8_t *const bounce = dynamic + wave * BOUNCE;
   const Lists lists(dynamic + UP_WAVES * BOUNCE, p.experts, p.tokens * p.top_k, words, ROOM, UP_WAVES);
   const int32_t *chosen = w.chosen;
@@ -425,8 +438,8 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
   }
   const uint32_t tiles = (p.inter + 15) / 16, line = tiles * __builtin_amdgcn_readfirstlane(list<UP_WAVES * 64>(lists, p, chosen, all, words, ROOM));
   const uint32_t steps = (p.hidden + S::STEP - 1) / S::STEP, s0 = steps * wave / UP_WAVES, n = steps * (wave + 1) / UP_WAVES - s0;   // this wave's steps of each tile
-  Rows<F8, ROOM, 2> of;
-  Step<F8, ROOM, 2, TAIL> t[AHEAD] = {};
+  Rows<F8, ROOM, 2, FULL> of;
+  Step<F8, ROOM, 2, TAIL, FULL> t[AHEAD] = {};
   auto go_to = [&](uint32_t tile) {
     const uint32_t part = by_tiles.div(tile), row0 = (tile - part * tiles) * 16, height = min(16u, p.inter - row0);
     const Part q = lists.parts[part];
@@ -438,7 +451,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
     go_to(blockIdx.x);
 #pragma unroll
     for (int a = 0; a < AHEAD; a++)
-      if (uint32_t(a) < n) t[a].fetch(of, s0 + a, int(p.hidden), false);
+      if (uint32_t(a) < n) t[a].fetch(of, s0 + a, int(p.hidden));
   }
   uint32_t turn = 0;
   for (uint32_t tile = blockIdx.x; tile < line; tile += gridDim.x, turn ^= 1) {
@@ -450,7 +463,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
       for (int a = 0; a < AHEAD; a++) {
         if (at + a < n) t[a].multiply(acc, bounce);
         const uint32_t next = last ? uint32_t(a) : at + a + AHEAD;
-        if (next < n && (!last || more)) t[a].fetch(of, s0 + next, int(p.hidden), false);
+        if (next < n && (!last || more)) t[a].fetch(of, s0 + next, int(p.hidden));
       }
     }
     v4f(&here)[UP_WAVES][2][64] = sums[turn];
@@ -469,20 +482,23 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
   }
 }
 
-// ---- Down: blockIdx.x: `height` rows, 8 or 16; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to eight steps of a part, of which a wave has every
-// WAVES-th: a workgroup's waves go through the same rows together. ----
-template <bool F8, int ROOM, int TAIL, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t height, uint32_t tokens_here, uint32_t words) {
-  constexpr int AHEAD = WAVES == 8 ? 6 : F8 ? ROOM == 16 ? 2 : 3 : 4, THREADS = WAVES * 64;
-  typedef Shape<F8, ROOM> S;
+// ---- Down: blockIdx.x: 16 rows, or 8; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to 1024 bytes of a part's rows, of which a wave has every
+// eighth: a workgroup's waves go through the same rows together.  (Eight rows PAIRED against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 112;
+// 8 of 1024 through 64 40.2 and 42.  Sixteen waves: 194 and 196 in bf16, 110 and 106 in e4m3.) ----
+constexpr int DOWN_WAVES = 8;
+template <bool F8, int ROOM, int TAIL, int HOW>
+__global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t tokens_here, uint32_t words) {
+  constexpr int WAVES = DOWN_WAVES, THREADS = WAVES * 64, AHEAD = HOW == PAIRED ? 4 : 6;   // (PAIRED: of twice the bytes)
+  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
+  typedef Shape<F8, ROOM, HOW> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
   float *const shares = (float *)(sums + WAVES * tokens_here * 4);   // [tokens_here * top_k]
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr uint32_t BOUNCE = TILE_BYTES + ROOM * S::X_BYTES;
+  constexpr uint32_t BOUNCE = TILE_BYTES + S::BOUNCE;
   uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * BOUNCE;
   const Lists lists(bounces + WAVES * BOUNCE, p.experts, tokens_here * p.top_k, words, ROOM, WAVES);
-  const uint32_t row0 = blockIdx.x * height, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(height, p.hidden - row0);
+  const uint32_t row0 = blockIdx.x * HEIGHT, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(HEIGHT, p.hidden - row0);
   if (t0 >= rows) return;
   const uint32_t here = min(tokens_here, rows - t0);
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
@@ -490,16 +506,16 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, ROOM));
   // Pieces of eight steps, or fewer where a seventh of the waves' last turn would be idle.
   const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP;
-  uint32_t size = 8, of_part, pieces;
+  uint32_t size = 8 / S::PAIR, of_part, pieces;
   for (;; size /= 2) {
     of_part = (steps + size - 1) / size, pieces = parts * of_part;
     if (size == 1 || pieces * 7 >= (pieces + WAVES - 1) / WAVES * WAVES * 6) break;
   }
   // The piece to fetch from, and the one to multiply.
   uint32_t fetch_piece = wave, fetch_s = 0, fetch_end = 0, piece = wave, s = 0, end = 0;
-  Rows<F8, ROOM, 1> of;
-  Step<F8, ROOM, 1, TAIL> t[AHEAD] = {};
-  auto fetch = [&](Step<F8, ROOM, 1, TAIL> &to) {
+  Rows<F8, ROOM, 1, HOW> of;
+  Step<F8, ROOM, 1, TAIL, HOW> t[AHEAD] = {};
+  auto fetch = [&](Step<F8, ROOM, 1, TAIL, HOW> &to) {
     if (fetch_s == fetch_end) {
       const uint32_t part = fetch_piece / of_part;
       const Part q = lists.parts[part];
@@ -507,7 +523,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
       of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
       of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + i]) * w.h_s; });
     }
-    to.fetch(of, fetch_s, int(p.inter), height <= 8);
+    to.fetch(of, fetch_s, int(p.inter));
     if (++fetch_s == fetch_end) fetch_piece += WAVES;
   };
   v4f acc[1] = {};
@@ -526,8 +542,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
       if (fetch_piece < pieces) fetch(t[a]);
       if (++s == end) {
         const Part q = lists.parts[piece / of_part];
-        if (li < q.count) {
-          const uint32_t choice = lists.choices[q.first + li];
+        const uint32_t i = HOW == PAIRED ? li - lg / 2 * 8 : li;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
+        if (i < q.count) {
+          const uint32_t choice = lists.choices[q.first + i];
           sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
         }
         acc[0] = v4f{0, 0, 0, 0};
@@ -538,9 +555,13 @@ __global__ __launch_bounds__(WAVES * 64) void k_experts_down(ExpertsArgs p, Plac
   __syncthreads();
   for (uint32_t i = tid; i < here * 4; i += THREADS) {
     v4f sum = sums[i];
+    const uint32_t row = i % 4 * 4;
 #pragma unroll
     for (uint32_t v = 1; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i];
-    const uint32_t row = i % 4 * 4;
+    if (HOW == PAIRED && row < 8) {
+#pragma unroll
+      for (uint32_t v = 0; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i + 2];
+    }
     if (row < rows_here) store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
   }
 }
@@ -551,8 +572,8 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   // 180, 32 tokens 110 and 112, 16 through 8 of 4096 x 14336 254 and 253.)
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
   const uint32_t grid = uint32_t(std::min<uint64_t>(uint64_t(most_parts(a.experts, choices, ROOM)) * tiles, 2 * g_compute_units));
-  static_assert(!FUSED || MOST_FUSED * 12 + MOST_FUSED_TOKENS * (8 + MOST_CHOSEN * 8) <= UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES), "");
-  const size_t lds = UP_WAVES * (2 * TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
+  static_assert(!FUSED || MOST_FUSED * 20 + MOST_FUSED_TOKENS * 8 <= UP_WAVES * (2 * TILE_BYTES + Shape<F8, ROOM, FULL>::BOUNCE), "");
+  const size_t lds = UP_WAVES * (2 * TILE_BYTES + Shape<F8, ROOM, FULL>::BOUNCE) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
     const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, TAIL>), 96 * 1024);
@@ -562,49 +583,48 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   return plan::last_error();
 }
 constexpr size_t MOST_LDS = 160 * 1024;
-template <bool F8, int ROOM, int TAIL, int WAVES>
+template <bool F8, int ROOM, int HOW>
 size_t down_lds(const ExpertsArgs &a, uint32_t here) {
-  return size_t(WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + WAVES * (TILE_BYTES + ROOM * Shape<F8, ROOM>::X_BYTES) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, ROOM, WAVES);
+  return size_t(DOWN_WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + DOWN_WAVES * (TILE_BYTES + Shape<F8, ROOM, HOW>::BOUNCE) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, ROOM, DOWN_WAVES);
 }
-template <bool F8, int ROOM, int TAIL, int WAVES>
-hipError_t launch_down_waves(const ExpertsArgs &a, const Places &w, uint32_t height, hipStream_t stream) {
+template <bool F8, int ROOM, int TAIL, int HOW>
+hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
   uint32_t here = a.tokens;   // of a workgroup: all, or as many as its sums have place for
-  while (down_lds<F8, ROOM, TAIL, WAVES>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
+  while (down_lds<F8, ROOM, HOW>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, WAVES>), MOST_LDS);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, HOW>), MOST_LDS);
     if (e != hipSuccess) return e;
   }
-  const size_t lds = down_lds<F8, ROOM, TAIL, WAVES>(a, here);
-  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, WAVES>), dim3((a.hidden + height - 1) / height, (a.tokens + here - 1) / here), dim3(WAVES * 64), lds, stream, a, w, height, here, (here + 31) / 32);
+  const size_t lds = down_lds<F8, ROOM, HOW>(a, here);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
   return plan::last_error();
-}
-template <bool F8, int ROOM, int TAIL>
-hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  // Eight rows where sixteen would leave half of the compute units without any.  (us of the layer, 8 and 16, in bf16 through 64 experts of 768, 8 chosen: 32 tokens of 2048 124.7 and 133.1, 8 of 1024 65.5 and 68.1,
-  // 8 of 2880 123.9 and 116.7, 1 of 5120 54.0 and 50.9; in e4m3 32 of 2048 76 and 81, 8 of 2880 88 and 71.)
-  const uint32_t height = a.hidden <= 8 * g_compute_units ? 8 : 16;
-  // A workgroup of sixteen waves to each unit where one is enough and its tokens are few enough for deep lookahead, else several of eight.  (us, 16 and 8 waves, 128 experts of 2048 x 768, 8 chosen, in bf16: 1 token 26.2 and 28.2,
-  // 32 204 and 221, 64 237 and 256, 128 323 and 276; in e4m3 64 132 and 147, 128 232 and 157, in parts of sixteen 64 tokens through 32 experts 61 and 55.)
-  if constexpr (TAIL != SHORT && !(F8 && ROOM == 16)) {
-    if (a.hidden <= height * g_compute_units && a.tokens <= 64) return launch_down_waves<F8, ROOM, TAIL, 16>(a, w, height, stream);
-  }
-  return launch_down_waves<F8, ROOM, TAIL, 8>(a, w, height, stream);
 }
 // How rows of k elements end.
 template <bool F8>
-Tail tail_of(uint32_t k) { return k * (F8 ? 1 : 2) < 16 || k * 2 < 16 ? SHORT : k % (F8 ? 128 : 64) ? INSIDE : WHOLE; }
+Tail tail_of(uint32_t k, uint32_t step = F8 ? 128 : 64) { return k * (F8 ? 1 : 2) < 16 || k * 2 < 16 ? SHORT : k % step ? INSIDE : WHOLE; }
+template <bool F8, int ROOM, int HOW>
+hipError_t launch_down_how(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  const Tail tail = tail_of<F8>(a.inter, Shape<F8, ROOM, HOW>::STEP);
+  return tail == WHOLE ? launch_down<F8, ROOM, WHOLE, HOW>(a, w, stream) : tail == INSIDE ? launch_down<F8, ROOM, INSIDE, HOW>(a, w, stream) : launch_down<F8, ROOM, SHORT, HOW>(a, w, stream);
+}
 template <bool F8, int ROOM, bool FUSED>
 hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   const double weight = 3.0 * a.inter * a.hidden * (F8 ? 1 : 2) * std::min(a.experts, a.tokens * a.top_k);
-  const Tail up = tail_of<F8>(a.hidden), down = tail_of<F8>(a.inter);
+  const Tail up = tail_of<F8>(a.hidden);
   plan::work(plan::UNIT_STREAM, 0, weight * 2 / 3);
   const hipError_t e = up == WHOLE    ? launch_up<F8, ROOM, FUSED, WHOLE>(a, w, stream)
                        : up == INSIDE ? launch_up<F8, ROOM, FUSED, INSIDE>(a, w, stream)
                                       : launch_up<F8, ROOM, FUSED, SHORT>(a, w, stream);
   if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  return down == WHOLE ? launch_down<F8, ROOM, WHOLE>(a, w, stream) : down == INSIDE ? launch_down<F8, ROOM, INSIDE>(a, w, stream) : launch_down<F8, ROOM, SHORT>(a, w, stream);
+  // Eight rows where these leave the compute unit with the most of them fewer; in parts of sixteen, where half of each instruction is lost on them, where sixteen would leave half of the units without any.
+  // (us of the layer, 8 and 16, in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; of 2880 275 and 270, 161 and 148; of 5120 475 and 498, 262 and 267; of 6144 548 and 568, 297 and 301;
+  // in parts of sixteen 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024 in e4m3 283 and 259.)
+  auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
+  const bool eight = ROOM == 8 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units;
+  return eight ? launch_down_how<F8, ROOM, ROOM == 8 ? PAIRED : HALF>(a, w, stream) : launch_down_how<F8, ROOM, FULL>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {

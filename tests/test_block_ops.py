@@ -115,7 +115,7 @@ def test_which_kernel_a_product_takes(m, n, k, out, strides, kernel, copied):
 
 
 @pytest.mark.parametrize("tokens,hidden,experts_,top_k,launches", [
-    (1, 2048, 128, 8, 3), (1, 2048, 129, 8, 4), (8, 2048, 45, 8, 3), (8, 2048, 46, 8, 4), (9, 2048, 8, 2, 4), (256, 2048, 512, 32, 4)])
+    (1, 2048, 181, 8, 3), (1, 2048, 182, 8, 4), (8, 2048, 32, 8, 3), (8, 2048, 33, 8, 4), (32, 2048, 8, 1, 3), (33, 2048, 7, 1, 4), (32, 2048, 8, 2, 4), (256, 2048, 512, 32, 4)])
 def test_which_kernels_a_layer_of_experts_takes(tokens, hidden, experts_, top_k, launches):
     for dtype in (M.bf16, M.f8e4m3):
         families = [s.family for s in M.Experts(dtype, tokens, hidden, 768, experts_, top_k).plan().steps]

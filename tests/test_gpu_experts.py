@@ -13,7 +13,7 @@ SIZES = [(1, 256, 128, 8, 2), (1, 1, 1, 1, 1), (1, 2048, 256, 64, 8), (2, 512, 1
          # logits of all tokens below, at and past the threads that choose; the last that one workgroup chooses for all, and one more
          (5, 264, 72, 60, 4), (2, 128, 64, 127, 5), (2, 128, 64, 128, 5), (3, 128, 64, 104, 7), (16, 136, 40, 45, 3), (32, 64, 48, 32, 4), (31, 64, 48, 32, 16), (33, 64, 48, 31, 4), (1, 64, 48, 181, 32),
          # the largest of whose choices every workgroup makes all, and those behind them
-         (8, 72, 40, 45, 32), (8, 72, 40, 46, 32), (4, 136, 64, 64, 6), (1, 136, 64, 128, 32), (1, 136, 64, 129, 32), (9, 64, 48, 8, 2),
+         (8, 72, 40, 32, 32), (8, 72, 40, 33, 32), (4, 136, 64, 64, 6), (1, 136, 64, 181, 32), (1, 136, 64, 182, 32), (32, 64, 48, 8, 2), (28, 64, 48, 9, 2), (29, 64, 48, 9, 2),
          # sixteen waves for the products with down, and one token more
          (64, 300, 136, 128, 8), (65, 300, 136, 128, 8), (64, 2050, 64, 40, 3), (64, 264, 128, 300, 32), (33, 4096, 48, 6, 2), (40, 4100, 48, 64, 2)]
 
@@ -68,6 +68,17 @@ def test_a_row_that_is_not_a_number(gpu):
     want, bound, which, _ = layer.want()
     others = np.arange(6) != 2
     assert np.array_equal(chosen[others], which[others]) and (np.abs(as_f64("bf16", out) - want) <= bound)[others].all()
+
+
+@pytest.mark.parametrize("hidden,inter", [(64, 300), (64, 129), (2050, 300), (64, 384)])
+def test_an_unbounded_scale_of_the_last_block(gpu, hidden, inter):
+    """Is that block's alone: with all else positive every element of the result is infinite, not NaN from what would lie behind it."""
+    layer = Layer("e4m3", 3, hidden, inter, 4, 1, seed=9)
+    layer.x &= 0x7fff
+    for name in ("gate", "up", "down"):
+        layer.stored[name] = layer.stored[name] & 0x3f | 0x20   # 2^-3 to 1.875
+    layer.scales["down"][:, :, -1] = np.inf
+    assert np.isposinf(as_f64("bf16", layer.run()[0])).all()
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
