@@ -20,13 +20,20 @@ struct Places {
   double *logits;       // [tokens][experts]
   int32_t *chosen;      // [tokens][top_k]
   float *shares;        // [tokens][top_k]
-  uint16_t *h;          // [tokens * top_k][h_s]
+  uint16_t *h;          // [tokens * top_k][in_two ? 2 : 1][h_s]: rounded to bf16, and what that left, rounded
   uint32_t h_s;
+  bool in_two;
 };
+// What is between the products in one bf16 number adds as much to a result's error as rounding that does, and on few numbers by chance half as much again.  In two it adds nothing; that is free for few tokens, and where it is small (us of
+// the layer, in one and in two: 1 token through 64 experts of 2048 x 1024 31.1 and 31.0, 8 of 1024 x 768 in e4m3 40.3 and 40.9, 32 through 128 of 2048 x 768 107 and 113, 16 through 8 of 4096 x 14336 in bf16 475 and 513).
+bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 15; }
+// Many tokens of each expert go in parts of sixteen, others in parts of eight, or four of what is in two.
+bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
+
 size_t places(const ExpertsArgs &a, Places *to) {
   Places w = {};
   const size_t choices = size_t(a.tokens) * a.top_k;
-  w.h_s = (a.inter + 63) / 64 * 64;
+  w.h_s = (a.inter + 63) / 64 * 64, w.in_two = few_of_each(a) && kept_in_two(a);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t *p = a.workspace ? a.workspace + at : nullptr;
@@ -36,7 +43,7 @@ size_t places(const ExpertsArgs &a, Places *to) {
   w.logits = (double *)take(sizeof(double) * a.tokens * a.experts);
   w.chosen = (int32_t *)take(4 * choices);
   w.shares = (float *)take(4 * choices);
-  w.h = (uint16_t *)take(2 * choices * w.h_s);
+  w.h = (uint16_t *)take((w.in_two ? 4 : 2) * choices * w.h_s);
   if (to) *to = w;
   return at;
 }
@@ -477,7 +484,19 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
       for (int i = 0; i < 4; i++) h[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
       const uint32_t part = by_tiles.div(tile), row = (tile - part * tiles) * 16 + lg * 4;
       const Part q = lists.parts[part];
-      if (li < q.count && row < p.inter) store4(w.h + uint64_t(lists.choices[q.first + li]) * w.h_s + row, h, int(p.inter - row));
+      if (li < q.count && row < p.inter) {
+        uint16_t *const to = w.h + (uint64_t(lists.choices[q.first + li]) << (w.in_two ? 1 : 0)) * w.h_s + row;
+        store4(to, h, int(p.inter - row));
+        if (w.in_two) {
+          v4f rest;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float r = h[i] - float((__bf16)h[i]);
+            rest[i] = fabsf(r) < __builtin_inff() ? r : 0.0f;
+          }
+          store4(to + w.h_s, rest, int(p.inter - row));
+        }
+      }
     }
   }
 }
@@ -486,10 +505,10 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
 // eighth: a workgroup's waves go through the same rows together.  (Eight rows PAIRED against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 112;
 // 8 of 1024 through 64 40.2 and 42.  Sixteen waves: 194 and 196 in bf16, 110 and 106 in e4m3.) ----
 constexpr int DOWN_WAVES = 8;
-template <bool F8, int ROOM, int TAIL, int HOW>
+template <bool F8, int ROOM, int TAIL, int HOW, bool IN_TWO>
 __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t tokens_here, uint32_t words) {
   constexpr int WAVES = DOWN_WAVES, THREADS = WAVES * 64, AHEAD = HOW == PAIRED ? 4 : 6;   // (PAIRED: of twice the bytes)
-  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
+  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8, EACH = IN_TWO ? 2 : 1, MOST = ROOM / EACH;   // (IN_TWO: a token's two next to each other, as two tokens)
   typedef Shape<F8, ROOM, HOW> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
@@ -497,13 +516,13 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   constexpr uint32_t BOUNCE = TILE_BYTES + S::BOUNCE;
   uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * BOUNCE;
-  const Lists lists(bounces + WAVES * BOUNCE, p.experts, tokens_here * p.top_k, words, ROOM, WAVES);
+  const Lists lists(bounces + WAVES * BOUNCE, p.experts, tokens_here * p.top_k, words, MOST, WAVES);
   const uint32_t row0 = blockIdx.x * HEIGHT, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(HEIGHT, p.hidden - row0);
   if (t0 >= rows) return;
   const uint32_t here = min(tokens_here, rows - t0);
   for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
   for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
-  const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, ROOM));
+  const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, MOST));
   // Pieces of eight steps, or fewer where a seventh of the waves' last turn would be idle.
   const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP;
   uint32_t size = 8 / S::PAIR, of_part, pieces;
@@ -521,7 +540,7 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       const Part q = lists.parts[part];
       fetch_s = (fetch_piece - part * of_part) * size, fetch_end = min(steps, fetch_s + size);
       of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
-      of.tokens(__builtin_amdgcn_readfirstlane(q.count), [&](uint32_t i) { return w.h + uint64_t(t0 * p.top_k + lists.choices[q.first + i]) * w.h_s; });
+      of.tokens(__builtin_amdgcn_readfirstlane(q.count) * EACH, [&](uint32_t i) { return w.h + (uint64_t(t0 * p.top_k + lists.choices[q.first + i / EACH]) * EACH + i % EACH) * w.h_s; });
     }
     to.fetch(of, fetch_s, int(p.inter));
     if (++fetch_s == fetch_end) fetch_piece += WAVES;
@@ -542,7 +561,15 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       if (fetch_piece < pieces) fetch(t[a]);
       if (++s == end) {
         const Part q = lists.parts[piece / of_part];
-        const uint32_t i = HOW == PAIRED ? li - lg / 2 * 8 : li;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
+        uint32_t i = HOW == PAIRED ? li - lg / 2 * 8 : li;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
+        if constexpr (IN_TWO) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {   // (and the next lane's, but where that is infinity times nothing)
+            const float x = acc[0][e], rest = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));
+            acc[0][e] = fabsf(x) < __builtin_inff() ? x + rest : x;
+          }
+          i = i % 2 ? ~0u : i / 2;
+        }
         if (i < q.count) {
           const uint32_t choice = lists.choices[q.first + i];
           sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
@@ -583,31 +610,33 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   return plan::last_error();
 }
 constexpr size_t MOST_LDS = 160 * 1024;
-template <bool F8, int ROOM, int HOW>
+template <bool F8, int ROOM, int HOW, bool IN_TWO>
 size_t down_lds(const ExpertsArgs &a, uint32_t here) {
-  return size_t(DOWN_WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + DOWN_WAVES * (TILE_BYTES + Shape<F8, ROOM, HOW>::BOUNCE) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, ROOM, DOWN_WAVES);
+  return size_t(DOWN_WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + DOWN_WAVES * (TILE_BYTES + Shape<F8, ROOM, HOW>::BOUNCE) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, IN_TWO ? ROOM / 2 : ROOM, DOWN_WAVES);
 }
-template <bool F8, int ROOM, int TAIL, int HOW>
+template <bool F8, int ROOM, int TAIL, int HOW, bool IN_TWO>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
   uint32_t here = a.tokens;   // of a workgroup: all, or as many as its sums have place for
-  while (down_lds<F8, ROOM, HOW>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
+  while (down_lds<F8, ROOM, HOW, IN_TWO>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, HOW>), MOST_LDS);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), MOST_LDS);
     if (e != hipSuccess) return e;
   }
-  const size_t lds = down_lds<F8, ROOM, HOW>(a, here);
-  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
+  const size_t lds = down_lds<F8, ROOM, HOW, IN_TWO>(a, here);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
   return plan::last_error();
 }
 // How rows of k elements end.
 template <bool F8>
 Tail tail_of(uint32_t k, uint32_t step = F8 ? 128 : 64) { return k * (F8 ? 1 : 2) < 16 || k * 2 < 16 ? SHORT : k % step ? INSIDE : WHOLE; }
-template <bool F8, int ROOM, int HOW>
+template <bool F8, int ROOM, int HOW, bool IN_TWO>
 hipError_t launch_down_how(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   const Tail tail = tail_of<F8>(a.inter, Shape<F8, ROOM, HOW>::STEP);
-  return tail == WHOLE ? launch_down<F8, ROOM, WHOLE, HOW>(a, w, stream) : tail == INSIDE ? launch_down<F8, ROOM, INSIDE, HOW>(a, w, stream) : launch_down<F8, ROOM, SHORT, HOW>(a, w, stream);
+  return tail == WHOLE    ? launch_down<F8, ROOM, WHOLE, HOW, IN_TWO>(a, w, stream)
+         : tail == INSIDE ? launch_down<F8, ROOM, INSIDE, HOW, IN_TWO>(a, w, stream)
+                          : launch_down<F8, ROOM, SHORT, HOW, IN_TWO>(a, w, stream);
 }
 template <bool F8, int ROOM, bool FUSED>
 hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
@@ -624,7 +653,11 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t st
   // in parts of sixteen 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024 in e4m3 283 and 259.)
   auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
   const bool eight = ROOM == 8 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units;
-  return eight ? launch_down_how<F8, ROOM, ROOM == 8 ? PAIRED : HALF>(a, w, stream) : launch_down_how<F8, ROOM, FULL>(a, w, stream);
+  constexpr int EIGHT = ROOM == 8 ? PAIRED : HALF;
+  if constexpr (ROOM == 8) {
+    if (w.in_two) return eight ? launch_down_how<F8, ROOM, EIGHT, true>(a, w, stream) : launch_down_how<F8, ROOM, FULL, true>(a, w, stream);
+  }
+  return eight ? launch_down_how<F8, ROOM, EIGHT, false>(a, w, stream) : launch_down_how<F8, ROOM, FULL, false>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
@@ -632,7 +665,7 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   // (a token to a workgroup while these still run side by side: the layer takes 31.5 us so and 32.3 with four for 1 token and 512 experts, 33 and 33 for 16 and 128, 202 and 185 for 200 and 256)
   if (a.experts * a.tokens <= 8 * g_compute_units) MRL_LAUNCH(k_experts_logits<1>, dim3(a.experts, a.tokens), dim3(ROUTER_THREADS), 0, stream, a, w);
   else MRL_LAUNCH(k_experts_logits<4>, dim3(a.experts, (a.tokens + 3) / 4), dim3(ROUTER_THREADS), 0, stream, a, w);
-  const bool few = !(a.tokens > 8 && a.tokens * a.top_k >= 6 * a.experts), fused = few && fused_choice(a);
+  const bool few = few_of_each(a), fused = few && fused_choice(a);
   if (!fused) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), Choice::bytes(a.experts, a.top_k, 1), stream, a, w, FastDiv(a.experts));

@@ -131,9 +131,9 @@ class Layer:
         shares = np.take_along_axis(p, order, 1)
         return order, shares / shares.sum(1, keepdims=True) if self.renormalise else shares
 
-    def want(self, rows=None):
+    def want(self, rows=None, h_step=2.0 ** -8):
         """(out, bound, chosen, shares).  A sum of n products is off by at most 2 n u times the sum of their sizes (in any order, with a share of it
-        for blocks and pieces); silu's derivative is at most 1.1 and its own steps good to 8 u; h is rounded to bf16; shares are good to 1e-6."""
+        for blocks and pieces); silu's derivative is at most 1.1 and its own steps good to 8 u; h is rounded by h_step: bf16's, or 2^-16 for two such numbers; shares are good to 1e-6."""
         rows = self.tokens if rows is None else rows
         chosen, shares = self.choice()
         out, bound = np.zeros((rows, self.hidden)), np.zeros((rows, self.hidden))
@@ -146,7 +146,7 @@ class Layer:
                 eg, eu = n * (np.abs(gate) @ np.abs(x)), n * (np.abs(up) @ np.abs(x))
                 silu = g / (1 + np.exp(-g))
                 h = silu * u
-                eh = 1.1 * eg * (np.abs(u) + eu) + np.abs(silu) * eu + (8 * U + 2.0 ** -8) * (np.abs(h) + 1.1 * eg * np.abs(u) + np.abs(silu) * eu)
+                eh = 1.1 * eg * (np.abs(u) + eu) + np.abs(silu) * eu + (8 * U + h_step) * (np.abs(h) + 1.1 * eg * np.abs(u) + np.abs(silu) * eu)
                 out[t] += share * (down @ h)
                 bound[t] += share * (np.abs(down) @ eh + (2 * (self.inter + 64) * U + 2e-6) * (np.abs(down) @ (np.abs(h) + eh)))
         half = HALF_STEP["bf16"]

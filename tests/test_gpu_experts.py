@@ -26,6 +26,31 @@ def test_layer(gpu, kind, tokens, hidden, inter, experts, top_k):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", [(1, 256, 300, 8, 1), (4, 512, 2100, 16, 4), (3, 2100, 640, 6, 2), (16, 128, 64, 32, 2), (40, 72, 100, 5, 1), (200, 2064, 40, 1, 1), (64, 128, 255, 90, 2)])
+def test_small_layers_round_once(gpu, kind, tokens, hidden, inter, experts, top_k):
+    """What is between the products in sixteen bits."""
+    layer = Layer(kind, tokens, hidden, inter, experts, top_k, seed=21)
+    want, bound, _, _ = layer.want(h_step=2.0 ** -16)
+    assert (np.abs(as_f64("bf16", layer.run()[0]) - want) <= bound).all()
+
+
+def test_results_without_bounds(gpu):
+    """What is past bf16 between the products, and infinite weights: infinite, not NaN, in one number and in two."""
+    for tokens, inter in ((2, 64), (40, 1024)):
+        layer = Layer("bf16", tokens, 64, inter, 4, 1, seed=22)
+        layer.x &= 0x7fff
+        for name in ("gate", "up", "down"):
+            layer.stored[name] &= 0x7fff
+        layer.stored["up"][:, 3] = 0x7f00   # 1.7e38
+        layer.stored["down"][:, 7, 5] = 0x7f80
+        layer.x[:] = np.maximum(layer.x, 0x4000)   # (2 and more: 64 such products past 3.4e38)
+        assert np.isposinf(as_f64("bf16", layer.run()[0])).all()
+        layer.stored["up"][:, 3] = 0
+        out = as_f64("bf16", layer.run()[0])
+        assert np.isposinf(out[:, 7]).all() and np.isfinite(np.delete(out, 7, 1)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("rows", [-3, 0, 1, 7, 20, 99])
 def test_rows_that_count(gpu, kind, rows):
     layer = Layer(kind, 20, 256, 128, 8, 2, seed=3)
