@@ -26,7 +26,7 @@ struct Places {
 };
 // What is between the products in one bf16 number adds as much to a result's error as rounding that does, and on few numbers by chance half as much again.  In two it adds nothing; that is free for few tokens, and where it is small (us of
 // the layer, in one and in two: 1 token through 64 experts of 2048 x 1024 31.1 and 31.0, 8 of 1024 x 768 in e4m3 40.3 and 40.9, 32 through 128 of 2048 x 768 107 and 113, 16 through 8 of 4096 x 14336 in bf16 475 and 513).
-bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 15; }
+bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 14; }
 // Many tokens of each expert go in parts of sixteen, others in parts of eight, or four of what is in two.
 bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
 
