@@ -4,6 +4,7 @@
 // of all these rows, and a's scales, go straight from memory into a ring of DEPTH blocks in LDS that is the wave's own, so that no wave waits for another
 // before the end, and what is under way is bounded by LDS and not by registers.  Eight lanes take a row's 128 bytes: sixteen cycles for an instruction's KiB, where the order in
 // which the matrix instructions want them (a lane of sixteen different rows next to each other) would take 64.
+// 8 x 4096 x 4096 5.1 us (17 MB; 5.8 with cold caches), 96 x 8192 x 8192 20.5 us (68 MB, 3.3 TB/s), 67 x 6144 x 4096 8.2 us: of a workgroup's 460 KB there 330 are a, which every one of them reads from L2.
 #include "matmul_blocks.h"
 
 namespace mrl {

@@ -3,7 +3,8 @@
 //
 // Four waves, 2 x 2, or GROUPS of four, each of which has every GROUPS-th block of K: one wave on a SIMD takes some 800 cycles from the barrier over reads from LDS, products and
 // sums to the next, of which the products are 128 (64 x 64) to 512, and groups fill them.  A block of all the tile's rows, and a's scales, go straight from memory into a
-// ring of DEPTH blocks in LDS that is the group's.
+// ring of DEPTH blocks in LDS that is the group's.  (1024 x 2048 x 4096 18.4 us, 0.93 PFLOP/s.)  Results in f32 pay for bf16: four matrix instructions of 16 cycles for one of 32, and sixteen conversions of each
+// sixteen rows for each wave that multiplies them: 1024 x 4096 x 4480 43 us, 0.87 PFLOP/s.
 #include "matmul_blocks.h"
 
 namespace mrl {
