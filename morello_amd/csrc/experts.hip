@@ -5,7 +5,7 @@
 // instructions take them: 16 rows of weights against up to 16 of the expert's tokens, 128 bytes of each row at a time, a lane 32 of them.
 // Each of the steps needs all of the one before, a launch each: logits; choice (with few tokens and experts every workgroup of the next launch makes it for itself);
 // gate and up to h, 16 rows of one expert at a time; down, a workgroup to some rows of all experts, so that a token's sum over
-// its experts is formed in one place and in one order.  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 475 (2.8 GB, 5.9 TB/s: up 309, down 154); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 105 (528 MB, 5.0 TB/s:
+// its experts is formed in one place and in one order (several workgroups to fewer rows than there are compute units for, and a launch that adds up what they have).  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 475 (2.8 GB, 5.9 TB/s: up 309, down 154); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 105 (528 MB, 5.0 TB/s:
 // logits and choice 5 each, up 59, down 34); 1 token, 8 of 64 of 2048 x 1024 in bf16 27 (101 MB: 3, 15, 9; each launch begins with 3 to 4 of reading what the one before left).  A choice is known by its number i = token * top_k + j; no lists go through memory but the chosen experts.
 #include <algorithm>
 
@@ -24,6 +24,9 @@ struct Places {
   uint16_t *h;          // [tokens * top_k][in_two ? 2 : 1][h_s]: rounded to bf16, and what that left, rounded
   uint32_t h_s;
   bool in_two;
+  uint32_t down_shares; // workgroups that share some rows of down; of more than one, what each has
+  float *sums;          // [down_shares][tokens][hidden_s]
+  uint32_t hidden_s;
 };
 // What is between the products in one bf16 number adds as much to a result's error as rounding that does, and on few numbers by chance half as much again.  In two it adds nothing; that is free for few tokens, and where it is small (us of
 // the layer, in one and in two: 1 token through 64 experts of 2048 x 1024 31.1 and 31.0, 8 of 1024 x 768 in e4m3 40.3 and 40.9, 32 through 128 of 2048 x 768 107 and 113, 16 through 8 of 4096 x 14336 in bf16 475 and 513).
@@ -31,6 +34,21 @@ bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.toke
 // Many tokens of each expert go in parts of sixteen, others in parts of eight, or four of what is in two.
 bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
 
+// Rows of down to a workgroup: eight where these leave the compute unit with the most of them fewer; in parts of sixteen, where half of each instruction is lost on them, where sixteen would leave half of the units without any.
+// (us of the layer, 8 and 16, in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; of 2880 275 and 270, 161 and 148; of 5120 475 and 498, 262 and 267; of 6144 548 and 568, 297 and 301;
+// in parts of sixteen 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024 in e4m3 283 and 259.)
+uint32_t rows_of_down(const ExpertsArgs &a) {
+  auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
+  return (few_of_each(a) ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units) ? 8 : 16;
+}
+// Workgroups that share some rows of down: as many as find a compute unit, with 48 steps of 2 KiB and more to each.  (us of the layer, one and as many: 94 tokens, 2 of 8 experts of 384 x 11652 in bf16 214 and 98, 1 token,
+// 8 of 64 of 384 x 9600 in e4m3 50 and 37, 109 tokens, 4 of 16 of 896 x 640 in bf16 47 and 38, 32 tokens, 8 of 128 of 1024 x 768 in e4m3 75 and 67; with less, 4 tokens, 4 of 64 of 1024 x 512 in bf16, 23.4 and 24.5.)
+uint32_t shares_of_down(const ExpertsArgs &a) {
+  const uint32_t height = rows_of_down(a), groups = (a.hidden + height - 1) / height, choices = a.tokens * a.top_k;
+  const uint32_t parts = std::max(std::min(a.experts, choices), choices / (few_of_each(a) ? 8 : 16));   // about
+  const uint64_t steps = uint64_t(parts) * ((uint64_t(a.inter) * (a.weight_dtype == MRL_BF16 ? 2 : 1) * height + 2047) / 2048);
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(g_compute_units / groups, steps / 48)));
+}
 size_t places(const ExpertsArgs &a, Places *to) {
   Places w = {};
   const size_t choices = size_t(a.tokens) * a.top_k;
@@ -44,6 +62,8 @@ size_t places(const ExpertsArgs &a, Places *to) {
   w.logits = (double *)take(sizeof(double) * a.tokens * a.experts);
   w.chosen = (int32_t *)take(4 * choices);
   w.shares = (float *)take(4 * choices);
+  w.down_shares = shares_of_down(a), w.hidden_s = (a.hidden + 3) / 4 * 4;
+  if (w.down_shares > 1) w.sums = (float *)take(sizeof(float) * w.down_shares * a.tokens * w.hidden_s);
   w.h = (uint16_t *)take((w.in_two ? 4 : 2) * choices * w.h_s);
   if (to) *to = w;
   return at;
@@ -526,13 +546,14 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
   const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, MOST));
   // Pieces of eight steps, or fewer where a seventh of the waves' last turn would be idle.
   const uint32_t steps = (p.inter + S::STEP - 1) / S::STEP;
+  const uint32_t all_waves = WAVES * gridDim.z, first = wave + blockIdx.z * WAVES;
   uint32_t size = 8 / S::PAIR, of_part, pieces;
   for (;; size /= 2) {
     of_part = (steps + size - 1) / size, pieces = parts * of_part;
-    if (size == 1 || pieces * 7 >= (pieces + WAVES - 1) / WAVES * WAVES * 6) break;
+    if (size == 1 || pieces * 7 >= (pieces + all_waves - 1) / all_waves * all_waves * 6) break;
   }
   // The piece to fetch from, and the one to multiply.
-  uint32_t fetch_piece = wave, fetch_s = 0, fetch_end = 0, piece = wave, s = 0, end = 0;
+  uint32_t fetch_piece = first, fetch_s = 0, fetch_end = 0, piece = first, s = 0, end = 0;
   Rows<F8, ROOM, 1, HOW> of;
   Step<F8, ROOM, 1, TAIL, HOW> t[AHEAD] = {};
   auto fetch = [&](Step<F8, ROOM, 1, TAIL, HOW> &to) {
@@ -544,7 +565,7 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       of.tokens(__builtin_amdgcn_readfirstlane(q.count) * EACH, [&](uint32_t i) { return w.h + (uint64_t(t0 * p.top_k + lists.choices[q.first + i / EACH]) * EACH + i % EACH) * w.h_s; });
     }
     to.fetch(of, fetch_s, int(p.inter));
-    if (++fetch_s == fetch_end) fetch_piece += WAVES;
+    if (++fetch_s == fetch_end) fetch_piece += all_waves;
   };
   v4f acc[1] = {};
 #pragma unroll
@@ -576,7 +597,7 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
           sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
         }
         acc[0] = v4f{0, 0, 0, 0};
-        piece += WAVES;
+        piece += all_waves;
       }
     }
   }
@@ -590,8 +611,21 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
 #pragma unroll
       for (uint32_t v = 0; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i + 2];
     }
-    if (row < rows_here) store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
+    if (row >= rows_here) continue;
+    if (gridDim.z > 1) *(v4f *)(w.sums + (uint64_t(blockIdx.z) * p.tokens + t0 + i / 4) * w.hidden_s + row0 + row) = sum;   // (hidden_s: whole fours)
+    else store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
   }
+}
+
+// What several workgroups have of the same rows, in their order.
+constexpr int JOIN_THREADS = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void k_experts_join(ExpertsArgs p, Places w) {
+  const uint32_t at = (blockIdx.x * JOIN_THREADS + threadIdx.x) * 4, token = blockIdx.y;
+  if (at >= p.hidden || token >= live_rows(p)) return;
+  const float *const from = w.sums + uint64_t(token) * w.hidden_s + at;
+  v4f sum = *(const v4f *)from;
+  for (uint32_t z = 1; z < w.down_shares; z++) sum += *(const v4f *)(from + uint64_t(z) * p.tokens * w.hidden_s);
+  store4(p.out + int64_t(token) * p.out_s + at, sum, int(p.hidden - at));
 }
 
 template <bool F8, int ROOM, bool FUSED, int TAIL>
@@ -626,7 +660,11 @@ hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream
     if (e != hipSuccess) return e;
   }
   const size_t lds = down_lds<F8, ROOM, HOW, IN_TWO>(a, here);
-  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here, w.down_shares), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
+  if (w.down_shares > 1) {
+    plan::work(plan::UNIT_STREAM, 0, (4.0 * w.down_shares + 2) * a.tokens * a.hidden);
+    MRL_LAUNCH(k_experts_join, dim3((a.hidden + JOIN_THREADS * 4 - 1) / (JOIN_THREADS * 4), a.tokens), dim3(JOIN_THREADS), 0, stream, a, w);
+  }
   return plan::last_error();
 }
 // How rows of k elements end.
@@ -649,11 +687,7 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t st
                                       : launch_up<F8, ROOM, FUSED, SHORT>(a, w, stream);
   if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  // Eight rows where these leave the compute unit with the most of them fewer; in parts of sixteen, where half of each instruction is lost on them, where sixteen would leave half of the units without any.
-  // (us of the layer, 8 and 16, in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; of 2880 275 and 270, 161 and 148; of 5120 475 and 498, 262 and 267; of 6144 548 and 568, 297 and 301;
-  // in parts of sixteen 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024 in e4m3 283 and 259.)
-  auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
-  const bool eight = ROOM == 8 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units;
+  const bool eight = rows_of_down(a) == 8;
   constexpr int EIGHT = ROOM == 8 ? PAIRED : HALF;
   if constexpr (ROOM == 8) {
     if (w.in_two) return eight ? launch_down_how<F8, ROOM, EIGHT, true>(a, w, stream) : launch_down_how<F8, ROOM, FULL, true>(a, w, stream);

@@ -122,6 +122,13 @@ def test_which_kernels_a_layer_of_experts_takes(tokens, hidden, experts_, top_k,
         assert families == ["k_experts_logits"] + ["k_experts_choose"] * (launches == 4) + ["k_experts_up", "k_experts_down"]
 
 
+@pytest.mark.parametrize("hidden,inter,joined", [(1024, 2048, True), (1024, 512, False), (2048, 1 << 15, False), (1032, 1 << 15, False), (384, 9600, True)])
+def test_few_rows_of_down_are_shared(hidden, inter, joined):
+    op = M.Experts(M.bf16, 1, hidden, inter, 64, 8)
+    assert ([s.family for s in op.plan().steps][-1] == "k_experts_join") == joined
+    assert (op.workspace_bytes() >= 2 * hidden * 4) or not joined
+
+
 def test_the_oracle_of_the_casts():
     """Every byte is its own nearest; between two numbers the nearer, halfway the even byte; a block reads back within half a step."""
     codes = np.array([c for c in range(256) if c & 127 != 127])
