@@ -787,8 +787,9 @@ int mrl_cast_blocks_plan(const mrl_cast_blocks *op, mrl_plan *plan, mrl_plan_ste
  *   2  b         e4m3 [n][k]
  *   3  b scales  f32 [ceil(n / 128)][ceil(k / 128)]
  *   4  out       [m][n]  (Out)
- *   5  workspace mrl_matmul_blocks_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's: 0 where a's and b's rows lie 16 bytes apart or a multiple of that and k is one, and for the
- *                smallest products; else room for copies of a, b or both whose rows do, which every call makes anew.  (Weights whose rows do are read where they lie.) */
+ *   5  workspace mrl_matmul_blocks_workspace_bytes() bytes, under the terms of mrl_run_paged_attention's: may be NULL where that is 0.  It holds
+ *                what workgroups that share K have of the sums, and copies of a, b or both where k or their strides are no multiple of 16, which every call makes anew (but for one or two rows and small
+ *                products): weights are better kept so that they are one. */
 typedef struct {
   int32_t out_dtype;   /* MRL_BF16 or MRL_F32 */
   uint32_t m, n, k;    /* each up to 2^23, m * n up to 2^40 */

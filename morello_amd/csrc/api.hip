@@ -1834,7 +1834,7 @@ uint32_t mrl_target_kernels(const char **names, uint32_t cap) {
       "k_softmax_generic", "k_softmax_cols_short", "k_parts", "k_parts_block", "k_parts_rows", "k_parts_cols", "k_broadcast", "k_broadcast_rows", "k_broadcast_fill_rows", "k_fill", "k_fill16", "k_fill_zero", "k_move_rows", "k_move_runs",
       "k_move_tiled", "k_move_tiled_as", "k_move_tiled8v", "k_move_tiled16", "k_move_tiled16v", "k_move_tiled32", "k_move_gather", "k_move_generic", "k_relayout", "k_convert4", "k_copy1",
       "k_copy16", "k_pad_rows", "k_pad_rows_pair", "k_widen_bf16", "k_page_tables", "k_rotary", "k_paged_attn", "k_paged_attn_merge", "k_paged_attn_generic",
-      "k_cast_rows", "k_cast_squares", "k_product_wide", "k_product_tile", "k_product_tile_any", "k_product_few", "k_product_few_any", "k_experts_logits", "k_experts_choose", "k_experts_up", "k_experts_down", "k_experts_join"};
+      "k_cast_rows", "k_cast_squares", "k_product_wide", "k_product_tile", "k_product_tile_any", "k_product_few", "k_product_join", "k_product_few_any", "k_experts_logits", "k_experts_choose", "k_experts_up", "k_experts_down", "k_experts_join"};
   const uint32_t n = sizeof families / sizeof families[0];
   for (uint32_t i = 0; i < n && i < cap && names; i++) names[i] = families[i];
   return n;

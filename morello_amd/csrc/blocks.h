@@ -22,7 +22,8 @@ struct ProductArgs {
   const float *a_scales, *b_scales;
   void *out;
   uint8_t *workspace;
-  uint32_t m, n, k;
+  float *parts;         // [shares][m][parts_s], where several workgroups share K
+  uint32_t m, n, k, shares, parts_s;
   int out_dtype;
   int64_t a_s, as_s, b_s, bs_s, out_s;   // strides of a row in elements (of a row of blocks for b's scales)
 };

@@ -1,5 +1,7 @@
 // What the kernels of products of blocks share (matmul_blocks.hip, matmul_blocks_wide.hip).
 #pragma once
+#include <algorithm>
+
 #include "blocks_device.h"
 
 namespace mrl {
@@ -104,6 +106,13 @@ __device__ inline void store_sums(uint8_t *lds, const v4f (&acc)[MT][NT], const 
   }
 }
 
+// This workgroup's part, where several share K.
+__device__ inline ProductArgs part_of(const ProductArgs &p) {
+  ProductArgs q = p;
+  q.out = p.parts + uint64_t(blockIdx.y) * p.m * p.parts_s, q.out_s = p.parts_s;
+  return q;
+}
+
 }  // namespace blocks
 
 hipError_t launch_product_wide(const ProductArgs &p, hipStream_t stream);
@@ -111,5 +120,7 @@ hipError_t launch_product_tile(const ProductArgs &p, hipStream_t stream);
 // Rows of whole chunks, scales of a within 2 GB.  (us, so and on tiles: 80 x 8192 x 8192 19.4 and 20.4, 96 x 4096 x 4096 10.4 and 11.8, 128 x 8192 x 8192 41.8 and 21.3, 128 x 4096 x 4096 13.4 and 12.0.)
 constexpr uint32_t MOST_FEW = 96;
 hipError_t launch_product_few(const ProductArgs &p, hipStream_t stream);
+// Workgroups that share the K of a tile; of more than one, sums go to parts.
+uint32_t shares_of_tiles(const ProductArgs &p);
 
 }  // namespace mrl

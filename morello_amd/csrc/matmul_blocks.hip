@@ -132,11 +132,33 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few_any(ProductArgs p) {
   }
 }
 
+// What several workgroups have of the same sums, in their order.
+template <class OUT>
+__global__ __launch_bounds__(TILE_THREADS) void k_product_join(ProductArgs p, FastDiv by_fours) {
+  const uint32_t at = blockIdx.x * TILE_THREADS + threadIdx.x, row = by_fours.div(at), col = (at - row * (p.parts_s / 4)) * 4;
+  if (row >= p.m) return;
+  const float *const from = p.parts + uint64_t(row) * p.parts_s + col;
+  v4f sum = *(const v4f *)from;
+  for (uint32_t z = 1; z < p.shares; z++) sum += *(const v4f *)(from + uint64_t(z) * p.m * p.parts_s);
+  store4((OUT *)p.out + int64_t(row) * p.out_s + col, sum, int(p.n - col));
+}
+template <class OUT>
+hipError_t launch_join(const ProductArgs &p, hipStream_t stream) {
+  const uint32_t fours = p.parts_s / 4;
+  plan::work(plan::UNIT_STREAM, 0, double(p.m) * p.n * (4.0 * p.shares + sizeof(OUT)));
+  MRL_LAUNCH(k_product_join<OUT>, dim3((p.m * fours + TILE_THREADS - 1) / TILE_THREADS), dim3(TILE_THREADS), 0, stream, p, FastDiv(fours));
+  return plan::last_error();
+}
+
 template <class OUT>
 hipError_t launch(const ProductArgs &p, hipStream_t stream) {
   plan::work(plan::UNIT_MFMA_I8, 2.0 * p.m * double(p.n) * p.k, (double(p.m) + p.n) * p.k + double(p.m) * p.n * sizeof(OUT), 0, 0, sizeof(OUT) == 2 ? 1.4 : 0.7);
   if (rows_of_chunks(p.a, p.a_s, p.k) && rows_of_chunks(p.b, p.b_s, p.k) && p.as_s < (1 << 21)) {
     if (p.m <= MOST_FEW) return launch_product_few(p, stream);
+    if (p.shares > 1) {
+      const hipError_t e = launch_product_tile(p, stream);
+      return e == hipSuccess ? launch_join<OUT>(p, stream) : e;
+    }
     // Tiles of 256 x 256 where the last of their rounds over the compute units is not too empty.  us, so and on the smaller ones: 2048 x 4096 x 4096 (128 tiles) 61 and 51, 2048 x 6144 x 2048
     // (192) 38.3 and 46, 4096 x 4096 x 1024 (256) 25.9 and 32.3.
     const uint64_t wide = uint64_t((p.m + 255) / 256) * ((p.n + 255) / 256), rounds = (wide + g_compute_units - 1) / g_compute_units;
@@ -179,14 +201,22 @@ PadRows rows_of(const void *from, uint32_t rows, uint32_t k, int64_t stride, voi
 
 }  // namespace
 
+// Workgroups that share K, by sizes and strides alone.
+uint32_t shares(const ProductArgs &p, const Copies &c) {
+  const bool a = c.a || (p.k % 16 == 0 && p.a_s % 16 == 0), b = c.b || (p.k % 16 == 0 && p.b_s % 16 == 0);
+  return p.m > MOST_FEW && a && b ? shares_of_tiles(p) : 1;
+}
+
 size_t product_workspace_bytes(const ProductArgs &p) {
   const Copies c = copies(p);
-  return c.a_bytes + c.b_bytes;
+  const uint32_t z = shares(p, c);
+  return c.a_bytes + c.b_bytes + (z > 1 ? sizeof(float) * z * p.m * ((p.n + 3) / 4 * 4) : 0);
 }
 
 hipError_t launch_product(const ProductArgs &given, hipStream_t stream) {
   ProductArgs p = given;
   const Copies c = copies(p);
+  p.shares = shares(p, c), p.parts = (float *)(p.workspace + c.a_bytes + c.b_bytes), p.parts_s = (p.n + 3) / 4 * 4;
   // (an operand that keeps its rows has to have them at such addresses, too)
   auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if ((c.a || c.b) && (c.a || aligned(p.a)) && (c.b || aligned(p.b))) {

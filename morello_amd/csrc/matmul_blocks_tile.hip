@@ -11,7 +11,7 @@ namespace mrl {
 namespace {
 using namespace blocks;
 
-template <int BM, int BN, int GROUPS, int DEPTH, class OUT>
+template <int BM, int BN, int GROUPS, int DEPTH, bool SHARED, class OUT>
 __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, uint32_t tiles_m, uint32_t tiles_n, uint32_t high) {
   constexpr int MT = BM / 32, NT = BN / 32, A_LOADS = BM / 32, B_LOADS = BN / 32, LOADS = A_LOADS + B_LOADS + 1;   // a wave's, a step
   constexpr int SLOT = (BM + BN) * int(BLOCK) + 4 * 256;   // (a's scales: 256 bytes from each wave, BM of them what is wanted)
@@ -24,7 +24,8 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
   const uint32_t at = xcd_run(blockIdx.x, gridDim.x), group = at / (high * tiles_n), here = min(high, tiles_m - group * high), in_group = at - group * high * tiles_n;
   const uint32_t tile_n = in_group / here, tile_m = group * high + in_group - tile_n * here;
   const uint32_t m0 = tile_m * BM, n0 = tile_n * BN, wm = wave / 2 * (BM / 2), wn = wave % 2 * (BN / 2);
-  const int steps = int((p.k + BLOCK - 1) / BLOCK), turns = (steps + GROUPS - 1) / GROUPS, mine = steps > my_group ? (steps - my_group + GROUPS - 1) / GROUPS : 0;   // mine: turns or one less
+  const int steps = int((p.k + BLOCK - 1) / BLOCK), all_groups = SHARED ? GROUPS * int(gridDim.y) : GROUPS;
+  const int first = SHARED ? int(blockIdx.y) * GROUPS + my_group : my_group, turns = (steps + all_groups - 1) / all_groups, mine = steps > first ? (steps - first + all_groups - 1) / all_groups : 0;   // mine: turns or one less
   // This wave's loads of a step: every fourth eight rows of a and of b, from the wave-th on.  Chunk c of a row at c ^ (row / 2 % 8) of its 128 bytes.
   const uint32_t row0 = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ (row0 >> 1 & 7), a_s = uint32_t(p.a_s), b_s = uint32_t(p.b_s);
   const uint32_t a_off = row0 * a_s + chunk * 16, b_off = row0 * b_s + chunk * 16;
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
   const uint32_t lds0 = lds_address(ring);
   uint32_t slot_in = 0;   // where the next step goes
   auto fetch = [&](int turn) {
-    const int step = turn * GROUPS + my_group;
+    const int step = turn * all_groups + first;
     const bool none = step == steps - 1 && chunk * 16 >= left_in_last;
     // (up to the last row's end: rows behind it bring zeros, or where rows overlap something, which nobody sees)
     const uint32_t left = p.k - step * BLOCK;
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
     if (i < mine) fetch(i);
   float sb[SCALES];
 #pragma unroll
-  for (int u = 0; u < SCALES; u++) sb[u] = b_scale[u][min(my_group, steps - 1)];
+  for (int u = 0; u < SCALES; u++) sb[u] = b_scale[u][min(first, steps - 1)];
   uint32_t slot = 0;
   for (int turn = 0; turn < turns; turn++) {
     if (turn + DEPTH - 1 <= mine) wait_for_all_but<(DEPTH - 2) * LOADS>();   // (DEPTH - 2 steps behind this one are under way)
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
     if (GROUPS > 1 && turn >= mine) break;                  // (the last turn, and no barrier behind it in the loop)
     float next[SCALES];
 #pragma unroll
-    for (int u = 0; u < SCALES; u++) next[u] = b_scale[u][min((turn + 1) * GROUPS + my_group, steps - 1)];
+    for (int u = 0; u < SCALES; u++) next[u] = b_scale[u][min((turn + 1) * all_groups + first, steps - 1)];
     const uint8_t *const from = ring + slot * SLOT;
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
     const float *const scales = (const float *)(from + (BM + BN) * BLOCK) + wm + li;
@@ -116,25 +117,27 @@ __global__ __launch_bounds__(GROUPS * 256) void k_product_tile(ProductArgs p, ui
   }
   if constexpr (GROUPS == 1) __syncthreads();   // (all waves have read their operands)
   else wait_for_lds();                          // (the sums of the others are in; each wave's lie where its own have been)
-  store_sums<MT, NT, OUT>(lds + wave * (MT * NT * 1024), acc, p, m0 + wm, n0 + wn);
+  if constexpr (SHARED) store_sums<MT, NT, float>(lds + wave * (MT * NT * 1024), acc, part_of(p), m0 + wm, n0 + wn);
+  else store_sums<MT, NT, OUT>(lds + wave * (MT * NT * 1024), acc, p, m0 + wm, n0 + wn);
 }
 
-template <int BM, int BN, int GROUPS, int DEPTH, class OUT>
+template <int BM, int BN, int GROUPS, int DEPTH, class OUT, bool SHARED = false>
 hipError_t launch(const ProductArgs &p, hipStream_t stream) {
   constexpr int BYTES = GROUPS * DEPTH * ((BM + BN) * int(BLOCK) + 4 * 256);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_product_tile<BM, BN, GROUPS, DEPTH, OUT>), BYTES);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_product_tile<BM, BN, GROUPS, DEPTH, SHARED, OUT>), BYTES);
     if (e != hipSuccess) return e;
   }
   const uint32_t tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
-  MRL_LAUNCH((k_product_tile<BM, BN, GROUPS, DEPTH, OUT>), dim3(tiles_m * tiles_n), dim3(GROUPS * 256), BYTES, stream, p, tiles_m, tiles_n, 512u / BM);
+  MRL_LAUNCH((k_product_tile<BM, BN, GROUPS, DEPTH, SHARED, OUT>), dim3(tiles_m * tiles_n, SHARED ? p.shares : 1), dim3(GROUPS * 256), BYTES, stream, p, tiles_m, tiles_n, 512u / BM);
   return plan::last_error();
 }
 
 template <class OUT>
 hipError_t choose(const ProductArgs &p, hipStream_t stream) {
   auto tiles = [&](uint32_t bm, uint32_t bn) { return uint64_t((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
+  if (p.shares > 1) return launch<64, 64, 3, 3, OUT, true>(p, stream);
   // The smallest tiles that the compute units take in one round, each with a workgroup of several groups; past a round of the largest, two workgroups of one to a unit.  us as 64 x 64
   // in 3 groups, 64 x 96, 128 x 64, 96 x 96, 128 x 96 and 128 x 128 in 2, and 128 x 128 in 1, bf16: 1024 x 1024 x 4096 (256 tiles of 64 x 64) 12.1, .., 18.4, .., .., 24.4, 28; 1024 x 1536 x 4096 22.4,
   // 15.3, 17.7, 18.7, 21.9, 23.6, 27.2; 1500 x 1500 x 2048 19.8, 16.6, 18.7, 12.0, 13.5, 14.8, 16.9; 1300 x 2600 x 2048 .., 23.3, 18.7, 20.6, 23.4, 14.6, 16.3; f32: 1001 x 2050 x 4432 .., 47.9, 58, 35,
@@ -150,6 +153,13 @@ hipError_t choose(const ProductArgs &p, hipStream_t stream) {
 }
 
 }  // namespace
+
+// As many as find a compute unit, of tiles that leave half of them without one, with four blocks and more to each group of waves.  (us, one and as many: 129 x 512 x 4992 12.0 and 9.2, 256 x 1024 x 8192 19.5 and 11.6,
+// 600 x 600 x 4096 in f32 15.5 and 13.2, 128 x 4096 x 4096 11.9 and 11.3; with two blocks 128 x 1024 x 2048 6.8 and 7.6.)
+uint32_t shares_of_tiles(const ProductArgs &p) {
+  const uint64_t tiles = uint64_t((p.m + 63) / 64) * ((p.n + 63) / 64);
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(g_compute_units / tiles, (p.k + BLOCK - 1) / BLOCK / 12)));
+}
 
 hipError_t launch_product_tile(const ProductArgs &p, hipStream_t stream) { return p.out_dtype == MRL_BF16 ? choose<uint16_t>(p, stream) : choose<float>(p, stream); }
 

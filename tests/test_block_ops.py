@@ -100,7 +100,7 @@ ODD = dict(a_stride=4097)
 
 
 @pytest.mark.parametrize("m,n,k,out,strides,kernel,copied", [
-    (1, 4096, 4096, M.bf16, {}, "k_product_few", 0), (96, 4096, 4096, M.f32, {}, "k_product_few", 0), (97, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
+    (1, 4096, 4096, M.bf16, {}, "k_product_few", 0), (96, 4096, 4096, M.f32, {}, "k_product_few", 0), (97, 8192, 4096, M.bf16, {}, "k_product_tile", 0),
     (4096, 4096, 4096, M.bf16, {}, "k_product_wide", 0), (4096, 4096, 4096, M.f32, {}, "k_product_tile", 0), (2048, 4096, 4096, M.bf16, {}, "k_product_tile", 0),
     (2048, 6144, 4096, M.bf16, {}, "k_product_wide", 0), (16, 100, 4095, M.bf16, {}, "k_product_few_any", 0), (17, 100, 4095, M.bf16, {}, "k_product_few", 117 * 4096),
     (2, 4000, 4095, M.f32, {}, "k_product_few_any", 0), (3, 4000, 4095, M.f32, {}, "k_product_few", 4003 * 4096),
@@ -112,6 +112,14 @@ def test_which_kernel_a_product_takes(m, n, k, out, strides, kernel, copied):
     assert op.workspace_bytes() == copied
     steps = op.plan().steps
     assert [s.family for s in steps][-1] == kernel and len(steps) == 1 + (copied > 0)
+
+
+@pytest.mark.parametrize("m,n,k,strides,shares,copied", [
+    (97, 4096, 4096, {}, 2, 0), (97, 4097, 4096, {}, 1, 0), (128, 512, 1535, {}, 1, 640 * 1536), (128, 512, 3200, {}, 2, 0), (129, 510, 4992, {}, 3, 0), (200, 130, 8192, dict(a_stride=8193), 5, 200 * 8192), (96, 512, 8192, {}, 1, 0)])
+def test_few_tiles_share_k(m, n, k, strides, shares, copied):
+    op = M.MatmulBlocks(M.f32, m, n, k, **strides)
+    assert op.workspace_bytes() == copied + (shares * m * (-(-n // 4) * 4) * 4 if shares > 1 else 0)
+    assert [s.family for s in op.plan().steps][copied > 0:] == (["k_product_tile", "k_product_join"] if shares > 1 else ["k_product_tile"] if m > 96 else ["k_product_few"])
 
 
 @pytest.mark.parametrize("tokens,hidden,experts_,top_k,launches", [

@@ -56,7 +56,9 @@ SIZES = [(20, 400, 1168), (38, 6200, 512), (50, 6160, 400), (77, 6200, 640), (90
          (64, 64, 64), (65, 300, 130), (100, 2048, 1024), (128, 128, 128), (129, 257, 640), (200, 520, 15), (300, 200, 1111), (513, 384, 2048), (1000, 1030, 1200), (257, 2000, 33),
          (2049, 2050, 256), (600, 800, 1040),
          # tiles of 64 x 96, 96 x 64, 96 x 96 and 128 x 96, whole ones and ones that the sizes cut
-         (1024, 1536, 400), (200, 6100, 272), (1536, 1024, 256), (1500, 1020, 1040), (1500, 1500, 528), (1001, 2050, 657), (1536, 1536, 128), (1537, 2000, 384), (2001, 1501, 1300), (768, 520, 128), (1025, 513, 2000)]
+         (1024, 1536, 400), (200, 6100, 272), (1536, 1024, 256), (1500, 1020, 1040), (1500, 1500, 528), (1001, 2050, 657), (1536, 1536, 128), (1537, 2000, 384), (2001, 1501, 1300),
+         # workgroups that share K
+         (97, 64, 3201), (129, 512, 3104), (130, 515, 4900), (200, 130, 8208), (600, 600, 3088), (97, 4096, 3090), (768, 520, 128), (1025, 513, 2000)]
 
 
 @pytest.mark.parametrize("out", ["bf16", "f32"])
@@ -80,6 +82,14 @@ def test_strides_and_odd_addresses(gpu, m, n, k):
                dict(a_stride=up, b_stride=k + 5, offset=8)):
         x.check(x.run("bf16", **kw), "bf16")
         x.check(x.run("f32", **kw), "f32")
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_strides_where_workgroups_share_k(gpu, out):
+    x = Operands(150, 130, 4000, 12, narrow=True)
+    for kw in (dict(a_stride=4032, b_stride=4048, a_scale_stride=33, b_scale_stride=40, out_stride=138), dict(a_stride=4003, b_stride=4001, offset=1, out_stride=131), dict(a_stride=4032, b_stride=4005),
+               dict(a_stride=4032, b_stride=4005, offset=8)):
+        x.check(x.run(out, **kw), out)
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 70, 512), (60, 90, 512), (600, 530, 256)])
@@ -118,7 +128,7 @@ def test_scales_far_apart(gpu, m, n, k):
 
 
 def test_repeats_bit_for_bit(gpu):
-    for m, n, k in ((8, 4096, 4096), (70, 1500, 3000), (400, 1100, 1024)):
+    for m, n, k in ((8, 4096, 4096), (70, 1500, 3000), (400, 1100, 1024), (130, 200, 5000)):
         x = Operands(m, n, k, 6)
         first = x.run("f32")
         assert np.array_equal(first, x.run("f32"))
