@@ -134,8 +134,19 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   }
 }
 
-// ---- Choice of experts, of some tokens by a workgroup: a token's j-th is the one that j others are before.  Where there are more threads than logits, a logit's threads
-// share the others. ----
+// ---- Choice of experts: a token's j-th is the one that j others are before.  Of some tokens by a workgroup: where there are more threads than logits, a logit's threads share the others. ----
+// The share of lane j's expert, of the j-th chosen (logits again: a NaN makes all shares of its token NaN).
+__device__ inline float share_of(const ExpertsArgs &p, const double *of_token, double most, int32_t chosen) {
+  const uint32_t lane = threadIdx.x & 63;
+  float sum = 0.0f, mine = 0.0f;
+  if (lane < p.top_k) mine = expf(float(of_token[chosen] - most));
+  if (p.renormalise) {
+    sum = mine;
+  } else {
+    for (uint32_t e = lane; e < p.experts; e += 64) sum += expf(float(of_token[e] - most));
+  }
+  return mine / __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_over_wave(sum)), 63));
+}
 struct Choice {          // in LDS, for `tokens` tokens
   double *key;           // [tokens][experts] logits; NaN as the lowest value
   double *most;          // [tokens]
@@ -149,7 +160,6 @@ struct Choice {          // in LDS, for `tokens` tokens
     expert = (int32_t *)at, at += tokens * p.top_k * 4;
     share = (float *)at;
   }
-  static size_t bytes(uint32_t experts, uint32_t top_k, uint32_t tokens) { return tokens * (experts * 12 + 8 + top_k * 8); }
 };
 // Tokens t0 .. t0 + tokens - 1.  Ends on a barrier.
 template <int THREADS>
@@ -181,17 +191,9 @@ __device__ inline void choose(const ExpertsArgs &p, const Places &w, uint32_t t0
     if (before < p.top_k) c.expert[t * p.top_k + before] = int32_t(i - t * p.experts);
   }
   __syncthreads();
-  for (uint32_t t = wave; t < tokens; t += THREADS / 64) {   // (logits again: a NaN makes all shares of its token NaN)
-    const double most = c.most[t], *const of_token = logits + t * p.experts;
-    float sum = 0.0f, mine = 0.0f;
-    if (lane < p.top_k) mine = expf(float(of_token[c.expert[t * p.top_k + lane]] - most));
-    if (p.renormalise) {
-      sum = mine;
-    } else {
-      for (uint32_t e = lane; e < p.experts; e += 64) sum += expf(float(of_token[e] - most));
-    }
-    sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_over_wave(sum)), 63));
-    if (lane < p.top_k) c.share[t * p.top_k + lane] = mine / sum;
+  for (uint32_t t = wave; t < tokens; t += THREADS / 64) {
+    const float share = share_of(p, logits + t * p.experts, c.most[t], lane < p.top_k ? c.expert[t * p.top_k + lane] : 0);
+    if (lane < p.top_k) c.share[t * p.top_k + lane] = share;
   }
   __syncthreads();
 }
@@ -204,13 +206,46 @@ __device__ inline void keep(const ExpertsArgs &p, const Places &w, uint32_t t0, 
     if (p.shares) p.shares[to] = c.share[i];
   }
 }
-constexpr int CHOOSE_THREADS = 512;
-__global__ __launch_bounds__(CHOOSE_THREADS) void k_experts_choose(ExpertsArgs p, Places w, FastDiv by_experts) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
-  if (blockIdx.x >= live_rows(p)) return;
-  const Choice c(dynamic, p, 1);
-  choose<CHOOSE_THREADS>(p, w, blockIdx.x, 1, by_experts, c);
-  keep<CHOOSE_THREADS>(p, w, blockIdx.x, 1, c);
+// Of a token by a workgroup: each wave ranks sixty-four experts among themselves, and the top_k of each are ranked among all of these.  (A rank among all experts takes four times the comparisons, in 64 bits, of
+// which 256 experts' take 4 us.)
+constexpr uint32_t MOST_CHUNKS = MOST_EXPERTS / 64;
+__global__ __launch_bounds__(MOST_EXPERTS) void k_experts_choose(ExpertsArgs p, Places w) {
+  __shared__ double keys[MOST_CHUNKS * MOST_CHOSEN], most;
+  __shared__ int32_t experts[MOST_CHUNKS * MOST_CHOSEN], chosen[MOST_CHOSEN];
+  const uint32_t token = blockIdx.x, e = threadIdx.x, lane = e & 63, chunk = e / 64, chunks = blockDim.x / 64;
+  if (token >= live_rows(p)) return;
+  const double *const logits = w.logits + uint64_t(token) * p.experts;
+  const double x = e < p.experts ? logits[e] : 0.0, mine = e < p.experts && x == x ? x : -__builtin_inf();   // (those that there are not are behind the lowest of those that there are)
+  uint32_t before = 0;
+#pragma unroll
+  for (int o = 0; o < 64; o++) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, mine);
+    const double other = __builtin_bit_cast(double, uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits >> 32)), o))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits)), o)));
+    before += (other > mine || (other == mine && uint32_t(o) < lane)) ? 1 : 0;
+  }
+  if (e < p.experts && before < p.top_k) keys[chunk * MOST_CHOSEN + before] = mine, experts[chunk * MOST_CHOSEN + before] = int32_t(e);
+  __syncthreads();
+  auto of_chunk = [&](uint32_t c) { return min(p.top_k, min(64u, p.experts - c * 64)); };
+  const uint32_t c = e / MOST_CHOSEN, rank = e % MOST_CHOSEN;
+  if (c < chunks && rank < of_chunk(c)) {
+    const double key = keys[e];
+    uint32_t place = rank;
+    for (uint32_t d = 0; d < chunks; d++) {
+      if (d == c) continue;
+      for (uint32_t i = 0, n = of_chunk(d); i < n; i++) place += (keys[d * MOST_CHOSEN + i] > key || (keys[d * MOST_CHOSEN + i] == key && d < c)) ? 1 : 0;
+    }
+    if (place < p.top_k) chosen[place] = experts[e];
+    if (place == 0) most = key;
+  }
+  __syncthreads();
+  if (chunk > 0) return;
+  const int32_t its = chosen[min(lane, p.top_k - 1)];
+  const float share = share_of(p, logits, most, its);
+  if (lane >= p.top_k) return;
+  const uint32_t to = token * p.top_k + lane;
+  w.chosen[to] = its, w.shares[to] = share;
+  if (p.chosen) p.chosen[to] = its;
+  if (p.shares) p.shares[to] = share;
 }
 // Whether every workgroup of the next launch makes all choices for itself: up to 128 comparisons a thread.  (us of the layer in a graph, so and with a launch for them, 2048 x 512, tokens and experts: 1 and 64 16.3
 // and 17.3, 1 and 128 20.6 and 21.4, 1 and 160 28.5 and 28.3, 1 and 512 49.8 and 38.1, 4 and 32 22.0 and 23.4, 4 and 64 24.1 and 23.8, 8 and 32 27.1 and 27.7, 8 and 128 84.9 and 74.8, 16 and 16 24.0 and 24.2,
@@ -703,7 +738,7 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   const bool few = few_of_each(a), fused = few && fused_choice(a);
   if (!fused) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
-    MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3(CHOOSE_THREADS), Choice::bytes(a.experts, a.top_k, 1), stream, a, w, FastDiv(a.experts));
+    MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3((a.experts + 63) / 64 * 64), 0, stream, a, w);
   }
   // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.  (us, 16 and 8, choices an expert: 2 113.6 and 111.6,
   // 4 33.3 and 31.5, 6 149.2 and 150.5, 137 and 145, 8 156 and 172, 91 and 101.)

@@ -84,6 +84,25 @@ def test_equal_logits_go_to_the_lowest_expert(gpu):
     assert (got[1] == np.arange(4)).all() and not as_f64("bf16", got[0]).any()
 
 
+@pytest.mark.parametrize("experts,top_k", [(65, 32), (130, 3), (192, 32), (257, 8), (512, 32), (449, 1), (64, 20)])
+def test_choices_among_many(gpu, experts, top_k):
+    """Logits with many equals, whole ones: the lowest numbers first, across the sixty-fours that are ranked together; rows of equals, and of the lowest there is."""
+    layer = Layer("bf16", 40, 16, 16, experts, top_k, seed=experts)
+    layer.x[:], layer.router[:] = 0, 0
+    rng = np.random.default_rng(experts)
+    layer.x[:, 0] = 0x3f80   # 1
+    layer.x[:, 1] = rng.choice([0, 0x3f80, 0xbf80, 0x4000], 40)   # 0, 1, -1, 2
+    layer.router[:, :2] = rng.choice([0, 0x3f80, 0x4000, 0x4040, 0xc000], (experts, 2))
+    layer.x[0, :2] = 0
+    layer.x[1, 0] = 0xff7f   # -3.4e38 times 2 and 3: past 32 bits
+    layer.x64, layer.router64 = as_f64("bf16", layer.x), as_f64("bf16", layer.router)
+    _, chosen, shares = layer.run()
+    want, share = layer.choice()
+    assert np.array_equal(chosen, want)
+    finite = np.arange(40) != 1
+    assert np.allclose(shares[finite], share[finite], rtol=2e-6, atol=1e-38)
+
+
 def test_a_row_that_is_not_a_number(gpu):
     """Its choice is the first experts, its results are NaN, and the other rows are what they are without it."""
     layer = Layer("e4m3", 6, 256, 128, 8, 3, seed=7)
