@@ -176,6 +176,69 @@ def test_a_workspace_that_two_recordings_share(gpu):
     stream.destroy()
 
 
+def test_sums_that_workgroups_share_in_graphs(gpu):
+    """A product and a layer whose sums meet in the workspace, recorded, replayed with other inputs and other rows between eager calls on workspaces full of NaN."""
+    hip = hip_runtime()
+    stream = M.Stream()
+    m, n, k = 130, 200, 5000
+    product, layer = M.MatmulBlocks(M.bf16, m, n, k), Layer("e4m3", 20, 64, 4000, 8, 2, seed=71)
+    experts = layer.op()
+    families = [s.family for op in (product, experts) for s in op.plan().steps]
+    assert "k_product_join" in families and "k_experts_join" in families
+    b8, b_scales = cast((synth.normal_f32(72, 0, (n, k)) * k ** -0.5).astype(np.float32), 128)
+    with Device() as d:
+        arrays = layer.arrays()
+        arrays[8] = np.array([20], np.int32)
+        at = [None if y is None else d.put(y) for y in arrays]
+        a8, a_scales = cast(synth.normal_f32(73, 0, (m, k)).astype(np.float32), 1)
+        fixed = [d.put(x) for x in (a8, a_scales, b8, b_scales)]
+        results = []
+        for _ in range(2):   # of the graph, of eager calls
+            results.append([d.put(np.zeros((m, n), np.uint16)), d.put(np.full((20, 64), POISON["bf16"], np.uint16))]
+                           + [d.put(np.full(op.workspace_bytes(), 0xff, np.uint8)) for op in (product, experts)])
+
+        def calls(where, s):
+            out, y, w0, w1 = results[where]
+            product.run_async(fixed + [out, w0], s)
+            experts.run_async(at[:9] + [y, at[10], at[11], w1], s)
+
+        class Calls:
+            enqueue = staticmethod(lambda s: calls(0, s))
+
+        lib = B.load()
+
+        def get(p, shape):
+            got = np.empty(shape, np.uint16)
+            M._check(lib.mrl_memcpy_d2h(got.ctypes.data, p, got.nbytes), "mrl_memcpy_d2h")
+            return got
+
+        def put(p, x):
+            M._check(lib.mrl_memcpy_h2d(p, np.ascontiguousarray(x).ctypes.data, x.nbytes), "mrl_memcpy_h2d")
+
+        graph = Recorded(hip, Calls, stream)
+        for i, rows in enumerate((20, 7, 0, 1, 20)):
+            a8, a_scales = cast(synth.normal_f32(74 + i, 0, (m, k)).astype(np.float32), 1)
+            x = values("bf16", 80 + i, 0, (20, 64))[0]
+            for p, y in ((fixed[0], a8), (fixed[1], a_scales), (at[0], x), (at[8], np.array([rows], np.int32))):
+                put(p, y)
+            for r in results:
+                put(r[1], np.full((20, 64), POISON["bf16"], np.uint16))
+            graph.launch(stream)
+            calls(1, None)
+            stream.synchronize()
+            M.synchronize()
+            assert np.array_equal(get(results[0][0], (m, n)), get(results[1][0], (m, n))) and np.array_equal(get(results[0][1], (20, 64)), get(results[1][1], (20, 64)))
+            a64, b64 = back(a8, a_scales, 1), back(b8, b_scales, 128)
+            want = a64 @ b64.T
+            assert (np.abs(as_f64("bf16", get(results[0][0], (m, n))) - want) <= product_bound(a64, b64, 41, HALF_STEP["bf16"], want, cut=True)).all()
+            layer.x, layer.x64 = x, as_f64("bf16", x)
+            want, bound, _, _ = layer.want(rows)
+            got = get(results[0][1], (20, 64))
+            assert (np.abs(as_f64("bf16", got[:rows]) - want) <= bound).all() and (got[rows:] == POISON["bf16"]).all()
+        graph.destroy()
+    stream.destroy()
+
+
 def test_refusals_of_a_run(gpu):
     """What only a run can see: missing pointers, workspaces off 16 bytes; nothing is launched."""
     layer = Layer("e4m3", 2, 128, 64, 4, 2, seed=7)
