@@ -5,7 +5,7 @@
 // instructions take them: 16 rows of weights against up to 16 of the expert's tokens, 128 bytes of each row at a time, a lane 32 of them.
 // Each of the steps needs all of the one before, a launch each: logits; choice (with few tokens and experts every workgroup of the next launch makes it for itself);
 // gate and up to h, 16 rows of one expert at a time; down, a workgroup to some rows of all experts, so that a token's sum over
-// its experts is formed in one place and in one order (several workgroups to fewer rows than there are compute units for, and a launch that adds up what they have).  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 475 (2.8 GB, 5.9 TB/s: up 309, down 154); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 105 (528 MB, 5.0 TB/s:
+// its experts is formed in one place and in one order (several workgroups to fewer rows than there are compute units for, and a launch that adds up what they have).  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 462 to 500 (2.8 GB, 5.6 to 6.0 TB/s: up 309, down 154); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 104 to 112 (528 MB, 4.7 to 5.1 TB/s:
 // logits and choice 5 each, up 59, down 34); 1 token, 8 of 64 of 2048 x 1024 in bf16 27 (101 MB: 3, 15, 9; each launch begins with 3 to 4 of reading what the one before left).  A choice is known by its number i = token * top_k + j; no lists go through memory but the chosen experts.
 #include <algorithm>
 
@@ -34,12 +34,13 @@ bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.toke
 // Many tokens of each expert go in parts of sixteen, others in parts of eight, or four of what is in two.
 bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
 
-// Rows of down to a workgroup: eight where these leave the compute unit with the most of them fewer; in parts of sixteen, where half of each instruction is lost on them, where sixteen would leave half of the units without any.
-// (us of the layer, 8 and 16, in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; of 2880 275 and 270, 161 and 148; of 5120 475 and 498, 262 and 267; of 6144 548 and 568, 297 and 301;
-// in parts of sixteen 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024 in e4m3 283 and 259.)
+// Rows of down to a workgroup at a time: eight where sixteen would leave half of the compute units without any, and in bf16 and parts of eight where these leave the unit with the most of them fewer.  (us of the layer, 8 and 16,
+// in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; 8 through 64 of 2880 x 768 124 and 118, 79 and 75; 32 through 64 of 6144 x 768 in bf16 294 and 308, 19 through 256 of 5376 x 320 in
+// e4m3 180 and 169, 2 through 60 of 6016 x 128 25.8 and 22.6; in parts of sixteen, where half of each instruction is lost on eight, 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024
+// in e4m3 283 and 259.)
 uint32_t rows_of_down(const ExpertsArgs &a) {
   auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
-  return (few_of_each(a) ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units) ? 8 : 16;
+  return (few_of_each(a) && a.weight_dtype == MRL_BF16 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units) ? 8 : 16;
 }
 // Workgroups that share some rows of down: as many as find a compute unit, with 48 steps of 2 KiB and more to each.  (us of the layer, one and as many: 94 tokens, 2 of 8 experts of 384 x 11652 in bf16 214 and 98, 1 token,
 // 8 of 64 of 384 x 9600 in e4m3 50 and 37, 109 tokens, 4 of 16 of 896 x 640 in bf16 47 and 38, 32 tokens, 8 of 128 of 1024 x 768 in e4m3 75 and 67; with less, 4 tokens, 4 of 64 of 1024 x 512 in bf16, 23.4 and 24.5.)
@@ -557,9 +558,10 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
   }
 }
 
-// ---- Down: blockIdx.x: 16 rows, or 8; blockIdx.y: tokens_here tokens.  All parts' steps in a line, cut into pieces of up to 1024 bytes of a part's rows, of which a wave has every
-// eighth: a workgroup's waves go through the same rows together.  (Eight rows PAIRED against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 112;
-// 8 of 1024 through 64 40.2 and 42.  Sixteen waves: 194 and 196 in bf16, 110 and 106 in e4m3.) ----
+// ---- Down: a workgroup to 16 rows, or 8, and behind them those gridDim.x further; blockIdx.y: tokens_here tokens; blockIdx.z: which of those that share the rows.  All parts' steps in a line, cut into pieces of up to
+// 1024 bytes of a part's rows, of which a wave has every eighth: a workgroup's waves go through the same rows together, and each asks for the next rows' weights while it multiplies the last of these.  (Eight rows PAIRED
+// against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 112; 8 of 1024 through 64 40.2 and 42.  A workgroup to each rows, 1 token, 2 of 8 of 4992 x 768 in e4m3 23.4
+// for 21.0; sixteen waves, 32 tokens as above 194 for 196 in bf16, 110 for 106 in e4m3.) ----
 constexpr int DOWN_WAVES = 8;
 template <bool F8, int ROOM, int TAIL, int HOW, bool IN_TWO>
 __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t tokens_here, uint32_t words) {
@@ -573,10 +575,11 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
   constexpr uint32_t BOUNCE = TILE_BYTES + S::BOUNCE;
   uint8_t *const bounces = (uint8_t *)(shares + (tokens_here * p.top_k + 3) / 4 * 4), *const bounce = bounces + wave * BOUNCE;
   const Lists lists(bounces + WAVES * BOUNCE, p.experts, tokens_here * p.top_k, words, MOST, WAVES);
-  const uint32_t row0 = blockIdx.x * HEIGHT, t0 = blockIdx.y * tokens_here, rows = live_rows(p), rows_here = min(HEIGHT, p.hidden - row0);
+  const uint32_t t0 = blockIdx.y * tokens_here, rows = live_rows(p), groups = (p.hidden + HEIGHT - 1) / HEIGHT;
   if (t0 >= rows) return;
   const uint32_t here = min(tokens_here, rows - t0);
-  for (uint32_t i = lane; i < here * 4; i += 64) sums[wave * tokens_here * 4 + i] = v4f{0, 0, 0, 0};
+  v4f *const mine = sums + wave * tokens_here * 4;
+  for (uint32_t i = lane; i < here * 4; i += 64) mine[i] = v4f{0, 0, 0, 0};
   for (uint32_t i = tid; i < here * p.top_k; i += THREADS) shares[i] = w.shares[t0 * p.top_k + i];
   const uint32_t parts = __builtin_amdgcn_readfirstlane(list<THREADS>(lists, p, w.chosen + t0 * p.top_k, here * p.top_k, words, MOST));
   // Pieces of eight steps, or fewer where a seventh of the waves' last turn would be idle.
@@ -587,8 +590,33 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
     of_part = (steps + size - 1) / size, pieces = parts * of_part;
     if (size == 1 || pieces * 7 >= (pieces + all_waves - 1) / all_waves * all_waves * 6) break;
   }
-  // The piece to fetch from, and the one to multiply.
-  uint32_t fetch_piece = first, fetch_s = 0, fetch_end = 0, piece = first, s = 0, end = 0;
+  // The waves' sums of some rows into one, and on to the next.
+  auto finish = [&](uint32_t group) {
+    __syncthreads();
+    const uint32_t row0 = group * HEIGHT, rows_here = min(HEIGHT, p.hidden - row0);
+    for (uint32_t i = tid; i < here * 4; i += THREADS) {
+      const uint32_t row = i % 4 * 4;
+      if (row >= rows_here) continue;
+      v4f sum = sums[i];
+#pragma unroll
+      for (uint32_t v = 1; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i];
+      if (HOW == PAIRED && row < 8) {
+#pragma unroll
+        for (uint32_t v = 0; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i + 2];
+      }
+      if (gridDim.z > 1) *(v4f *)(w.sums + (uint64_t(blockIdx.z) * p.tokens + t0 + i / 4) * w.hidden_s + row0 + row) = sum;   // (hidden_s: whole fours)
+      else store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
+    }
+    if (group + gridDim.x >= groups) return;
+    __syncthreads();
+    for (uint32_t i = lane; i < here * 4; i += 64) mine[i] = v4f{0, 0, 0, 0};
+  };
+  if (first >= pieces) {   // (of each row the same)
+    for (uint32_t group = blockIdx.x; group < groups; group += gridDim.x) finish(group);
+    return;
+  }
+  // The piece to fetch from, and the one to multiply, of which rows.
+  uint32_t fetch_group = blockIdx.x, fetch_piece = first, fetch_s = 0, fetch_end = 0, group = blockIdx.x, piece = first, s = 0, end = 0;
   Rows<F8, ROOM, 1, HOW> of;
   Step<F8, ROOM, 1, TAIL, HOW> t[AHEAD] = {};
   auto fetch = [&](Step<F8, ROOM, 1, TAIL, HOW> &to) {
@@ -596,26 +624,26 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       const uint32_t part = fetch_piece / of_part;
       const Part q = lists.parts[part];
       fetch_s = (fetch_piece - part * of_part) * size, fetch_end = min(steps, fetch_s + size);
-      of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), row0, rows_here);
+      of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), fetch_group * HEIGHT, min(HEIGHT, p.hidden - fetch_group * HEIGHT));
       of.tokens(__builtin_amdgcn_readfirstlane(q.count) * EACH, [&](uint32_t i) { return w.h + (uint64_t(t0 * p.top_k + lists.choices[q.first + i / EACH]) * EACH + i % EACH) * w.h_s; });
     }
     to.fetch(of, fetch_s, int(p.inter));
-    if (++fetch_s == fetch_end) fetch_piece += all_waves;
+    if (++fetch_s == fetch_end && (fetch_piece += all_waves) >= pieces) fetch_piece = first, fetch_group += gridDim.x;
   };
   v4f acc[1] = {};
 #pragma unroll
   for (int a = 0; a < AHEAD; a++)
-    if (fetch_piece < pieces) fetch(t[a]);
-  while (piece < pieces) {
+    if (fetch_group < groups) fetch(t[a]);
+  while (group < groups) {
 #pragma unroll
     for (int a = 0; a < AHEAD; a++) {
-      if (piece >= pieces) break;
+      if (group >= groups) break;
       if (s == end) {
         const uint32_t part = piece / of_part;
         s = (piece - part * of_part) * size, end = min(steps, s + size);
       }
       t[a].multiply(acc, bounce);
-      if (fetch_piece < pieces) fetch(t[a]);
+      if (fetch_group < groups) fetch(t[a]);
       if (++s == end) {
         const Part q = lists.parts[piece / of_part];
         uint32_t i = HOW == PAIRED ? li - lg / 2 * 8 : li;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
@@ -632,23 +660,9 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
           sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
         }
         acc[0] = v4f{0, 0, 0, 0};
-        piece += all_waves;
+        if ((piece += all_waves) >= pieces) finish(group), group += gridDim.x, piece = first;
       }
     }
-  }
-  __syncthreads();
-  for (uint32_t i = tid; i < here * 4; i += THREADS) {
-    v4f sum = sums[i];
-    const uint32_t row = i % 4 * 4;
-#pragma unroll
-    for (uint32_t v = 1; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i];
-    if (HOW == PAIRED && row < 8) {
-#pragma unroll
-      for (uint32_t v = 0; v < WAVES; v++) sum += sums[v * tokens_here * 4 + i + 2];
-    }
-    if (row >= rows_here) continue;
-    if (gridDim.z > 1) *(v4f *)(w.sums + (uint64_t(blockIdx.z) * p.tokens + t0 + i / 4) * w.hidden_s + row0 + row) = sum;   // (hidden_s: whole fours)
-    else store4(p.out + int64_t(t0 + i / 4) * p.out_s + row0 + row, sum, int(rows_here - row));
   }
 }
 
@@ -695,7 +709,7 @@ hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream
     if (e != hipSuccess) return e;
   }
   const size_t lds = down_lds<F8, ROOM, HOW, IN_TWO>(a, here);
-  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3((a.hidden + HEIGHT - 1) / HEIGHT, (a.tokens + here - 1) / here, w.down_shares), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
+  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3(std::min((a.hidden + HEIGHT - 1) / HEIGHT, uint32_t(g_compute_units)), (a.tokens + here - 1) / here, w.down_shares), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
   if (w.down_shares > 1) {
     plan::work(plan::UNIT_STREAM, 0, (4.0 * w.down_shares + 2) * a.tokens * a.hidden);
     MRL_LAUNCH(k_experts_join, dim3((a.hidden + JOIN_THREADS * 4 - 1) / (JOIN_THREADS * 4), a.tokens), dim3(JOIN_THREADS), 0, stream, a, w);
