@@ -481,8 +481,7 @@ __device__ inline uint32_t list(const Lists &to, const ExpertsArgs &p, const int
 // ---- Gate and up.  All parts' tiles of 16 rows lie on a line, of which workgroup b has the tiles b, b + gridDim.x, ..: what is under way at a time lies close together (equal runs of the line for each
 // took 10 % longer over 1.9 GB).  The waves share a tile's steps; their loads run AHEAD steps in front, from one tile into the next, and the
 // waves' sums meet behind each.  FUSED: from logits, the choices made here. ----
-constexpr int UP_WAVES = 4;
-template <bool F8, int ROOM, bool FUSED, int TAIL>
+template <bool F8, int ROOM, bool FUSED, int TAIL, int UP_WAVES>
 __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, Places w, uint32_t words, FastDiv by_tiles, FastDiv by_experts) {
   constexpr int AHEAD = 3;
   typedef Shape<F8, ROOM, FULL> S;
@@ -677,8 +676,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_experts_join(ExpertsArgs p, Pl
   store4(p.out + int64_t(token) * p.out_s + at, sum, int(p.hidden - at));
 }
 
-template <bool F8, int ROOM, bool FUSED, int TAIL>
-hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+template <bool F8, int ROOM, bool FUSED, int TAIL, int UP_WAVES>
+hipError_t launch_up_waves(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   // Two workgroups to a compute unit, what their registers allow, or one to a tile.  (us, two with three steps ahead and three with two: 128 tokens through 128 experts of 2048 x 768 in e4m3 155 and
   // 180, 32 tokens 110 and 112, 16 through 8 of 4096 x 14336 254 and 253.)
   const uint32_t tiles = (a.inter + 15) / 16, words = (a.tokens + 31) / 32, choices = a.tokens * a.top_k;
@@ -687,11 +686,21 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   const size_t lds = UP_WAVES * (2 * TILE_BYTES + Shape<F8, ROOM, FULL>::BOUNCE) + Lists::bytes(a.experts, choices, words, ROOM, UP_WAVES);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, TAIL>), 96 * 1024);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_up<F8, ROOM, FUSED, TAIL, UP_WAVES>), 96 * 1024);
     if (e != hipSuccess) return e;
   }
-  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, TAIL>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles), FastDiv(a.experts));
+  MRL_LAUNCH((k_experts_up<F8, ROOM, FUSED, TAIL, UP_WAVES>), dim3(grid), dim3(UP_WAVES * 64), lds, stream, a, w, words, FastDiv(tiles), FastDiv(a.experts));
   return plan::last_error();
+}
+template <bool F8, int ROOM, bool FUSED, int TAIL>
+hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
+  // Eight waves to a tile where at least half of the compute units have none and its rows are 2 KiB and more.  (us of the layer, four and eight, 1 token: 2 of 8 experts of 4096 x 512 in bf16 18.7 and 16.8, 4 of 64 of
+  // 7168 x 512 in e4m3 23.9 and 22.5; 4 of 16 of 4096 x 1024 19.9 and 20.6, of 1024 x 256 12.3 and 12.4.)
+  const uint64_t tiles = uint64_t(most_parts(a.experts, a.tokens * a.top_k, ROOM)) * ((a.inter + 15) / 16);
+  if constexpr (ROOM == 8 && TAIL != SHORT) {
+    if (tiles * 2 <= uint64_t(g_compute_units) && a.hidden * (F8 ? 1 : 2) >= 2048) return launch_up_waves<F8, ROOM, FUSED, TAIL, 8>(a, w, stream);
+  }
+  return launch_up_waves<F8, ROOM, FUSED, TAIL, 4>(a, w, stream);
 }
 constexpr size_t MOST_LDS = 160 * 1024;
 template <bool F8, int ROOM, int HOW, bool IN_TWO>
