@@ -7,7 +7,7 @@
 namespace mrl {
 namespace blocks {
 
-// Results in bf16 come from products in e4m3, whose cuts they do not show (2^-9 of a result against 2^-13 of a block's largest product); results in f32 from the same numbers
+// Results in bf16 come from products in e4m3, whose cuts, 2^-13 of a block's largest product, they show only where products cancel to some 2^-7 of it; results in f32 from the same numbers
 // in bf16.
 template <class OUT> struct Operand;
 template <> struct Operand<uint16_t> {
