@@ -745,12 +745,13 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t st
                                       : launch_up<F8, ROOM, FUSED, SHORT>(a, w, stream);
   if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  const bool eight = rows_of_down(a) == 8;
-  constexpr int EIGHT = ROOM == 8 ? PAIRED : HALF;
+  // Of rows of a single run of 128 bytes there is no pair.  (us of the layer, HALF and PAIRED, in e4m3: 44 tokens, 6 of 64 experts of 640 x 128 27.2 and 31.1, 4 tokens, 8 of 64 of 2048 x 128 21.1 and 22.9.)
+  const bool eight = rows_of_down(a) == 8, pair = ROOM == 8 && eight && a.inter * (F8 ? 1 : 2) > 128;
   if constexpr (ROOM == 8) {
-    if (w.in_two) return eight ? launch_down_how<F8, ROOM, EIGHT, true>(a, w, stream) : launch_down_how<F8, ROOM, FULL, true>(a, w, stream);
+    if (w.in_two) return pair ? launch_down_how<F8, ROOM, PAIRED, true>(a, w, stream) : eight ? launch_down_how<F8, ROOM, HALF, true>(a, w, stream) : launch_down_how<F8, ROOM, FULL, true>(a, w, stream);
+    if (pair) return launch_down_how<F8, ROOM, PAIRED, false>(a, w, stream);
   }
-  return eight ? launch_down_how<F8, ROOM, EIGHT, false>(a, w, stream) : launch_down_how<F8, ROOM, FULL, false>(a, w, stream);
+  return eight ? launch_down_how<F8, ROOM, HALF, false>(a, w, stream) : launch_down_how<F8, ROOM, FULL, false>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {

@@ -15,7 +15,7 @@ SIZES = [(1, 256, 128, 8, 2), (1, 1, 1, 1, 1), (1, 2048, 256, 64, 8), (2, 512, 1
          # the largest of whose choices every workgroup makes all, and those behind them
          (8, 72, 40, 32, 32), (8, 72, 40, 33, 32), (4, 136, 64, 64, 6), (1, 136, 64, 181, 32), (1, 136, 64, 182, 32), (32, 64, 48, 8, 2), (28, 64, 48, 9, 2), (29, 64, 48, 9, 2),
          # sixteen waves for the products with down, and one token more
-         (64, 300, 136, 128, 8), (65, 300, 136, 128, 8), (64, 2050, 64, 40, 3), (64, 264, 128, 300, 32), (33, 4096, 48, 6, 2), (40, 4100, 48, 64, 2), (1, 5000, 64, 2, 1), (3, 9003, 300, 4, 2), (2, 4096, 48, 8, 2), (5, 2048, 30, 100, 1), (7, 2000, 40, 9, 1),
+         (64, 300, 136, 128, 8), (65, 300, 136, 128, 8), (64, 2050, 64, 40, 3), (64, 264, 128, 300, 32), (33, 4096, 48, 6, 2), (40, 4100, 48, 64, 2), (1, 5000, 64, 2, 1), (3, 9003, 300, 4, 2), (2, 4096, 48, 8, 2), (5, 2048, 30, 100, 1), (7, 2000, 40, 9, 1), (44, 640, 128, 64, 6), (44, 640, 129, 64, 6), (40, 300, 64, 64, 6), (3, 200, 65, 12, 4),
          # several workgroups to the same rows of down
          (40, 72, 2100, 24, 4), (3, 250, 4000, 8, 3), (128, 65, 900, 16, 4), (1, 1, 8200, 8, 8), (256, 130, 1300, 4, 2)]
 
