@@ -1684,7 +1684,7 @@ int mrl_spec_parameter_direction(const mrl_spec *spec, uint32_t idx) {
 
 size_t mrl_spec_parameter_bytes(const mrl_spec *spec, uint32_t idx) {
   uint32_t shape[MRL_MAX_RANK], rank;
-  if (mrl_spec_parameter_shape(spec, idx, shape, &rank) != MRL_OK) return 0;
+  if (mrl_spec_parameter_shape(spec, idx, shape, &rank) != MRL_OK || !valid_dtype(spec->dtypes[idx])) return 0;
   return size_t(volume(shape, rank)) * mrl_dtype_size(spec->dtypes[idx]);
 }
 
@@ -1762,7 +1762,7 @@ uint32_t mrl_target_destination_memories(uint32_t slower, uint32_t *out, uint32_
 }
 
 uint32_t mrl_target_layouts_for_shape(const uint32_t *shape, uint32_t rank, int dtype, mrl_layout *out, uint32_t cap) {
-  if (!shape || rank == 0 || rank > MRL_MAX_RANK || mrl_dtype_size(dtype) == 0) return 0;
+  if (!shape || rank == 0 || rank > MRL_MAX_RANK || !valid_dtype(dtype)) return 0;
   const uint32_t es = uint32_t(mrl_dtype_size(dtype));
   std::vector<mrl_layout> base(1), result;
   mrl_layout_row_major(shape, rank, &base[0]);

@@ -34,6 +34,15 @@ def test_the_type_of_eight_bits():
     assert M.Matmul([1, 4, 4, 4], [M.f8e4m3] * 3).check() == BAD_SPEC
 
 
+def test_the_type_of_eight_bits_is_of_no_spec():
+    """What a search asks about Specs knows as little of it as of numbers that are no type."""
+    for dtype in (M.f8e4m3, 9, -1):
+        assert M.Target.all_layouts_for_shape([64, 64], dtype) == []
+    lib = B.load()
+    spec = M.Matmul([1, 4, 4, 4], [M.u8, M.f8e4m3, M.i32])
+    assert [lib.mrl_spec_parameter_bytes(C.byref(spec._c), i) for i in range(3)] == [16, 0, 64]
+
+
 @pytest.mark.parametrize("given,status", [
     (dict(), OK), (dict(dtype=M.f32), OK), (dict(dtype=M.i8), UNSUPPORTED), (dict(dtype=M.f8e4m3), BAD_SPEC), (dict(dtype=99), BAD_SPEC), (dict(rows=0), BAD_SPEC), (dict(cols=0), BAD_SPEC),
     (dict(block_rows=128), OK), (dict(block_rows=0), BAD_SPEC), (dict(block_rows=64), BAD_SPEC), (dict(rows=1 << 27, cols=128), OK), (dict(rows=1 << 27, cols=129), TOO_LARGE),
