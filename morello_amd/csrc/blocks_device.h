@@ -17,6 +17,12 @@ typedef v4i v4i_any __attribute__((aligned(1)));
 typedef v4f v4f_any __attribute__((aligned(4)));
 typedef v4bf v4bf_any __attribute__((aligned(2)));
 
+// What lanes of a wave have written to LDS is there for its others, and what they have read may be written over: a wave's LDS accesses complete in order, and this keeps the compiler from changing theirs.
+__device__ inline void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ inline v4i chunk_at(const uint8_t *p) { return *(const v4i_any *)p; }
 // A row's last sixteen bytes moved down to where its last n of them belong, zeros behind them (n: 0 or less: zeros; 16 and more: as they are).
 __device__ inline v4i last_of_row(v4i x, int n) {

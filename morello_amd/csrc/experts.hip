@@ -349,6 +349,7 @@ struct Step {
       if (F8 && HOW == PAIRED && left + int(lane % S::LANES) * 16 <= int(lane / 32) * 128) scale = 0;   // (no such block; the last one's may be infinite)
     }
     uint8_t *const of_x = bounce + N * TILE_BYTES;
+    lanes_meet();   // (over what the step before was multiplied from)
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
@@ -363,6 +364,7 @@ struct Step {
         const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS + lane % S::X_CHUNKS / CHUNKS * 8;
         *(v4i *)(of_x + token * S::ROW_BYTES + (lane % CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[i];
       }
+    lanes_meet();
     const uint32_t mine = li & (S::IN_LDS - 1);
     const uint8_t *const my_x = of_x + mine * S::ROW_BYTES;
     float scales[2] = {0, 0};
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
     }
     if (group + gridDim.x >= groups) return;
     __syncthreads();
-    for (uint32_t i = lane; i < here * 4; i += 64) mine[i] = v4f{0, 0, 0, 0};
+    for (uint32_t i = lane; i < here * 4; i += 64) mine[i] = v4f{0, 0, 0, 0};   // (lanes meet in the next multiply, before any of them adds)
   };
   if (first >= pieces) {   // (of each row the same)
     for (uint32_t group = blockIdx.x; group < groups; group += gridDim.x) finish(group);

@@ -86,6 +86,7 @@ __device__ inline void store_sums(uint8_t *lds, const v4f (&acc)[MT][NT], const 
       if constexpr (SIZE == 2) *(v4bf *)to = v4bf{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
       else *(v4f *)to = x;
     }
+  lanes_meet();
   const uint32_t row_end = p.m - min(p.m, row0);
   OUT *const out = (OUT *)p.out + int64_t(row0) * p.out_s + col0;
 #pragma unroll

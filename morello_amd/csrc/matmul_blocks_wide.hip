@@ -131,6 +131,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_product_wide(ProductArgs p, uint
       const v4f &x = acc[t][u];
       *(v4bf *)(mine + (t * 16 + li) * 128 + ((u * 2 + lg / 2) ^ (li & 7)) * 16 + lg % 2 * 8) = v4bf{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
     }
+  lanes_meet();
   const uint32_t col = n0 + wn * 64 + (lane & 7) * 8, row_end = min(128u, p.m - min(p.m, m0 + wm * 128));
   uint16_t *const out = (uint16_t *)p.out + int64_t(m0 + wm * 128) * p.out_s + col;
 #pragma unroll
