@@ -87,8 +87,8 @@ __device__ inline float sum_over_wave(float x) {
 __device__ inline float lo_f32(int x) { return __uint_as_float(uint32_t(x) << 16); }
 __device__ inline float hi_f32(int x) { return __uint_as_float(uint32_t(x) & 0xffff0000u); }
 
-// ---- Logits: a workgroup to an expert and TOKENS tokens, in 64 bits (a product of two bf16 numbers is exact in 32), so that which experts are chosen
-// does not hang on the order of a sum. ----
+// ---- Logits: a workgroup to an expert and TOKENS tokens, in 64 bits, products too (of two bf16 numbers they have sixteen bits, but twice the range of 32-bit numbers), so that which experts are chosen
+// does not hang on the order of a sum, and finite inputs have finite logits. ----
 constexpr int ROUTER_THREADS = 256;
 template <int TOKENS>
 __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p, Places w) {
@@ -101,9 +101,11 @@ __global__ __launch_bounds__(ROUTER_THREADS) void k_experts_logits(ExpertsArgs p
   double sum[TOKENS] = {};
   auto add = [&](v4i r, const v4i (&y)[TOKENS]) {
 #pragma unroll
-    for (int t = 0; t < TOKENS; t++)
+    for (int i = 0; i < 4; i++) {
+      const double lo = lo_f32(r[i]), hi = hi_f32(r[i]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) sum[t] += double(lo_f32(r[i]) * lo_f32(y[t][i])), sum[t] += double(hi_f32(r[i]) * hi_f32(y[t][i]));
+      for (int t = 0; t < TOKENS; t++) sum[t] = __builtin_fma(hi, double(hi_f32(y[t][i])), __builtin_fma(lo, double(lo_f32(y[t][i])), sum[t]));
+    }
   };
   uint32_t k = threadIdx.x * 8;
   for (; k + 8 <= p.hidden; k += ROUTER_THREADS * 8) {

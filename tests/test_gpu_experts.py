@@ -103,6 +103,27 @@ def test_choices_among_many(gpu, experts, top_k):
     assert np.allclose(shares[finite], share[finite], rtol=2e-6, atol=1e-38)
 
 
+@pytest.mark.parametrize("tokens,experts,top_k", [(2, 12, 3), (4, 12, 12), (40, 12, 4), (9, 130, 5)])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_logits_out_of_the_range_of_32_bits(gpu, tokens, experts, top_k, renormalise):
+    """Products of finite numbers past 3.4e38 and below 1e-45: all different, the later expert's the larger, and shares are numbers."""
+    layer = Layer("bf16", tokens, 24, 16, experts, top_k, seed=23, renormalise=renormalise)
+    layer.x[:], layer.router[:] = 0, 0
+    e = np.arange(experts)
+    layer.router[:, 5] = 0x3f80 + e          # 1 and more, up to 2 and more
+    layer.router[:, 17] = 0x1f80 + e         # the same times 2^-64
+    layer.router[:, 22] = e % 2 * 0x4000     # 2, and nothing
+    layer.x[0::2, 5] = 0x7f7f                # 3.4e38
+    layer.x[1::2, 17] = 0x1000               # 2^-95: products at 2^-159 and above, where 32 bits have nothing
+    layer.x[0, 22] = 0xc0a0                  # -5
+    layer.x64, layer.router64 = as_f64("bf16", layer.x), as_f64("bf16", layer.router)
+    _, chosen, shares = layer.run()
+    want, share = layer.choice()
+    assert np.array_equal(want, np.tile(experts - 1 - np.arange(top_k), (tokens, 1)))
+    assert np.array_equal(chosen, want)
+    assert np.isfinite(shares).all() and np.allclose(shares, share, rtol=2e-6, atol=1e-38)
+
+
 def test_a_row_that_is_not_a_number(gpu):
     """Its choice is the first experts, its results are NaN, and the other rows are what they are without it."""
     layer = Layer("e4m3", 6, 256, 128, 8, 3, seed=7)
