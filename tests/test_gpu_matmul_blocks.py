@@ -143,3 +143,51 @@ def test_whole_chunks_at_odd_addresses(gpu, m, n, k):
         for kw in (dict(a_stride=up, b_stride=up), dict(a_stride=up, b_stride=up + 3), dict(a_stride=k + 1, b_stride=up)):
             for out in ("bf16", "f32"):
                 x.check(x.run(out, offset=offset, **kw), out)
+
+
+# On tiles of 256 x 256 (169 of them): blocks of K that the ring's two and the scales' eight go around once and more, whole last ones and cut ones; scales of a in fours (blocks a multiple of four) and one by one
+WIDE = [(3100, 3100, 1200), (3100, 3101, 1424), (3099, 3100, 2304), (3100, 3100, 2560), (3100, 3100, 1300), (3090, 3100, 128), (3100, 3090, 272), (3100, 3100, 4096)]
+# On tiles of 128 x 64, and past a round of 128 x 128, of many blocks
+MORE_TILES = [(1280, 1216, 400), (1279, 1217, 1552), (1280, 1216, 1024), (2049, 2050, 1168), (2049, 2050, 1024), (2170, 2060, 1300)]
+
+
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_product_on_wide_tiles(gpu, m, n, k):
+    x = Operands(m, n, k, m + n + k, narrow=True)
+    first = x.run("bf16")
+    x.check(first, "bf16")
+    assert np.array_equal(first, x.run("bf16"))
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", MORE_TILES)
+def test_product_on_more_tiles(gpu, m, n, k, out):
+    x = Operands(m, n, k, m + n + k, narrow=True)
+    x.check(x.run(out), out)
+
+
+@pytest.mark.parametrize("k,a_scale_stride", [(1424, 13), (1424, 16), (2560, 21), (1200, 12)])
+def test_strides_on_wide_tiles(gpu, k, a_scale_stride):
+    x = Operands(3100, 3100, k, 13, narrow=True)
+    x.check(x.run("bf16", a_stride=k + 32, b_stride=k + 16, a_scale_stride=a_scale_stride, b_scale_stride=a_scale_stride + 3, out_stride=3109), "bf16")
+
+
+@pytest.mark.parametrize("k", [1424, 1200])
+def test_scales_far_apart_on_wide_tiles(gpu, k):
+    """Every block of K has a scale of its own, by 2^10 apart: none is multiplied by another's."""
+    x = Operands(3100, 3100, k, 14, narrow=True)
+    for q in range(x.steps):
+        x.a_scales[:, q] *= np.float32(2.0 ** (10 * (q % 5) - 20))
+        x.b_scales[:, q] *= np.float32(2.0 ** (7 * (q % 3) - 7))
+    x.check(x.run("bf16"), "bf16")
+
+
+@pytest.mark.parametrize("k", [1424, 1200])
+def test_what_is_not_a_number_on_wide_tiles(gpu, k):
+    m = n = 3100
+    x = Operands(m, n, k, 15, narrow=True)
+    x.a[m - 1, k - 1], x.a[300, 0], x.b[n // 3, k - 17] = 0x7f, 0xff, 0xff
+    got = as_f64("bf16", x.run("bf16"))
+    nan = np.zeros((m, n), bool)
+    nan[[m - 1, 300]], nan[:, n // 3] = True, True
+    assert np.array_equal(np.isnan(got), nan)
