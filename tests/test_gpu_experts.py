@@ -197,3 +197,18 @@ def test_repeats_bit_for_bit(gpu, kind):
     first = layer.run()
     second = layer.run()
     assert all(np.array_equal(a, b) for a, b in zip(first, second))
+
+
+# Sixteen rows of down at a time, in several turns and in one, of tokens that one workgroup has all of and that several share; rows of all ends; eight rows off and on steps of 256 bytes
+MORE = [(64, 4112, 256, 8, 2), (20, 2100, 300, 6, 2), (256, 2100, 140, 8, 2), (256, 2056, 7, 16, 8), (256, 64, 7, 16, 8), (35, 2112, 512, 6, 1), (35, 2100, 500, 6, 1), (80, 2056, 7, 430, 32),
+        (80, 64, 7, 430, 32), (40, 200, 64, 64, 8), (90, 200, 40, 80, 5), (12, 320, 1536, 16, 4), (32, 1800, 256, 24, 3), (35, 4200, 512, 6, 1), (3, 2100, 256, 4, 2), (2, 2056, 5, 4, 2),
+        (256, 7, 64, 16, 8), (33, 4100, 48, 6, 2), (40, 5, 40, 64, 2)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", MORE)
+def test_more_layers(gpu, kind, tokens, hidden, inter, experts, top_k):
+    layer = Layer(kind, tokens, hidden, inter, experts, top_k, seed=tokens + hidden, renormalise=bool(tokens % 2))
+    first = layer.run()
+    layer.check(first)
+    assert all(np.array_equal(a, b) for a, b in zip(first, layer.run()))
