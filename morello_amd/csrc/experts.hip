@@ -735,9 +735,10 @@ Tail tail_of(uint32_t k, uint32_t step = F8 ? 128 : 64) { return k * (F8 ? 1 : 2
 template <bool F8, int ROOM, int HOW, bool IN_TWO>
 hipError_t launch_down_how(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   const Tail tail = tail_of<F8>(a.inter, Shape<F8, ROOM, HOW>::STEP);
-  return tail == WHOLE    ? launch_down<F8, ROOM, WHOLE, HOW, IN_TWO>(a, w, stream)
-         : tail == INSIDE ? launch_down<F8, ROOM, INSIDE, HOW, IN_TWO>(a, w, stream)
-                          : launch_down<F8, ROOM, SHORT, HOW, IN_TWO>(a, w, stream);
+  if constexpr (HOW != PAIRED) {   // (pairs are of rows of more than 128 bytes)
+    if (tail == SHORT) return launch_down<F8, ROOM, SHORT, HOW, IN_TWO>(a, w, stream);
+  }
+  return tail == WHOLE ? launch_down<F8, ROOM, WHOLE, HOW, IN_TWO>(a, w, stream) : launch_down<F8, ROOM, INSIDE, HOW, IN_TWO>(a, w, stream);
 }
 template <bool F8, int ROOM, bool FUSED>
 hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t stream) {

@@ -146,6 +146,31 @@ def test_few_rows_of_down_are_shared(hidden, inter, joined):
     assert (op.workspace_bytes() >= 2 * hidden * 4) or not joined
 
 
+def test_values_are_compared_of_every_form_of_the_kernels():
+    """The sizes whose results are compared with the oracle's reach every kernel that the library chooses between, with all its template arguments."""
+    import test_gpu_experts as E
+    import test_gpu_matmul_blocks as P
+
+    ops = [M.MatmulBlocks(out, *s) for out in (M.bf16, M.f32) for s in P.SIZES + P.MORE_TILES] + [M.MatmulBlocks(M.bf16, *s) for s in P.WIDE]
+    ops += [M.Experts(kind, *s) for kind in (M.bf16, M.f8e4m3) for s in E.SIZES + E.MORE]
+    reached = {s.kernel for op in ops for s in op.plan().steps}
+    tiles = [(128, 128, 1, 2), (128, 128, 2, 2), (128, 96, 2, 2), (128, 64, 2, 3), (96, 96, 2, 3), (96, 64, 2, 3), (64, 96, 2, 3), (64, 64, 3, 3)]
+    few = [(1, 1, 8, 4), (2, 1, 8, 3), (3, 1, 8, 2), (3, 2, 4, 3), (4, 1, 4, 3), (4, 2, 4, 3), (5, 1, 6, 2), (5, 2, 4, 2), (6, 1, 4, 2), (6, 2, 4, 2)]
+    want = {f"k_product_wide [CHUNKS = {c}]" for c in ("false", "true")}
+    for out in ("float", "unsigned short"):
+        want |= {"k_product_tile [BM = %d, BN = %d, GROUPS = %d, DEPTH = %d, OUT = %s, SHARED = false]" % (*t, out) for t in tiles}
+        want |= {f"k_product_tile [BM = 64, BN = 64, GROUPS = 3, DEPTH = 3, OUT = {out}, SHARED = true]", f"k_product_join [OUT = {out}]", f"k_product_few_any [OUT = {out}]"}
+        want |= {"k_product_few [MT = %d, NT = %d, WAVES = %d, DEPTH = %d, OUT = %s]" % (*f, out) for f in few}
+    for f8 in ("false", "true"):
+        for tail in range(3):
+            want |= {f"k_experts_up [F8 = {f8}, ROOM = 16, FUSED = false, TAIL = {tail}, UP_WAVES = 4]"}
+            want |= {f"k_experts_up [F8 = {f8}, ROOM = 8, FUSED = {fused}, TAIL = {tail}, UP_WAVES = {waves}]" for fused in ("false", "true") for waves in (4, 8) if (waves, tail) != (8, 2)}
+            want |= {f"k_experts_down [F8 = {f8}, ROOM = 16, TAIL = {tail}, HOW = {how}, IN_TWO = false]" for how in range(2)}
+            want |= {f"k_experts_down [F8 = {f8}, ROOM = 8, TAIL = {tail}, HOW = {how}, IN_TWO = {two}]" for how in range(3) for two in ("false", "true") if (how, tail) != (2, 2)}
+    assert want <= reached, sorted(want - reached)
+    assert {k for k in reached - want if "[" in k and not k.startswith(("k_experts_logits", "k_pad_rows"))} == set()
+
+
 def test_the_oracle_of_the_casts():
     """Every byte is its own nearest; between two numbers the nearer, halfway the even byte; a block reads back within half a step."""
     codes = np.array([c for c in range(256) if c & 127 != 127])
