@@ -159,10 +159,13 @@ hipError_t launch(const ProductArgs &p, hipStream_t stream) {
       const hipError_t e = launch_product_tile(p, stream);
       return e == hipSuccess ? launch_join<OUT>(p, stream) : e;
     }
-    // Tiles of 256 x 256 where the last of their rounds over the compute units is not too empty.  us, so and on the smaller ones: 2048 x 4096 x 4096 (128 tiles) 61 and 51, 2048 x 6144 x 2048
-    // (192) 38.3 and 46, 4096 x 4096 x 1024 (256) 25.9 and 32.3.
-    const uint64_t wide = uint64_t((p.m + 255) / 256) * ((p.n + 255) / 256), rounds = (wide + g_compute_units - 1) / g_compute_units;
-    return sizeof(OUT) == 2 && wide * 100 >= 62 * rounds * g_compute_units ? launch_product_wide(p, stream) : launch_product_tile(p, stream);
+    // Tiles of 256 x 256 where they make one round over the compute units and those of 128 x 128, of which a unit takes two at a time, more than one; in more rounds, and where rows of the result are off 16 bytes and cost the
+    // larger tiles' stores, all at one time, more, where the last round is not too empty.  us, so and on the smaller ones: 2048 x 4096 x 4096 (128 tiles, 512 of the smaller) 54.3 and 48.7, 2304 x 4096 x 4096 (144, 576) 54.5 and 65.7,
+    // 2304 x 4096 x 1040 23.6 and 25.0, 2944 x 2944 x 2048 (144, 529) 31.5 and 34.7, 130 x 40000 x 2048 (157, 626) 33.3 and 40.4, 4096 x 4096 x 512 (256) 17.6 and 18.9; off 16 bytes 2900 x 2950 x 1040 (144) 28.1 and 25.0, 3300 x 3300 x 1024 (169) 24.0 and 21.0,
+    // 2304 x 4090 x 4096 57.1 and 64.3, 4000 x 4001 x 1040 (256) 26.3 and 32.1; two rounds 4608 x 4096 x 4096 (288) 111.6 and 106.1, 5120 x 4096 x 4096 (320) 111.9 and 112.5, 5632 x 4096 x 4096 (352) 112.8 and 126.
+    const uint64_t wide = uint64_t((p.m + 255) / 256) * ((p.n + 255) / 256), small = uint64_t((p.m + 127) / 128) * ((p.n + 127) / 128), rounds = (wide + g_compute_units - 1) / g_compute_units;
+    const bool few_rounds = rounds == 1 && p.out_s % 8 == 0 ? small > 2 * g_compute_units : wide * 100 >= 62 * rounds * g_compute_units;
+    return sizeof(OUT) == 2 && few_rounds ? launch_product_wide(p, stream) : launch_product_tile(p, stream);
   }
   if (p.m <= 16) MRL_LAUNCH((k_product_few_any<1, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);
   else if (p.m <= MOST_FEW_ANY) MRL_LAUNCH((k_product_few_any<2, 8, OUT>), dim3((p.n + 15) / 16), dim3(512), 0, stream, p);

@@ -123,6 +123,16 @@ def test_which_kernel_a_product_takes(m, n, k, out, strides, kernel, copied):
     assert [s.family for s in steps][-1] == kernel and len(steps) == 1 + (copied > 0)
 
 
+@pytest.mark.parametrize("m,n,k,kernel", [
+    (2048, 4096, 4096, "k_product_tile"), (2049, 4096, 4096, "k_product_wide"), (2304, 4096, 1024, "k_product_wide"), (3000, 3000, 2000, "k_product_wide"), (2816, 2816, 2048, "k_product_tile"),
+    (2944, 2944, 2048, "k_product_wide"), (4608, 4096, 512, "k_product_tile"), (5120, 4096, 4096, "k_product_wide"), (2000, 16384, 512, "k_product_wide"), (130, 40000, 256, "k_product_wide"),
+    (2900, 2950, 1040, "k_product_tile"), (3100, 3100, 1040, "k_product_wide")])
+def test_where_products_take_wide_tiles(m, n, k, kernel):
+    """In one round of them where the smaller tiles make more than one; past a round, and of results whose rows are off 16 bytes, where the last is full enough."""
+    assert [s.family for s in M.MatmulBlocks(M.bf16, m, n, k).plan().steps] == [kernel]
+    assert [s.family for s in M.MatmulBlocks(M.f32, m, n, k).plan().steps] == ["k_product_tile"]
+
+
 @pytest.mark.parametrize("m,n,k,strides,shares,copied", [
     (97, 4096, 4096, {}, 2, 0), (97, 4097, 4096, {}, 1, 0), (128, 512, 1535, {}, 1, 640 * 1536), (128, 512, 3200, {}, 2, 0), (129, 510, 4992, {}, 3, 0), (200, 130, 8192, dict(a_stride=8193), 5, 200 * 8192), (96, 512, 8192, {}, 1, 0)])
 def test_few_tiles_share_k(m, n, k, strides, shares, copied):

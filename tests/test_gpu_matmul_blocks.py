@@ -145,8 +145,9 @@ def test_whole_chunks_at_odd_addresses(gpu, m, n, k):
                 x.check(x.run(out, offset=offset, **kw), out)
 
 
-# On tiles of 256 x 256 (169 of them): blocks of K that the ring's two and the scales' eight go around once and more, whole last ones and cut ones; scales of a in fours (blocks a multiple of four) and one by one
-WIDE = [(3100, 3100, 1200), (3100, 3101, 1424), (3099, 3100, 2304), (3100, 3100, 2560), (3100, 3100, 1300), (3090, 3100, 128), (3100, 3090, 272), (3100, 3100, 4096)]
+# On tiles of 256 x 256 (130 to 169 of them): blocks of K that the ring's two and the scales' eight go around once and more, whole last ones and cut ones; scales of a in fours (blocks a multiple of four) and one by one
+WIDE = [(3100, 3100, 1200), (3100, 3101, 1424), (3099, 3100, 2304), (3100, 3100, 2560), (3100, 3100, 1300), (3090, 3100, 128), (3100, 3090, 272), (3100, 3100, 4096),
+        (130, 33104, 272), (2049, 4096, 400), (2944, 2888, 1424)]
 # On tiles of 128 x 64, and past a round of 128 x 128, of many blocks
 MORE_TILES = [(1280, 1216, 400), (1279, 1217, 1552), (1280, 1216, 1024), (2049, 2050, 1168), (2049, 2050, 1024), (2170, 2060, 1300)]
 
