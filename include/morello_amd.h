@@ -803,9 +803,9 @@ int mrl_matmul_blocks_plan(const mrl_matmul_blocks *op, mrl_plan *plan, mrl_plan
 /* A layer of experts for few tokens.  For each token x: p = softmax over the experts of router x; the top_k experts of largest p are chosen (of equal ones the
  * lowest; a logit that is NaN counts as the lowest), their shares p, or p over the sum of the chosen's with `renormalise`;
  *     out = sum over the chosen e of share_e * down_e (silu(gate_e x) * up_e x)
- * Logits are summed in 64 bits, all else in 32; silu(gate x) * up x is rounded to bf16 before down, or to the sum of two bf16 numbers where
- * that costs nothing (up to 4 tokens, small layers).  Weights of experts that no token chooses are not read.
- * A token's results do not depend on the other tokens of the call but for their rounding.
+ * Logits are summed in 64 bits, all else in 32; silu(gate x) * up x is rounded to the sum of two bf16 numbers (sixteen bits) before down, so that results are
+ * rounded once.  Weights of experts that no token chooses are not read.
+ * A token's results do not depend on the other tokens of the call but for the order of sums in 32 bits.
  * params:
  *   0  x            bf16 [tokens][hidden]
  *   1  router       bf16 [experts][hidden]

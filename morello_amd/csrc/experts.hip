@@ -21,39 +21,44 @@ struct Places {
   double *logits;       // [tokens][experts]
   int32_t *chosen;      // [tokens][top_k]
   float *shares;        // [tokens][top_k]
-  uint16_t *h;          // [tokens * top_k][in_two ? 2 : 1][h_s]: rounded to bf16, and what that left, rounded
+  uint16_t *h;          // [tokens * top_k][2][h_s]: rounded to bf16, and what that left, rounded
   uint32_t h_s;
-  bool in_two;
   uint32_t down_shares; // workgroups that share some rows of down; of more than one, what each has
   float *sums;          // [down_shares][tokens][hidden_s]
   uint32_t hidden_s;
 };
-// What is between the products in one bf16 number adds as much to a result's error as rounding that does, and on few numbers by chance half as much again.  In two it adds nothing; that is free for few tokens, and where it is small (us of
-// the layer, in one and in two: 1 token through 64 experts of 2048 x 1024 31.1 and 31.0, 8 of 1024 x 768 in e4m3 40.3 and 40.9, 32 through 128 of 2048 x 768 107 and 113, 16 through 8 of 4096 x 14336 in bf16 475 and 513).
-bool kept_in_two(const ExpertsArgs &a) { return a.tokens <= 4 || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 14; }
-// Many tokens of each expert go in parts of sixteen, others in parts of eight, or four of what is in two.
-bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
+// What is between the products is in two bf16 numbers, sixteen bits of it, so that a result is rounded once, whatever other tokens there are: in one number results are off by 1.4 times as much (rms 0.0024 for 0.0017).  (us of the layer, in
+// one and in two, each in the forms that are fastest: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 114, 16 through 8 of 4096 x 14336 476 and 483, in e4m3 250 and 265, 100 tokens, 8 of 64 of 2048 x 768 150 and 149,
+// in e4m3 101 and 106, 128, 4 of 16 of 4096 x 1024 in e4m3 95 and 110: beside the weights every workgroup reads all tokens' h, which is twice as much.)
 
-// Rows of down to a workgroup at a time: eight where sixteen would leave half of the compute units without any, and in bf16 and parts of eight where these leave the unit with the most of them fewer.  (us of the layer, 8 and 16,
-// in bf16 and e4m3: 32 tokens through 128 experts of 2048 x 768 196 and 220, 106 and 119; 8 through 64 of 2880 x 768 124 and 118, 79 and 75; 32 through 64 of 6144 x 768 in bf16 294 and 308, 19 through 256 of 5376 x 320 in
-// e4m3 180 and 169, 2 through 60 of 6016 x 128 25.8 and 22.6; in parts of sixteen, where half of each instruction is lost on eight, 100 tokens through 64 of 2048 x 768 154 and 162, 100 and 106, 64 through 64 of 6144 x 1024
-// in e4m3 283 and 259.)
+// Many tokens of each expert, and more than a little of all, go through gate and up in parts of sixteen, others in parts of eight.
+bool few_of_each(const ExpertsArgs &a) { return a.tokens <= 8 || a.tokens * a.top_k < 6 * a.experts || uint64_t(a.tokens) * a.top_k * a.inter <= 1u << 13; }
+// Through down in parts of four, whose two numbers each leave a matrix instruction room for a pair of runs (PAIRED), or of sixteen.  (us of the layer, 4 and 16: 32 tokens, 8 of 128 experts of 2048 x 768 in bf16 197 and 200, 20 of 64 117 and 119, 1 of 64 of
+// 2048 x 1024 29 and 31; 16, 2 of 8 of 4096 x 14336 515 and 483, 48, 8 of 128 of 2048 x 768 in e4m3 133 and 127, 40, 4 of 60 of 1280 x 512 in bf16 66 and 62.)
+uint32_t parts_of_down(const ExpertsArgs &a) { return a.tokens <= 4 || a.tokens * a.top_k * 2 <= 5 * a.experts ? 4 : 16; }
+
+// Rows of down to a workgroup at a time.  In parts of four eight where sixteen would leave half of the compute units without any, and in bf16 where these leave the unit with the most of them fewer.  In parts of sixteen sixteen, several workgroups to the
+// same rows where units would have none: that halves what all of them read of h.  (us of the layer, 8 and 16: 64 tokens, 8 of 64 experts of 2048 x 768 in bf16 153 and 134, in e4m3 100 and 89, 128, 2 of 8 of 2048 x 1024 61 and 57, 100, 6 of 64 of 640 x 192 in e4m3 47 and 39; in parts of
+// four 16, 8 of 128 of 2048 x 768 in bf16 145 and 150.)
 uint32_t rows_of_down(const ExpertsArgs &a) {
+  if (parts_of_down(a) == 16) return 16;
   auto most_rows = [&](uint32_t h) { return ((a.hidden + h - 1) / h + g_compute_units - 1) / g_compute_units * h; };
-  return (few_of_each(a) && a.weight_dtype == MRL_BF16 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units) ? 8 : 16;
+  return (a.weight_dtype == MRL_BF16 ? most_rows(8) < most_rows(16) : a.hidden <= 8 * g_compute_units) ? 8 : 16;
 }
-// Workgroups that share some rows of down: as many as find a compute unit, with 48 steps of 2 KiB and more to each.  (us of the layer, one and as many: 94 tokens, 2 of 8 experts of 384 x 11652 in bf16 214 and 98, 1 token,
-// 8 of 64 of 384 x 9600 in e4m3 50 and 37, 109 tokens, 4 of 16 of 896 x 640 in bf16 47 and 38, 32 tokens, 8 of 128 of 1024 x 768 in e4m3 75 and 67; with less, 4 tokens, 4 of 64 of 1024 x 512 in bf16, 23.4 and 24.5.)
+uint32_t tokens_of_down(const ExpertsArgs &a);   // that a workgroup has sums for
+// Workgroups that share some rows of down: as many as find a compute unit, with 50 steps of 2 KiB and more to each.  (us of the layer, one and as many: 94 tokens, 2 of 8 experts of 384 x 11652 in bf16 214 and 103, 1 token,
+// 8 of 64 of 384 x 9600 in e4m3 50 and 37, 32 tokens, 8 of 128 of 1024 x 768 in e4m3 75 and 71; with 96 steps and with 48, 128 tokens, 4 of 16 of 512 x 512 in bf16 37 and 31, 100, 6 of 64 of 640 x 192 in e4m3 44.6 and 39.4; with less, 4 tokens, 4 of 64
+// of 1024 x 512 in bf16, 23.4 and 24.5.)
 uint32_t shares_of_down(const ExpertsArgs &a) {
-  const uint32_t height = rows_of_down(a), groups = (a.hidden + height - 1) / height, choices = a.tokens * a.top_k;
-  const uint32_t parts = std::max(std::min(a.experts, choices), choices / (few_of_each(a) ? 8 : 16));   // about
+  const uint32_t height = rows_of_down(a), here = tokens_of_down(a), groups = (a.hidden + height - 1) / height * ((a.tokens + here - 1) / here), choices = a.tokens * a.top_k;
+  const uint32_t parts = std::max(std::min(a.experts, choices), choices / parts_of_down(a));   // about
   const uint64_t steps = uint64_t(parts) * ((uint64_t(a.inter) * (a.weight_dtype == MRL_BF16 ? 2 : 1) * height + 2047) / 2048);
-  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(g_compute_units / groups, steps / 48)));
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(g_compute_units / groups, steps / 50)));
 }
 size_t places(const ExpertsArgs &a, Places *to) {
   Places w = {};
   const size_t choices = size_t(a.tokens) * a.top_k;
-  w.h_s = (a.inter + 63) / 64 * 64, w.in_two = few_of_each(a) && kept_in_two(a);
+  w.h_s = (a.inter + 63) / 64 * 64;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t *p = a.workspace ? a.workspace + at : nullptr;
@@ -65,7 +70,7 @@ size_t places(const ExpertsArgs &a, Places *to) {
   w.shares = (float *)take(4 * choices);
   w.down_shares = shares_of_down(a), w.hidden_s = (a.hidden + 3) / 4 * 4;
   if (w.down_shares > 1) w.sums = (float *)take(sizeof(float) * w.down_shares * a.tokens * w.hidden_s);
-  w.h = (uint16_t *)take((w.in_two ? 4 : 2) * choices * w.h_s);
+  w.h = (uint16_t *)take(4 * choices * w.h_s);
   if (to) *to = w;
   return at;
 }
@@ -259,7 +264,8 @@ bool fused_choice(const ExpertsArgs &a) { return a.tokens <= MOST_FUSED_TOKENS &
 // ---- Products with experts' weights: 16 rows of each of N matrices against the x of a part's tokens, a step of 128 bytes of the rows at a time.  Loads take a row's 128 bytes with eight
 // lanes, x's with eight or sixteen, and LDS brings both into the order in which the matrix instructions want them: what bounds such loops else is the rate at which a compute
 // unit's address unit takes cache lines, of which a load of 16 bytes of sixteen rows next to each other has four times as many. ----
-// ROOM: tokens that a part may have, 8 or 16.  HOW a step fills an instruction: FULL as above; HALF: with eight rows, and nothing for the others; PAIRED, of parts of eight: eight rows and tokens, 256 bytes of the
+// ROOM: tokens that a part may have, 8 or 16, or where a token has two numbers for each twice what it may have, 8 or 32: "tokens" below are then a token's first numbers and, next to them, its second.  More than sixteen are
+// multiplied sixteen after sixteen by the same rows in registers.  HOW a step fills an instruction: FULL as above; HALF: with eight rows, and nothing for the others; PAIRED, of a ROOM of eight: eight rows and tokens, 256 bytes of the
 // rows, whose second 128 go where rows and tokens 8 to 15 would be: the instruction's sums of rows 0 to 7 with tokens 0 to 7, and of 8 to 15 with 8 to 15, are what is wanted.
 enum How { FULL = 0, HALF = 1, PAIRED = 2 };
 template <bool F8, int ROOM, int HOW>
@@ -269,7 +275,8 @@ struct Shape {
   static constexpr int LANES = BYTES / 16, LOADS = HOW == HALF ? 1 : 2;                 // of a row in a load; loads for all rows
   static constexpr int X_BYTES = STEP * 2, X_CHUNKS = X_BYTES / 16;                     // of a token's x
   static constexpr int X_LOADS = ROOM * X_BYTES / 1024, X_TOKENS = 64 / X_CHUNKS;       // for all tokens; tokens of a load
-  static constexpr int IN_LDS = ROOM * PAIR, ROW_BYTES = X_BYTES / PAIR;                // tokens as the instruction has them, and of one of these
+  static constexpr int GROUPS = ROOM > 16 ? ROOM / 16 : 1, GROUP_LOADS = X_LOADS / GROUPS;  // sixteens that the same rows are multiplied by, one after the other
+  static constexpr int IN_LDS = ROOM / GROUPS * PAIR, ROW_BYTES = X_BYTES / PAIR;       // tokens as the instruction has them, and of one of these
   static constexpr int BOUNCE = IN_LDS * ROW_BYTES;
   static_assert(HOW != PAIRED || ROOM == 8, "");
 };
@@ -339,7 +346,7 @@ struct Step {
   }
   // bounce: LDS of this wave's, N tiles and x of IN_LDS tokens.  Chunk c of a row of 128 bytes at c ^ (row / 2 % 8), of 256 bytes at c ^ row: sixteen lanes with a
   // chunk of sixteen rows each reach every bank once.
-  __device__ inline void multiply(v4f (&acc)[N], uint8_t *bounce) {
+  __device__ inline void multiply(v4f (&acc)[N][S::GROUPS], uint8_t *bounce) {
     const uint32_t lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     if (TAIL == INSIDE && __any(left < 16 || x_left < 16)) {
 #pragma unroll
@@ -351,6 +358,15 @@ struct Step {
       if (F8 && HOW == PAIRED && left + int(lane % S::LANES) * 16 <= int(lane / 32) * 128) scale = 0;   // (no such block; the last one's may be infinite)
     }
     uint8_t *const of_x = bounce + N * TILE_BYTES;
+    auto put_x = [&](int g) {
+#pragma unroll
+      for (int i = 0; i < S::GROUP_LOADS; i++)
+        if (g * S::GROUP_LOADS + i < x_loads) {
+          constexpr uint32_t CHUNKS = S::ROW_BYTES / 16;
+          const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS + lane % S::X_CHUNKS / CHUNKS * 8;
+          *(v4i *)(of_x + token * S::ROW_BYTES + (lane % CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[g * S::GROUP_LOADS + i];
+        }
+    };
     lanes_meet();   // (over what the step before was multiplied from)
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -359,47 +375,73 @@ struct Step {
         const uint32_t row = lane / S::LANES + i * (64 / S::LANES) + lane % S::LANES / 8 * 8;
         *(v4i *)(bounce + n * TILE_BYTES + row * 128 + (lane % 8 ^ (row / 2 & 7)) * 16) = q[n][i];
       }
-#pragma unroll
-    for (int i = 0; i < S::X_LOADS; i++)
-      if (i < x_loads) {
-        constexpr uint32_t CHUNKS = S::ROW_BYTES / 16;
-        const uint32_t token = lane / S::X_CHUNKS + i * S::X_TOKENS + lane % S::X_CHUNKS / CHUNKS * 8;
-        *(v4i *)(of_x + token * S::ROW_BYTES + (lane % CHUNKS ^ (F8 ? token : token / 2 % 8)) * 16) = y[i];
-      }
+    put_x(0);
     lanes_meet();
     const uint32_t mine = li & (S::IN_LDS - 1);
     const uint8_t *const my_x = of_x + mine * S::ROW_BYTES;
     float scales[2] = {0, 0};
     if constexpr (F8 && HOW == PAIRED) scales[0] = scale;
     else if constexpr (F8) scales[0] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale))), scales[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 32));
+    auto weights = [&](int n, int i) { return *(const v4i *)(bounce + n * TILE_BYTES + li * 128 + ((i * 4 + lg) ^ (li >> 1)) * 16); };
+    auto next_group = [&](int g) {   // (of a part that has tokens for it)
+      lanes_meet();
+      put_x(g);
+      lanes_meet();
+    };
     if constexpr (F8) {
-      v4i u[2][2];
+      v4i b[S::GROUPS > 1 ? 2 : 1][2];   // (a group's alone: as they are wanted)
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) u[i][j] = *(const v4i *)(my_x + ((i * 8 + lg * 2 + j) ^ mine) * 16);
-#pragma unroll
-      for (int n = 0; n < N; n++) {
-        v4f part = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const v4i w = *(const v4i *)(bounce + n * TILE_BYTES + li * 128 + ((i * 4 + lg) ^ (li >> 1)) * 16);
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            int b[4];
-            widen4(w[2 * j], b[0], b[1]);
-            widen4(w[2 * j + 1], b[2], b[3]);
-            part = mma_bf16(v4i{b[0], b[1], b[2], b[3]}, u[i][j], part);
-          }
+      for (int g = 0; g < S::GROUPS; g++) {
+        if (g > 0) {
+          if (g * S::GROUP_LOADS >= x_loads) break;
+          next_group(g);
         }
-        acc[n] += part * scales[n];
+        v4i u[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) u[i][j] = *(const v4i *)(my_x + ((i * 8 + lg * 2 + j) ^ mine) * 16);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+          v4f part = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            v4i(&wide)[2] = b[S::GROUPS > 1 ? i : 0];
+            if (g == 0) {
+              const v4i w = weights(n, i);
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                int x[4];
+                widen4(w[2 * j], x[0], x[1]);
+                widen4(w[2 * j + 1], x[2], x[3]);
+                wide[j] = v4i{x[0], x[1], x[2], x[3]};
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) part = mma_bf16(wide[j], u[i][j], part);
+          }
+          acc[n][g] += part * scales[n];
+        }
       }
     } else {
+      v4i b[2];
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const v4i u = *(const v4i *)(my_x + ((i * 4 + lg) ^ (mine >> 1)) * 16);
+      for (int g = 0; g < S::GROUPS; g++) {
+        if (g > 0) {
+          if (g * S::GROUP_LOADS >= x_loads) break;
+          next_group(g);
+        }
 #pragma unroll
-        for (int n = 0; n < N; n++) acc[n] = mma_bf16(*(const v4i *)(bounce + n * TILE_BYTES + li * 128 + ((i * 4 + lg) ^ (li >> 1)) * 16), u, acc[n]);
+        for (int i = 0; i < 2; i++) {
+          const v4i u = *(const v4i *)(my_x + ((i * 4 + lg) ^ (mine >> 1)) * 16);
+          if constexpr (S::GROUPS > 1) {
+            if (g == 0) b[i] = weights(0, i);
+            acc[0][g] = mma_bf16(b[i], u, acc[0][g]);
+          } else {
+#pragma unroll
+            for (int n = 0; n < N; n++) acc[n][g] = mma_bf16(weights(n, i), u, acc[n][g]);
+          }
+        }
       }
     }
   }
@@ -522,7 +564,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
   }
   uint32_t turn = 0;
   for (uint32_t tile = blockIdx.x; tile < line; tile += gridDim.x, turn ^= 1) {
-    v4f acc[2] = {};
+    v4f acc[2][1] = {};
     for (uint32_t at = 0; at < n; at += AHEAD) {
       const bool last = at + AHEAD >= n, more = tile + gridDim.x < line;
       if (last && more) go_to(tile + gridDim.x);
@@ -534,7 +576,7 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
       }
     }
     v4f(&here)[UP_WAVES][2][64] = sums[turn];
-    here[wave][0][lane] = acc[0], here[wave][1][lane] = acc[1];
+    here[wave][0][lane] = acc[0][0], here[wave][1][lane] = acc[1][0];
     __syncthreads();   // (the tile before the last has been read: its readers are here)
     if (wave == tile / gridDim.x % UP_WAVES) {
       v4f g = here[0][0][lane], u = here[0][1][lane], h;
@@ -545,17 +587,15 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
       const uint32_t part = by_tiles.div(tile), row = (tile - part * tiles) * 16 + lg * 4;
       const Part q = lists.parts[part];
       if (li < q.count && row < p.inter) {
-        uint16_t *const to = w.h + (uint64_t(lists.choices[q.first + li]) << (w.in_two ? 1 : 0)) * w.h_s + row;
+        uint16_t *const to = w.h + uint64_t(lists.choices[q.first + li]) * 2 * w.h_s + row;
         store4(to, h, int(p.inter - row));
-        if (w.in_two) {
-          v4f rest;
+        v4f rest;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float r = h[i] - float((__bf16)h[i]);
-            rest[i] = fabsf(r) < __builtin_inff() ? r : 0.0f;
-          }
-          store4(to + w.h_s, rest, int(p.inter - row));
+        for (int i = 0; i < 4; i++) {
+          const float r = h[i] - float((__bf16)h[i]);
+          rest[i] = fabsf(r) < __builtin_inff() ? r : 0.0f;
         }
+        store4(to + w.h_s, rest, int(p.inter - row));
       }
     }
   }
@@ -563,13 +603,13 @@ __global__ __launch_bounds__(UP_WAVES * 64, 2) void k_experts_up(ExpertsArgs p, 
 
 // ---- Down: a workgroup to 16 rows, or 8, and behind them those gridDim.x further; blockIdx.y: tokens_here tokens; blockIdx.z: which of those that share the rows.  All parts' steps in a line, cut into pieces of up to
 // 1024 bytes of a part's rows, of which a wave has every eighth: a workgroup's waves go through the same rows together, and each asks for the next rows' weights while it multiplies the last of these.  (Eight rows PAIRED
-// against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 193 and 197, in e4m3 110 and 112; 8 of 1024 through 64 40.2 and 42.  A workgroup to each rows, 1 token, 2 of 8 of 4992 x 768 in e4m3 23.4
-// for 21.0; sixteen waves, 32 tokens as above 194 for 196 in bf16, 110 for 106 in e4m3.) ----
+// against HALF, us of the layer: 32 tokens through 128 experts of 2048 x 768 in bf16 199 and 221, in e4m3 114 and 120; 8 of 1024 through 64 40.6 and 42.5.  A workgroup to each rows, 1 token, 2 of 8 of 4992 x 768 in e4m3 23.4
+// for 21.0; sixteen waves, with h in one number, 32 tokens as above 194 for 196 in bf16, 110 for 106 in e4m3.) ----
 constexpr int DOWN_WAVES = 8;
-template <bool F8, int ROOM, int TAIL, int HOW, bool IN_TWO>
+template <bool F8, int MOST, int TAIL, int HOW>
 __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p, Places w, uint32_t tokens_here, uint32_t words) {
-  constexpr int WAVES = DOWN_WAVES, THREADS = WAVES * 64, AHEAD = HOW == PAIRED ? 4 : 6;   // (PAIRED: of twice the bytes)
-  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8, EACH = IN_TWO ? 2 : 1, MOST = ROOM / EACH;   // (IN_TWO: a token's two next to each other, as two tokens)
+  constexpr int ROOM = MOST * 2, WAVES = DOWN_WAVES, THREADS = WAVES * 64, AHEAD = F8 && ROOM == 32 ? 3 : HOW == PAIRED || ROOM == 32 ? 4 : 6;   // (what registers take: PAIRED has twice a step's bytes, ROOM 32 four times those of x)
+  constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
   typedef Shape<F8, ROOM, HOW> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t dynamic[];
   v4f *const sums = (v4f *)dynamic;                            // [WAVES][tokens_here][4]
@@ -628,12 +668,12 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       const Part q = lists.parts[part];
       fetch_s = (fetch_piece - part * of_part) * size, fetch_end = min(steps, fetch_s + size);
       of.matrix(0, p.down, __builtin_amdgcn_readfirstlane(q.expert), fetch_group * HEIGHT, min(HEIGHT, p.hidden - fetch_group * HEIGHT));
-      of.tokens(__builtin_amdgcn_readfirstlane(q.count) * EACH, [&](uint32_t i) { return w.h + (uint64_t(t0 * p.top_k + lists.choices[q.first + i / EACH]) * EACH + i % EACH) * w.h_s; });
+      of.tokens(__builtin_amdgcn_readfirstlane(q.count) * 2, [&](uint32_t i) { return w.h + (uint64_t(t0 * p.top_k + lists.choices[q.first + i / 2]) * 2 + i % 2) * w.h_s; });
     }
     to.fetch(of, fetch_s, int(p.inter));
     if (++fetch_s == fetch_end && (fetch_piece += all_waves) >= pieces) fetch_piece = first, fetch_group += gridDim.x;
   };
-  v4f acc[1] = {};
+  v4f acc[1][S::GROUPS] = {};
 #pragma unroll
   for (int a = 0; a < AHEAD; a++)
     if (fetch_group < groups) fetch(t[a]);
@@ -649,20 +689,21 @@ __global__ __launch_bounds__(DOWN_WAVES * 64) void k_experts_down(ExpertsArgs p,
       if (fetch_group < groups) fetch(t[a]);
       if (++s == end) {
         const Part q = lists.parts[piece / of_part];
-        uint32_t i = HOW == PAIRED ? li - lg / 2 * 8 : li;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
-        if constexpr (IN_TWO) {
+#pragma unroll
+        for (int g = 0; g < S::GROUPS; g++) {
+          const uint32_t column = (HOW == PAIRED ? li - lg / 2 * 8 : li) + g * 16;   // (PAIRED: below 8 where the lane's sums are wanted, or far above)
+          v4f both;
 #pragma unroll
           for (int e = 0; e < 4; e++) {   // (and the next lane's, but where that is infinity times nothing)
-            const float x = acc[0][e], rest = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));
-            acc[0][e] = fabsf(x) < __builtin_inff() ? x + rest : x;
+            const float x = acc[0][g][e], rest = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));
+            both[e] = fabsf(x) < __builtin_inff() ? x + rest : x;
           }
-          i = i % 2 ? ~0u : i / 2;
+          if (column % 2 == 0 && column / 2 < q.count) {
+            const uint32_t choice = lists.choices[q.first + column / 2];
+            sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += both * shares[choice];
+          }
+          acc[0][g] = v4f{0, 0, 0, 0};
         }
-        if (i < q.count) {
-          const uint32_t choice = lists.choices[q.first + i];
-          sums[(wave * tokens_here + choice / p.top_k) * 4 + lg] += acc[0] * shares[choice];
-        }
-        acc[0] = v4f{0, 0, 0, 0};
         if ((piece += all_waves) >= pieces) finish(group), group += gridDim.x, piece = first;
       }
     }
@@ -707,22 +748,33 @@ hipError_t launch_up(const ExpertsArgs &a, const Places &w, hipStream_t stream) 
   return launch_up_waves<F8, ROOM, FUSED, TAIL, 4>(a, w, stream);
 }
 constexpr size_t MOST_LDS = 160 * 1024;
-template <bool F8, int ROOM, int HOW, bool IN_TWO>
+template <bool F8, int MOST, int HOW>
 size_t down_lds(const ExpertsArgs &a, uint32_t here) {
-  return size_t(DOWN_WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + DOWN_WAVES * (TILE_BYTES + Shape<F8, ROOM, HOW>::BOUNCE) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, IN_TWO ? ROOM / 2 : ROOM, DOWN_WAVES);
+  return size_t(DOWN_WAVES) * here * 64 + size_t(here * a.top_k + 3) / 4 * 16 + DOWN_WAVES * (TILE_BYTES + Shape<F8, MOST * 2, HOW>::BOUNCE) + Lists::bytes(a.experts, here * a.top_k, (here + 31) / 32, MOST, DOWN_WAVES);
 }
-template <bool F8, int ROOM, int TAIL, int HOW, bool IN_TWO>
+// Of rows of a single run of 128 bytes there is no pair.  (us of the layer, HALF and PAIRED, in e4m3, 4 tokens, 8 of 64 experts of 2048 x 128 21.1 and 22.9.)
+How how_of_down(const ExpertsArgs &a) { return rows_of_down(a) == 16 ? FULL : a.inter * (a.weight_dtype == MRL_BF16 ? 2 : 1) > 128 ? PAIRED : HALF; }
+template <bool F8>
+size_t down_lds(const ExpertsArgs &a, uint32_t here) {
+  const How how = how_of_down(a);
+  return how == PAIRED ? down_lds<F8, 4, PAIRED>(a, here) : how == HALF ? down_lds<F8, 4, HALF>(a, here) : parts_of_down(a) == 4 ? down_lds<F8, 4, FULL>(a, here) : down_lds<F8, 16, FULL>(a, here);
+}
+uint32_t tokens_of_down(const ExpertsArgs &a) {
+  uint32_t here = a.tokens;   // all, or as many as LDS has place for
+  while ((a.weight_dtype == MRL_BF16 ? down_lds<false>(a, here) : down_lds<true>(a, here)) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
+  return here;
+}
+template <bool F8, int MOST, int TAIL, int HOW>
 hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
   constexpr uint32_t HEIGHT = HOW == FULL ? 16 : 8;
-  uint32_t here = a.tokens;   // of a workgroup: all, or as many as its sums have place for
-  while (down_lds<F8, ROOM, HOW, IN_TWO>(a, here) > MOST_LDS) here -= (here + 31) / 32 > 1 ? here - (here - 1) / 32 * 32 : here / 2;
+  const uint32_t here = tokens_of_down(a);
   static std::atomic<uint64_t> raised{0};
   if (!plan::recording()) {
-    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), MOST_LDS);
+    const hipError_t e = raise_lds_limit(raised, reinterpret_cast<const void *>(&k_experts_down<F8, MOST, TAIL, HOW>), MOST_LDS);
     if (e != hipSuccess) return e;
   }
-  const size_t lds = down_lds<F8, ROOM, HOW, IN_TWO>(a, here);
-  MRL_LAUNCH((k_experts_down<F8, ROOM, TAIL, HOW, IN_TWO>), dim3(std::min((a.hidden + HEIGHT - 1) / HEIGHT, uint32_t(g_compute_units)), (a.tokens + here - 1) / here, w.down_shares), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
+  const size_t lds = down_lds<F8, MOST, HOW>(a, here);
+  MRL_LAUNCH((k_experts_down<F8, MOST, TAIL, HOW>), dim3(std::min((a.hidden + HEIGHT - 1) / HEIGHT, uint32_t(g_compute_units)), (a.tokens + here - 1) / here, w.down_shares), dim3(DOWN_WAVES * 64), lds, stream, a, w, here, (here + 31) / 32);
   if (w.down_shares > 1) {
     plan::work(plan::UNIT_STREAM, 0, (4.0 * w.down_shares + 2) * a.tokens * a.hidden);
     MRL_LAUNCH(k_experts_join, dim3((a.hidden + JOIN_THREADS * 4 - 1) / (JOIN_THREADS * 4), a.tokens), dim3(JOIN_THREADS), 0, stream, a, w);
@@ -732,13 +784,13 @@ hipError_t launch_down(const ExpertsArgs &a, const Places &w, hipStream_t stream
 // How rows of k elements end.
 template <bool F8>
 Tail tail_of(uint32_t k, uint32_t step = F8 ? 128 : 64) { return k * (F8 ? 1 : 2) < 16 || k * 2 < 16 ? SHORT : k % step ? INSIDE : WHOLE; }
-template <bool F8, int ROOM, int HOW, bool IN_TWO>
+template <bool F8, int MOST, int HOW>
 hipError_t launch_down_how(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
-  const Tail tail = tail_of<F8>(a.inter, Shape<F8, ROOM, HOW>::STEP);
-  if constexpr (HOW != PAIRED) {   // (pairs are of rows of more than 128 bytes)
-    if (tail == SHORT) return launch_down<F8, ROOM, SHORT, HOW, IN_TWO>(a, w, stream);
+  const Tail tail = tail_of<F8>(a.inter, Shape<F8, MOST * 2, HOW>::STEP);
+  if constexpr (HOW != PAIRED) {
+    if (tail == SHORT) return launch_down<F8, MOST, SHORT, HOW>(a, w, stream);
   }
-  return tail == WHOLE ? launch_down<F8, ROOM, WHOLE, HOW, IN_TWO>(a, w, stream) : launch_down<F8, ROOM, INSIDE, HOW, IN_TWO>(a, w, stream);
+  return tail == WHOLE ? launch_down<F8, MOST, WHOLE, HOW>(a, w, stream) : launch_down<F8, MOST, INSIDE, HOW>(a, w, stream);
 }
 template <bool F8, int ROOM, bool FUSED>
 hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
@@ -750,13 +802,11 @@ hipError_t launch_products(const ExpertsArgs &a, const Places &w, hipStream_t st
                                       : launch_up<F8, ROOM, FUSED, SHORT>(a, w, stream);
   if (e != hipSuccess) return e;
   plan::work(plan::UNIT_STREAM, 0, weight / 3);
-  // Of rows of a single run of 128 bytes there is no pair.  (us of the layer, HALF and PAIRED, in e4m3: 44 tokens, 6 of 64 experts of 640 x 128 27.2 and 31.1, 4 tokens, 8 of 64 of 2048 x 128 21.1 and 22.9.)
-  const bool eight = rows_of_down(a) == 8, pair = ROOM == 8 && eight && a.inter * (F8 ? 1 : 2) > 128;
-  if constexpr (ROOM == 8) {
-    if (w.in_two) return pair ? launch_down_how<F8, ROOM, PAIRED, true>(a, w, stream) : eight ? launch_down_how<F8, ROOM, HALF, true>(a, w, stream) : launch_down_how<F8, ROOM, FULL, true>(a, w, stream);
-    if (pair) return launch_down_how<F8, ROOM, PAIRED, false>(a, w, stream);
+  switch (how_of_down(a)) {
+    case PAIRED: return launch_down_how<F8, 4, PAIRED>(a, w, stream);
+    case HALF: return launch_down_how<F8, 4, HALF>(a, w, stream);
+    default: return parts_of_down(a) == 4 ? launch_down_how<F8, 4, FULL>(a, w, stream) : launch_down_how<F8, 16, FULL>(a, w, stream);
   }
-  return eight ? launch_down_how<F8, ROOM, HALF, false>(a, w, stream) : launch_down_how<F8, ROOM, FULL, false>(a, w, stream);
 }
 template <bool F8>
 hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
@@ -769,7 +819,7 @@ hipError_t launch(const ExpertsArgs &a, const Places &w, hipStream_t stream) {
     plan::work(plan::UNIT_STREAM, 0, 8.0 * a.experts * a.tokens);
     MRL_LAUNCH(k_experts_choose, dim3(a.tokens), dim3((a.experts + 63) / 64 * 64), 0, stream, a, w);
   }
-  // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.  (us, 16 and 8, choices an expert: 2 113.6 and 111.6,
+  // Parts of sixteen are what a matrix instruction takes; of eight take less LDS, fewer registers, and less of x where few of an expert's are there.  (us, 16 and 8 for up and down alike, with h in one number, choices an expert: 2 113.6 and 111.6,
   // 4 33.3 and 31.5, 6 149.2 and 150.5, 137 and 145, 8 156 and 172, 91 and 101.)
   return !few ? launch_products<F8, 16, false>(a, w, stream) : fused ? launch_products<F8, 8, true>(a, w, stream) : launch_products<F8, 8, false>(a, w, stream);
 }

@@ -175,8 +175,8 @@ def test_values_are_compared_of_every_form_of_the_kernels():
         for tail in range(3):
             want |= {f"k_experts_up [F8 = {f8}, ROOM = 16, FUSED = false, TAIL = {tail}, UP_WAVES = 4]"}
             want |= {f"k_experts_up [F8 = {f8}, ROOM = 8, FUSED = {fused}, TAIL = {tail}, UP_WAVES = {waves}]" for fused in ("false", "true") for waves in (4, 8) if (waves, tail) != (8, 2)}
-            want |= {f"k_experts_down [F8 = {f8}, ROOM = 16, TAIL = {tail}, HOW = {how}, IN_TWO = false]" for how in range(2)}
-            want |= {f"k_experts_down [F8 = {f8}, ROOM = 8, TAIL = {tail}, HOW = {how}, IN_TWO = {two}]" for how in range(3) for two in ("false", "true") if (how, tail) != (2, 2)}
+            want |= {f"k_experts_down [F8 = {f8}, MOST = 16, TAIL = {tail}, HOW = 0]"}
+            want |= {f"k_experts_down [F8 = {f8}, MOST = 4, TAIL = {tail}, HOW = {how}]" for how in range(3) if (how, tail) != (2, 2)}
     assert want <= reached, sorted(want - reached)
     assert {k for k in reached - want if "[" in k and not k.startswith(("k_experts_logits", "k_pad_rows"))} == set()
 
