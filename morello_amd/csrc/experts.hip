@@ -5,8 +5,8 @@
 // instructions take them: 16 rows of weights against up to 16 of the expert's tokens, 128 bytes of each row at a time, a lane 32 of them.
 // Each of the steps needs all of the one before, a launch each: logits; choice (with few tokens and experts every workgroup of the next launch makes it for itself);
 // gate and up to h, 16 rows of one expert at a time; down, a workgroup to some rows of all experts, so that a token's sum over
-// its experts is formed in one place and in one order (several workgroups to fewer rows than there are compute units for, and a launch that adds up what they have).  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 462 to 500 (2.8 GB, 5.6 to 6.0 TB/s: up 309, down 154); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 104 to 112 (528 MB, 4.7 to 5.1 TB/s:
-// logits and choice 5 each, up 59, down 34); 1 token, 8 of 64 of 2048 x 1024 in bf16 27 (101 MB: 3, 15, 9; each launch begins with 3 to 4 of reading what the one before left).  A choice is known by its number i = token * top_k + j; no lists go through memory but the chosen experts.
+// its experts is formed in one place and in one order (several workgroups to fewer rows than there are compute units for, and a launch that adds up what they have).  us: 16 tokens, 2 of 8 experts of 4096 x 14336 in bf16 475 to 492 (2.8 GB, 5.7 to 5.9 TB/s: up 314, down 157); 32 tokens, 8 of 128 of 2048 x 768 in e4m3 110 to 115 (528 MB, 4.6 to 4.8 TB/s:
+// logits and choice 5 each, up 62, down 40); 1 token, 8 of 64 of 2048 x 1024 in bf16 27 (101 MB: 3, 15, 9; each launch begins with 3 to 4 of reading what the one before left).  A choice is known by its number i = token * top_k + j; no lists go through memory but the chosen experts.
 #include <algorithm>
 
 #include "blocks_device.h"
